@@ -24,7 +24,10 @@ STATUS = {0: "CIA_OK", 1: "CIA_ERR_NULL", 2: "CIA_ERR_ALIGN", 3: "CIA_ERR_ARG",
           4: "CIA_ERR_HIP", 5: "CIA_ERR_STATE", 6: "CIA_ERR_NOSLOT",
           7: "CIA_ERR_IO"}
 
-# Every symbol include/cuda_inf_attn.h declares, with its ctypes signature.
+MOE_MAX_EXPERTS, MOE_MAX_TOP_K = 256, 16  # include/cuda_inf_ffn.h
+SCORES = {"sigmoid": 0, "softmax": 1}
+
+# Every symbol the headers in include/ declare, with its ctypes signature.
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
@@ -66,6 +69,15 @@ SIGNATURES = {
     "cia_decode_loop_ex": (_I, [_P, _I, _P, _P, _P, _P, _I, _I, _F, _I, _P, _P]),
     "cia_decode_loop_runs": (_I, [_P, _I, _P, _P, _P, _P, _I, _I, _F, _I, _I, _P, _P]),
     "cia_decode_fault": (_I, [_P, ctypes.c_int64, _P]),
+    # include/cuda_inf_ffn.h
+    "cia_add_rmsnorm": (_I, [_P, _P, _P, _F, _P, _P, _I, _I, _P]),
+    "cia_moe_route": (_I, [_P] * 7 + [_I, _I, _P]),
+    "cia_moe_select": (_I, [_P] * 5 + [_I, _P]),
+    "cia_moe_up_int4": (_I, [_P] * 5 + [_I] * 5 + [_P, ctypes.c_int64, _P]),
+    "cia_moe_down_int4": (_I, [_P] * 6 + [_I] * 5 + [_P, ctypes.c_int64, _P]),
+    "cia_moe_workspace_bytes": (ctypes.c_int64, [_I] * 5),
+    "cia_moe_block_workspace_bytes": (ctypes.c_int64, [_P, _I]),
+    "cia_moe_block_forward": (_I, [_P, _P, _I, _P]),
     # include/cuda_inf_model.h
     "cia_index_read": (_I, [ctypes.c_char_p, _P, ctypes.c_int64, _P]),
     "cia_file_size": (_I, [ctypes.c_char_p, _P]),
@@ -171,3 +183,22 @@ class cia_layer(ctypes.Structure):
         ("d_dst", _P), ("n_live", _I), ("ws_mass", _P),
         ("qw", _P), ("kw", _P), ("eps", _F), ("theta", _F), ("prep_ws", _P), ("prep_cap", _I),
     ]
+
+
+class cia_moe_gating(ctypes.Structure):
+    """Mirror of ``cia_moe_gating`` in include/cuda_inf_ffn.h."""
+    _fields_ = [("n_experts", _I), ("top_k", _I), ("score", _I), ("n_group", _I),
+                ("topk_group", _I), ("renorm", _I), ("eps", _F), ("scale", _F)]
+
+
+class cia_q4_experts(ctypes.Structure):
+    """Mirror of ``cia_q4_experts`` in include/cuda_inf_ffn.h."""
+    _fields_ = [("packed", _P), ("scales", _P), ("packed_stride", ctypes.c_int64),
+                ("scales_stride", ctypes.c_int64)]
+
+
+class cia_moe(ctypes.Structure):
+    """Mirror of ``cia_moe`` in include/cuda_inf_ffn.h."""
+    _fields_ = [("norm_w", _P), ("norm_eps", _F), ("H", _I), ("F", _I), ("gate", _P), ("bias", _P),
+                ("gating", cia_moe_gating), ("w1", cia_q4_experts), ("w3", cia_q4_experts),
+                ("w2", cia_q4_experts), ("ws", _P), ("ws_bytes", ctypes.c_int64), ("cap", _I)]

@@ -254,3 +254,95 @@ def qkv_proj_int4(x, wq, wk, wv, q, k, v, M: int, K: int = 2048) -> None:
     call("cia_qkv_proj_int4", _dev(x, "x", _F16, M * K), pq, sq, Nq, pk, sk, pv, sv, Nkv, K, M,
          _dev(q, "q", _F16, M * Nq), _dev(k, "k", _F16, M * Nkv), _dev(v, "v", _F16, M * Nkv),
          stream_handle())
+
+
+# ------------------------------------------------------------ feed-forward branch
+def add_rmsnorm(h, w, out, S: int, H: int, eps: float = 1e-5, add=None, hsum=None) -> None:
+    """engine.cu:867, 870: hsum = h + add (fp32 [S, H]; add and hsum optional,
+    hsum may be h or add), out = fp16(hsum * rsqrt(mean(hsum^2) + eps) * w)."""
+    f32 = (torch.float32,)
+    call("cia_add_rmsnorm", _dev(h, "h", f32, S * H), _opt(add, "add", f32, S * H), _dev(w, "w", _F16, H),
+         float(eps), _opt(hsum, "hsum", f32, S * H), _dev(out, "out", _F16, S * H), S, H, stream_handle())
+
+
+def moe_gating(E: int, k: int, score: str = "sigmoid", n_group: int = 1, topk_group: int = 1,
+               renorm: bool = True, eps: float = 1e-6, scale: float = 1.0):
+    """How a router chooses, as moe_route and moe_select take it."""
+    if score not in _lib.SCORES:
+        raise ValueError(f"score: {score!r} is not one of {sorted(_lib.SCORES)}")
+    return _lib.cia_moe_gating(E, k, _lib.SCORES[score], n_group, topk_group, int(bool(renorm)),
+                               float(eps), float(scale))
+
+
+def moe_route(x, gate, ids, weights, S: int, H: int, E: int, k: int, bias=None, logits=None,
+              **gating) -> None:
+    """engine.cu:878-893 on the device: the k experts of each of the S rows of x
+    (fp16 [S, H]; gate fp16 [E, H]; bias fp32 [E], for the choice alone) into
+    ids int32 [S, k] and weights fp32 [S, k]; logits fp32 [S, E], optional.
+    gating: score, n_group, topk_group, renorm, eps, scale, as moe_gating."""
+    f32 = (torch.float32,)
+    call("cia_moe_route", _dev(x, "x", _F16, S * H), _dev(gate, "gate", _F16, E * H),
+         _opt(bias, "bias", f32, E), ctypes.byref(moe_gating(E, k, **gating)),
+         _dev(ids, "ids", (torch.int32,), S * k), _dev(weights, "weights", f32, S * k),
+         _opt(logits, "logits", f32, S * E), S, H, stream_handle())
+
+
+def moe_select(logits, ids, weights, S: int, E: int, k: int, bias=None, **gating) -> None:
+    """moe_route's choice from logits fp32 [S, E]."""
+    f32 = (torch.float32,)
+    call("cia_moe_select", _dev(logits, "logits", f32, S * E), _opt(bias, "bias", f32, E),
+         ctypes.byref(moe_gating(E, k, **gating)), _dev(ids, "ids", (torch.int32,), S * k),
+         _dev(weights, "weights", f32, S * k), S, stream_handle())
+
+
+def q4_experts(w, name: str):
+    """(cia_q4_experts, E, rows, cols) of INT4 group-128 experts: w = (packed u8
+    [E, rows, cols / 2], scales fp16 [E, rows, cols / 128]) on the device.  Each
+    expert is contiguous; the experts may lie apart, at one stride."""
+    packed, scales = w
+    for t, part, dtypes in ((packed, ".packed", (torch.uint8,)), (scales, ".scales", _F16)):
+        if not isinstance(t, torch.Tensor) or t.dim() != 3:
+            raise ValueError(f"{name}{part}: need a tensor [experts, rows, columns]")
+        if not t.is_cuda:
+            raise ValueError(f"{name}{part}: must be a device tensor")
+        if t.dtype not in dtypes:
+            raise TypeError(f"{name}{part}: dtype {t.dtype} not in {dtypes}")
+        if t.shape[0] and not t[0].is_contiguous():
+            raise ValueError(f"{name}{part}: an expert must be contiguous")
+    E, rows, half = packed.shape
+    if half % 64 or tuple(scales.shape) != (E, rows, half // 64):
+        raise ValueError(f"{name}: packed {tuple(packed.shape)} and scales {tuple(scales.shape)} do not fit: "
+                         "[E, rows, cols / 2] and [E, rows, cols / 128], cols a multiple of 128")
+    return (_lib.cia_q4_experts(packed.data_ptr(), scales.data_ptr(), packed.stride(0), scales.stride(0)),
+            E, rows, 2 * half)
+
+
+def moe_workspace_bytes(S: int, k: int, E: int, H: int, F: int) -> int:
+    """Workspace bytes of moe_up_int4 and moe_down_int4 for up to S tokens."""
+    return int(_lib.lib().cia_moe_workspace_bytes(S, k, E, H, F))
+
+
+def moe_up_int4(x, ids, w1, w3, act, S: int, k: int, ws) -> None:
+    """engine.cu:896-899 for every token and chosen expert: act [S, k, F] fp16 =
+    silu(W1[e] x) * (W3[e] x), e = ids[s, j]; x fp16 [S, H], ids int32 [S, k]
+    (outside [0, E): the pair's act row is left as it was; None: one expert,
+    every row), w1 and w3 as q4_experts takes them, [E, F, H]."""
+    q1, E, F, H = q4_experts(w1, "w1")
+    q3, E3, F3, H3 = q4_experts(w3, "w3")
+    if (E3, F3, H3) != (E, F, H):
+        raise ValueError(f"w3: experts {(E3, F3, H3)}, but w1 has {(E, F, H)}")
+    call("cia_moe_up_int4", _dev(x, "x", _F16, S * H), _opt(ids, "ids", (torch.int32,), S * k),
+         ctypes.byref(q1), ctypes.byref(q3), _dev(act, "act", _F16, S * k * F), S, k, E, H, F,
+         _dev(ws, "ws", (torch.uint8,)), ws.numel(), stream_handle())
+
+
+def moe_down_int4(act, ids, weights, w2, res, out, S: int, k: int, ws) -> None:
+    """engine.cu:900-904 for every token and chosen expert: out [S, H] fp32 = res
+    + sum over j of weights[s, j] * (W2[e] act[s, j]); out may be res; weights
+    fp32 [S, k] or None (1); ids as moe_up_int4's; w2 [E, H, F]."""
+    q2, E, H, F = q4_experts(w2, "w2")
+    f32 = (torch.float32,)
+    call("cia_moe_down_int4", _dev(act, "act", _F16, S * k * F), _opt(ids, "ids", (torch.int32,), S * k),
+         _opt(weights, "weights", f32, S * k), ctypes.byref(q2), _dev(res, "res", f32, S * H),
+         _dev(out, "out", f32, S * H), S, k, E, H, F, _dev(ws, "ws", (torch.uint8,)), ws.numel(),
+         stream_handle())

@@ -14,8 +14,9 @@ import torch
 
 from . import _lib
 from ._lib import (D, KVGROUP, NH, NKV, NSPLIT_DEFAULT, call, cia_append_op, cia_attn_proj,
-                   cia_layer)
-from .kernels import decode_workspace_bytes, h2o_workspace_bytes, stream_handle
+                   cia_layer, cia_moe)
+from .kernels import (decode_workspace_bytes, h2o_workspace_bytes, moe_gating, q4_experts,
+                      stream_handle)
 
 HIDDEN = _lib.HIDDEN
 
@@ -213,3 +214,60 @@ def attn_block_loop(layers, x, h, past: int, steps: int, scale: float = 0.125, e
     finally:
         for L, s in zip(layers, arr):  # host counters advance in the copies
             L._s.committed, L._s.n_live = s.committed, s.n_live
+
+
+# ------------------------------------------------------------ the feed-forward branch
+class MoeBlock:
+    """The feed-forward branch of one layer (engine.cu:869-905): ffn_norm, the
+    router, and the chosen experts' INT4 products, into the residual.
+
+    ``norm_w``: fp16 [H].  ``w1``, ``w3`` ([E, F, H]) and ``w2`` ([E, H, F]):
+    INT4 group-128 experts as (packed u8 [E, rows, cols / 2], scales fp16
+    [E, rows, cols / 128]) pairs of device tensors.  ``gate`` (fp16 [E, H]) with
+    ``top_k`` and the other arguments of ``kernels.moe_gating`` routes; without
+    it the layer is dense (E = 1).  ``bias``: fp32 [E], for the choice alone.
+    ``max_batch``: tokens a call may bring.
+    """
+
+    def __init__(self, norm_w, w1, w3, w2, *, gate=None, bias=None, top_k: int = 1, eps: float = 1e-5,
+                 max_batch: int = 4096, device="cuda", **gating):
+        dev = torch.device(device)
+        M = cia_moe()
+        M.w1, E, F, H = q4_experts(w1, "w1")
+        M.w3, *s3 = q4_experts(w3, "w3")
+        M.w2, *s2 = q4_experts(w2, "w2")
+        if s3 != [E, F, H] or s2 != [E, H, F]:
+            raise ValueError(f"w3 {s3} and w2 {s2} do not go with w1 {[E, F, H]}")
+        if gate is None and (E != 1 or bias is not None or top_k != 1 or gating):
+            raise ValueError("experts need a gate (a dense layer has one expert and no router)")
+        for t, name, dtype, shape in ((norm_w, "norm_w", torch.float16, (H,)),
+                                      (gate, "gate", torch.float16, (E, H)),
+                                      (bias, "bias", torch.float32, (E,))):
+            if t is not None and (t.dtype != dtype or not t.is_cuda or not t.is_contiguous()
+                                  or tuple(t.shape) != shape):
+                raise ValueError(f"{name}: need a contiguous device {dtype} tensor {shape}")
+        for t in (norm_w, *w1, *w3, *w2, gate, bias):
+            if t is not None and dev.index is not None and t.device != dev:
+                raise ValueError(f"a weight is on {t.device}, the layer on {dev}")
+        self.H, self.max_batch = H, max_batch
+        self._keep = (norm_w, w1, w3, w2, gate, bias)
+        M.norm_w, M.norm_eps, M.H, M.F = norm_w.data_ptr(), float(eps), H, F
+        if gate is not None:
+            M.gate = gate.data_ptr()
+            M.bias = None if bias is None else bias.data_ptr()
+            M.gating = moe_gating(E, top_k, **gating)
+        M.cap = max_batch
+        M.ws_bytes = _lib.lib().cia_moe_block_workspace_bytes(ctypes.byref(M), max_batch)
+        self.ws = torch.empty(max(M.ws_bytes, 16), dtype=torch.uint8, device=dev)
+        M.ws = self.ws.data_ptr()
+        self._m = M
+
+    def forward(self, h) -> None:
+        """h fp32 [S, H], the residual, in place; S up to max_batch."""
+        S = h.numel() // self.H
+        if (h.dtype != torch.float32 or not h.is_cuda or not h.is_contiguous()
+                or h.numel() != S * self.H):
+            raise ValueError(f"h: need a contiguous device fp32 tensor [S, {self.H}]")
+        if S > self.max_batch:
+            raise ValueError(f"S={S} exceeds max_batch={self.max_batch}")
+        call("cia_moe_block_forward", ctypes.byref(self._m), h.data_ptr(), S, stream_handle())

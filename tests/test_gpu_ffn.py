@@ -1,0 +1,413 @@
+"""The feed-forward branch's operators on the GPU against 64-bit forms."""
+import numpy as np
+import pytest
+import torch
+
+import ffn_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def K(cia, dev):
+    from cuda_inf_amd import kernels
+    return kernels
+
+
+def t(a, dev):
+    return None if a is None else torch.from_numpy(np.ascontiguousarray(a)).to(dev)
+
+
+def within(got, want, bound, what):
+    err = np.abs(np.asarray(got, np.float64) - want)
+    bad = ~(err <= bound)
+    assert not bad.any(), f"{what}: {bad.sum()} of {bad.size} outside, worst {np.nanmax(err / bound)} of the bound"
+
+
+# ------------------------------------------------------------------ norm
+@pytest.mark.parametrize("S,H,add", [(1, 2048, False), (1, 8, True), (5, 64, True), (3, 1000, False),
+                                     (2, 2056, True), (7, 4096, False), (2, 8200, True), (4, 20000, False),
+                                     (513, 2048, True)])
+def test_norm(K, dev, S, H, add):
+    rng = np.random.default_rng(S * 7 + H)
+    h = (rng.standard_normal((S, H)) * (1 + 50 * (rng.random(H) < 0.02))).astype(np.float32)
+    b = rng.standard_normal((S, H)).astype(np.float32) if add else None
+    w = (1 + 0.3 * rng.standard_normal(H)).astype(np.float16)
+    hd, bd = t(h, dev), t(b, dev)
+    out = torch.full((S, H), 7.0, dtype=torch.float16, device=dev)
+    hs = torch.empty_like(hd)
+    K.add_rmsnorm(hd, t(w, dev), out, S, H, 1e-5, add=bd, hsum=hs)
+    _, y, bound = ref.norm(h, b, w, 1e-5)
+    within(out.cpu().numpy(), y, bound, "norm")
+    assert torch.equal(hs, hd if bd is None else hd + bd)
+    # in place, and without the sum
+    out2 = torch.empty_like(out)
+    K.add_rmsnorm(hd, t(w, dev), out2, S, H, 1e-5, add=bd)
+    assert torch.equal(out, out2)
+    K.add_rmsnorm(hd, t(w, dev), out2, S, H, 1e-5, add=bd, hsum=hd)
+    assert torch.equal(out, out2) and torch.equal(hd, hs)
+
+
+def test_norm_rows_of_zeros_and_beyond_numbers(K, dev):
+    h = torch.zeros((4, 256), device=dev)
+    h[1, 3], h[2, 5] = float("nan"), float("inf")
+    h[3] = 1e18  # (squares past fp32's range would need 2e19)
+    w = torch.ones(256, dtype=torch.float16, device=dev)
+    out = torch.empty((4, 256), dtype=torch.float16, device=dev)
+    K.add_rmsnorm(h, w, out, 4, 256)
+    o = out.float().cpu()
+    assert (o[0] == 0).all() and o[1].isnan().all()
+    assert o[2, 5].isnan() and (o[2, :5] == 0).all()
+    assert (o[3] == 1).all()
+
+
+# ------------------------------------------------------------------ router
+@pytest.mark.parametrize("S,H,E,kw", [
+    (1, 2048, 32, dict(k=4)),
+    (5, 256, 1, dict(k=1)),
+    (3, 8, 7, dict(k=7, renorm=False)),
+    (17, 1000, 33, dict(k=5, score="softmax")),
+    (65, 512, 64, dict(k=8, score="softmax", renorm=False, scale=2.5)),
+    (9, 1280, 128, dict(k=6, n_group=8, topk_group=3)),
+    (4, 384, 256, dict(k=16, n_group=16, topk_group=1, score="softmax")),
+    (6, 128, 24, dict(k=2, n_group=24, topk_group=2)),
+    (40, 640, 200, dict(k=3)),
+    (300, 2048, 32, dict(k=4, eps=0.0)),
+])
+@pytest.mark.parametrize("bias", [False, True])
+def test_route(K, dev, S, H, E, kw, bias):
+    kw = dict(kw)
+    k = kw.pop("k")
+    rng = np.random.default_rng(S + 3 * H + E)
+    x = rng.standard_normal((S, H)).astype(np.float16)
+    gate = (rng.standard_normal((E, H)) / np.sqrt(H)).astype(np.float16)
+    b = (0.1 * rng.standard_normal(E)).astype(np.float32) if bias else None
+    l = x.astype(np.float64) @ gate.astype(np.float64).T
+    ids, wt = ref.choose(l, b, k, **kw)
+    gi = torch.full((S, k), -7, dtype=torch.int32, device=dev)
+    gw, gl = torch.zeros((S, k), device=dev), torch.zeros((S, E), device=dev)
+    K.moe_route(t(x, dev), t(gate, dev), gi, gw, S, H, E, k, bias=t(b, dev), logits=gl, **kw)
+    assert np.array_equal(gi.cpu().numpy(), ids)
+    # one rounding of a value that 64 bits hold to 1e-12
+    within(gl.cpu().numpy(), l, ref.U24 * np.abs(l) + 1e-12, "logits")
+    within(gw.cpu().numpy(), wt, 1.001 * ref.U24 * np.abs(wt) + 1e-12, "weights")
+    # the logits are optional
+    g2, w2 = torch.empty_like(gi), torch.empty_like(gw)
+    K.moe_route(t(x, dev), t(gate, dev), g2, w2, S, H, E, k, bias=t(b, dev), **kw)
+    assert torch.equal(gi, g2) and torch.equal(gw, w2)
+    # a token's experts and weights do not depend on the tokens beside it
+    if S > 1:
+        i = S // 2
+        K.moe_route(t(x[i:i + 1], dev), t(gate, dev), g2, w2, 1, H, E, k, bias=t(b, dev), **kw)
+        assert torch.equal(gi[i], g2[0]) and torch.equal(gw[i], w2[0])
+
+
+@pytest.mark.parametrize("E,kw", [(32, dict(k=4)), (9, dict(k=3, score="softmax")),
+                                  (64, dict(k=5, n_group=8, topk_group=2, score="softmax", renorm=False)),
+                                  (256, dict(k=8, n_group=4, topk_group=2)), (100, dict(k=10))])
+@pytest.mark.parametrize("bias", [False, True])
+def test_select_of_logits(K, dev, E, kw, bias):
+    """Equal logits, infinities and what is not a number among them."""
+    kw = dict(kw)
+    k = kw.pop("k")
+    rng = np.random.default_rng(E)
+    l = rng.standard_normal((70, E)).astype(np.float32)
+    l[1] = 0.25                                  # all equal
+    l[2, ::2] = l[2, 1]                          # many equal
+    l[3, rng.random(E) < 0.9] = -np.inf
+    l[4] = -np.inf
+    l[5] *= 1e30
+    l[6, 0] = np.inf if kw.get("score") != "softmax" else 90.0
+    l[7] = np.round(l[7])
+    b = np.round(rng.standard_normal(E), 1).astype(np.float32) if bias else None
+    if bias:
+        b[E // 2:] = -np.inf                     # experts that are shut
+    ids, wt = ref.choose(l.astype(np.float64), b, k, **kw)
+    gi, gw = torch.empty((70, k), dtype=torch.int32, device=dev), torch.empty((70, k), device=dev)
+    K.moe_select(t(l, dev), gi, gw, 70, E, k, bias=t(b, dev), **kw)
+    assert np.array_equal(gi.cpu().numpy(), ids)
+    within(gw.cpu().numpy(), wt, 1.001 * ref.U24 * np.abs(wt) + 1e-12, "weights")
+
+
+def test_select_of_nan(K, dev):
+    """A row with a NaN: the experts stay distinct and in range, the weights of NaN
+    scores are NaN; other rows are not touched."""
+    l = torch.randn((3, 16), device=dev)
+    l[1, 5] = float("nan")
+    ids, w = torch.empty((3, 4), dtype=torch.int32, device=dev), torch.empty((3, 4), device=dev)
+    K.moe_select(l, ids, w, 3, 16, 4)
+    assert 5 not in ids[1].tolist() and not w.isnan().any()
+    K.moe_select(l, ids, w, 3, 16, 4, score="softmax")
+    assert ids[1].tolist() == [0, 1, 2, 3] and w[1].isnan().all()
+    assert not w[0].isnan().any() and not w[2].isnan().any()
+
+
+# ------------------------------------------------------------------ experts
+def make(rng, S, k, E, H, F, how="even"):
+    ids = None
+    if how != "dense":
+        ids = np.stack([rng.permutation(E)[:k] if k <= E else rng.integers(0, E, k) for _ in range(S)]).astype(np.int32)
+    if how == "one":      # every pair on one expert
+        ids[:] = E - 1
+    if how == "holes":
+        ids[rng.random((S, k)) < 0.3] = -1
+        ids[0] = [E, -5, 2 ** 31 - 1, -2 ** 31][:k] + [-1] * max(0, k - 4)
+    if how == "none":
+        ids[:] = -1
+    if how == "skew":
+        ids[:S * 3 // 4] = 0
+    return ids
+
+
+SIZES = [
+    # S, k, E, H, F, how
+    (1, 4, 32, 2048, 256, "even"),
+    (1, 1, 1, 128, 128, "dense"),
+    (1, 16, 16, 256, 128, "even"),
+    (2, 6, 3, 384, 256, "even"),        # ids repeat within a token
+    (7, 4, 8, 1792, 384, "holes"),
+    (16, 1, 1, 640, 256, "dense"),
+    (17, 1, 1, 256, 512, "dense"),
+    (33, 2, 4, 512, 1792, "holes"),
+    (45, 4, 32, 256, 384, "holes"),
+    (60, 4, 5, 896, 256, "skew"),
+    (64, 1, 1, 2048, 128, "dense"),
+    (129, 1, 1, 384, 384, "dense"),
+    (150, 2, 256, 128, 128, "even"),
+    (3, 2, 2, 128, 7168, "even"),
+    (5, 1, 1, 8320, 128, "dense"),
+    (90, 3, 7, 4096, 128, "skew"),
+    (9, 2, 4, 256, 256, "none"),
+    (257, 2, 3, 256, 640, "one"),
+    (300, 3, 6, 384, 256, "holes"),
+    (700, 4, 8, 256, 256, "skew"),
+    (1111, 1, 1, 256, 384, "dense"),
+    (1500, 2, 16, 2048, 128, "even"),
+    (1300, 2, 4, 128, 2304, "holes"),
+]
+
+
+@pytest.mark.parametrize("S,k,E,H,F,how", SIZES)
+def test_up(K, dev, S, k, E, H, F, how):
+    rng = np.random.default_rng(S + k + E + H + F)
+    x = rng.standard_normal((S, H)).astype(np.float16)
+    p1, s1, W1 = ref.quant(rng, E, F, H)
+    p3, s3, W3 = ref.quant(rng, E, F, H)
+    ids = make(rng, S, k, E, H, F, how)
+    want, bound = ref.up(x, ids, W1, W3, k)
+    act = torch.full((S, k, F), 3.0, dtype=torch.float16, device=dev)
+    ws = torch.full((K.moe_workspace_bytes(S, k, E, H, F),), 0xAB, dtype=torch.uint8, device=dev)
+    args = (t(x, dev), t(ids, dev), (t(p1, dev), t(s1, dev)), (t(p3, dev), t(s3, dev)))
+    K.moe_up_int4(*args, act, S, k, ws)
+    got = act.view(S * k, F).cpu().numpy()
+    out = np.isnan(want[:, 0])
+    assert (got[out] == 3.0).all(), "rows of pairs that take no part were written"
+    within(got[~out], want[~out], bound[~out], "act")
+    first = act.clone()
+    K.moe_up_int4(*args, act, S, k, ws)
+    assert torch.equal(first, act)
+
+
+@pytest.mark.parametrize("S,k,E,H,F,how", SIZES)
+@pytest.mark.parametrize("weighted", [True, False])
+def test_down(K, dev, S, k, E, H, F, how, weighted):
+    H, F = F, H  # the same contraction lengths as test_up
+    rng = np.random.default_rng(S + k + E + H + F + 1)
+    act = rng.standard_normal((S * k, F)).astype(np.float16)
+    p2, s2, W2 = ref.quant(rng, E, H, F)
+    ids = make(rng, S, k, E, F, H, how)
+    wt = rng.standard_normal((S, k)).astype(np.float32) if weighted else None
+    res = rng.standard_normal((S, H)).astype(np.float32)
+    want, bound = ref.down(act, ids, wt, W2, res, k)
+    if ids is not None:  # what the rows of pairs that take no part hold is not read
+        dead = (ids.reshape(-1) < 0) | (ids.reshape(-1) >= E)
+        act[dead] = np.nan
+        if weighted:
+            wt.reshape(-1)[dead] = np.nan
+    rd = t(res, dev)
+    out = torch.full((S, H), 5.0, device=dev)
+    ws = torch.full((K.moe_workspace_bytes(S, k, E, H, F),), 0xFF, dtype=torch.uint8, device=dev)
+    args = (t(act, dev), t(ids, dev), t(wt, dev), (t(p2, dev), t(s2, dev)))
+    K.moe_down_int4(*args, rd, out, S, k, ws)
+    within(out.cpu().numpy(), want, bound, "out")
+    K.moe_down_int4(*args, rd, rd, S, k, ws)  # in place
+    assert torch.equal(rd, out)
+
+
+def test_experts_apart(K, dev):
+    """Experts at a stride larger than an expert, as tensors of a weight blob lie."""
+    rng = np.random.default_rng(11)
+    S, k, E, H, F = 21, 2, 5, 256, 384
+    x = rng.standard_normal((S, H)).astype(np.float16)
+    p, s, W = ref.quant(rng, 2 * E, F, H)
+    ids = make(rng, S, k, E, H, F)
+    pd, sd = t(p, dev).view(E, 2, F, H // 2), t(s, dev).view(E, 2, F, H // 128)
+    act = torch.empty((S, k, F), dtype=torch.float16, device=dev)
+    ws = torch.empty(K.moe_workspace_bytes(S, k, E, H, F), dtype=torch.uint8, device=dev)
+    K.moe_up_int4(t(x, dev), t(ids, dev), (pd[:, 0], sd[:, 0]), (pd[:, 1], sd[:, 1]), act, S, k, ws)
+    want, bound = ref.up(x, ids, W[0::2], W[1::2], k)
+    within(act.view(S * k, F).cpu().numpy(), want, bound, "act")
+
+
+@pytest.mark.parametrize("S", [3, 40, 600])
+def test_a_bad_row_stays_alone(K, dev, S):
+    """NaN and infinities in one token's row reach no other token's outputs."""
+    rng = np.random.default_rng(S)
+    k, E, H, F = 2, 4, 256, 256
+    x = rng.standard_normal((S, H)).astype(np.float16)
+    p1, s1, W1 = ref.quant(rng, E, F, H)
+    p2, s2, W2 = ref.quant(rng, E, H, F)
+    ids = make(rng, S, k, E, H, F)
+    want, bound = ref.up(x, ids, W1, W1, k)
+    bad = S // 2
+    xb = x.copy()
+    xb[bad] = np.nan
+    w1 = (t(p1, dev), t(s1, dev))
+    act = torch.empty((S, k, F), dtype=torch.float16, device=dev)
+    ws = torch.empty(K.moe_workspace_bytes(S, k, E, H, F), dtype=torch.uint8, device=dev)
+    K.moe_up_int4(t(xb, dev), t(ids, dev), w1, w1, act, S, k, ws)
+    got = act.cpu().numpy()
+    assert np.isnan(got[bad]).all()
+    keep = np.arange(S) != bad
+    within(got[keep], want.reshape(S, k, F)[keep], bound.reshape(S, k, F)[keep], "act")
+    a = got.copy()
+    a[bad] = np.inf
+    res = np.zeros((S, H), np.float32)
+    out = torch.empty((S, H), device=dev)
+    K.moe_down_int4(t(a, dev), t(ids, dev), None, (t(p2, dev), t(s2, dev)), t(res, dev), out, S, k, ws)
+    o = out.cpu().numpy()
+    assert not np.isfinite(o[bad]).any() and np.isfinite(o[keep]).all()
+
+
+# ------------------------------------------------------------------ together
+def block(dev, rng, E, k, H, F, max_batch, **kw):
+    from cuda_inf_amd.layer import MoeBlock
+    (p1, s1, W1), (p3, s3, W3), (p2, s2, W2) = (ref.quant(rng, E, r, c) for r, c in ((F, H), (F, H), (H, F)))
+    nw = (1 + 0.2 * rng.standard_normal(H)).astype(np.float16)
+    gate = bias = None
+    if E > 1:
+        gate = (rng.standard_normal((E, H)) / np.sqrt(H)).astype(np.float16)
+        bias = (0.1 * rng.standard_normal(E)).astype(np.float32)
+        kw.update(gate=t(gate, dev), bias=t(bias, dev), top_k=k)
+    B = MoeBlock(t(nw, dev), *((t(p, dev), t(s, dev)) for p, s in ((p1, s1), (p3, s3), (p2, s2))),
+                 max_batch=max_batch, device=dev, **kw)
+    return B, (nw, gate, bias, W1, W3, W2)
+
+
+def plain_block(h, w, k, **kw):
+    """The branch in 64 bits; what lies between its operators is rounded as they hand it on."""
+    nw, gate, bias, W1, W3, W2 = w
+    x = ref.norm(h, None, nw, 1e-5)[1].astype(np.float16)
+    ids = wt = None
+    if gate is not None:
+        ids, wt = ref.choose(x.astype(np.float64) @ gate.astype(np.float64).T, bias, k, **kw)
+        wt = wt.astype(np.float32)
+    act = ref.up(x, ids, W1, W3, k)[0].astype(np.float16)
+    return ref.down(act, ids, wt, W2, h, k)[0]
+
+
+@pytest.mark.parametrize("S,E,k,H,F", [(1, 32, 4, 2048, 256), (6, 8, 3, 256, 384), (50, 1, 1, 256, 512),
+                                       (400, 8, 2, 256, 256)])
+def test_block(K, dev, S, E, k, H, F):
+    rng = np.random.default_rng(S + E)
+    B, w = block(dev, rng, E, k, H, F, max_batch=S + 3)
+    h = rng.standard_normal((S, H)).astype(np.float32)
+    hd = t(h, dev)
+    B.forward(hd)
+    want = plain_block(h, w, k)
+    # an fp16 step of x or act may fall the other way: 2^-10 of some terms of the sums
+    err = np.abs(hd.cpu().numpy() - want)
+    assert np.linalg.norm(err) <= 2.0 ** -10 * np.linalg.norm(want - h)
+    # operators one by one give the branch's bits
+    x = torch.empty((S, H), dtype=torch.float16, device=dev)
+    act = torch.empty((S, k, F), dtype=torch.float16, device=dev)
+    ws = torch.empty(K.moe_workspace_bytes(S, k, E, H, F), dtype=torch.uint8, device=dev)
+    h2 = t(h, dev)
+    norm_w, w1, w3, w2, gate, bias = B._keep
+    K.add_rmsnorm(h2, norm_w, x, S, H)
+    ids = wt = None
+    if E > 1:
+        ids, wt = torch.empty((S, k), dtype=torch.int32, device=dev), torch.empty((S, k), device=dev)
+        K.moe_route(x, gate, ids, wt, S, H, E, k, bias=bias)
+    K.moe_up_int4(x, ids, w1, w3, act, S, k, ws)
+    K.moe_down_int4(act, ids, wt, w2, h2, h2, S, k, ws)
+    assert torch.equal(hd, h2)
+
+
+def test_layer_of_attention_and_experts(K, dev):
+    """Two layers -- norm, attention branch, feed-forward branch -- over a prompt
+    and decode tokens, against the plain forms fed with the same attention."""
+    from cuda_inf_amd.layer import HIDDEN, AttnLayer
+    rng = np.random.default_rng(5)
+    E, k, F, prompt = 8, 2, 256, 70
+    layers = []
+    for _ in range(2):
+        L = AttnLayer(256, nsplit=0, max_batch=prompt, device=dev,
+                      qk_norm=(torch.ones(64, dtype=torch.float16), torch.ones(64, dtype=torch.float16)))
+        proj = []
+        for n in (2048, 512, 512, 2048):
+            p, s, _ = ref.quant(rng, 1, n, HIDDEN)
+            proj.append((t(p[0], dev), t(s[0], dev)))
+        L.set_projections(*proj)
+        nw = t((1 + 0.2 * rng.standard_normal(HIDDEN)).astype(np.float16), dev)
+        B, w = block(dev, rng, E, k, HIDDEN, F, max_batch=prompt)
+        layers.append((L, nw, B, w))
+    past = 0
+    for S in (prompt, 1, 1, 3):
+        h = t(rng.standard_normal((S, HIDDEN)).astype(np.float32), dev)
+        x = torch.empty((S, HIDDEN), dtype=torch.float16, device=dev)
+        for L, nw, B, w in layers:
+            K.add_rmsnorm(h, nw, x, S, HIDDEN)
+            L.block_forward(x, h, past)
+            before = h.cpu().numpy()
+            B.forward(h)
+            want = plain_block(before, w, k)
+            err = np.abs(h.cpu().numpy() - want)
+            assert np.linalg.norm(err) <= 2.0 ** -10 * np.linalg.norm(want - before)
+        past += S
+
+
+def test_block_captured(K, dev):
+    """A branch in a graph: every replay gives the eager result, with eager calls of
+    the same branch between the replays."""
+    rng = np.random.default_rng(9)
+    for S, E in ((1, 8), (5, 8), (300, 8), (40, 1)):
+        k = 2 if E > 1 else 1
+        B, _ = block(dev, rng, E, k, 256, 384, max_batch=S)
+        hs = [torch.from_numpy(rng.standard_normal((S, 256)).astype(np.float32)).to(dev) for _ in range(3)]
+        want = []
+        for h in hs:
+            o = h.clone()
+            B.forward(o)
+            want.append(o)
+        buf = hs[0].clone()
+        g = torch.cuda.CUDAGraph()
+        side = torch.cuda.Stream(dev)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            with torch.cuda.graph(g, stream=side):
+                B.forward(buf)
+        torch.cuda.synchronize()
+        for h, o in zip(hs * 2, want * 2):
+            buf.copy_(h)
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(buf, o)
+            e = h.clone()
+            B.forward(e)
+            torch.cuda.synchronize()
+            assert torch.equal(e, o)
+
+
+def test_another_stream(K, dev):
+    rng = np.random.default_rng(10)
+    B, _ = block(dev, rng, 8, 2, 256, 384, max_batch=64)
+    h = torch.from_numpy(rng.standard_normal((64, 256)).astype(np.float32)).to(dev)
+    want = h.clone()
+    B.forward(want)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream(dev)
+    with torch.cuda.stream(s):
+        B.forward(h)
+    s.synchronize()
+    assert torch.equal(h, want)
