@@ -31,8 +31,16 @@ struct MoeArgs {
   int S, k, E;
   uint16_t* act;          // up: [S k][N]
   float* y;               // down: [S k][N]
-  const int* plan;        // offs[E + 1], rows[S k]
+  const int* plan;        // offs[E + 1], tiles, (expert, first) of each, rows[S k]
+  int splits;             // down: parts of K, each into its own y
 };
+
+// Rows of a row tile.  The plan lists the tiles: expert e's are its rows 128 at a time.
+constexpr int kTileRows = 128;
+
+// The most row tiles P pairs of E experts can make
+__host__ __device__ constexpr int64_t max_tiles(int64_t P, int E) { return P / kTileRows + (P < E ? P : E); }
+__host__ __device__ constexpr int64_t plan_rows_at(int64_t P, int E) { return E + 2 + 2 * max_tiles(P, E); }
 
 // ---------------------------------------------------------------- plan
 // Rows by expert: offs[e] .. offs[e + 1] - 1 of rows are expert e's.  Their order
@@ -49,14 +57,24 @@ __global__ __launch_bounds__(1024) void k_moe_plan(const int32_t* ids, int P, in
   }
   __syncthreads();
   if (tid < E) {
-    int o = 0;
-    for (int j = 0; j < tid; j++) o += cnt[j];
+    int o = 0, t = 0;
+    for (int j = 0; j < tid; j++) {
+      o += cnt[j];
+      t += (cnt[j] + kTileRows - 1) / kTileRows;
+    }
     at[tid] = o;
     plan[tid] = o;
-    if (tid == E - 1) plan[E] = o + cnt[tid];
+    for (int i = 0; i < cnt[tid]; i += kTileRows, t++) {
+      plan[E + 2 + 2 * t] = tid;
+      plan[E + 3 + 2 * t] = o + i;
+    }
+    if (tid == E - 1) {
+      plan[E] = o + cnt[tid];
+      plan[E + 1] = t;
+    }
   }
   __syncthreads();
-  int* rows = plan + E + 1;
+  int* rows = plan + plan_rows_at(P, E);
   for (int i = tid; i < P; i += 1024) {
     const int e = ids ? ids[i] : 0;
     if ((unsigned)e < (unsigned)E) rows[atomicAdd(&at[e], 1)] = i;
@@ -81,12 +99,29 @@ __device__ __forceinline__ f16x8 nib8(uint32_t u) {
   return r;
 }
 
-__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + fast_exp(-g)) * u; }
+// The product is rounded to fp32 before its caller rounds it to fp16.  (Left to
+// itself the compiler multiplies and converts in one instruction at some places
+// and in two at others, and a row's bits would depend on its place in a tile.)
+__device__ __forceinline__ float silu_mul(float g, float u) {
+  float v = g / (1.0f + fast_exp(-g)) * u;
+  asm("" : "+v"(v));
+  return v;
+}
 
 // the value of the neighbouring lane (l ^ 1)
 __device__ __forceinline__ float lane_pair(float v) {
   return __builtin_bit_cast(
       float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, false));
+}
+
+// A kernel argument as a scalar value.  (Left visible, the choice below between
+// the two matrices' arguments becomes a choice of address in the argument
+// segment, and a vector load from it.)
+template <class T>
+__device__ __forceinline__ T arg(T v) {
+  uint64_t u = (uint64_t)v;
+  asm("" : "+s"(u));
+  return (T)u;
 }
 
 // Column c of a tile: up interleaves the two matrices (even W1, odd W3), so
@@ -96,57 +131,257 @@ struct Col {
   const uint8_t* w;
   const uint16_t* s;
   __device__ __forceinline__ Col(const MoeArgs& a, int e, int c) {
-    const int m = kUp ? c & 1 : 0, n0 = kUp ? c >> 1 : c, n = n0 < a.N ? n0 : a.N - 1;
-    w = (m ? a.packed[1] : a.packed[0]) + (size_t)e * (m ? a.pstride[1] : a.pstride[0]) + (size_t)n * (a.K >> 1);
-    s = (m ? a.scales[1] : a.scales[0]) + (size_t)e * (m ? a.sstride[1] : a.sstride[0]) + (size_t)n * (a.K >> 7);
+    const int n0 = kUp ? c >> 1 : c, n = n0 < a.N ? n0 : a.N - 1;
+    const uint8_t* w0 = arg(a.packed[0]) + (size_t)e * a.pstride[0];
+    const uint16_t* s0 = arg(a.scales[0]) + (size_t)e * a.sstride[0];
+    if constexpr (kUp) {
+      const uint8_t* w1 = arg(a.packed[1]) + (size_t)e * arg(a.pstride[1]);
+      const uint16_t* s1 = arg(a.scales[1]) + (size_t)e * arg(a.sstride[1]);
+      w0 = c & 1 ? w1 : w0;
+      s0 = c & 1 ? s1 : s0;
+    }
+    w = w0 + (size_t)n * (a.K >> 1);
+    s = s0 + (size_t)n * (a.K >> 7);
   }
 };
 
-// One wave: 16 rows x 32 columns, operands straight from memory.
-template <bool kUp>
-__global__ __launch_bounds__(64) void k_moe_simple(MoeArgs a) {
-  const int l = threadIdx.x, n16 = l & 15, q = l >> 4, ng = a.K >> 7;
-  const int nct = (kUp ? 2 * a.N : a.N) / 32;
-  int e = 0, t = blockIdx.x / nct;
-  for (; e < a.E; e++) {
-    const int nt = (a.plan[e + 1] - a.plan[e] + 15) >> 4;
-    if (t < nt) break;
-    t -= nt;
+// ---------------------------------------------------------------- tiles
+// Many rows an expert: a workgroup of 8 waves computes 128 rows x (128 kNT)
+// columns, a wave all the rows of its own 16 kNT columns, so that a dequantised
+// operand serves 128 rows and no column is dequantised twice.  The K loop runs
+// over the scale groups in two LDS slots, filled by DMA one group ahead:
+//   X  128 rows x 16 chunks of 16 bytes, fetched from the rows of the tile
+//      wherever they are (a row's address is the lane's own).  Row r's chunk c at
+//      c ^ xsw(r): a 16-byte read is served 32 lanes, 512 bytes of banks, at a
+//      time, and so reaches 32 different places.
+//   W  each wave's own columns, 4 chunks of nibbles; column c's chunk q at
+//      q ^ ((c >> 2) & 3).
+// Inside a group lane q = l >> 4 of an operand holds k = 32q + 8s .. + 7 at step
+// s, so one 16-byte read brings a column's nibbles for all four steps.
+// Scales lie in an LDS table, filled once for up to kTabGroups groups.
+typedef __attribute__((address_space(3))) void lds_void_t;
+typedef __attribute__((address_space(1))) void gbl_void_t;
+
+constexpr int kTileWaves = 8;
+constexpr int kTabGroups = 32;
+
+__device__ __forceinline__ int xsw(int r) { return ((r >> 1) & 3) | ((r & 1) << 2) | (r & 8); }
+
+__device__ __forceinline__ void dma16(const void* src, void* dst) {
+  __builtin_amdgcn_global_load_lds((gbl_void_t*)src, (lds_void_t*)dst, 16, 0, 0);
+}
+
+template <bool kUp, int kNT>
+struct Tile {
+  static constexpr int kCols = 16 * kNT;  // of a wave
+  static constexpr int kX = kTileRows * 256, kW = kTileWaves * kCols * 64, kSlot = kX + kW;
+  static constexpr int kTab = kTileWaves * kTabGroups * kCols * 2;
+  static constexpr int kLds = 2 * kSlot + kTab + kTileRows * 4;
+};
+
+// A lane's DMA sources in group 0
+template <int kNT>
+struct TileSrc {
+  const uint8_t *x0, *x1, *x2, *x3, *w0, *w1, *w2;
+  __device__ __forceinline__ const uint8_t* x(int t) const { return t == 0 ? x0 : t == 1 ? x1 : t == 2 ? x2 : x3; }
+  __device__ __forceinline__ const uint8_t* w(int t) const { return t == 0 ? w0 : t == 1 ? w1 : w2; }
+};
+
+template <bool kUp, int kNT, int kPR>
+__device__ __forceinline__ void tile_fetch(uint8_t* slot, const TileSrc<kNT>& src, int w, int g) {
+  using T = Tile<kUp, kNT>;
+#pragma unroll
+  for (int t = 0; t < 4; t++)
+    if (kPR == 4 || 16 * w + 4 * t < 32 * kPR) dma16(src.x(t) + 256 * (size_t)g, slot + (4 * w + t) * 1024);
+#pragma unroll
+  for (int t = 0; t < kNT; t++)
+    dma16(src.w(t) + 64 * (size_t)g, slot + T::kX + w * T::kCols * 64 + t * 1024);
+}
+
+// One scale group: group g + 1 (if more) is fetched into next while cur is
+// multiplied.
+template <bool kUp, int kNT, int kPR>
+__device__ __forceinline__ void tile_group(const uint8_t* cur, uint8_t* next, const uint16_t* scales, const TileSrc<kNT>& src, int w, int g,
+                                           bool more, f32x4 (&C)[2 * kPR][kNT]) {
+  using T = Tile<kUp, kNT>;
+  const int l = threadIdx.x & 63, n16 = l & 15, q = l >> 4;
+  if (more) tile_fetch<kUp, kNT, kPR>(next, src, w, g + 1);
+  const uint16_t* xs = (const uint16_t*)cur + n16 * 128;
+  const uint8_t* ws = cur + T::kX + w * T::kCols * 64;
+  // Units of two row tiles x two k steps: a unit's x operands are requested
+  // before the products of the unit before it.
+  f16x8 A[2][4];
+  auto load_a = [&](int u, f16x8 (&o)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int s = 0; s < 2; s++)
+        o[2 * i + s] = *(const f16x8*)(xs + 16 * (2 * (u >> 1) + i) * 128 + 8 * ((4 * q + 2 * (u & 1) + s) ^ xsw(n16)));
+  };
+  u32x4 wq[kNT];
+  float scl[kNT];
+#pragma unroll
+  for (int j = 0; j < kNT; j++) {
+    const int c = 16 * j + n16;
+    wq[j] = *(const u32x4*)(ws + c * 64 + 16 * (q ^ ((c >> 2) & 3)));
+    scl[j] = h2f(scales[c]);
   }
-  if (e == a.E) return;
-  const int r0 = a.plan[e] + 16 * t, r1 = a.plan[e + 1];
-  const int* rows = a.plan + a.E + 1;
-  const int ra = rows[r0 + n16 < r1 ? r0 + n16 : r1 - 1];
-  const uint16_t* xr = a.x + (size_t)(kUp ? ra / a.k : ra) * a.K;
-  const int c0 = blockIdx.x % nct * 32;
-  f32x4 acc[2] = {};
-  const Col<kUp> col[2] = {Col<kUp>(a, e, c0 + n16), Col<kUp>(a, e, c0 + 16 + n16)};
-  for (int g = 0; g < ng; g++)
+  load_a(0, A[0]);
+  f16x8 B[kNT][4];
+  f32x4 P[2][2][kNT];  // of a pair of row tiles, and of the pair before
+  auto scale_add = [&](int pr) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-      const u32x4 wq = *(const u32x4*)(col[j].w + 64 * g + 16 * q);
-      f32x4 p = {};
+    for (int i = 0; i < 2; i++)
 #pragma unroll
-      for (int s = 0; s < 4; s++)
-        p = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const f16x8*)(xr + 128 * g + 32 * q + 8 * s), nib8(wq[s]), p, 0, 0, 0);
-      const float sc = h2f(col[j].s[g]);
+      for (int j = 0; j < kNT; j++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) acc[j][i] = __builtin_fmaf(p[i], sc, acc[j][i]);
-    }
+        for (int r = 0; r < 4; r++)
+          C[2 * pr + i][j][r] = __builtin_fmaf(P[pr & 1][i][j][r], scl[j], C[2 * pr + i][j][r]);
+  };
 #pragma unroll
-  for (int j = 0; j < 2; j++) {
-    const int c = c0 + 16 * j + n16;
+  for (int u = 0; u < 2 * kPR; u++) {
+    if (u + 1 < 2 * kPR) load_a(u + 1, A[(u + 1) & 1]);
+    __builtin_amdgcn_sched_barrier(0);
+    const int s0 = 2 * (u & 1), pr = u >> 1;
+    if (u < 2)
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int r = r0 + 4 * q + i;
-      const float v = acc[j][i], o = lane_pair(v);
-      if constexpr (kUp) {
-        if (!(c & 1) && r < r1 && (c >> 1) < a.N)
-          a.act[(size_t)rows[r] * a.N + (c >> 1)] = f2h(silu_mul(v, o));
-      } else if (r < r1 && c < a.N) {
-        a.y[(size_t)rows[r] * a.N + c] = v;
+      for (int j = 0; j < kNT; j++) {
+        B[j][s0] = nib8(wq[j][s0]);
+        B[j][s0 + 1] = nib8(wq[j][s0 + 1]);
+      }
+#pragma unroll
+    for (int s = 0; s < 2; s++)
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < kNT; j++)
+          P[pr & 1][i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              A[u & 1][2 * i + s], B[j][s0 + s], s0 + s == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : P[pr & 1][i][j], 0, 0, 0);
+    // the pair before is scaled between this pair's first products
+    if (pr > 0 && (u & 1) == 0) {
+      scale_add(pr - 1);
+#pragma unroll
+      for (int k = 0; k < 4 * kNT; k++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // one MFMA
+        __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);  // two vector instructions
       }
     }
+  }
+  scale_add(kPR - 1);
+}
+
+// The K loop of a tile of up to 32 kPR rows
+template <bool kUp, int kNT, int kPR>
+__device__ __forceinline__ void tile_loop(const MoeArgs& a, uint8_t* lds, uint16_t* tab, TileSrc<kNT> src, int e, int c0,
+                                          int g0, int g1, f32x4 (&C)[2 * kPR][kNT]) {
+  using T = Tile<kUp, kNT>;
+  const int l = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  tile_fetch<kUp, kNT, kPR>(lds, src, w, g0);
+#pragma unroll
+  for (int i = 0; i < 2 * kPR; i++)
+#pragma unroll
+    for (int j = 0; j < kNT; j++) C[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int g = g0; g < g1; g++) {
+    const int i = g - g0, slot = (i & 1) * T::kSlot;
+    if (i % kTabGroups == 0)  // this wave's scales of the next groups
+      for (int k = l; k < T::kCols * kTabGroups; k += 64) {
+        const int c = k / kTabGroups, gg = g + k % kTabGroups;
+        if (gg < g1) tab[(k % kTabGroups) * T::kCols + c] = Col<kUp>(a, e, c0 + c).s[gg];
+      }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): this wave's DMA and scales landed
+    __builtin_amdgcn_s_barrier();        // every wave's did; the other slot is read
+    asm volatile("" ::: "memory");
+    tile_group<kUp, kNT, kPR>(lds + slot, lds + (T::kSlot - slot), tab + i % kTabGroups * T::kCols, src, w, g,
+                              g + 1 < g1, C);
+  }
+}
+
+template <bool kUp, int kNT, int kPR>
+__device__ __forceinline__ void tile_run(const MoeArgs& a, uint8_t* lds, uint16_t* tab, TileSrc<kNT> src,
+                                         const int* rows, int nrows, int e, int c0,
+                                         int g0, int g1, float* y) {
+  const int l = threadIdx.x & 63, n16 = l & 15, q = l >> 4;
+  f32x4 C[2 * kPR][kNT];
+  tile_loop<kUp, kNT, kPR>(a, lds, tab, src, e, c0, g0, g1, C);
+  // lane holds rows 4q .. 4q + 3 of row tile i, column n16 of column tile j
+#pragma unroll
+  for (int i = 0; i < 2 * kPR; i++) {
+    auto row = [&](int r) __attribute__((always_inline)) {
+      const int t = 16 * i + 4 * q + r;
+      return t < nrows ? rows[t] : -1;
+    };
+    const int p0 = row(0), p1 = row(1), p2 = row(2), p3 = row(3);
+#pragma unroll
+    for (int j = 0; j < kNT; j++) {
+      const int c = c0 + 16 * j + n16;
+      const f32x4 v = C[i][j];
+      if constexpr (kUp) {
+        // the even lane takes rows 0 and 1 of the pair's column, the odd one 2, 3
+        const bool odd = c & 1;
+        const int n = c >> 1, pa = odd ? p2 : p0, pb = odd ? p3 : p1;
+        const float o0 = lane_pair(v[0]), o1 = lane_pair(v[1]), o2 = lane_pair(v[2]), o3 = lane_pair(v[3]);
+        const float va = silu_mul(odd ? o2 : v[0], odd ? v[2] : o0), vb = silu_mul(odd ? o3 : v[1], odd ? v[3] : o1);
+        if (n < a.N) {
+          if (pa >= 0) a.act[(size_t)pa * a.N + n] = f2h(va);
+          if (pb >= 0) a.act[(size_t)pb * a.N + n] = f2h(vb);
+        }
+      } else if (c < a.N) {
+        if (p0 >= 0) y[(size_t)p0 * a.N + c] = v[0];
+        if (p1 >= 0) y[(size_t)p1 * a.N + c] = v[1];
+        if (p2 >= 0) y[(size_t)p2 * a.N + c] = v[2];
+        if (p3 >= 0) y[(size_t)p3 * a.N + c] = v[3];
+      }
+    }
+  }
+}
+
+// grid = max_tiles x column tiles x splits, up to a multiple of 8; block = 512
+template <bool kUp, int kNT>
+__global__ __launch_bounds__(64 * kTileWaves) void k_moe_tile(MoeArgs a) {
+  using T = Tile<kUp, kNT>;
+  // (one LDS variable: with two the compiler tells their accesses apart, takes the
+  // DMA's target for known, and waits for it before any read of that variable)
+  __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
+  int* const srows = (int*)(lds + T::kLds) - kTileRows;
+  const int tid = threadIdx.x, l = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int nv = kUp ? 2 * a.N : a.N, nct = (nv + T::kCols * kTileWaves - 1) / (T::kCols * kTileWaves);
+  // Workgroups go to the 8 XCDs in turn: each takes a run of tiles, row tiles
+  // slowest, so that its L2 holds what neighbours share.
+  const int ntiles = a.plan[a.E + 1] * nct * a.splits, per = (ntiles + 7) >> 3;
+  int tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || tile >= ntiles) return;
+  const int ct = tile % nct;
+  tile /= nct;
+  const int sp = tile % a.splits;
+  tile /= a.splits;
+  const int e = a.plan[a.E + 2 + 2 * tile], r0 = a.plan[a.E + 3 + 2 * tile];
+  const int left = a.plan[e + 1] - r0, nrows = left < kTileRows ? left : kTileRows;
+  if (tid < kTileRows) {
+    const int* rows = a.plan + plan_rows_at((int64_t)a.S * a.k, a.E);
+    srows[tid] = rows[r0 + (tid < nrows ? tid : nrows - 1)];
+  }
+  __syncthreads();
+  const int c0 = ct * T::kCols * kTileWaves + w * T::kCols;
+  const int ng = a.K >> 7, g0 = ng * sp / a.splits, g1 = ng * (sp + 1) / a.splits;
+  auto xsrc = [&](int t) {
+    const int r = 16 * w + 4 * t + (l >> 4), p = srows[r];
+    return (const uint8_t*)(a.x + (size_t)(kUp ? p / a.k : p) * a.K) + 16 * ((l & 15) ^ xsw(r));
+  };
+  auto wsrc = [&](int t) {
+    const int c = 16 * t + (l >> 2);
+    return Col<kUp>(a, e, c0 + c).w + 16 * ((l & 3) ^ ((c >> 2) & 3));
+  };
+  const TileSrc<kNT> src = {xsrc(0), xsrc(1), xsrc(2), xsrc(3), wsrc(0), wsrc(1), kNT > 2 ? wsrc(2) : nullptr};
+  uint16_t* tab = (uint16_t*)(lds + 2 * T::kSlot) + w * kTabGroups * T::kCols;
+  float* y = kUp ? nullptr : a.y + (size_t)sp * a.S * a.k * a.N;
+  switch ((nrows + 31) >> 5) {
+    case 1: return tile_run<kUp, kNT, 1>(a, lds, tab, src, srows, nrows, e, c0, g0, g1, y);
+    case 2: return tile_run<kUp, kNT, 2>(a, lds, tab, src, srows, nrows, e, c0, g0, g1, y);
+    case 3: return tile_run<kUp, kNT, 3>(a, lds, tab, src, srows, nrows, e, c0, g0, g1, y);
+    default: return tile_run<kUp, kNT, 4>(a, lds, tab, src, srows, nrows, e, c0, g0, g1, y);
   }
 }
 
@@ -157,7 +392,7 @@ struct CombineArgs {
   const float* weights;  // or null: 1
   const float* res;
   float* out;
-  int S, k, E, H;
+  int S, k, E, H, splits;
 };
 
 // out = res + the k weighted rows of each token, in the order of j
@@ -170,7 +405,8 @@ __global__ __launch_bounds__(256) void k_moe_combine(CombineArgs a) {
     const int p = s * a.k + j, e = a.ids ? a.ids[p] : 0;
     if ((unsigned)e >= (unsigned)a.E) continue;
     const float w = a.weights ? a.weights[p] : 1.0f;
-    const f32x4 y = *(const f32x4*)(a.y + (size_t)p * a.H + c);
+    f32x4 y = *(const f32x4*)(a.y + (size_t)p * a.H + c);
+    for (int i = 1; i < a.splits; i++) y += *(const f32x4*)(a.y + ((size_t)i * a.S * a.k + p) * a.H + c);
 #pragma unroll
     for (int i = 0; i < 4; i++) v[i] = __builtin_fmaf(w, y[i], v[i]);
   }
@@ -178,7 +414,10 @@ __global__ __launch_bounds__(256) void k_moe_combine(CombineArgs a) {
 }
 
 // ---------------------------------------------------------------- host
-static int64_t plan_bytes(int64_t P, int E) { return ((E + 1 + P) * 4 + 255) / 256 * 256; }
+static int64_t plan_bytes(int64_t P, int E) { return ((plan_rows_at(P, E) + P) * 4 + 255) / 256 * 256; }
+
+// Rows of y: P, and room for parts of K where few pairs leave the chip empty
+static int64_t y_rows(int64_t P) { return P >= 4096 ? P : (8 * P < 4096 ? 8 * P : 4096); }
 
 static int moe_check(int S, int k, int E, int H, int F, const int32_t* ids) {
   CIA_REQUIRE(S >= 0 && k >= 1 && k <= kMoeMaxK && E >= 1 && E <= kMoeMaxE && H > 0 && F > 0 &&
@@ -207,11 +446,13 @@ static void set_w(MoeArgs& a, int i, const cia_q4_experts* w) {
 
 template <bool kUp>
 static int products(MoeArgs& a, void* ws, hipStream_t s) {
+  constexpr int kNT = 2;
   const int P = a.S * a.k;
   a.plan = (const int*)ws;
   hipLaunchKernelGGL(k_moe_plan, dim3(1), dim3(1024), 0, s, a.ids, P, a.E, (int*)ws);
-  const int nv = kUp ? 2 * a.N : a.N;
-  hipLaunchKernelGGL((k_moe_simple<kUp>), dim3((unsigned)(nv / 32) * (unsigned)(P / 16 + a.E)), dim3(64), 0, s, a);
+  const int nv = kUp ? 2 * a.N : a.N, cols = 128 * kNT;
+  const int64_t tiles = max_tiles(P, a.E) * ((nv + cols - 1) / cols) * a.splits;
+  hipLaunchKernelGGL((k_moe_tile<kUp, kNT>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * kTileWaves), 0, s, a);
   return launch_status();
 }
 
@@ -222,7 +463,7 @@ using namespace cia;
 extern "C" int64_t cia_moe_workspace_bytes(int S, int k, int E, int H, int F) {
   if (S < 0 || k < 1 || E < 1 || H < 1 || F < 1) return 0;
   const int64_t P = (int64_t)S * k;
-  return plan_bytes(P, E) + P * H * 4;
+  return plan_bytes(P, E) + y_rows(P) * H * 4;
 }
 
 extern "C" int cia_moe_up_int4(const uint16_t* x, const int32_t* ids, const cia_q4_experts* w1,
@@ -246,6 +487,7 @@ extern "C" int cia_moe_up_int4(const uint16_t* x, const int32_t* ids, const cia_
   a.k = k;
   a.E = E;
   a.act = act;
+  a.splits = 1;
   return products<true>(a, ws, (hipStream_t)stream);
 }
 
@@ -272,9 +514,10 @@ extern "C" int cia_moe_down_int4(const uint16_t* act, const int32_t* ids, const 
   a.k = k;
   a.E = E;
   a.y = (float*)((char*)ws + plan_bytes((int64_t)S * k, E));
+  a.splits = 1;
   hipStream_t s = (hipStream_t)stream;
   if ((st = products<false>(a, ws, s))) return st;
-  const CombineArgs c{a.y, ids, weights, res, out, S, k, E, H};
+  const CombineArgs c{a.y, ids, weights, res, out, S, k, E, H, a.splits};
   hipLaunchKernelGGL(k_moe_combine, dim3((unsigned)((H + 1023) / 1024) * (unsigned)S), dim3(256), 0, s, c);
   return launch_status();
 }
