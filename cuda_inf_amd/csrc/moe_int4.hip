@@ -31,68 +31,134 @@ struct MoeArgs {
   int S, k, E;
   uint16_t* act;          // up: [S k][N]
   float* y;               // down: [S k][N]
-  const int* plan;        // offs[E + 1], tiles, (expert, first) of each, rows[S k]
+  const int* plan;        // k_moe_plan's
   int splits;             // down: parts of K, each into its own y
 };
 
-// Rows of a row tile.  The plan lists the tiles: expert e's are its rows 128 at a time.
+// Rows of a row tile.  The plan lists the tiles: the whole ones of all experts,
+// then the experts' last, partly filled ones.
 constexpr int kTileRows = 128;
 
 // The most row tiles P pairs of E experts can make
 __host__ __device__ constexpr int64_t max_tiles(int64_t P, int E) { return P / kTileRows + (P < E ? P : E); }
-__host__ __device__ constexpr int64_t plan_rows_at(int64_t P, int E) { return E + 2 + 2 * max_tiles(P, E); }
+// plan: offs[E + 1], whole tiles, tiles, (expert, first) of each, rows[P]
+__host__ __device__ constexpr int64_t plan_rows_at(int64_t P, int E) { return E + 3 + 2 * max_tiles(P, E); }
 
 // ---------------------------------------------------------------- plan
 // Rows by expert: offs[e] .. offs[e + 1] - 1 of rows are expert e's.  Their order
 // within an expert does not matter: a row's results do not depend on its
 // neighbours.
-__global__ __launch_bounds__(1024) void k_moe_plan(const int32_t* ids, int P, int E, int* plan) {
-  __shared__ int cnt[kMoeMaxE], at[kMoeMaxE];
-  const int tid = threadIdx.x;
-  if (tid < kMoeMaxE) cnt[tid] = 0;
-  __syncthreads();
-  for (int i = tid; i < P; i += 1024) {
-    const int e = ids ? ids[i] : 0;
-    if ((unsigned)e < (unsigned)E) atomicAdd(&cnt[e], 1);
-  }
-  __syncthreads();
-  if (tid < E) {
-    int o = 0, t = 0;
-    for (int j = 0; j < tid; j++) {
-      o += cnt[j];
-      t += (cnt[j] + kTileRows - 1) / kTileRows;
-    }
-    at[tid] = o;
-    plan[tid] = o;
-    for (int i = 0; i < cnt[tid]; i += kTileRows, t++) {
-      plan[E + 2 + 2 * t] = tid;
-      plan[E + 3 + 2 * t] = o + i;
-    }
-    if (tid == E - 1) {
-      plan[E] = o + cnt[tid];
-      plan[E + 1] = t;
-    }
-  }
-  __syncthreads();
+//   Bound by latency.  One workgroup; up to 16384 pairs are read once, 16 to a
+// thread, and counted by wave: the count before is a pair's rank.  (16384 pairs:
+// 16.3 us with two reads and shared counts.)
+constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+
+__global__ __launch_bounds__(kPlanThreads) void k_moe_plan(const int32_t* ids, int P, int E, int* plan) {
+  __shared__ int cnt[kPlanWaves][kMoeMaxE];  // of a wave, then the first place of its pairs
+  __shared__ int part[3][4];  // of 64 experts
+  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63;
   int* rows = plan + plan_rows_at(P, E);
-  for (int i = tid; i < P; i += 1024) {
-    const int e = ids ? ids[i] : 0;
-    if ((unsigned)e < (unsigned)E) rows[atomicAdd(&at[e], 1)] = i;
+  constexpr int kPer = 16;
+  const bool once = P <= kPer * kPlanThreads;
+  for (int i = tid; i < kPlanWaves * kMoeMaxE; i += kPlanThreads) (&cnt[0][0])[i] = 0;
+  __syncthreads();
+  // pair i = 1024 j + tid
+  int id[kPer], rank[kPer];
+  if (!ids) {
+    if (tid == 0) cnt[0][0] = P;
+  } else if (once) {
+#pragma unroll
+    for (int j = 0; j < kPer; j++) {
+      const int i = kPlanThreads * j + tid;
+      id[j] = i < P ? ids[i] : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; j++)
+      if ((unsigned)id[j] < (unsigned)E) rank[j] = atomicAdd(&cnt[w][id[j]], 1);
+  } else {
+    for (int i = tid; i < P; i += kPlanThreads) {
+      const int e = ids[i];
+      if ((unsigned)e < (unsigned)E) atomicAdd(&cnt[w][e], 1);
+    }
+  }
+  __syncthreads();
+  // thread e: its pairs, whole tiles and partly filled tile, and how many of each
+  // the experts before it have
+  int n = 0, before[3] = {};
+  if (tid < kMoeMaxE) {
+    for (int i = 0; i < kPlanWaves; i++) n += cnt[i][tid];
+    const int own[3] = {n, n / kTileRows, n % kTileRows != 0};
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+      int v = own[k];
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int u = __shfl_up(v, d);
+        if (l >= d) v += u;
+      }
+      before[k] = v - own[k];
+      if (l == 63) part[k][w] = v;
+    }
+  }
+  __syncthreads();
+  if (tid < kMoeMaxE) {
+    const int whole = part[1][0] + part[1][1] + part[1][2] + part[1][3];
+#pragma unroll
+    for (int k = 0; k < 3; k++)
+      for (int i = 0; i < w; i++) before[k] += part[k][i];
+    if (tid < E) {
+      plan[tid] = before[0];
+      int* tiles = plan + E + 3;
+      const int full = n / kTileRows, other = whole + before[2];
+      for (int i = 0; i < full; i++) {
+        tiles[2 * (before[1] + i)] = tid;
+        tiles[2 * (before[1] + i) + 1] = before[0] + i * kTileRows;
+      }
+      if (n % kTileRows) {
+        tiles[2 * other] = tid;
+        tiles[2 * other + 1] = before[0] + full * kTileRows;
+      }
+      if (tid == E - 1) {
+        plan[E] = before[0] + n;
+        plan[E + 1] = whole;
+        plan[E + 2] = other + (n % kTileRows != 0);
+      }
+    }
+    int at = before[0];
+    for (int i = 0; i < kPlanWaves; i++) {
+      const int c = cnt[i][tid];
+      cnt[i][tid] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+  if (!ids) {
+    for (int i = tid; i < P; i += kPlanThreads) rows[i] = i;
+  } else if (once) {
+#pragma unroll
+    for (int j = 0; j < kPer; j++)
+      if ((unsigned)id[j] < (unsigned)E) rows[cnt[w][id[j]] + rank[j]] = kPlanThreads * j + tid;
+  } else {
+    for (int i = tid; i < P; i += kPlanThreads) {
+      const int e = ids[i];
+      if ((unsigned)e < (unsigned)E) rows[atomicAdd(&cnt[w][e], 1)] = i;
+    }
   }
 }
 
 // ---------------------------------------------------------------- products
-// 8 nibbles (k even in the low one) -> 8 fp16 (nibble - 8), exact: byte b twice
-// into a word, its low nibble under the exponent of 1024 and its high one, not
-// shifted, 16 fold; one fma takes {1, 1/16} and the offsets back out.
+// 8 nibbles (k even in the low one) -> 8 fp16 (nibble - 8), exact, in 12
+// instructions: a permute puts byte b under the exponent of 1024 in both halves
+// of a word, an and leaves the low half its low nibble and the high half its high
+// one, not shifted and so 16 fold, and one fma takes {1, 1/16} and the offsets
+// back out.
 __device__ __forceinline__ f16x8 nib8(uint32_t u) {
   const f16x2 mul = {(_Float16)1.0f, (_Float16)0.0625f}, off = {(_Float16)-1032.0f, (_Float16)-72.0f};
   f16x8 r;
 #pragma unroll
   for (int b = 0; b < 4; b++) {
-    const uint32_t t = __builtin_amdgcn_perm(u, u, 0x0C000C00u | (uint32_t)b << 16 | (uint32_t)b);
-    const f16x2 h = __builtin_elementwise_fma(
-        __builtin_bit_cast(f16x2, (t & 0x00F0000Fu) | 0x64006400u), mul, off);
+    const uint32_t t = __builtin_amdgcn_perm(0x64646464u, u, 0x04000400u | (uint32_t)b << 16 | (uint32_t)b);
+    const f16x2 h = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, t & 0x64F0640Fu), mul, off);
     r[2 * b] = h[0];
     r[2 * b + 1] = h[1];
   }
@@ -103,7 +169,7 @@ __device__ __forceinline__ f16x8 nib8(uint32_t u) {
 // itself the compiler multiplies and converts in one instruction at some places
 // and in two at others, and a row's bits would depend on its place in a tile.)
 __device__ __forceinline__ float silu_mul(float g, float u) {
-  float v = g / (1.0f + fast_exp(-g)) * u;
+  float v = g * __builtin_amdgcn_rcpf(1.0f + fast_exp(-g)) * u;
   asm("" : "+v"(v));
   return v;
 }
@@ -124,46 +190,60 @@ __device__ __forceinline__ T arg(T v) {
   return (T)u;
 }
 
-// Column c of a tile: up interleaves the two matrices (even W1, odd W3), so
-// that a gate and its up product are in neighbouring lanes.
+// Columns of a tile: up interleaves the two matrices (even W1, odd W3), so that a
+// gate and its up product are in neighbouring lanes.  A lane's columns are all
+// even or all odd.
 template <bool kUp>
-struct Col {
+struct Cols {
   const uint8_t* w;
   const uint16_t* s;
-  __device__ __forceinline__ Col(const MoeArgs& a, int e, int c) {
-    const int n0 = kUp ? c >> 1 : c, n = n0 < a.N ? n0 : a.N - 1;
-    const uint8_t* w0 = arg(a.packed[0]) + (size_t)e * a.pstride[0];
-    const uint16_t* s0 = arg(a.scales[0]) + (size_t)e * a.sstride[0];
+  int last, ng;
+  __device__ __forceinline__ Cols(const MoeArgs& a, int e, bool odd) {
+    w = arg(a.packed[0]) + (size_t)e * a.pstride[0];
+    s = arg(a.scales[0]) + (size_t)e * a.sstride[0];
     if constexpr (kUp) {
       const uint8_t* w1 = arg(a.packed[1]) + (size_t)e * arg(a.pstride[1]);
       const uint16_t* s1 = arg(a.scales[1]) + (size_t)e * arg(a.sstride[1]);
-      w0 = c & 1 ? w1 : w0;
-      s0 = c & 1 ? s1 : s0;
+      w = odd ? w1 : w;
+      s = odd ? s1 : s;
     }
-    w = w0 + (size_t)n * (a.K >> 1);
-    s = s0 + (size_t)n * (a.K >> 7);
+    last = a.N - 1;
+    ng = a.K >> 7;
+  }
+  // (an expert's bytes and scales: at most 2^39 and 2^33)
+  __device__ __forceinline__ size_t row(int c) const {
+    const int n = kUp ? c >> 1 : c;
+    return (size_t)((uint64_t)(uint32_t)(n < last ? n : last) * (uint32_t)ng);
+  }
+  __device__ __forceinline__ const uint8_t* packed(int c) const { return w + row(c) * 64; }
+  // (through a pointer to global memory: the choice of matrix hides where it points)
+  __device__ __forceinline__ uint16_t scale(int c, int g) const {
+    return ((const __attribute__((address_space(1))) uint16_t*)s)[row(c) + g];
   }
 };
 
 // ---------------------------------------------------------------- tiles
-// Many rows an expert: a workgroup of 8 waves computes 128 rows x (128 kNT)
+// Many rows an expert: a workgroup of 4 waves computes 128 rows x (64 kNT)
 // columns, a wave all the rows of its own 16 kNT columns, so that a dequantised
-// operand serves 128 rows and no column is dequantised twice.  The K loop runs
-// over the scale groups in two LDS slots, filled by DMA one group ahead:
-//   X  128 rows x 16 chunks of 16 bytes, fetched from the rows of the tile
-//      wherever they are (a row's address is the lane's own).  Row r's chunk c at
-//      c ^ xsw(r): a 16-byte read is served 32 lanes, 512 bytes of banks, at a
-//      time, and so reaches 32 different places.
-//   W  each wave's own columns, 4 chunks of nibbles; column c's chunk q at
-//      q ^ ((c >> 2) & 3).
+// operand serves 128 rows and no column is dequantised twice.  Two workgroups a
+// compute unit, so that one's first loads, dequantisation and outputs lie under
+// the other's products.  The K loop runs over the scale groups, operands through
+// LDS by DMA:
+//   X  half a group, 64 rows x 16 chunks of 16 bytes, a slot, three slots; fetched
+//      from the rows of the tile wherever they are (a row's address is the lane's
+//      own).  Row r's chunk c at c ^ xsw(r): a 16-byte read is served 32 lanes,
+//      512 bytes of banks, at a time, and so reaches 32 different places.
+//   W  each wave's own columns, 4 chunks of nibbles, two slots; column c's chunk q
+//      at q ^ ((c >> 2) & 3).
 // Inside a group lane q = l >> 4 of an operand holds k = 32q + 8s .. + 7 at step
 // s, so one 16-byte read brings a column's nibbles for all four steps.
-// Scales lie in an LDS table, filled once for up to kTabGroups groups.
+//   One barrier a half: past the one before half h, h has landed, and all have
+// read h - 1, whose slot h + 2 takes.
 typedef __attribute__((address_space(3))) void lds_void_t;
 typedef __attribute__((address_space(1))) void gbl_void_t;
 
-constexpr int kTileWaves = 8;
-constexpr int kTabGroups = 32;
+constexpr int kTileWaves = 4;
+constexpr int kTabGroups = 16;  // groups whose scales the LDS table holds
 
 __device__ __forceinline__ int xsw(int r) { return ((r >> 1) & 3) | ((r & 1) << 2) | (r & 8); }
 
@@ -171,217 +251,302 @@ __device__ __forceinline__ void dma16(const void* src, void* dst) {
   __builtin_amdgcn_global_load_lds((gbl_void_t*)src, (lds_void_t*)dst, 16, 0, 0);
 }
 
-template <bool kUp, int kNT>
+template <int kNT>
 struct Tile {
   static constexpr int kCols = 16 * kNT;  // of a wave
-  static constexpr int kX = kTileRows * 256, kW = kTileWaves * kCols * 64, kSlot = kX + kW;
+  static constexpr int kX = 64 * 256, kW = kTileWaves * kCols * 64;  // of a slot
   static constexpr int kTab = kTileWaves * kTabGroups * kCols * 2;
-  static constexpr int kLds = 2 * kSlot + kTab + kTileRows * 4;
+  static constexpr int kLds = 3 * kX + 2 * kW + kTab + 2 * kTileRows * 4;
 };
 
-// A lane's DMA sources in group 0
+// A lane's DMA sources in group 0: X of the first and second half, W
 template <int kNT>
 struct TileSrc {
-  const uint8_t *x0, *x1, *x2, *x3, *w0, *w1, *w2;
-  __device__ __forceinline__ const uint8_t* x(int t) const { return t == 0 ? x0 : t == 1 ? x1 : t == 2 ? x2 : x3; }
+  const uint8_t *x0, *x1, *x2, *x3, *y0, *y1, *y2, *y3, *w0, *w1, *w2;
+  __device__ __forceinline__ const uint8_t* x(int half, int t) const {
+    return half == 0 ? (t == 0 ? x0 : t == 1 ? x1 : t == 2 ? x2 : x3) : (t == 0 ? y0 : t == 1 ? y1 : t == 2 ? y2 : y3);
+  }
   __device__ __forceinline__ const uint8_t* w(int t) const { return t == 0 ? w0 : t == 1 ? w1 : w2; }
 };
 
-template <bool kUp, int kNT, int kPR>
-__device__ __forceinline__ void tile_fetch(uint8_t* slot, const TileSrc<kNT>& src, int w, int g) {
-  using T = Tile<kUp, kNT>;
-#pragma unroll
-  for (int t = 0; t < 4; t++)
-    if (kPR == 4 || 16 * w + 4 * t < 32 * kPR) dma16(src.x(t) + 256 * (size_t)g, slot + (4 * w + t) * 1024);
-#pragma unroll
-  for (int t = 0; t < kNT; t++)
-    dma16(src.w(t) + 64 * (size_t)g, slot + T::kX + w * T::kCols * 64 + t * 1024);
-}
-
-// One scale group: group g + 1 (if more) is fetched into next while cur is
-// multiplied.
-template <bool kUp, int kNT, int kPR>
-__device__ __forceinline__ void tile_group(const uint8_t* cur, uint8_t* next, const uint16_t* scales, const TileSrc<kNT>& src, int w, int g,
-                                           bool more, f32x4 (&C)[2 * kPR][kNT]) {
-  using T = Tile<kUp, kNT>;
-  const int l = threadIdx.x & 63, n16 = l & 15, q = l >> 4;
-  if (more) tile_fetch<kUp, kNT, kPR>(next, src, w, g + 1);
-  const uint16_t* xs = (const uint16_t*)cur + n16 * 128;
-  const uint8_t* ws = cur + T::kX + w * T::kCols * 64;
-  // Units of two row tiles x two k steps: a unit's x operands are requested
-  // before the products of the unit before it.
-  f16x8 A[2][4];
-  auto load_a = [&](int u, f16x8 (&o)[4]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-      for (int s = 0; s < 2; s++)
-        o[2 * i + s] = *(const f16x8*)(xs + 16 * (2 * (u >> 1) + i) * 128 + 8 * ((4 * q + 2 * (u & 1) + s) ^ xsw(n16)));
-  };
-  u32x4 wq[kNT];
-  float scl[kNT];
-#pragma unroll
-  for (int j = 0; j < kNT; j++) {
-    const int c = 16 * j + n16;
-    wq[j] = *(const u32x4*)(ws + c * 64 + 16 * (q ^ ((c >> 2) & 3)));
-    scl[j] = h2f(scales[c]);
-  }
-  load_a(0, A[0]);
+// The K loop of a wave over up to 32 kPR rows, in kHalves halves of a group.
+template <int kNT, int kPR>
+struct TileLoop {
+  static_assert(kNT <= 3, "the columns' sources");
+  using T = Tile<kNT>;
+  static constexpr int kUnits = 2 * kPR;  // of a row tile
+  static constexpr int kHalves = kPR > 2 ? 2 : 1;
+  static constexpr int kLast = kPR > 2 ? 2 * (kPR - 2) : 2 * kPR;  // DMA instructions a wave in the last half: its row tiles
+  uint8_t* lds;
+  uint16_t* tab;  // this wave's scales
+  TileSrc<kNT> src;
+  int w, n16, q, g1;
+  f32x4 C[kUnits][kNT];
+  f32x4 P[2][kNT];  // of a row tile, and of the one before
+  f16x8 A[2][4];    // of a row tile, and of the next
   f16x8 B[kNT][4];
-  f32x4 P[2][2][kNT];  // of a pair of row tiles, and of the pair before
-  auto scale_add = [&](int pr) __attribute__((always_inline)) {
+  float scl[kNT], scl_old[kNT];  // of a group, and of the one before
+
+  // Half of group g into the slot at byte at; past the last group that one again
+  // (a branch here would part the block that products and vector instructions are
+  // mixed in)
+  template <int kHalf>
+  __device__ __forceinline__ void fetch_x(int at, int g) const {
+    constexpr int n = kHalf == kHalves - 1 ? kLast : 4;
+    g = g < g1 ? g : g1 - 1;
 #pragma unroll
-    for (int i = 0; i < 2; i++)
+    for (int t = 0; t < n; t++) dma16(src.x(kHalf, t) + 256 * (size_t)g, lds + at + (n * w + t) * 1024);
+  }
+  __device__ __forceinline__ uint8_t* wslot(int i) const { return lds + 3 * T::kX + (i & 1) * T::kW + w * T::kCols * 64; }
+  __device__ __forceinline__ void fetch_w(int i, int g) const {
+    g = g < g1 ? g : g1 - 1;
 #pragma unroll
-      for (int j = 0; j < kNT; j++)
+    for (int t = 0; t < kNT; t++) dma16(src.w(t) + 64 * (size_t)g, wslot(i) + t * 1024);
+  }
+  __device__ __forceinline__ void load_a(int at, int u, f16x8 (&o)[4]) const {
+    const uint16_t* xs = (const uint16_t*)(lds + at) + n16 * 128;
 #pragma unroll
-        for (int r = 0; r < 4; r++)
-          C[2 * pr + i][j][r] = __builtin_fmaf(P[pr & 1][i][j][r], scl[j], C[2 * pr + i][j][r]);
-  };
+    for (int s = 0; s < 4; s++) o[s] = *(const f16x8*)(xs + 16 * (u & 3) * 128 + 8 * ((4 * q + s) ^ xsw(n16)));
+  }
+  __device__ __forceinline__ void scale(int row_tile, int p, const float (&sc)[kNT]) {
 #pragma unroll
-  for (int u = 0; u < 2 * kPR; u++) {
-    if (u + 1 < 2 * kPR) load_a(u + 1, A[(u + 1) & 1]);
-    __builtin_amdgcn_sched_barrier(0);
-    const int s0 = 2 * (u & 1), pr = u >> 1;
-    if (u < 2)
+    for (int j = 0; j < kNT; j++)
 #pragma unroll
-      for (int j = 0; j < kNT; j++) {
-        B[j][s0] = nib8(wq[j][s0]);
-        B[j][s0 + 1] = nib8(wq[j][s0 + 1]);
+      for (int r = 0; r < 4; r++) C[row_tile][j][r] = __builtin_fmaf(P[p][j][r], sc[j], C[row_tile][j][r]);
+  }
+  __device__ __forceinline__ static int after(int at) { return at == 2 * T::kX ? 0 : at + T::kX; }
+  // all but the last kLeft fetches have landed
+  template <int kLeft>
+  __device__ __forceinline__ static void meet() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0F70 | kLeft);  // vmcnt
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
+
+  // The i-th group, group g, its first half in the slot at at; returns the next's.
+  __device__ __forceinline__ int group(int i, int g, int at) {
+    u32x4 wq[kNT];
+#pragma unroll
+    for (int u = 0; u < kUnits; u++) {
+      if (u == 0) {
+        // what may be in flight: the half after this one, fetched last
+        meet<kLast>();
+        fetch_w(i + 1, g + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        fetch_x<0>(after(after(at)), kHalves == 2 ? g + 1 : g + 2);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < kNT; j++) {
+          const int c = 16 * j + n16;
+          wq[j] = *(const u32x4*)(wslot(i) + c * 64 + 16 * (q ^ ((c >> 2) & 3)));
+          scl_old[j] = scl[j];
+          scl[j] = h2f(tab[i % kTabGroups * T::kCols + c]);
+          asm("" : "+v"(scl[j]));  // (an fp32 register: no conversion in every fma)
+        }
+        load_a(at, 0, A[0]);
       }
-#pragma unroll
-    for (int s = 0; s < 2; s++)
-#pragma unroll
-      for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int j = 0; j < kNT; j++)
-          P[pr & 1][i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              A[u & 1][2 * i + s], B[j][s0 + s], s0 + s == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : P[pr & 1][i][j], 0, 0, 0);
-    // the pair before is scaled between this pair's first products
-    if (pr > 0 && (u & 1) == 0) {
-      scale_add(pr - 1);
-#pragma unroll
-      for (int k = 0; k < 4 * kNT; k++) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // one MFMA
-        __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);  // two vector instructions
+      if (u == 4) {
+        meet<kNT + 4>();
+        at = after(at);
+        fetch_x<1>(after(after(at)), g + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        load_a(at, 0, A[0]);
       }
+      __builtin_amdgcn_sched_barrier(0);
+      if (u + 1 < kUnits && u != 3) load_a(at, u + 1, A[(u + 1) & 1]);
+#pragma unroll
+      for (int s = 0; s < 4; s++)
+#pragma unroll
+        for (int j = 0; j < kNT; j++) {
+          if (u == 0) B[j][s] = nib8(wq[j][s]);
+          P[u & 1][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[u & 1][s], B[j][s],
+                                                               s == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : P[u & 1][j], 0, 0, 0);
+        }
+      // the row tile before (of the group before, at a group's start)
+      if (u == 0)
+        scale(kUnits - 1, 1, scl_old);
+      else
+        scale(u - 1, (u - 1) & 1, scl);
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (u == 0) {
+#pragma unroll
+          for (int j = 0; j < kNT; j++) {
+            __builtin_amdgcn_sched_group_barrier(0x002, 13, 0);  // vector instructions
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // one MFMA
+          }
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // one LDS read
+        } else {
+#pragma unroll
+          for (int j = 0; j < kNT; j++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 1, 0);
+          }
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
     }
+    return after(at);
   }
-  scale_add(kPR - 1);
-}
 
-// The K loop of a tile of up to 32 kPR rows
-template <bool kUp, int kNT, int kPR>
-__device__ __forceinline__ void tile_loop(const MoeArgs& a, uint8_t* lds, uint16_t* tab, TileSrc<kNT> src, int e, int c0,
-                                          int g0, int g1, f32x4 (&C)[2 * kPR][kNT]) {
-  using T = Tile<kUp, kNT>;
-  const int l = threadIdx.x & 63;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  tile_fetch<kUp, kNT, kPR>(lds, src, w, g0);
+  // groups g0 .. g1 - 1; scales(c, g) is column c's
+  template <class F>
+  __device__ __forceinline__ void run(int g0, const F& scales) {
+    const int l = threadIdx.x & 63;
+    auto refill = [&](int g) __attribute__((always_inline)) {
+      constexpr int n = T::kCols * kTabGroups / 64;  // 16 neighbouring lanes a column
+      const int gg = g + l % kTabGroups;
+      uint16_t v[n];
 #pragma unroll
-  for (int i = 0; i < 2 * kPR; i++)
+      for (int k = 0; k < n; k++) v[k] = scales((64 * k + l) / kTabGroups, gg < g1 ? gg : g1 - 1);
 #pragma unroll
-    for (int j = 0; j < kNT; j++) C[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int g = g0; g < g1; g++) {
-    const int i = g - g0, slot = (i & 1) * T::kSlot;
-    if (i % kTabGroups == 0)  // this wave's scales of the next groups
-      for (int k = l; k < T::kCols * kTabGroups; k += 64) {
-        const int c = k / kTabGroups, gg = g + k % kTabGroups;
-        if (gg < g1) tab[(k % kTabGroups) * T::kCols + c] = Col<kUp>(a, e, c0 + c).s[gg];
-      }
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): this wave's DMA and scales landed
-    __builtin_amdgcn_s_barrier();        // every wave's did; the other slot is read
-    asm volatile("" ::: "memory");
-    tile_group<kUp, kNT, kPR>(lds + slot, lds + (T::kSlot - slot), tab + i % kTabGroups * T::kCols, src, w, g,
-                              g + 1 < g1, C);
-  }
-}
-
-template <bool kUp, int kNT, int kPR>
-__device__ __forceinline__ void tile_run(const MoeArgs& a, uint8_t* lds, uint16_t* tab, TileSrc<kNT> src,
-                                         const int* rows, int nrows, int e, int c0,
-                                         int g0, int g1, float* y) {
-  const int l = threadIdx.x & 63, n16 = l & 15, q = l >> 4;
-  f32x4 C[2 * kPR][kNT];
-  tile_loop<kUp, kNT, kPR>(a, lds, tab, src, e, c0, g0, g1, C);
-  // lane holds rows 4q .. 4q + 3 of row tile i, column n16 of column tile j
-#pragma unroll
-  for (int i = 0; i < 2 * kPR; i++) {
-    auto row = [&](int r) __attribute__((always_inline)) {
-      const int t = 16 * i + 4 * q + r;
-      return t < nrows ? rows[t] : -1;
+      for (int k = 0; k < n; k++) tab[l % kTabGroups * T::kCols + (64 * k + l) / kTabGroups] = v[k];
     };
-    const int p0 = row(0), p1 = row(1), p2 = row(2), p3 = row(3);
+    fetch_w(0, g0);
+    fetch_x<0>(0, g0);
+    if constexpr (kHalves == 2)
+      fetch_x<1>(T::kX, g0);
+    else
+      fetch_x<0>(T::kX, g0 + 1);
+    refill(g0);
 #pragma unroll
     for (int j = 0; j < kNT; j++) {
-      const int c = c0 + 16 * j + n16;
-      const f32x4 v = C[i][j];
-      if constexpr (kUp) {
+#pragma unroll
+      for (int i = 0; i < kUnits; i++) C[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      P[1][j] = f32x4{0.f, 0.f, 0.f, 0.f};  // (of the group before the first)
+      scl[j] = 0.f;
+    }
+    int at = 0;
+    for (int i = 0; g0 + i < g1; i++) {
+      if (i > 0 && i % kTabGroups == 0) refill(g0 + i);
+      at = group(i, g0 + i, at);
+    }
+    scale(kUnits - 1, 1, scl);
+  }
+};
+
+template <bool kUp, int kNT, int kPR>
+__device__ __forceinline__ void tile_run(const MoeArgs& a, uint8_t* lds, uint16_t* tab, const int* rows, int nrows, int e,
+                                         int c0, int g0, int g1, float* y) {
+  using T = Tile<kNT>;
+  const int l = threadIdx.x & 63, n16 = l & 15, q = l >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  TileLoop<kNT, kPR> loop;
+  // X instruction t of wave w fills rows 4 (n w + t) .. + 3 of its half, n
+  // instructions a wave; W instruction t this wave's columns 16 t .. + 15
+  auto xsrc = [&](int half, int t) __attribute__((always_inline)) {
+    const int n = half == loop.kHalves - 1 ? loop.kLast : 4;
+    const int r = half >= loop.kHalves || t >= n ? 0 : 64 * half + 4 * (n * w + t) + (l >> 4);
+    return (const uint8_t*)(a.x + (uint64_t)(uint32_t)rows[kTileRows + r] * (uint32_t)a.K) + 16 * ((l & 15) ^ xsw(r));
+  };
+  const Cols<kUp> wcols(a, e, (l >> 2) & 1), scols(a, e, (l >> 4) & 1);
+  auto wsrc = [&](int t) __attribute__((always_inline)) {
+    const int c = 16 * t + (l >> 2);
+    return wcols.packed(c0 + c) + 16 * ((l & 3) ^ ((c >> 2) & 3));
+  };
+  loop.lds = lds;
+  loop.tab = tab;
+  loop.src = {xsrc(0, 0), xsrc(0, 1), xsrc(0, 2), xsrc(0, 3), xsrc(1, 0), xsrc(1, 1),
+              xsrc(1, 2), xsrc(1, 3), wsrc(0),    wsrc(1),    wsrc(kNT > 2 ? 2 : 0)};
+  loop.w = w;
+  loop.n16 = n16;
+  loop.q = q;
+  loop.g1 = g1;
+  loop.run(g0, [&](int c, int g) { return scols.scale(c0 + c, g); });
+  // Lane holds rows 4q .. 4q + 3 of row tile i, column n16 of column tile j.  They
+  // change places in LDS, where all have read, and go out 16 bytes a lane.
+  loop.template meet<0>();
+  uint8_t* const out = lds + w * ((3 * T::kX + 2 * T::kW) / kTileWaves);
+  if constexpr (kUp) {
+    constexpr int kN = T::kCols / 2;  // outputs of a row
+    uint16_t* st = (uint16_t*)out + (4 * q + (n16 & 1) * 2) * kN + (n16 >> 1);
+#pragma unroll
+    for (int i = 0; i < 2 * kPR; i++)
+#pragma unroll
+      for (int j = 0; j < kNT; j++) {
         // the even lane takes rows 0 and 1 of the pair's column, the odd one 2, 3
-        const bool odd = c & 1;
-        const int n = c >> 1, pa = odd ? p2 : p0, pb = odd ? p3 : p1;
+        const f32x4 v = loop.C[i][j];
+        const bool odd = n16 & 1;
         const float o0 = lane_pair(v[0]), o1 = lane_pair(v[1]), o2 = lane_pair(v[2]), o3 = lane_pair(v[3]);
-        const float va = silu_mul(odd ? o2 : v[0], odd ? v[2] : o0), vb = silu_mul(odd ? o3 : v[1], odd ? v[3] : o1);
-        if (n < a.N) {
-          if (pa >= 0) a.act[(size_t)pa * a.N + n] = f2h(va);
-          if (pb >= 0) a.act[(size_t)pb * a.N + n] = f2h(vb);
-        }
-      } else if (c < a.N) {
-        if (p0 >= 0) y[(size_t)p0 * a.N + c] = v[0];
-        if (p1 >= 0) y[(size_t)p1 * a.N + c] = v[1];
-        if (p2 >= 0) y[(size_t)p2 * a.N + c] = v[2];
-        if (p3 >= 0) y[(size_t)p3 * a.N + c] = v[3];
+        st[16 * i * kN + 8 * j] = f2h(silu_mul(odd ? o2 : v[0], odd ? v[2] : o0));
+        st[(16 * i + 1) * kN + 8 * j] = f2h(silu_mul(odd ? o3 : v[1], odd ? v[3] : o1));
+      }
+#pragma unroll
+    for (int k = 0; k < (32 * kPR * kNT + 63) / 64; k++) {
+      const int i = 64 * k + l, r = i / kNT, n = c0 / 2 + 8 * (i % kNT);
+      if (r < nrows && n < a.N)
+        *(u32x4*)(a.act + (uint64_t)(uint32_t)rows[r] * (uint32_t)a.N + n) = *(const u32x4*)(out + 16 * i);
+    }
+  } else {
+    constexpr int kRow = T::kCols + 4;  // floats: the four row groups of a store on different banks
+#pragma unroll
+    for (int half = 0; half < (kPR + 1) / 2; half++) {  // 64 rows at a time
+      float* st = (float*)out + 4 * q * kRow + n16;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (4 * half + i < 2 * kPR)
+#pragma unroll
+          for (int j = 0; j < kNT; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) st[(16 * i + r) * kRow + 16 * j] = loop.C[4 * half + i < 2 * kPR ? 4 * half + i : 0][j][r];
+#pragma unroll
+      for (int k = 0; k < 4 * kNT; k++) {
+        const int i = 64 * k + l, r = i / (4 * kNT), ch = i % (4 * kNT), n = c0 + 4 * ch;
+        if (64 * half + r < nrows && n < a.N)
+          *(f32x4*)(y + (uint64_t)(uint32_t)rows[64 * half + r] * (uint32_t)a.N + n) =
+              *(const f32x4*)((const float*)out + r * kRow + 4 * ch);
       }
     }
   }
 }
 
-// grid = max_tiles x column tiles x splits, up to a multiple of 8; block = 512
+// grid = max_tiles x column tiles x splits, up to a multiple of 8, and 8; block = 256
 template <bool kUp, int kNT>
-__global__ __launch_bounds__(64 * kTileWaves) void k_moe_tile(MoeArgs a) {
-  using T = Tile<kUp, kNT>;
+__global__ __launch_bounds__(64 * kTileWaves, 2) void k_moe_tile(MoeArgs a) {
+  using T = Tile<kNT>;
   // (one LDS variable: with two the compiler tells their accesses apart, takes the
   // DMA's target for known, and waits for it before any read of that variable)
   __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
-  int* const srows = (int*)(lds + T::kLds) - kTileRows;
-  const int tid = threadIdx.x, l = tid & 63;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int* const srows = (int*)(lds + T::kLds) - 2 * kTileRows;  // rows, and their rows of x
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nv = kUp ? 2 * a.N : a.N, nct = (nv + T::kCols * kTileWaves - 1) / (T::kCols * kTileWaves);
   // Workgroups go to the 8 XCDs in turn: each takes a run of tiles, row tiles
   // slowest, so that its L2 holds what neighbours share.
-  const int ntiles = a.plan[a.E + 1] * nct * a.splits, per = (ntiles + 7) >> 3;
-  int tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per || tile >= ntiles) return;
+  // The whole tiles first: the others fill the last round.
+  const int whole = a.plan[a.E + 1], n0 = whole * nct * a.splits, n1 = (a.plan[a.E + 2] - whole) * nct * a.splits;
+  const int per0 = (n0 + 7) >> 3, per1 = (n1 + 7) >> 3;
+  int tile = blockIdx.x >> 3;
+  if (tile < per0) {
+    tile += (blockIdx.x & 7) * per0;
+    if (tile >= n0) return;
+  } else {
+    tile -= per0;
+    if (tile >= per1) return;
+    tile += (blockIdx.x & 7) * per1;
+    if (tile >= n1) return;
+    tile += n0;
+  }
   const int ct = tile % nct;
   tile /= nct;
   const int sp = tile % a.splits;
   tile /= a.splits;
-  const int e = a.plan[a.E + 2 + 2 * tile], r0 = a.plan[a.E + 3 + 2 * tile];
+  const int e = a.plan[a.E + 3 + 2 * tile], r0 = a.plan[a.E + 4 + 2 * tile];
   const int left = a.plan[e + 1] - r0, nrows = left < kTileRows ? left : kTileRows;
   if (tid < kTileRows) {
-    const int* rows = a.plan + plan_rows_at((int64_t)a.S * a.k, a.E);
-    srows[tid] = rows[r0 + (tid < nrows ? tid : nrows - 1)];
+    const int p = a.plan[plan_rows_at((int64_t)a.S * a.k, a.E) + r0 + (tid < nrows ? tid : nrows - 1)];
+    srows[tid] = p;
+    srows[kTileRows + tid] = kUp ? p / a.k : p;
   }
   __syncthreads();
   const int c0 = ct * T::kCols * kTileWaves + w * T::kCols;
   const int ng = a.K >> 7, g0 = ng * sp / a.splits, g1 = ng * (sp + 1) / a.splits;
-  auto xsrc = [&](int t) {
-    const int r = 16 * w + 4 * t + (l >> 4), p = srows[r];
-    return (const uint8_t*)(a.x + (size_t)(kUp ? p / a.k : p) * a.K) + 16 * ((l & 15) ^ xsw(r));
-  };
-  auto wsrc = [&](int t) {
-    const int c = 16 * t + (l >> 2);
-    return Col<kUp>(a, e, c0 + c).w + 16 * ((l & 3) ^ ((c >> 2) & 3));
-  };
-  const TileSrc<kNT> src = {xsrc(0), xsrc(1), xsrc(2), xsrc(3), wsrc(0), wsrc(1), kNT > 2 ? wsrc(2) : nullptr};
-  uint16_t* tab = (uint16_t*)(lds + 2 * T::kSlot) + w * kTabGroups * T::kCols;
+  uint16_t* tab = (uint16_t*)(lds + 3 * T::kX + 2 * T::kW) + w * kTabGroups * T::kCols;
   float* y = kUp ? nullptr : a.y + (size_t)sp * a.S * a.k * a.N;
   switch ((nrows + 31) >> 5) {
-    case 1: return tile_run<kUp, kNT, 1>(a, lds, tab, src, srows, nrows, e, c0, g0, g1, y);
-    case 2: return tile_run<kUp, kNT, 2>(a, lds, tab, src, srows, nrows, e, c0, g0, g1, y);
-    case 3: return tile_run<kUp, kNT, 3>(a, lds, tab, src, srows, nrows, e, c0, g0, g1, y);
-    default: return tile_run<kUp, kNT, 4>(a, lds, tab, src, srows, nrows, e, c0, g0, g1, y);
+    case 1: return tile_run<kUp, kNT, 1>(a, lds, tab, srows, nrows, e, c0, g0, g1, y);
+    case 2: return tile_run<kUp, kNT, 2>(a, lds, tab, srows, nrows, e, c0, g0, g1, y);
+    case 3: return tile_run<kUp, kNT, 3>(a, lds, tab, srows, nrows, e, c0, g0, g1, y);
+    default: return tile_run<kUp, kNT, 4>(a, lds, tab, srows, nrows, e, c0, g0, g1, y);
   }
 }
 
@@ -419,6 +584,16 @@ static int64_t plan_bytes(int64_t P, int E) { return ((plan_rows_at(P, E) + P) *
 // Rows of y: P, and room for parts of K where few pairs leave the chip empty
 static int64_t y_rows(int64_t P) { return P >= 4096 ? P : (8 * P < 4096 ? 8 * P : 4096); }
 
+// Parts of K of a down launch: as many as the chip's 512 places hold where the
+// tiles alone leave most of them empty, each of 4 groups or more.
+static int k_splits(int64_t P, int E, int H, int F) {
+  const int64_t tiles = ((P + kTileRows - 1) / kTileRows + (P < E - 1 ? P : E - 1)) * ((H + 191) / 192);
+  int64_t n = 512 / tiles;
+  n = n < y_rows(P) / P ? n : y_rows(P) / P;
+  n = n < F / 512 ? n : F / 512;
+  return n < 1 ? 1 : (int)n;
+}
+
 static int moe_check(int S, int k, int E, int H, int F, const int32_t* ids) {
   CIA_REQUIRE(S >= 0 && k >= 1 && k <= kMoeMaxK && E >= 1 && E <= kMoeMaxE && H > 0 && F > 0 &&
                   H % 128 == 0 && F % 128 == 0 && H <= (1 << 20) && F <= (1 << 20) &&
@@ -446,13 +621,13 @@ static void set_w(MoeArgs& a, int i, const cia_q4_experts* w) {
 
 template <bool kUp>
 static int products(MoeArgs& a, void* ws, hipStream_t s) {
-  constexpr int kNT = 2;
+  constexpr int kNT = 3;
   const int P = a.S * a.k;
   a.plan = (const int*)ws;
   hipLaunchKernelGGL(k_moe_plan, dim3(1), dim3(1024), 0, s, a.ids, P, a.E, (int*)ws);
-  const int nv = kUp ? 2 * a.N : a.N, cols = 128 * kNT;
+  const int nv = kUp ? 2 * a.N : a.N, cols = 16 * kNT * kTileWaves;
   const int64_t tiles = max_tiles(P, a.E) * ((nv + cols - 1) / cols) * a.splits;
-  hipLaunchKernelGGL((k_moe_tile<kUp, kNT>), dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(64 * kTileWaves), 0, s, a);
+  hipLaunchKernelGGL((k_moe_tile<kUp, kNT>), dim3((unsigned)((tiles + 7) / 8 * 8 + 8)), dim3(64 * kTileWaves), 0, s, a);
   return launch_status();
 }
 
@@ -514,7 +689,7 @@ extern "C" int cia_moe_down_int4(const uint16_t* act, const int32_t* ids, const 
   a.k = k;
   a.E = E;
   a.y = (float*)((char*)ws + plan_bytes((int64_t)S * k, E));
-  a.splits = 1;
+  a.splits = k_splits((int64_t)S * k, E, H, F);
   hipStream_t s = (hipStream_t)stream;
   if ((st = products<false>(a, ws, s))) return st;
   const CombineArgs c{a.y, ids, weights, res, out, S, k, E, H, a.splits};
