@@ -177,7 +177,7 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
 // the value of the neighbouring lane (l ^ 1)
 __device__ __forceinline__ float lane_pair(float v) {
   return __builtin_bit_cast(
-      float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, false));
+      float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true));
 }
 
 // A kernel argument as a scalar value.  (Left visible, the choice below between

@@ -32,101 +32,318 @@ struct RouteArgs {
   float eps, scale;
 };
 
+typedef double f64x2 __attribute__((ext_vector_type(2)));
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+// Sums and maxima over the wave without the LDS unit, in 64 bits; every lane gets
+// the same value.
+__device__ __forceinline__ double f64_of(uint32_t lo, uint32_t hi) {
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int kN>
+__device__ __forceinline__ double row_ror_f64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  return f64_of((uint32_t)__builtin_amdgcn_mov_dpp((int)u, 0x120 + kN, 0xF, 0xF, true),
+                (uint32_t)__builtin_amdgcn_mov_dpp((int)(u >> 32), 0x120 + kN, 0xF, 0xF, true));
+}
+// the value of the lane 16 (32) on or back
+template <bool k32>
+__device__ __forceinline__ f64x2 swap_f64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)u, hi = (uint32_t)(u >> 32);
+  if constexpr (k32) {
+    const auto a = __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+    const auto b = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+    return f64x2{f64_of(a[0], b[0]), f64_of(a[1], b[1])};
+  } else {
+    const auto a = __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
+    const auto b = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+    return f64x2{f64_of(a[0], b[0]), f64_of(a[1], b[1])};
+  }
+}
+template <class F>
+__device__ __forceinline__ double wave_fold(double v, const F& f) {
+  v = f(v, row_ror_f64<8>(v));
+  v = f(v, row_ror_f64<4>(v));
+  v = f(v, row_ror_f64<2>(v));
+  v = f(v, row_ror_f64<1>(v));
+  f64x2 r = swap_f64<false>(v);
+  v = f(r[0], r[1]);
+  r = swap_f64<true>(v);
+  return f(r[0], r[1]);
+}
 __device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off);
-  return v;
+  return wave_fold(v, [](double a, double b) { return a + b; });
+}
+// (of values that are numbers)
+__device__ __forceinline__ double wave_max_f64(double v) {
+  return wave_fold(v, [](double a, double b) { return a > b ? a : b; });
 }
 
-// one token a workgroup of 256
-__global__ __launch_bounds__(256) void k_moe_route(RouteArgs a) {
-  __shared__ double lg[kRouteMaxE], ch[kRouteMaxE], gs[kRouteMaxE], red[4];
-  __shared__ double top[kRouteMaxK];
-  const int s = blockIdx.x, tid = threadIdx.x, w = tid >> 6, l = tid & 63;
-  if (a.x) {
-    const uint16_t* xr = a.x + (size_t)s * a.H;
-    for (int e = w; e < a.E; e += 4) {
-      const uint16_t* gr = a.gate + (size_t)e * a.H;
-      double acc = 0.0;
-      for (int c = l; c < a.H; c += 64) acc += (double)h2f(xr[c]) * (double)h2f(gr[c]);
-      acc = wave_sum_f64(acc);
-      if (l == 0) lg[e] = acc;
-    }
-  } else if (tid < a.E) {
-    lg[tid] = (double)a.logits_in[(size_t)s * a.E + tid];
+// A token's choice by one wave: lg, its logits in LDS; ch, E doubles of LDS for
+// the wave.  Lane l has experts l, l + 64, ..
+__device__ __forceinline__ void choose(const RouteArgs& a, int s, const double* lg, double* ch) {
+  constexpr int kPer = kRouteMaxE / 64;
+  const int l = threadIdx.x & 63;
+  const double ninf = -__builtin_inf();
+  double sc[kPer], c[kPer];
+  bool bad = false;
+  double m = ninf;
+#pragma unroll
+  for (int i = 0; i < kPer; i++) {
+    const int e = l + 64 * i;
+    sc[i] = e < a.E ? lg[e] : ninf;
+    if (e < a.E && a.logits) a.logits[(size_t)s * a.E + e] = (float)sc[i];
+    bad = bad || sc[i] != sc[i];
+    m = sc[i] > m ? sc[i] : m;
   }
-  __syncthreads();
-  if (a.logits && tid < a.E) a.logits[(size_t)s * a.E + tid] = (float)lg[tid];
-  double sc = 0.0;
   if (a.softmax) {
-    double m = -__builtin_inf();
-    for (int e = 0; e < a.E; e++) m = lg[e] > m || lg[e] != lg[e] ? lg[e] : m;
-    const double p = tid < a.E && m > -__builtin_inf() ? exp(lg[tid] - m) : (m != m ? m : 0.0);
-    const double ws = wave_sum_f64(tid < a.E ? p : 0.0);
-    if (l == 0) red[w] = ws;
-    __syncthreads();
-    const double sum = red[0] + red[1] + red[2] + red[3];
-    sc = sum == 0.0 ? 0.0 : p / sum;
-  } else if (tid < a.E) {
-    sc = 1.0 / (1.0 + exp(-lg[tid]));
+    m = wave_max_f64(m);
+    // no number among infinities (inf - inf) or beside a NaN; all -inf: scores of 0
+    bad = __any(bad || m == __builtin_inf());
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPer; i++) {
+      if (i > 0 && 64 * i >= a.E) break;
+      sc[i] = sc[i] > ninf ? exp(sc[i] - m) : 0.0;
+      sum += sc[i];
+    }
+    sum = wave_sum_f64(sum);
+#pragma unroll
+    for (int i = 0; i < kPer; i++) sc[i] = bad ? __builtin_nan("") : (sum == 0.0 ? 0.0 : sc[i] / sum);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; i++) {
+      if (i > 0 && 64 * i >= a.E) break;
+      sc[i] = 1.0 / (1.0 + exp(-sc[i]));
+    }
   }
   // a choice that is not a number ranks with the last
-  double c = tid < a.E ? sc + (a.bias ? (double)a.bias[tid] : 0.0) : 0.0;
-  if (c != c) c = -__builtin_inf();
-  if (tid < a.E) ch[tid] = c;
-  __syncthreads();
-  bool in = tid < a.E;
+#pragma unroll
+  for (int i = 0; i < kPer; i++) {
+    const int e = l + 64 * i;
+    c[i] = ninf;
+    if (e < a.E) {
+      c[i] = sc[i] + (a.bias ? (double)a.bias[e] : 0.0);
+      if (c[i] != c[i]) c[i] = ninf;
+      ch[e] = c[i];
+    }
+  }
+  uint32_t in = 0;  // bit i: expert l + 64 i may be chosen
+#pragma unroll
+  for (int i = 0; i < kPer; i++) in |= (l + 64 * i < a.E ? 1u : 0u) << i;
   if (a.n_group > 1) {
+    // lane l has groups l, l + 64, ..: the sum of a group's two best choices
     const int per = a.E / a.n_group;
-    if (tid < a.n_group) {
-      double b0 = -__builtin_inf(), b1 = b0;
-      for (int i = 0; i < per; i++) {
-        const double v = ch[tid * per + i];
-        if (v > b0) {
-          b1 = b0;
-          b0 = v;
-        } else if (v > b1) {
-          b1 = v;
+    double best[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; i++) {
+      const int g = l + 64 * i;
+      double b0 = ninf, b1 = ninf;
+      if (g < a.n_group)
+        for (int j = 0; j < per; j++) {
+          const double v = ch[g * per + j];
+          b1 = v > b0 ? b0 : (v > b1 ? v : b1);
+          b0 = v > b0 ? v : b0;
+        }
+      best[i] = per > 1 ? b0 + b1 : b0;
+      if (best[i] != best[i]) best[i] = ninf;
+    }
+    // (the choices are read: their place takes the groups' sums, then which are in)
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < kPer; i++)
+      if (l + 64 * i < a.n_group) ch[l + 64 * i] = best[i];
+    uint32_t keep = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; i++) {
+      const int g = l + 64 * i;
+      if (64 * i >= a.n_group) break;
+      int rank = 0;
+      for (int j = 0; j < a.n_group; j++) rank += ch[j] > best[i] || (ch[j] == best[i] && j < g);
+      keep |= (g < a.n_group && rank < a.topk_group ? 1u : 0u) << i;
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < kPer; i++)
+      if (l + 64 * i < a.n_group) ch[l + 64 * i] = keep >> i & 1 ? 1.0 : 0.0;
+    in = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; i++)
+      if (l + 64 * i < a.E && ch[(l + 64 * i) / per] != 0.0) in |= 1u << i;
+  }
+  // k rounds: the best choice left, the lowest index among equals; lane j keeps
+  // round j's
+  int id = 0;
+  double w = 0.0;
+  for (int j = 0; j < a.k; j++) {
+    double v = ninf, vs = 0.0;
+    int ve = kRouteMaxE;  // (none left)
+#pragma unroll
+    for (int i = 0; i < kPer; i++)
+      if (in >> i & 1 && (ve == kRouteMaxE || c[i] > v)) {
+        v = c[i];
+        vs = sc[i];
+        ve = l + 64 * i;
+      }
+    const double top = wave_max_f64(v);
+    uint64_t at = __ballot(ve < kRouteMaxE && v == top);
+    int win = ve, lane = 0;
+    if (a.E > 64) {
+      // (a lane's own equals are in order; among lanes the lowest index)
+      win = ve < kRouteMaxE && v == top ? ve : kRouteMaxE;
+#pragma unroll
+      for (int d = 32; d >= 1; d >>= 1) {
+        const int o = __shfl_xor(win, d);
+        win = o < win ? o : win;
+      }
+      lane = win & 63;
+    } else {
+      lane = __builtin_ctzll(at);
+      win = lane;
+    }
+    const double ws = __shfl(vs, lane);
+    if (l == lane) in &= ~(1u << (win >> 6));
+    if (l == j) {
+      id = win;
+      w = ws;
+    }
+  }
+  double f = (double)a.scale;
+  if (a.renorm) {
+    const double sum = wave_sum_f64(l < a.k ? w : 0.0) + (double)a.eps;
+    f = sum == 0.0 ? 0.0 : f / sum;
+  }
+  if (l < a.k) {
+    a.ids[(size_t)s * a.k + l] = id;
+    a.weights[(size_t)s * a.k + l] = (float)(w * f);
+  }
+}
+
+// Few tokens: kT a workgroup of 8 waves, a wave every 8th expert, so that a
+// token's gate is read by all of a compute unit.  x lies in LDS in 64 bits, a
+// lane's 8 elements in four 16-byte pieces kSpan / 8 lanes apart.
+constexpr int kTokWaves = 8;
+
+template <int kT>
+__global__ __launch_bounds__(64 * kTokWaves) void k_route_tok(RouteArgs a) {
+  constexpr int kSpan = 4096 / kT;  // elements of a row in LDS at a time
+  __shared__ f64x2 xs[kT][4][kSpan / 8];
+  __shared__ double lg[kT][kRouteMaxE];
+  __shared__ double ch[kT][kRouteMaxE];
+  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, s0 = blockIdx.x * kT;
+  if (a.x) {
+    for (int h0 = 0; h0 < a.H; h0 += kSpan) {
+      const int n8 = (a.H - h0 < kSpan ? a.H - h0 : kSpan) / 8;
+      if (h0) __syncthreads();
+      for (int i = tid; i < kT * n8; i += 64 * kTokWaves) {
+        const int t = kT > 1 ? i / n8 : 0, c = i - t * n8;
+        const int s = s0 + t < a.S ? s0 + t : a.S - 1;
+        const f16x8 v = *(const f16x8*)(a.x + (size_t)s * a.H + h0 + 8 * c);
+#pragma unroll
+        for (int p = 0; p < 4; p++) xs[t][p][c] = f64x2{(double)(float)v[2 * p], (double)(float)v[2 * p + 1]};
+      }
+      __syncthreads();
+      for (int e = w; e < a.E; e += kTokWaves) {
+        const uint16_t* gr = a.gate + (size_t)e * a.H + h0;
+        double acc[kT][2] = {};
+        for (int c = l; c < n8; c += 64) {
+          const f16x8 g = *(const f16x8*)(gr + 8 * c);
+#pragma unroll
+          for (int p = 0; p < 4; p++) {
+            const double g0 = (double)(float)g[2 * p], g1 = (double)(float)g[2 * p + 1];
+#pragma unroll
+            for (int t = 0; t < kT; t++) {
+              const f64x2 xv = xs[t][p][c];
+              acc[t][0] = __builtin_fma(xv[0], g0, acc[t][0]);
+              acc[t][1] = __builtin_fma(xv[1], g1, acc[t][1]);
+            }
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < kT; t++) {
+          const double v = wave_sum_f64(acc[t][0] + acc[t][1]);
+          if (l == 0) lg[t][e] = h0 ? lg[t][e] + v : v;
         }
       }
-      const double t = per > 1 ? b0 + b1 : b0;
-      gs[tid] = t != t ? -__builtin_inf() : t;
     }
     __syncthreads();
-    if (in) {
-      const int g = tid / per;
-      int rank = 0;
-      for (int j = 0; j < a.n_group; j++) rank += gs[j] > gs[g] || (gs[j] == gs[g] && j < g);
-      in = rank < a.topk_group;
+  } else {
+    for (int i = tid; i < kT * a.E; i += 64 * kTokWaves) {
+      const int t = i / a.E, e = i - t * a.E;
+      lg[t][e] = s0 + t < a.S ? (double)a.logits_in[(size_t)(s0 + t) * a.E + e] : 0.0;
     }
     __syncthreads();
-    if (tid < a.E) gs[tid] = in ? 1.0 : 0.0;
+  }
+  if (w < kT && s0 + w < a.S) choose(a, s0 + w, lg[w], ch[w]);
+}
+
+// Many tokens: 16 a workgroup on the matrix cores in 64 bits
+// (v_mfma_f64_16x16x4_f64), 16 experts a tile, the 8 waves a part of H each.  A
+// lane's 8 elements of 16 bytes are eight k steps: at step i lane (r, q) holds k =
+// 8q + i of row r, in both operands.
+constexpr int kTileToks = 16, kMfmaWaves = 8;
+
+__global__ __launch_bounds__(64 * kMfmaWaves) void k_route_mfma(RouteArgs a) {
+  constexpr int kTiles = 2;  // of experts at a time
+  __shared__ double part[kMfmaWaves][kTiles][256];
+  __shared__ double lg[kTileToks][kRouteMaxE];
+  __shared__ double ch[kMfmaWaves][kRouteMaxE];
+  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, r16 = l & 15, q = l >> 4;
+  const int s0 = blockIdx.x * kTileToks;
+  const int s = s0 + r16 < a.S ? s0 + r16 : a.S - 1;
+  const int n32 = (a.H + 31) / 32;  // steps of 32 elements
+  for (int e0 = 0; e0 < a.E; e0 += 16 * kTiles) {
+    f64x4 acc[kTiles] = {};
+    const uint16_t* gr[kTiles];
+#pragma unroll
+    for (int t = 0; t < kTiles; t++) {
+      const int e = e0 + 16 * t + r16;
+      gr[t] = a.gate + (size_t)(e < a.E ? e : a.E - 1) * a.H;
+    }
+    for (int i = w; i < n32; i += kMfmaWaves) {
+      const int k = 32 * i + 8 * q;
+      f16x8 x = {}, g[kTiles] = {};
+      if (k < a.H) {
+        x = *(const f16x8*)(a.x + (size_t)s * a.H + k);
+#pragma unroll
+        for (int t = 0; t < kTiles; t++) g[t] = *(const f16x8*)(gr[t] + k);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const double xv = (double)(float)x[j];
+#pragma unroll
+        for (int t = 0; t < kTiles; t++)
+          acc[t] = __builtin_amdgcn_mfma_f64_16x16x4f64(xv, (double)(float)g[t][j], acc[t], 0, 0, 0);
+      }
+    }
+    // lane holds tokens 4 i + q, i = 0 .. 3, of expert r16
+#pragma unroll
+    for (int t = 0; t < kTiles; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) part[w][t][64 * i + l] = acc[t][i];
+    __syncthreads();
+    for (int i = tid; i < 256 * kTiles; i += 64 * kMfmaWaves) {
+      const int t = i >> 8, j = i & 255, e = e0 + 16 * t + (j & 15);
+      double v = 0.0;
+#pragma unroll
+      for (int k = 0; k < kMfmaWaves; k++) v += part[k][t][j];
+      if (e < a.E) lg[j >> 4][e] = v;
+    }
     __syncthreads();
   }
-  int rank = a.k;
-  if (in) {
-    rank = 0;
-    for (int j = 0; j < a.E; j++)
-      if (a.n_group == 1 || gs[j] != 0.0) rank += ch[j] > c || (ch[j] == c && j < tid);
-  }
-  if (rank < a.k) {
-    top[rank] = sc;
-    a.ids[(size_t)s * a.k + rank] = tid;
-  }
-  __syncthreads();
-  if (tid < a.k) {
-    double f = (double)a.scale;
-    if (a.renorm) {
-      double sum = (double)a.eps;
-      for (int j = 0; j < a.k; j++) sum += top[j];
-      f = sum == 0.0 ? 0.0 : f / sum;
-    }
-    a.weights[(size_t)s * a.k + tid] = (float)(top[tid] * f);
-  }
+  for (int t = w; t < kTileToks && s0 + t < a.S; t += kMfmaWaves) choose(a, s0 + t, lg[t], ch[w]);
 }
 
 static int route_run(const RouteArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL(k_moe_route, dim3((unsigned)a.S), dim3(256), 0, s, a);
+  if (a.x && a.S >= 1024)
+    hipLaunchKernelGGL(k_route_mfma, dim3((unsigned)((a.S + kTileToks - 1) / kTileToks)), dim3(64 * kMfmaWaves), 0, s, a);
+  else if (!a.x && a.S >= 64)  // (nothing but the choice: a wave a token)
+    hipLaunchKernelGGL(k_route_tok<8>, dim3((unsigned)((a.S + 7) / 8)), dim3(64 * kTokWaves), 0, s, a);
+  else if (a.S <= 256)
+    hipLaunchKernelGGL(k_route_tok<1>, dim3((unsigned)a.S), dim3(64 * kTokWaves), 0, s, a);
+  else
+    hipLaunchKernelGGL(k_route_tok<2>, dim3((unsigned)((a.S + 1) / 2)), dim3(64 * kTokWaves), 0, s, a);
   return launch_status();
 }
 

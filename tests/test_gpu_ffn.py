@@ -73,6 +73,10 @@ def test_norm_rows_of_zeros_and_beyond_numbers(K, dev):
     (6, 128, 24, dict(k=2, n_group=24, topk_group=2)),
     (40, 640, 200, dict(k=3)),
     (300, 2048, 32, dict(k=4, eps=0.0)),
+    (2, 8200, 20, dict(k=2)),
+    (1030, 72, 40, dict(k=4)),
+    (1024, 256, 17, dict(k=5, score="softmax")),
+    (2050, 136, 100, dict(k=3, n_group=4, topk_group=2)),
 ])
 @pytest.mark.parametrize("bias", [False, True])
 def test_route(K, dev, S, H, E, kw, bias):
