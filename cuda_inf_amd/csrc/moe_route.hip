@@ -141,6 +141,7 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int s, const double* 
       const int g = l + 64 * i;
       double b0 = ninf, b1 = ninf;
       if (g < a.n_group)
+#pragma unroll 8
         for (int j = 0; j < per; j++) {
           const double v = ch[g * per + j];
           b1 = v > b0 ? b0 : (v > b1 ? v : b1);
@@ -160,6 +161,7 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int s, const double* 
       const int g = l + 64 * i;
       if (64 * i >= a.n_group) break;
       int rank = 0;
+#pragma unroll 8
       for (int j = 0; j < a.n_group; j++) rank += ch[j] > best[i] || (ch[j] == best[i] && j < g);
       keep |= (g < a.n_group && rank < a.topk_group ? 1u : 0u) << i;
     }
@@ -177,35 +179,30 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int s, const double* 
   int id = 0;
   double w = 0.0;
   for (int j = 0; j < a.k; j++) {
-    double v = ninf, vs = 0.0;
-    int ve = kRouteMaxE;  // (none left)
+    double v = ninf;
 #pragma unroll
     for (int i = 0; i < kPer; i++)
-      if (in >> i & 1 && (ve == kRouteMaxE || c[i] > v)) {
-        v = c[i];
-        vs = sc[i];
-        ve = l + 64 * i;
-      }
+      if (in >> i & 1 && c[i] > v) v = c[i];
     const double top = wave_max_f64(v);
-    uint64_t at = __ballot(ve < kRouteMaxE && v == top);
-    int win = ve, lane = 0;
-    if (a.E > 64) {
-      // (a lane's own equals are in order; among lanes the lowest index)
-      win = ve < kRouteMaxE && v == top ? ve : kRouteMaxE;
+    uint64_t at = 0;
+    int wi = 0;
+    double vs = 0.0;
 #pragma unroll
-      for (int d = 32; d >= 1; d >>= 1) {
-        const int o = __shfl_xor(win, d);
-        win = o < win ? o : win;
+    for (int i = kPer - 1; i >= 0; i--) {
+      const uint64_t b = __ballot(in >> i & 1 && c[i] == top);
+      if (b) {
+        at = b;
+        wi = i;
+        vs = sc[i];
       }
-      lane = win & 63;
-    } else {
-      lane = __builtin_ctzll(at);
-      win = lane;
     }
-    const double ws = __shfl(vs, lane);
-    if (l == lane) in &= ~(1u << (win >> 6));
+    const int lane = __builtin_ctzll(at);
+    const uint64_t u = __builtin_bit_cast(uint64_t, vs);
+    const double ws = f64_of((uint32_t)__builtin_amdgcn_readlane((int)u, lane),
+                             (uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), lane));
+    if (l == lane) in &= ~(1u << wi);
     if (l == j) {
-      id = win;
+      id = lane + 64 * wi;
       w = ws;
     }
   }
@@ -244,26 +241,52 @@ __global__ __launch_bounds__(64 * kTokWaves) void k_route_tok(RouteArgs a) {
         for (int p = 0; p < 4; p++) xs[t][p][c] = f64x2{(double)(float)v[2 * p], (double)(float)v[2 * p + 1]};
       }
       __syncthreads();
-      for (int e = w; e < a.E; e += kTokWaves) {
-        const uint16_t* gr = a.gate + (size_t)e * a.H + h0;
-        double acc[kT][2] = {};
-        for (int c = l; c < n8; c += 64) {
-          const f16x8 g = *(const f16x8*)(gr + 8 * c);
+      // 4 experts at a time, w, w + 8, .., a step's 8 elements of each fetched a
+      // step ahead, across experts too
+      const int steps = (n8 + 63) / 64, rounds = (a.E + 4 * kTokWaves - 1) / (4 * kTokWaves);
+      f16x8 g[4], gn[4];
+      auto fetch = [&](int round, int step, f16x8 (&o)[4]) __attribute__((always_inline)) {
+        const int c = 64 * step + l;
 #pragma unroll
-          for (int p = 0; p < 4; p++) {
-            const double g0 = (double)(float)g[2 * p], g1 = (double)(float)g[2 * p + 1];
+        for (int j = 0; j < 4; j++) {
+          const int e = 4 * kTokWaves * round + kTokWaves * j + w;
+          o[j] = *(const f16x8*)(a.gate + (size_t)(e < a.E ? e : a.E - 1) * a.H + h0 + 8 * (c < n8 ? c : n8 - 1));
+        }
+      };
+      fetch(0, 0, gn);
+      for (int round = 0; round < rounds; round++) {
+        double acc[kT][4][2] = {};
+        for (int step = 0; step < steps; step++) {
 #pragma unroll
-            for (int t = 0; t < kT; t++) {
-              const f64x2 xv = xs[t][p][c];
-              acc[t][0] = __builtin_fma(xv[0], g0, acc[t][0]);
-              acc[t][1] = __builtin_fma(xv[1], g1, acc[t][1]);
+          for (int j = 0; j < 4; j++) g[j] = gn[j];
+          const bool last = step + 1 == steps;
+          if (!last || round + 1 < rounds) fetch(last ? round + 1 : round, last ? 0 : step + 1, gn);
+          const int c = 64 * step + l;
+          if (c < n8)
+#pragma unroll
+            for (int p = 0; p < 4; p++) {
+              f64x2 xv[kT];
+#pragma unroll
+              for (int t = 0; t < kT; t++) xv[t] = xs[t][p][c];
+#pragma unroll
+              for (int j = 0; j < 4; j++) {
+                const double g0 = (double)(float)g[j][2 * p], g1 = (double)(float)g[j][2 * p + 1];
+#pragma unroll
+                for (int t = 0; t < kT; t++) {
+                  acc[t][j][0] = __builtin_fma(xv[t][0], g0, acc[t][j][0]);
+                  acc[t][j][1] = __builtin_fma(xv[t][1], g1, acc[t][j][1]);
+                }
+              }
             }
-          }
         }
 #pragma unroll
-        for (int t = 0; t < kT; t++) {
-          const double v = wave_sum_f64(acc[t][0] + acc[t][1]);
-          if (l == 0) lg[t][e] = h0 ? lg[t][e] + v : v;
+        for (int j = 0; j < 4; j++) {
+          const int e = 4 * kTokWaves * round + kTokWaves * j + w;
+#pragma unroll
+          for (int t = 0; t < kT; t++) {
+            const double v = wave_sum_f64(acc[t][j][0] + acc[t][j][1]);
+            if (l == 0 && e < a.E) lg[t][e] = h0 ? lg[t][e] + v : v;
+          }
         }
       }
     }
@@ -279,16 +302,16 @@ __global__ __launch_bounds__(64 * kTokWaves) void k_route_tok(RouteArgs a) {
 }
 
 // Many tokens: 16 a workgroup on the matrix cores in 64 bits
-// (v_mfma_f64_16x16x4_f64), 16 experts a tile, the 8 waves a part of H each.  A
+// (v_mfma_f64_16x16x4_f64), 16 experts a tile, the 16 waves a part of H each.  A
 // lane's 8 elements of 16 bytes are eight k steps: at step i lane (r, q) holds k =
 // 8q + i of row r, in both operands.
-constexpr int kTileToks = 16, kMfmaWaves = 8;
+constexpr int kTileToks = 16, kMfmaWaves = 16;
 
 __global__ __launch_bounds__(64 * kMfmaWaves) void k_route_mfma(RouteArgs a) {
   constexpr int kTiles = 2;  // of experts at a time
-  __shared__ double part[kMfmaWaves][kTiles][256];
+  __shared__ double part[kMfmaWaves][kTiles][256];  // in the end the waves' choices
   __shared__ double lg[kTileToks][kRouteMaxE];
-  __shared__ double ch[kMfmaWaves][kRouteMaxE];
+  static_assert(kTiles * 256 >= kRouteMaxE, "a wave's choices");
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, r16 = l & 15, q = l >> 4;
   const int s0 = blockIdx.x * kTileToks;
   const int s = s0 + r16 < a.S ? s0 + r16 : a.S - 1;
@@ -301,14 +324,24 @@ __global__ __launch_bounds__(64 * kMfmaWaves) void k_route_mfma(RouteArgs a) {
       const int e = e0 + 16 * t + r16;
       gr[t] = a.gate + (size_t)(e < a.E ? e : a.E - 1) * a.H;
     }
-    for (int i = w; i < n32; i += kMfmaWaves) {
-      const int k = 32 * i + 8 * q;
-      f16x8 x = {}, g[kTiles] = {};
-      if (k < a.H) {
-        x = *(const f16x8*)(a.x + (size_t)s * a.H + k);
+    // (elements past H: the last ones of the row times zeros)
+    auto fetch = [&](int i, f16x8& x, f16x8 (&g)[kTiles]) __attribute__((always_inline)) {
+      const int k0 = 32 * i + 8 * q, k = k0 < a.H ? k0 : a.H - 8;
+      x = *(const f16x8*)(a.x + (size_t)s * a.H + k);
 #pragma unroll
-        for (int t = 0; t < kTiles; t++) g[t] = *(const f16x8*)(gr[t] + k);
+      for (int t = 0; t < kTiles; t++) {
+        g[t] = *(const f16x8*)(gr[t] + k);
+        if (k0 >= a.H) g[t] = f16x8{};
       }
+      if (k0 >= a.H) x = f16x8{};
+    };
+    f16x8 x, g[kTiles], xn, gn[kTiles];
+    fetch(w, xn, gn);
+    for (int i = w; i < n32; i += kMfmaWaves) {
+      x = xn;
+#pragma unroll
+      for (int t = 0; t < kTiles; t++) g[t] = gn[t];
+      fetch(i + kMfmaWaves, xn, gn);
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         const double xv = (double)(float)x[j];
@@ -332,7 +365,7 @@ __global__ __launch_bounds__(64 * kMfmaWaves) void k_route_mfma(RouteArgs a) {
     }
     __syncthreads();
   }
-  for (int t = w; t < kTileToks && s0 + t < a.S; t += kMfmaWaves) choose(a, s0 + t, lg[t], ch[w]);
+  for (int t = w; t < kTileToks && s0 + t < a.S; t += kMfmaWaves) choose(a, s0 + t, lg[t], part[w][0]);
 }
 
 static int route_run(const RouteArgs& a, hipStream_t s) {
