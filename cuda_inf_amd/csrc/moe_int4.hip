@@ -216,6 +216,7 @@ struct Cols {
     return (size_t)((uint64_t)(uint32_t)(n < last ? n : last) * (uint32_t)ng);
   }
   __device__ __forceinline__ const uint8_t* packed(int c) const { return w + row(c) * 64; }
+  __device__ __forceinline__ const uint16_t* scales(int c) const { return s + row(c); }
   // (through a pointer to global memory: the choice of matrix hides where it points)
   __device__ __forceinline__ uint16_t scale(int c, int g) const {
     return ((const __attribute__((address_space(1))) uint16_t*)s)[row(c) + g];
@@ -550,6 +551,225 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void k_moe_tile(MoeArgs a) {
   }
 }
 
+// ---------------------------------------------------------------- streams
+// Few rows an expert: the experts' weights are read once, at the memory's rate,
+// and everything else lies under that.  A workgroup of 8 waves takes a run of
+// column tiles (16 columns) of one expert; its waves split K, each keeping its
+// scale groups' x of up to 16 kMT rows in registers for the whole run, so that
+// x is fetched once a run and a weight passes through one wave only.
+//   W     4 lanes to a column's 64 bytes of a group, as a load is quick (a lane's
+//         16 bytes in a line of its own takes four times as long), kRing tiles
+//         ahead in registers; then through the wave's own LDS into operand order.
+//   sums  a wave's products are scaled in its registers; the 8 waves' sums of
+//         kRing tiles meet in LDS and are added there in the order of the groups.
+// Rows by expert are found by the workgroup itself, from up to kStreamPairs ids:
+// no launch before this one.
+constexpr int kStreamWaves = 8, kStreamPairs = 1024, kStreamGrid = 256;
+constexpr int kStreamMaxK = 8 * 8 * 128;  // 8 groups a wave
+
+// groups a wave -> row tiles that x leaves registers for
+__host__ __device__ constexpr int stream_mt(int kg) { return kg <= 2 ? 4 : (kg <= 4 ? 2 : 1); }
+
+template <bool kUp, int kG>
+struct Stream {
+  static constexpr int kRing = kG <= 2 ? 4 : 2;
+  static constexpr int kMaxMT = stream_mt(kG), kRows = 16 * kMaxMT;
+  static constexpr int kPart = kRing * kMaxMT > 8 ? 16 : 8;  // row tiles x tiles that the LDS holds of each wave
+  struct Lds {
+    f32x4 part[kPart][kStreamWaves][64];
+    u32x4 stage[kStreamWaves][2][64];
+    int cnt[kMoeMaxE], seg[kMoeMaxE];
+    int sum[4], wave[2][kStreamWaves], rows[kRows], expert[2];
+  };
+};
+
+// tiles t0 .. t1 - 1 of expert e for its n rows in L.rows
+template <bool kUp, int kG, int kMT>
+__device__ __forceinline__ void stream_run(const MoeArgs& a, typename Stream<kUp, kG>::Lds& L, int e, int n, int t0, int t1) {
+  using St = Stream<kUp, kG>;
+  constexpr int kRing = St::kRing;
+  constexpr bool kTwo = 2 * kRing * kMT <= St::kPart;  // two batches fit
+  const int tid = threadIdx.x, l = tid & 63, n16 = l & 15, q = l >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int ng = a.K >> 7, g0 = w * ng / kStreamWaves, mine = (w + 1) * ng / kStreamWaves - g0;  // <= kG
+  const Cols<kUp> wc(a, e, (l >> 2) & 1), sc(a, e, n16 & 1);
+  typedef const __attribute__((address_space(1))) uint16_t* gs_t;
+  typedef const __attribute__((address_space(1))) u32x4* gw_t;
+  const uint8_t* wp = wc.packed(16 * t0 + (l >> 2)) + 64 * (size_t)g0 + 16 * (l & 3);
+  const uint16_t* sp = sc.scales(16 * t0 + n16) + g0;
+  const size_t step = (size_t)(kUp ? 8 : 16) * ng;  // groups from a tile to the next
+  u32x4 wr[kRing][kG];
+  uint32_t sr[kRing][kG];
+  auto fetch = [&](int t, int d) __attribute__((always_inline)) {
+    const size_t o = step * (size_t)((t < t1 ? t : t1 - 1) - t0);
+#pragma unroll
+    for (int g = 0; g < kG; g++) {
+      const int gg = g < mine ? g : 0;
+      wr[d][g] = *(gw_t)(wp + 64 * (o + gg));
+      sr[d][g] = *(gs_t)(sp + o + gg);
+    }
+  };
+  if (mine > 0)
+#pragma unroll
+    for (int d = 0; d < kRing; d++) fetch(t0 + d, d);
+  // x of this wave's groups: lane (n16, q) holds row 16 i + n16, k = 32q + 8s .. + 7
+  f16x8 A[kMT][kG][4];
+#pragma unroll
+  for (int i = 0; i < kMT; i++) {
+    const int r = 16 * i + n16;
+    const int p = L.rows[r < n ? r : 0];
+    const uint16_t* xr = a.x + (uint64_t)(uint32_t)(kUp ? p / a.k : p) * (uint32_t)a.K + 128 * g0 + 32 * q;
+#pragma unroll
+    for (int g = 0; g < kG; g++)
+#pragma unroll
+      for (int s = 0; s < 4; s++) {
+        A[i][g][s] = f16x8{};
+        if (r < n && g < mine) A[i][g][s] = *(const f16x8*)(xr + 128 * g + 8 * s);
+      }
+  }
+  for (int tb = t0, batch = 0; tb < t1; tb += kRing, batch++) {
+    f32x4(*part)[kStreamWaves][64] = L.part + (kTwo && (batch & 1) ? kRing * kMT : 0);
+#pragma unroll
+    for (int d = 0; d < kRing; d++) {
+      if (tb + d >= t1) break;
+      f32x4 acc[kMT] = {};
+      if (mine > 0) {
+        float scl[kG];
+#pragma unroll
+        for (int g = 0; g < kG; g++) scl[g] = g < mine ? h2f((uint16_t)sr[d][g]) : 0.f;
+        u32x4 wq[kG];
+#pragma unroll
+        for (int g = 0; g < kG; g++) {
+          u32x4* st = L.stage[w][g & 1];
+          // column l >> 2's chunk l & 3 at chunk ^ (column >> 2) & 3: a read's 16 columns on all banks
+          st[(l & ~3) | ((l & 3) ^ ((l >> 4) & 3))] = wr[d][g];
+          wq[g] = st[4 * n16 + (q ^ ((n16 >> 2) & 3))];
+        }
+        fetch(tb + d + kRing, d);
+#pragma unroll
+        for (int g = 0; g < kG; g++) {
+          f32x4 P[kMT];
+#pragma unroll
+          for (int s = 0; s < 4; s++) {
+            const f16x8 B = nib8(wq[g][s]);
+#pragma unroll
+            for (int i = 0; i < kMT; i++)
+              P[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[i][g][s], B, s == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : P[i], 0, 0, 0);
+          }
+#pragma unroll
+          for (int i = 0; i < kMT; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) acc[i][r] = __builtin_fmaf(P[i][r], scl[g], acc[i][r]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kMT; i++) part[d * kMT + i][w][l] = acc[i];
+    }
+    __syncthreads();
+    // sums of tile d, row tile i: wave d kMT + i, 4 on in every second batch
+#pragma unroll
+    for (int u = 0; u < (kRing * kMT + 7) / 8; u++) {
+      const int it = ((w + (kRing * kMT <= 4 ? 4 * (batch & 1) : 0)) & 7) + 8 * u, d = it / kMT, i = it % kMT;
+      if (it >= kRing * kMT || tb + d >= t1) continue;
+      f32x4 v = {};
+#pragma unroll
+      for (int k = 0; k < kStreamWaves; k++) v += part[it][k][l];
+      const int c = 16 * (tb + d) + n16, r = 16 * i + 4 * q;
+      if constexpr (kUp) {
+        // the even lane takes rows 0 and 1 of the pair's column, the odd one 2, 3
+        const bool odd = n16 & 1;
+        const float o0 = lane_pair(v[0]), o1 = lane_pair(v[1]), o2 = lane_pair(v[2]), o3 = lane_pair(v[3]);
+        const float va = silu_mul(odd ? o2 : v[0], odd ? v[2] : o0), vb = silu_mul(odd ? o3 : v[1], odd ? v[3] : o1);
+        const int ra = r + (odd ? 2 : 0);
+        if (ra < n) a.act[(uint64_t)(uint32_t)L.rows[ra] * (uint32_t)a.N + (c >> 1)] = f2h(va);
+        if (ra + 1 < n) a.act[(uint64_t)(uint32_t)L.rows[ra + 1] * (uint32_t)a.N + (c >> 1)] = f2h(vb);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          if (r + k < n) a.y[(uint64_t)(uint32_t)L.rows[r + k] * (uint32_t)a.N + c] = v[k];
+      }
+    }
+    if (!kTwo) __syncthreads();  // the sums are read
+  }
+}
+
+// grid = kStreamGrid, block = 512; S k <= kStreamPairs, ceil(K / 1024) <= kG
+template <bool kUp, int kG>
+__global__ __launch_bounds__(64 * kStreamWaves) void k_moe_stream(MoeArgs a) {
+  using St = Stream<kUp, kG>;
+  __shared__ typename St::Lds L;
+  const int tid = threadIdx.x, l = tid & 63, w = tid >> 6, P = a.S * a.k;
+  int id[2];
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    const int i = 512 * j + tid;
+    id[j] = i < P ? (a.ids ? a.ids[i] : 0) : -1;
+    if ((unsigned)id[j] >= (unsigned)a.E) id[j] = -1;
+  }
+  if (tid < kMoeMaxE) L.cnt[tid] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 2; j++)
+    if (id[j] >= 0) atomicAdd(&L.cnt[id[j]], 1);
+  __syncthreads();
+  // segments: an expert's rows kRows at a time; expert e's are seg[e] .. + its number - 1
+  const int segs = tid < kMoeMaxE ? (L.cnt[tid] + St::kRows - 1) / St::kRows : 0;
+  int before = segs;
+  if (tid < kMoeMaxE) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int u = __shfl_up(before, d);
+      if (l >= d) before += u;
+    }
+    if (l == 63) L.sum[w] = before;
+  }
+  __syncthreads();
+  before -= segs;
+  if (tid < kMoeMaxE)
+    for (int i = 0; i < w; i++) before += L.sum[i];
+  const int nseg = L.sum[0] + L.sum[1] + L.sum[2] + L.sum[3];
+  // this workgroup's column tiles of all the segments' tiles
+  const int nct = (kUp ? 2 * a.N : a.N) >> 4;
+  const int64_t all = (int64_t)nseg * nct;
+  int64_t u0 = all * blockIdx.x / gridDim.x;
+  const int64_t u1 = all * (blockIdx.x + 1) / gridDim.x;
+  while (u0 < u1) {
+    const int sg = (int)(u0 / nct), t0 = (int)(u0 - (int64_t)sg * nct);
+    const int t1 = u1 - u0 < nct - t0 ? t0 + (int)(u1 - u0) : nct;
+    u0 += t1 - t0;
+    if (segs > 0 && sg >= before && sg < before + segs) {
+      L.expert[0] = tid;
+      L.expert[1] = sg - before;
+    }
+    __syncthreads();
+    const int e = __builtin_amdgcn_readfirstlane(L.expert[0]);
+    const int r0 = __builtin_amdgcn_readfirstlane(L.expert[1]) * St::kRows;
+    // its rows r0 on, in the order of the pairs, the same in every workgroup
+    uint64_t b[2];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      b[j] = __ballot(id[j] == e);
+      if (l == 0) L.wave[j][w] = __popcll(b[j]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      int r = __popcll(b[j] & ((1ull << l) - 1)) - r0;
+      for (int k = 0; k < 8 * j + w; k++) r += L.wave[k >> 3][k & 7];
+      if (id[j] == e && r >= 0 && r < St::kRows) L.rows[r] = 512 * j + tid;
+    }
+    __syncthreads();
+    const int left = L.cnt[e] - r0, n = __builtin_amdgcn_readfirstlane(left < St::kRows ? left : St::kRows);
+    if (St::kMaxMT >= 4 && n > 32)
+      stream_run<kUp, kG, St::kMaxMT >= 4 ? 4 : 1>(a, L, e, n, t0, t1);
+    else if (St::kMaxMT >= 2 && n > 16)
+      stream_run<kUp, kG, St::kMaxMT >= 2 ? 2 : 1>(a, L, e, n, t0, t1);
+    else
+      stream_run<kUp, kG, 1>(a, L, e, n, t0, t1);
+    __syncthreads();  // the sums and rows are read
+  }
+}
+
 // ---------------------------------------------------------------- combine
 struct CombineArgs {
   const float* y;
@@ -619,12 +839,31 @@ static void set_w(MoeArgs& a, int i, const cia_q4_experts* w) {
   a.sstride[i] = w->scales_stride;
 }
 
+// Whether the weights are streamed rather than multiplied in tiles: while the
+// rows of an expert, on average over those that can have any, are few.
+static bool streams(int64_t P, int E, int K) {
+  return P <= kStreamPairs && K <= kStreamMaxK && P <= 48 * (int64_t)E;
+}
+
 template <bool kUp>
 static int products(MoeArgs& a, void* ws, hipStream_t s) {
-  constexpr int kNT = 3;
   const int P = a.S * a.k;
+  if (streams(P, a.E, a.K)) {
+    const int kg = (a.K + 1023) / 1024;
+    const dim3 grid(kStreamGrid), block(64 * kStreamWaves);
+    if (kg <= 1)
+      hipLaunchKernelGGL((k_moe_stream<kUp, 1>), grid, block, 0, s, a);
+    else if (kg <= 2)
+      hipLaunchKernelGGL((k_moe_stream<kUp, 2>), grid, block, 0, s, a);
+    else if (kg <= 4)
+      hipLaunchKernelGGL((k_moe_stream<kUp, 4>), grid, block, 0, s, a);
+    else
+      hipLaunchKernelGGL((k_moe_stream<kUp, 8>), grid, block, 0, s, a);
+    return launch_status();
+  }
+  constexpr int kNT = 3;
   a.plan = (const int*)ws;
-  hipLaunchKernelGGL(k_moe_plan, dim3(1), dim3(1024), 0, s, a.ids, P, a.E, (int*)ws);
+  hipLaunchKernelGGL(k_moe_plan, dim3(1), dim3(kPlanThreads), 0, s, a.ids, P, a.E, (int*)ws);
   const int nv = kUp ? 2 * a.N : a.N, cols = 16 * kNT * kTileWaves;
   const int64_t tiles = max_tiles(P, a.E) * ((nv + cols - 1) / cols) * a.splits;
   hipLaunchKernelGGL((k_moe_tile<kUp, kNT>), dim3((unsigned)((tiles + 7) / 8 * 8 + 8)), dim3(64 * kTileWaves), 0, s, a);
@@ -689,7 +928,7 @@ extern "C" int cia_moe_down_int4(const uint16_t* act, const int32_t* ids, const 
   a.k = k;
   a.E = E;
   a.y = (float*)((char*)ws + plan_bytes((int64_t)S * k, E));
-  a.splits = k_splits((int64_t)S * k, E, H, F);
+  a.splits = streams((int64_t)S * k, E, F) ? 1 : k_splits((int64_t)S * k, E, H, F);
   hipStream_t s = (hipStream_t)stream;
   if ((st = products<false>(a, ws, s))) return st;
   const CombineArgs c{a.y, ids, weights, res, out, S, k, E, H, a.splits};
