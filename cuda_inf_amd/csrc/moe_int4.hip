@@ -693,12 +693,62 @@ __device__ __forceinline__ void stream_run(const MoeArgs& a, typename Stream<kUp
   }
 }
 
+template <bool kUp, int kG>
+__device__ __forceinline__ void stream_rows(const MoeArgs& a, typename Stream<kUp, kG>::Lds& L, int e, int n, int t0, int t1) {
+  constexpr int kMax = Stream<kUp, kG>::kMaxMT;
+  if (kMax >= 4 && n > 32)
+    stream_run<kUp, kG, kMax >= 4 ? 4 : 1>(a, L, e, n, t0, t1);
+  else if (kMax >= 2 && n > 16)
+    stream_run<kUp, kG, kMax >= 2 ? 2 : 1>(a, L, e, n, t0, t1);
+  else
+    stream_run<kUp, kG, 1>(a, L, e, n, t0, t1);
+  __syncthreads();  // the sums and rows are read
+}
+
 // grid = kStreamGrid, block = 512; S k <= kStreamPairs, ceil(K / 1024) <= kG
 template <bool kUp, int kG>
 __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_stream(MoeArgs a) {
   using St = Stream<kUp, kG>;
   __shared__ typename St::Lds L;
   const int tid = threadIdx.x, l = tid & 63, w = tid >> 6, P = a.S * a.k;
+  const int nct = (kUp ? 2 * a.N : a.N) >> 4;
+  // Segments: an expert's rows kRows at a time, in the order of the pairs, the same
+  // in every workgroup.  Each takes an equal run of all the segments' column tiles.
+  if (P <= 64) {
+    // every wave finds its own, lane i with pair i, and waits for no other
+    int id = l < P ? (a.ids ? a.ids[l] : 0) : -1;
+    if ((unsigned)id >= (unsigned)a.E) id = -1;
+    uint64_t same = __ballot(id >= 0);
+#pragma unroll
+    for (int b = 0; b < 8; b++) {
+      const uint64_t v = __ballot(id >> b & 1);
+      same &= id >> b & 1 ? v : ~v;
+    }
+    const uint64_t below = (1ull << l) - 1;
+    const bool first = id >= 0 && !(same & below);  // of its expert
+    const int segs = first ? (__popcll(same) + St::kRows - 1) / St::kRows : 0;
+    int before = 0, nseg = 0;
+#pragma unroll
+    for (int k = 1; k <= 64 / St::kRows; k++) {
+      const uint64_t v = __ballot(segs >= k);
+      before += __popcll(v & below);
+      nseg += __popcll(v);
+    }
+    int u0 = (int)((int64_t)nseg * nct * blockIdx.x / gridDim.x);
+    const int u1 = (int)((int64_t)nseg * nct * (blockIdx.x + 1) / gridDim.x);
+    while (u0 < u1) {
+      const int sg = u0 / nct, t0 = u0 - sg * nct, t1 = u1 - u0 < nct - t0 ? t0 + (u1 - u0) : nct;
+      u0 += t1 - t0;
+      const int at = __builtin_ctzll(__ballot(segs > 0 && sg >= before && sg < before + segs));
+      const int e = __builtin_amdgcn_readlane(id, at);
+      const int r0 = (sg - __builtin_amdgcn_readlane(before, at)) * St::kRows;
+      const uint64_t rows = __ballot(id == e);
+      const int r = __popcll(rows & below) - r0, left = __popcll(rows) - r0;
+      if (id == e && r >= 0 && r < St::kRows) L.rows[r] = l;  // (all waves the same)
+      stream_rows<kUp, kG>(a, L, e, left < St::kRows ? left : St::kRows, t0, t1);
+    }
+    return;
+  }
   int id[2];
 #pragma unroll
   for (int j = 0; j < 2; j++) {
@@ -712,7 +762,6 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_stream(MoeArgs a) {
   for (int j = 0; j < 2; j++)
     if (id[j] >= 0) atomicAdd(&L.cnt[id[j]], 1);
   __syncthreads();
-  // segments: an expert's rows kRows at a time; expert e's are seg[e] .. + its number - 1
   const int segs = tid < kMoeMaxE ? (L.cnt[tid] + St::kRows - 1) / St::kRows : 0;
   int before = segs;
   if (tid < kMoeMaxE) {
@@ -727,10 +776,7 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_stream(MoeArgs a) {
   before -= segs;
   if (tid < kMoeMaxE)
     for (int i = 0; i < w; i++) before += L.sum[i];
-  const int nseg = L.sum[0] + L.sum[1] + L.sum[2] + L.sum[3];
-  // this workgroup's column tiles of all the segments' tiles
-  const int nct = (kUp ? 2 * a.N : a.N) >> 4;
-  const int64_t all = (int64_t)nseg * nct;
+  const int64_t all = (int64_t)(L.sum[0] + L.sum[1] + L.sum[2] + L.sum[3]) * nct;
   int64_t u0 = all * blockIdx.x / gridDim.x;
   const int64_t u1 = all * (blockIdx.x + 1) / gridDim.x;
   while (u0 < u1) {
@@ -744,7 +790,6 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_stream(MoeArgs a) {
     __syncthreads();
     const int e = __builtin_amdgcn_readfirstlane(L.expert[0]);
     const int r0 = __builtin_amdgcn_readfirstlane(L.expert[1]) * St::kRows;
-    // its rows r0 on, in the order of the pairs, the same in every workgroup
     uint64_t b[2];
 #pragma unroll
     for (int j = 0; j < 2; j++) {
@@ -760,13 +805,7 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_stream(MoeArgs a) {
     }
     __syncthreads();
     const int left = L.cnt[e] - r0, n = __builtin_amdgcn_readfirstlane(left < St::kRows ? left : St::kRows);
-    if (St::kMaxMT >= 4 && n > 32)
-      stream_run<kUp, kG, St::kMaxMT >= 4 ? 4 : 1>(a, L, e, n, t0, t1);
-    else if (St::kMaxMT >= 2 && n > 16)
-      stream_run<kUp, kG, St::kMaxMT >= 2 ? 2 : 1>(a, L, e, n, t0, t1);
-    else
-      stream_run<kUp, kG, 1>(a, L, e, n, t0, t1);
-    __syncthreads();  // the sums and rows are read
+    stream_rows<kUp, kG>(a, L, e, n, t0, t1);
   }
 }
 

@@ -307,10 +307,10 @@ def q4_experts(w, name: str):
             raise ValueError(f"{name}{part}: must be a device tensor")
         if t.dtype not in dtypes:
             raise TypeError(f"{name}{part}: dtype {t.dtype} not in {dtypes}")
-        if t.shape[0] and not t[0].is_contiguous():
+        if t.stride()[1:] != (t.shape[2], 1):
             raise ValueError(f"{name}{part}: an expert must be contiguous")
     E, rows, half = packed.shape
-    if half % 64 or tuple(scales.shape) != (E, rows, half // 64):
+    if half % 64 or scales.shape != (E, rows, half // 64):
         raise ValueError(f"{name}: packed {tuple(packed.shape)} and scales {tuple(scales.shape)} do not fit: "
                          "[E, rows, cols / 2] and [E, rows, cols / 128], cols a multiple of 128")
     return (_lib.cia_q4_experts(packed.data_ptr(), scales.data_ptr(), packed.stride(0), scales.stride(0)),
