@@ -564,34 +564,38 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void k_moe_tile(MoeArgs a) {
 //         kRing tiles meet in LDS and are added there in the order of the groups.
 // Rows by expert are found by the workgroup itself, from up to kStreamPairs ids:
 // no launch before this one.
-constexpr int kStreamWaves = 8, kStreamPairs = 1024, kStreamGrid = 256;
-constexpr int kStreamMaxK = 8 * 8 * 128;  // 8 groups a wave
+constexpr int kStreamWaves = 8, kStreamPairs = 1024, kUnits = 256;  // compute units
+constexpr int kStreamMaxK = 4 * 8 * 128;  // 4 groups a wave, of one part of K
 
 // groups a wave -> row tiles that x leaves registers for
-__host__ __device__ constexpr int stream_mt(int kg) { return kg <= 2 ? 4 : (kg <= 4 ? 2 : 1); }
+__host__ __device__ constexpr int stream_mt(int kg) { return kg <= 2 ? 4 : 2; }
 
-template <bool kUp, int kG>
+template <int kG, int kMT>
 struct Stream {
   static constexpr int kRing = kG <= 2 ? 4 : 2;
-  static constexpr int kMaxMT = stream_mt(kG), kRows = 16 * kMaxMT;
-  static constexpr int kPart = kRing * kMaxMT > 8 ? 16 : 8;  // row tiles x tiles that the LDS holds of each wave
+  static constexpr int kMaxMT = kMT, kRows = 16 * kMT;
+  // row tiles x tiles that the LDS holds of each wave; operand slots of a wave
+  static constexpr int kPart = kRing * kMT > 8 ? 16 : 8, kStage = kMT == 1 ? 1 : 2;
+  // 16 rows: registers and LDS for two workgroups a compute unit
+  static constexpr int kPerUnit = kMT == 1 && kG <= 2 ? 2 : 1;
   struct Lds {
     f32x4 part[kPart][kStreamWaves][64];
-    u32x4 stage[kStreamWaves][2][64];
+    u32x4 stage[kStreamWaves][kStage][64];
     int cnt[kMoeMaxE], seg[kMoeMaxE];
     int sum[4], wave[2][kStreamWaves], rows[kRows], expert[2];
   };
 };
 
-// tiles t0 .. t1 - 1 of expert e for its n rows in L.rows
-template <bool kUp, int kG, int kMT>
-__device__ __forceinline__ void stream_run(const MoeArgs& a, typename Stream<kUp, kG>::Lds& L, int e, int n, int t0, int t1) {
-  using St = Stream<kUp, kG>;
+// tiles t0 .. t1 - 1 of expert e, part part_k of K, for its n rows in L.rows
+template <bool kUp, int kG, int kMT, class St>
+__device__ __forceinline__ void stream_run(const MoeArgs& a, typename St::Lds& L, int e, int part_k, int n, int t0, int t1) {
   constexpr int kRing = St::kRing;
   constexpr bool kTwo = 2 * kRing * kMT <= St::kPart;  // two batches fit
   const int tid = threadIdx.x, l = tid & 63, n16 = l & 15, q = l >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int ng = a.K >> 7, g0 = w * ng / kStreamWaves, mine = (w + 1) * ng / kStreamWaves - g0;  // <= kG
+  const int ng = a.K >> 7, k0 = kUp ? 0 : ng * part_k / a.splits, nk = (kUp ? ng : ng * (part_k + 1) / a.splits) - k0;
+  const int g0 = k0 + w * nk / kStreamWaves, mine = k0 + (w + 1) * nk / kStreamWaves - g0;  // <= kG
+  float* const y = kUp ? nullptr : a.y + (size_t)part_k * a.S * a.k * a.N;
   const Cols<kUp> wc(a, e, (l >> 2) & 1), sc(a, e, n16 & 1);
   typedef const __attribute__((address_space(1))) uint16_t* gs_t;
   typedef const __attribute__((address_space(1))) u32x4* gw_t;
@@ -640,7 +644,7 @@ __device__ __forceinline__ void stream_run(const MoeArgs& a, typename Stream<kUp
         u32x4 wq[kG];
 #pragma unroll
         for (int g = 0; g < kG; g++) {
-          u32x4* st = L.stage[w][g & 1];
+          u32x4* st = L.stage[w][g % St::kStage];
           // column l >> 2's chunk l & 3 at chunk ^ (column >> 2) & 3: a read's 16 columns on all banks
           st[(l & ~3) | ((l & 3) ^ ((l >> 4) & 3))] = wr[d][g];
           wq[g] = st[4 * n16 + (q ^ ((n16 >> 2) & 3))];
@@ -686,32 +690,32 @@ __device__ __forceinline__ void stream_run(const MoeArgs& a, typename Stream<kUp
       } else {
 #pragma unroll
         for (int k = 0; k < 4; k++)
-          if (r + k < n) a.y[(uint64_t)(uint32_t)L.rows[r + k] * (uint32_t)a.N + c] = v[k];
+          if (r + k < n) y[(uint64_t)(uint32_t)L.rows[r + k] * (uint32_t)a.N + c] = v[k];
       }
     }
     if (!kTwo) __syncthreads();  // the sums are read
   }
 }
 
-template <bool kUp, int kG>
-__device__ __forceinline__ void stream_rows(const MoeArgs& a, typename Stream<kUp, kG>::Lds& L, int e, int n, int t0, int t1) {
-  constexpr int kMax = Stream<kUp, kG>::kMaxMT;
+template <bool kUp, int kG, class St>
+__device__ __forceinline__ void stream_rows(const MoeArgs& a, typename St::Lds& L, int e, int part_k, int n, int t0, int t1) {
+  constexpr int kMax = St::kMaxMT;
   if (kMax >= 4 && n > 32)
-    stream_run<kUp, kG, kMax >= 4 ? 4 : 1>(a, L, e, n, t0, t1);
+    stream_run<kUp, kG, kMax >= 4 ? 4 : 1, St>(a, L, e, part_k, n, t0, t1);
   else if (kMax >= 2 && n > 16)
-    stream_run<kUp, kG, kMax >= 2 ? 2 : 1>(a, L, e, n, t0, t1);
+    stream_run<kUp, kG, kMax >= 2 ? 2 : 1, St>(a, L, e, part_k, n, t0, t1);
   else
-    stream_run<kUp, kG, 1>(a, L, e, n, t0, t1);
+    stream_run<kUp, kG, 1, St>(a, L, e, part_k, n, t0, t1);
   __syncthreads();  // the sums and rows are read
 }
 
-// grid = kStreamGrid, block = 512; S k <= kStreamPairs, ceil(K / 1024) <= kG
-template <bool kUp, int kG>
-__global__ __launch_bounds__(64 * kStreamWaves) void k_moe_stream(MoeArgs a) {
-  using St = Stream<kUp, kG>;
+// grid = any, block = 512; S k <= kStreamPairs, a part of K at most 1024 kG
+template <bool kUp, int kG, int kMT>
+__global__ __launch_bounds__(64 * kStreamWaves, (2 * Stream<kG, kMT>::kPerUnit)) void k_moe_stream(MoeArgs a) {
+  using St = Stream<kG, kMT>;
   __shared__ typename St::Lds L;
   const int tid = threadIdx.x, l = tid & 63, w = tid >> 6, P = a.S * a.k;
-  const int nct = (kUp ? 2 * a.N : a.N) >> 4;
+  const int nct = (kUp ? 2 * a.N : a.N) >> 4, parts = kUp ? 1 : a.splits;
   // Segments: an expert's rows kRows at a time, in the order of the pairs, the same
   // in every workgroup.  Each takes an equal run of all the segments' column tiles.
   if (P <= 64) {
@@ -734,18 +738,21 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_stream(MoeArgs a) {
       before += __popcll(v & below);
       nseg += __popcll(v);
     }
-    int u0 = (int)((int64_t)nseg * nct * blockIdx.x / gridDim.x);
-    const int u1 = (int)((int64_t)nseg * nct * (blockIdx.x + 1) / gridDim.x);
+    int u0 = (int)((int64_t)nseg * parts * nct * blockIdx.x / gridDim.x);
+    const int u1 = (int)((int64_t)nseg * parts * nct * (blockIdx.x + 1) / gridDim.x);
     while (u0 < u1) {
-      const int sg = u0 / nct, t0 = u0 - sg * nct, t1 = u1 - u0 < nct - t0 ? t0 + (u1 - u0) : nct;
+      int sg = u0 / nct;
+      const int t0 = u0 - sg * nct, t1 = u1 - u0 < nct - t0 ? t0 + (u1 - u0) : nct;
       u0 += t1 - t0;
+      const int part_k = sg % parts;
+      sg /= parts;
       const int at = __builtin_ctzll(__ballot(segs > 0 && sg >= before && sg < before + segs));
       const int e = __builtin_amdgcn_readlane(id, at);
       const int r0 = (sg - __builtin_amdgcn_readlane(before, at)) * St::kRows;
       const uint64_t rows = __ballot(id == e);
       const int r = __popcll(rows & below) - r0, left = __popcll(rows) - r0;
       if (id == e && r >= 0 && r < St::kRows) L.rows[r] = l;  // (all waves the same)
-      stream_rows<kUp, kG>(a, L, e, left < St::kRows ? left : St::kRows, t0, t1);
+      stream_rows<kUp, kG, St>(a, L, e, part_k, left < St::kRows ? left : St::kRows, t0, t1);
     }
     return;
   }
@@ -776,13 +783,15 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_stream(MoeArgs a) {
   before -= segs;
   if (tid < kMoeMaxE)
     for (int i = 0; i < w; i++) before += L.sum[i];
-  const int64_t all = (int64_t)(L.sum[0] + L.sum[1] + L.sum[2] + L.sum[3]) * nct;
+  const int64_t all = (int64_t)(L.sum[0] + L.sum[1] + L.sum[2] + L.sum[3]) * parts * nct;
   int64_t u0 = all * blockIdx.x / gridDim.x;
   const int64_t u1 = all * (blockIdx.x + 1) / gridDim.x;
   while (u0 < u1) {
-    const int sg = (int)(u0 / nct), t0 = (int)(u0 - (int64_t)sg * nct);
-    const int t1 = u1 - u0 < nct - t0 ? t0 + (int)(u1 - u0) : nct;
+    int sg = (int)(u0 / nct);
+    const int t0 = (int)(u0 - (int64_t)sg * nct), t1 = u1 - u0 < nct - t0 ? t0 + (int)(u1 - u0) : nct;
     u0 += t1 - t0;
+    const int part_k = sg % parts;
+    sg /= parts;
     if (segs > 0 && sg >= before && sg < before + segs) {
       L.expert[0] = tid;
       L.expert[1] = sg - before;
@@ -805,7 +814,7 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_stream(MoeArgs a) {
     }
     __syncthreads();
     const int left = L.cnt[e] - r0, n = __builtin_amdgcn_readfirstlane(left < St::kRows ? left : St::kRows);
-    stream_rows<kUp, kG>(a, L, e, n, t0, t1);
+    stream_rows<kUp, kG, St>(a, L, e, part_k, n, t0, t1);
   }
 }
 
@@ -880,24 +889,34 @@ static void set_w(MoeArgs& a, int i, const cia_q4_experts* w) {
 
 // Whether the weights are streamed rather than multiplied in tiles: while the
 // rows of an expert, on average over those that can have any, are few.
-static bool streams(int64_t P, int E, int K) {
-  return P <= kStreamPairs && K <= kStreamMaxK && P <= 48 * (int64_t)E;
+// (down takes a K of two parts as well)
+static bool streams(bool up, int64_t P, int E, int K) {
+  return P <= kStreamPairs && K <= (up ? 1 : 2) * kStreamMaxK && P <= 48 * (int64_t)E;
+}
+
+// 16 rows at a time with two workgroups a compute unit where experts hardly have
+// more
+template <bool kUp, int kG>
+static void stream_launch(const MoeArgs& a, hipStream_t s) {
+  constexpr int kMT = stream_mt(kG);
+  const dim3 block(64 * kStreamWaves);
+  if ((int64_t)a.S * a.k <= 8 * (int64_t)a.E)
+    hipLaunchKernelGGL((k_moe_stream<kUp, kG, 1>), dim3(kUnits * Stream<kG, 1>::kPerUnit), block, 0, s, a);
+  else
+    hipLaunchKernelGGL((k_moe_stream<kUp, kG, kMT>), dim3(kUnits), block, 0, s, a);
 }
 
 template <bool kUp>
 static int products(MoeArgs& a, void* ws, hipStream_t s) {
   const int P = a.S * a.k;
-  if (streams(P, a.E, a.K)) {
-    const int kg = (a.K + 1023) / 1024;
-    const dim3 grid(kStreamGrid), block(64 * kStreamWaves);
-    if (kg <= 1)
-      hipLaunchKernelGGL((k_moe_stream<kUp, 1>), grid, block, 0, s, a);
-    else if (kg <= 2)
-      hipLaunchKernelGGL((k_moe_stream<kUp, 2>), grid, block, 0, s, a);
-    else if (kg <= 4)
-      hipLaunchKernelGGL((k_moe_stream<kUp, 4>), grid, block, 0, s, a);
+  if (streams(kUp, P, a.E, a.K)) {
+    const int part = ((a.K >> 7) + a.splits - 1) / a.splits;  // groups
+    if (part <= 8)
+      stream_launch<kUp, 1>(a, s);
+    else if (part <= 16)
+      stream_launch<kUp, 2>(a, s);
     else
-      hipLaunchKernelGGL((k_moe_stream<kUp, 8>), grid, block, 0, s, a);
+      stream_launch<kUp, 4>(a, s);
     return launch_status();
   }
   constexpr int kNT = 3;
@@ -967,7 +986,7 @@ extern "C" int cia_moe_down_int4(const uint16_t* act, const int32_t* ids, const 
   a.k = k;
   a.E = E;
   a.y = (float*)((char*)ws + plan_bytes((int64_t)S * k, E));
-  a.splits = streams((int64_t)S * k, E, F) ? 1 : k_splits((int64_t)S * k, E, H, F);
+  a.splits = streams(false, (int64_t)S * k, E, F) ? (F + kStreamMaxK - 1) / kStreamMaxK : k_splits((int64_t)S * k, E, H, F);
   hipStream_t s = (hipStream_t)stream;
   if ((st = products<false>(a, ws, s))) return st;
   const CombineArgs c{a.y, ids, weights, res, out, S, k, E, H, a.splits};
