@@ -818,6 +818,162 @@ __global__ __launch_bounds__(64 * kStreamWaves, (2 * Stream<kG, kMT>::kPerUnit))
   }
 }
 
+// Down for up to kFewPairs pairs: a workgroup takes 16 columns of out through all
+// the experts that have a row, so that it can weight the rows and add them to the
+// residual itself, and no launch follows.  The waves split K as above, the weights
+// of the next kRing segments in flight; 8 segments' sums meet at a time.
+// (1 token, 4 of 32 experts of 1792: 5.3 us and 2.4 for the rows' sum so far.)
+constexpr int kFewPairs = 64;
+
+struct FewArgs {
+  MoeArgs m;
+  const float* weights;  // or null: 1
+  const float* res;
+  float* out;
+};
+
+// grid = N / 16, block = 512; K <= 1024 kG
+template <int kG>
+__global__ __launch_bounds__(64 * kStreamWaves) void k_moe_few(FewArgs f) {
+  constexpr int kRing = kG <= 2 ? 4 : 2, kBatch = 8;
+  const MoeArgs& a = f.m;
+  __shared__ f32x4 part[kBatch][kStreamWaves][64];
+  __shared__ u32x4 stage[kStreamWaves][2][64];
+  __shared__ float sums[kFewPairs][16];
+  __shared__ int rows[kStreamWaves][2 * kBatch][16];
+  const int tid = threadIdx.x, l = tid & 63, n16 = l & 15, q = l >> 4, P = a.S * a.k;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c0 = 16 * blockIdx.x;
+  // the rows by expert, 16 a segment, as in k_moe_stream
+  int id = l < P ? (a.ids ? a.ids[l] : 0) : -1;
+  if ((unsigned)id >= (unsigned)a.E) id = -1;
+  // this thread's outputs: column tid & 15 of tokens (tid >> 4) and 32 on
+  float old[2], wt = l < P && f.weights ? f.weights[l] : 1.0f;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int s = 32 * i + (tid >> 4);
+    old[i] = f.res[(size_t)(s < a.S ? s : 0) * a.N + c0 + (tid & 15)];
+  }
+  uint64_t same = __ballot(id >= 0);
+  const uint64_t live = same;
+#pragma unroll
+  for (int b = 0; b < 8; b++) {
+    const uint64_t v = __ballot(id >> b & 1);
+    same &= id >> b & 1 ? v : ~v;
+  }
+  const uint64_t below = (1ull << l) - 1;
+  const int segs = id >= 0 && !(same & below) ? (__popcll(same) + 15) >> 4 : 0;
+  int before = 0, nseg = 0;
+#pragma unroll
+  for (int k = 1; k <= kFewPairs / 16; k++) {
+    const uint64_t v = __ballot(segs >= k);
+    before += __popcll(v & below);
+    nseg += __popcll(v);
+  }
+  const int ng = a.K >> 7, g0 = w * ng / kStreamWaves, mine = (w + 1) * ng / kStreamWaves - g0;
+  typedef const __attribute__((address_space(1))) uint16_t* gs_t;
+  typedef const __attribute__((address_space(1))) u32x4* gw_t;
+  u32x4 wr[kRing][kG];
+  uint32_t sr[kRing][kG];
+  // segment sg's expert and its first row's place among the expert's
+  auto expert = [&](int sg, int& r0) __attribute__((always_inline)) {
+    const int at = __builtin_ctzll(__ballot(segs > 0 && sg >= before && sg < before + segs));
+    r0 = (sg - __builtin_amdgcn_readlane(before, at)) * 16;
+    return __builtin_amdgcn_readlane(id, at);
+  };
+  // its weights, scales and x rows of this wave's groups
+  f16x8 A[kRing][kG][4];
+  auto fetch = [&](int sg, int d) __attribute__((always_inline)) {
+    if (sg >= nseg) return;
+    int r0;
+    const int e = expert(sg, r0);
+    const uint64_t m = __ballot(id == e);
+    const int r = __popcll(m & below) - r0;
+    int* const list = rows[w][sg % (2 * kBatch)];
+    if (id == e && r >= 0 && r < 16) list[r] = l;
+    if (mine == 0) return;
+    const Cols<false> col(a, e, false);
+    const gw_t wp = (gw_t)(col.packed(c0 + (l >> 2)) + 64 * (size_t)g0 + 16 * (l & 3));
+    const gs_t sp = (gs_t)(col.scales(c0 + n16) + g0);
+#pragma unroll
+    for (int g = 0; g < kG; g++) {
+      const int gg = g < mine ? g : 0;
+      wr[d][g] = wp[4 * gg];
+      sr[d][g] = sp[gg];
+    }
+    // (rows past the last one: the first, its products are not read)
+    const int p = list[n16 < __popcll(m) - r0 ? n16 : 0];
+    const gw_t xr = (gw_t)(a.x + (uint64_t)(uint32_t)p * (uint32_t)a.K + 128 * g0 + 32 * q);
+    if (n16 < __popcll(m) - r0)
+#pragma unroll
+      for (int g = 0; g < kG; g++)
+#pragma unroll
+        for (int s = 0; s < 4; s++) A[d][g][s] = __builtin_bit_cast(f16x8, xr[16 * (g < mine ? g : 0) + s]);
+  };
+#pragma unroll
+  for (int d = 0; d < kRing; d++) {
+#pragma unroll
+    for (int g = 0; g < kG; g++)
+#pragma unroll
+      for (int s = 0; s < 4; s++) A[d][g][s] = f16x8{};
+    fetch(d, d);
+  }
+  for (int sb = 0; sb < nseg; sb += kBatch) {
+#pragma unroll
+    for (int b = 0; b < kBatch; b++) {
+      const int sg = sb + b, d = b % kRing;
+      if (sg >= nseg) break;
+      f32x4 acc = {};
+      if (mine > 0) {
+        u32x4 wq[kG];
+        float scl[kG];
+#pragma unroll
+        for (int g = 0; g < kG; g++) {
+          u32x4* st = stage[w][g & 1];
+          st[(l & ~3) | ((l & 3) ^ ((l >> 4) & 3))] = wr[d][g];
+          wq[g] = st[4 * n16 + (q ^ ((n16 >> 2) & 3))];
+          scl[g] = g < mine ? h2f((uint16_t)sr[d][g]) : 0.f;
+        }
+#pragma unroll
+        for (int g = 0; g < kG; g++) {
+          f32x4 Pg = {};
+#pragma unroll
+          for (int s = 0; s < 4; s++) Pg = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[d][g][s], nib8(wq[g][s]), Pg, 0, 0, 0);
+          if (g < mine)
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[i] = __builtin_fmaf(Pg[i], scl[g], acc[i]);
+        }
+      }
+      fetch(sg + kRing, d);
+      part[b][w][l] = acc;
+    }
+    __syncthreads();
+    // wave b adds up segment sb + b (its own list of its rows)
+    if (sb + w < nseg) {
+      f32x4 v = {};
+#pragma unroll
+      for (int k = 0; k < kStreamWaves; k++) v += part[w][k][l];
+      int r0;
+      const int e = expert(sb + w, r0), left = __popcll(__ballot(id == e)) - r0;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (4 * q + i < left) sums[rows[w][(sb + w) % (2 * kBatch)][4 * q + i]][n16] = v[i];
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int s = 32 * i + (tid >> 4);
+    float v = old[i];
+    for (int j = 0; j < a.k; j++) {
+      const int p = s < a.S ? s * a.k + j : 0;
+      const float wp = __shfl(wt, p);
+      if (live >> p & 1) v = __builtin_fmaf(wp, sums[p][tid & 15], v);
+    }
+    if (s < a.S) f.out[(size_t)s * a.N + c0 + (tid & 15)] = v;
+  }
+}
+
 // ---------------------------------------------------------------- combine
 struct CombineArgs {
   const float* y;
@@ -887,11 +1043,16 @@ static void set_w(MoeArgs& a, int i, const cia_q4_experts* w) {
   a.sstride[i] = w->scales_stride;
 }
 
-// Whether the weights are streamed rather than multiplied in tiles: while the
-// rows of an expert, on average over those that can have any, are few.
-// (down takes a K of two parts as well)
+// Whether the weights are streamed rather than multiplied in tiles: up to 8 rows
+// an expert on average, or few pairs at all.  Calls in us, streamed / in tiles:
+// 4 of 32 experts of 1792, H = 2048, 40 tokens up 31 / 34, down 26.5 / 28.1; 64
+// 37 / 41, 31.6 / 32.9; 100 49 / 45, 37.6 / 34.7.  2 of 8 of 2048, H = 1024, 64
+// tokens 15.2 / 18.9, 19.4 / 19.4; 100 17.8 / 21.1, 24.7 / 21.2; 256 25.0 / 26.5,
+// 34 / 26.  The dense form of 7168, H = 2048, 128 rows 23 / 36, 22 / 28; 256 31 /
+// 38, 29 / 30; 400 54 / 41, 48 / 39.  (Down takes a K of two parts as well.)
 static bool streams(bool up, int64_t P, int E, int K) {
-  return P <= kStreamPairs && K <= (up ? 1 : 2) * kStreamMaxK && P <= 48 * (int64_t)E;
+  const int64_t few = up ? 256 : 128;
+  return P <= kStreamPairs && K <= (up ? 1 : 2) * kStreamMaxK && (P <= 8 * (int64_t)E || P <= few);
 }
 
 // 16 rows at a time with two workgroups a compute unit where experts hardly have
@@ -900,8 +1061,13 @@ template <bool kUp, int kG>
 static void stream_launch(const MoeArgs& a, hipStream_t s) {
   constexpr int kMT = stream_mt(kG);
   const dim3 block(64 * kStreamWaves);
-  if ((int64_t)a.S * a.k <= 8 * (int64_t)a.E)
-    hipLaunchKernelGGL((k_moe_stream<kUp, kG, 1>), dim3(kUnits * Stream<kG, 1>::kPerUnit), block, 0, s, a);
+  const int64_t P = (int64_t)a.S * a.k;
+  if (P <= 8 * (int64_t)a.E) {
+    // (as many workgroups as tiles to take 4 of)
+    const int64_t tiles = (P < a.E ? P : a.E) * ((kUp ? 2 * a.N : a.N) >> 4) * (kUp ? 1 : a.splits);
+    const int n = tiles <= 4 * kUnits ? kUnits : kUnits * Stream<kG, 1>::kPerUnit;
+    hipLaunchKernelGGL((k_moe_stream<kUp, kG, 1>), dim3(n), block, 0, s, a);
+  }
   else
     hipLaunchKernelGGL((k_moe_stream<kUp, kG, kMT>), dim3(kUnits), block, 0, s, a);
 }
@@ -988,6 +1154,17 @@ extern "C" int cia_moe_down_int4(const uint16_t* act, const int32_t* ids, const 
   a.y = (float*)((char*)ws + plan_bytes((int64_t)S * k, E));
   a.splits = streams(false, (int64_t)S * k, E, F) ? (F + kStreamMaxK - 1) / kStreamMaxK : k_splits((int64_t)S * k, E, H, F);
   hipStream_t s = (hipStream_t)stream;
+  if (S * (int64_t)k <= kFewPairs && F <= kStreamMaxK) {
+    const FewArgs f{a, weights, res, out};
+    const dim3 grid((unsigned)(H / 16)), block(64 * kStreamWaves);
+    if (F <= 1024)
+      hipLaunchKernelGGL(k_moe_few<1>, grid, block, 0, s, f);
+    else if (F <= 2048)
+      hipLaunchKernelGGL(k_moe_few<2>, grid, block, 0, s, f);
+    else
+      hipLaunchKernelGGL(k_moe_few<4>, grid, block, 0, s, f);
+    return launch_status();
+  }
   if ((st = products<false>(a, ws, s))) return st;
   const CombineArgs c{a.y, ids, weights, res, out, S, k, E, H, a.splits};
   hipLaunchKernelGGL(k_moe_combine, dim3((unsigned)((H + 1023) / 1024) * (unsigned)S), dim3(256), 0, s, c);

@@ -300,21 +300,26 @@ def q4_experts(w, name: str):
     [E, rows, cols / 2], scales fp16 [E, rows, cols / 128]) on the device.  Each
     expert is contiguous; the experts may lie apart, at one stride."""
     packed, scales = w
-    for t, part, dtypes in ((packed, ".packed", (torch.uint8,)), (scales, ".scales", _F16)):
-        if not isinstance(t, torch.Tensor) or t.dim() != 3:
-            raise ValueError(f"{name}{part}: need a tensor [experts, rows, columns]")
-        if not t.is_cuda:
-            raise ValueError(f"{name}{part}: must be a device tensor")
-        if t.dtype not in dtypes:
-            raise TypeError(f"{name}{part}: dtype {t.dtype} not in {dtypes}")
-        if t.stride()[1:] != (t.shape[2], 1):
-            raise ValueError(f"{name}{part}: an expert must be contiguous")
+    if not (isinstance(packed, torch.Tensor) and isinstance(scales, torch.Tensor) and packed.dim() == 3
+            and scales.dim() == 3):
+        raise ValueError(f"{name}: need two tensors [experts, rows, columns], packed and scales")
     E, rows, half = packed.shape
-    if half % 64 or scales.shape != (E, rows, half // 64):
+    groups = half // 64
+    ps, ss = packed.stride(), scales.stride()
+    # (one condition: a decode token's call is bound by the host)
+    if not (packed.is_cuda and scales.is_cuda and packed.dtype is torch.uint8 and scales.dtype in _F16
+            and half == 64 * groups and scales.shape == (E, rows, groups)
+            and ps[1] == half and ps[2] == 1 and ss[1] == groups and ss[2] == 1):
+        for t, part, dtypes in ((packed, ".packed", (torch.uint8,)), (scales, ".scales", _F16)):
+            if not t.is_cuda:
+                raise ValueError(f"{name}{part}: must be a device tensor")
+            if t.dtype not in dtypes:
+                raise TypeError(f"{name}{part}: dtype {t.dtype} not in {dtypes}")
+            if t.stride()[1:] != (t.shape[2], 1):
+                raise ValueError(f"{name}{part}: an expert must be contiguous")
         raise ValueError(f"{name}: packed {tuple(packed.shape)} and scales {tuple(scales.shape)} do not fit: "
                          "[E, rows, cols / 2] and [E, rows, cols / 128], cols a multiple of 128")
-    return (_lib.cia_q4_experts(packed.data_ptr(), scales.data_ptr(), packed.stride(0), scales.stride(0)),
-            E, rows, 2 * half)
+    return _lib.cia_q4_experts(packed.data_ptr(), scales.data_ptr(), ps[0], ss[0]), E, rows, 2 * half
 
 
 def moe_workspace_bytes(S: int, k: int, E: int, H: int, F: int) -> int:

@@ -197,10 +197,10 @@ def test_wrapper_refusals(cia):
         K.moe_route(x, x, None, None, 2, 256, 4, 2)
     with pytest.raises(ValueError, match="score"):
         K.moe_gating(4, 2, score="tanh")
-    with pytest.raises(ValueError, match=r"w1.packed: need a tensor \[experts"):
+    with pytest.raises(ValueError, match=r"w1: need two tensors \[experts"):
         K.moe_up_int4(x, None, (x, x), (x, x), x, 2, 1, x)
     with pytest.raises(ValueError, match="w2.packed: must be a device tensor"):
-        K.moe_down_int4(x, None, None, (torch.zeros((1, 2, 64), dtype=torch.uint8), x), x, x, 2, 1, x)
+        K.moe_down_int4(x, None, None, (torch.zeros((1, 2, 64), dtype=torch.uint8), x[None]), x, x, 2, 1, x)
 
 
 def test_choice_oracle():
