@@ -19,7 +19,7 @@ namespace cia {
 
 constexpr int kMoeMaxE = CIA_MOE_MAX_EXPERTS;
 constexpr int kMoeMaxK = CIA_MOE_MAX_TOP_K;
-constexpr int kMoeMaxPairs = 1 << 24;
+constexpr int kMoeMaxPairs = CIA_MOE_MAX_PAIRS, kMoeMaxCols = CIA_MOE_MAX_WIDTH;
 
 struct MoeArgs {
   const uint16_t* x;      // fp16: [S][K] (up), [S k][K] (down)
@@ -31,7 +31,7 @@ struct MoeArgs {
   int S, k, E;
   uint16_t* act;          // up: [S k][N]
   float* y;               // down: [S k][N]
-  const int* plan;        // k_moe_plan's
+  const int* plan;        // k_moe_plan's; null: every workgroup finds its tile
   int splits;             // down: parts of K, each into its own y
 };
 
@@ -42,20 +42,23 @@ constexpr int kTileRows = 128;
 // The most row tiles P pairs of E experts can make
 __host__ __device__ constexpr int64_t max_tiles(int64_t P, int E) { return P / kTileRows + (P < E ? P : E); }
 // plan: offs[E + 1], whole tiles, tiles, (expert, first) of each, rows[P]
-__host__ __device__ constexpr int64_t plan_rows_at(int64_t P, int E) { return E + 3 + 2 * max_tiles(P, E); }
+// (rows 16-byte aligned, and written 4 at a time)
+__host__ __device__ constexpr int64_t plan_rows_at(int64_t P, int E) { return (E + 3 + 2 * max_tiles(P, E) + 3) / 4 * 4; }
 
 // ---------------------------------------------------------------- plan
 // Rows by expert: offs[e] .. offs[e + 1] - 1 of rows are expert e's.  Their order
 // within an expert does not matter: a row's results do not depend on its
 // neighbours.
 //   Bound by latency.  One workgroup; up to 16384 pairs are read once, 16 to a
-// thread, and counted by wave: the count before is a pair's rank.  (16384 pairs:
-// 16.3 us with two reads and shared counts.)
+// thread, and counted by wave: the count before is a pair's rank.  They are put in
+// order in LDS and leave it 16 bytes a lane.  (16384 pairs: 16.3 us with two reads
+// and shared counts, 10.8 with each pair stored on its own.)
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 
 __global__ __launch_bounds__(kPlanThreads) void k_moe_plan(const int32_t* ids, int P, int E, int* plan) {
   __shared__ int cnt[kPlanWaves][kMoeMaxE];  // of a wave, then the first place of its pairs
   __shared__ int part[3][4];  // of 64 experts
+  __shared__ __attribute__((aligned(16))) int order[16 * kPlanThreads];
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63;
   int* rows = plan + plan_rows_at(P, E);
   constexpr int kPer = 16;
@@ -137,7 +140,10 @@ __global__ __launch_bounds__(kPlanThreads) void k_moe_plan(const int32_t* ids, i
   } else if (once) {
 #pragma unroll
     for (int j = 0; j < kPer; j++)
-      if ((unsigned)id[j] < (unsigned)E) rows[cnt[w][id[j]] + rank[j]] = kPlanThreads * j + tid;
+      if ((unsigned)id[j] < (unsigned)E) order[cnt[w][id[j]] + rank[j]] = kPlanThreads * j + tid;
+    __syncthreads();
+    const int total = (part[0][0] + part[0][1] + part[0][2] + part[0][3] + 3) / 4;
+    for (int i = tid; i < total; i += kPlanThreads) ((u32x4*)rows)[i] = ((const u32x4*)order)[i];
   } else {
     for (int i = tid; i < P; i += kPlanThreads) {
       const int e = ids[i];
@@ -448,7 +454,7 @@ __device__ __forceinline__ void tile_run(const MoeArgs& a, uint8_t* lds, uint16_
   loop.lds = lds;
   loop.tab = tab;
   loop.src = {xsrc(0, 0), xsrc(0, 1), xsrc(0, 2), xsrc(0, 3), xsrc(1, 0), xsrc(1, 1),
-              xsrc(1, 2), xsrc(1, 3), wsrc(0),    wsrc(1),    wsrc(kNT > 2 ? 2 : 0)};
+              xsrc(1, 2), xsrc(1, 3), wsrc(0),    wsrc(kNT > 1 ? 1 : 0), wsrc(kNT > 2 ? 2 : 0)};
   loop.w = w;
   loop.n16 = n16;
   loop.q = q;
@@ -501,6 +507,142 @@ __device__ __forceinline__ void tile_run(const MoeArgs& a, uint8_t* lds, uint16_
   }
 }
 
+// A workgroup's tile: its expert, rows and their rows of x, in rows[128] and
+// rows[128 + ..].  From the plan, or from up to kOwnPairs ids by itself (which
+// saves the plan's launch, 4 us).
+constexpr int kOwnPairs = 1024;
+
+struct TileOf {
+  int e, n;  // n = 0: none
+  int ct, sp;
+};
+
+// Workgroups go to the 8 XCDs in turn: each takes a run of tiles, row tiles
+// slowest, so that its L2 holds what neighbours share.  The whole tiles first: the
+// others fill the last round.  Returns the row tile, or -1.
+__device__ __forceinline__ int tile_index(int whole, int others, int nct, int splits, TileOf& t) {
+  const int n0 = whole * nct * splits, n1 = others * nct * splits;
+  const int per0 = (n0 + 7) >> 3, per1 = (n1 + 7) >> 3;
+  int i = blockIdx.x >> 3;
+  if (i < per0) {
+    i += (blockIdx.x & 7) * per0;
+    if (i >= n0) return -1;
+  } else {
+    i -= per0;
+    if (i >= per1) return -1;
+    i += (blockIdx.x & 7) * per1;
+    if (i >= n1) return -1;
+    i += n0;
+  }
+  t.ct = i % nct;
+  i /= nct;
+  t.sp = i % splits;
+  return i / splits;
+}
+
+template <bool kUp>
+__device__ __forceinline__ TileOf planned_tile(const MoeArgs& a, int nct, int* rows) {
+  const int tid = threadIdx.x, whole = a.plan[a.E + 1];
+  TileOf t{};
+  const int tile = tile_index(whole, a.plan[a.E + 2] - whole, nct, a.splits, t);
+  if (tile < 0) return t;
+  t.e = a.plan[a.E + 3 + 2 * tile];
+  const int r0 = a.plan[a.E + 4 + 2 * tile], left = a.plan[t.e + 1] - r0;
+  t.n = left < kTileRows ? left : kTileRows;
+  if (tid < kTileRows) {
+    const int p = a.plan[plan_rows_at((int64_t)a.S * a.k, a.E) + r0 + (tid < t.n ? tid : t.n - 1)];
+    rows[tid] = p;
+    rows[kTileRows + tid] = kUp ? p / a.k : p;
+  }
+  __syncthreads();
+  return t;
+}
+
+// scratch: LDS that the tile's loop takes afterwards
+template <bool kUp>
+__device__ __forceinline__ TileOf own_tile(const MoeArgs& a, int nct, int* rows, int* scratch) {
+  constexpr int kPer = kOwnPairs / (64 * kTileWaves);
+  static_assert(kMoeMaxE <= 64 * kTileWaves, "a thread an expert");
+  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, P = a.S * a.k;
+  int* const cnt = scratch;               // [256]
+  int* const part = scratch + kMoeMaxE;   // [2][4]: whole tiles and others of 64 experts
+  int* const found = part + 2 * kTileWaves;
+  int* const wave = found + 2;            // [kPer][4]: pairs of the expert
+  int id[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; j++) {
+    const int i = 64 * kTileWaves * j + tid;
+    id[j] = i < P ? (a.ids ? a.ids[i] : 0) : -1;
+    if ((unsigned)id[j] >= (unsigned)a.E) id[j] = -1;
+  }
+  cnt[tid] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kPer; j++)
+    if (id[j] >= 0) atomicAdd(&cnt[id[j]], 1);
+  __syncthreads();
+  const int mine = cnt[tid], own[2] = {mine / kTileRows, mine % kTileRows != 0};
+  int before[2];
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    int v = own[k];
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int u = __shfl_up(v, d);
+      if (l >= d) v += u;
+    }
+    before[k] = v - own[k];
+    if (l == 63) part[k * kTileWaves + w] = v;
+  }
+  __syncthreads();
+  int total[2] = {};
+#pragma unroll
+  for (int k = 0; k < 2; k++)
+#pragma unroll
+    for (int i = 0; i < kTileWaves; i++) {
+      const int v = part[k * kTileWaves + i];
+      if (i < w) before[k] += v;
+      total[k] += v;
+    }
+  TileOf t{};
+  const int tile = tile_index(total[0], total[1], nct, a.splits, t);
+  if (tile < 0) return t;
+  if (tile >= before[0] && tile < before[0] + own[0]) {
+    found[0] = tid;
+    found[1] = (tile - before[0]) * kTileRows;
+  }
+  if (own[1] && tile == total[0] + before[1]) {
+    found[0] = tid;
+    found[1] = own[0] * kTileRows;
+  }
+  __syncthreads();
+  t.e = __builtin_amdgcn_readfirstlane(found[0]);
+  const int r0 = __builtin_amdgcn_readfirstlane(found[1]), left = __builtin_amdgcn_readfirstlane(cnt[t.e]) - r0;
+  t.n = left < kTileRows ? left : kTileRows;
+  // its rows from r0 on, in the order of the pairs, the same in every workgroup
+  uint64_t b[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; j++) {
+    b[j] = __ballot(id[j] == t.e);
+    if (l == 0) wave[kTileWaves * j + w] = __popcll(b[j]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kPer; j++) {
+    int r = __popcll(b[j] & ((1ull << l) - 1)) - r0;
+    for (int i = 0; i < kTileWaves * j + w; i++) r += wave[i];
+    const int p = 64 * kTileWaves * j + tid;
+    if (id[j] == t.e && r >= 0 && r < kTileRows) {
+      rows[r] = p;
+      rows[kTileRows + r] = kUp ? p / a.k : p;
+    }
+  }
+  __syncthreads();
+  if (tid >= t.n && tid < kTileRows) rows[kTileRows + tid] = rows[kTileRows];  // (read, and not used)
+  __syncthreads();
+  return t;
+}
+
 // grid = max_tiles x column tiles x splits, up to a multiple of 8, and 8; block = 256
 template <bool kUp, int kNT>
 __global__ __launch_bounds__(64 * kTileWaves, 2) void k_moe_tile(MoeArgs a) {
@@ -509,45 +651,19 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void k_moe_tile(MoeArgs a) {
   // DMA's target for known, and waits for it before any read of that variable)
   __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
   int* const srows = (int*)(lds + T::kLds) - 2 * kTileRows;  // rows, and their rows of x
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nv = kUp ? 2 * a.N : a.N, nct = (nv + T::kCols * kTileWaves - 1) / (T::kCols * kTileWaves);
-  // Workgroups go to the 8 XCDs in turn: each takes a run of tiles, row tiles
-  // slowest, so that its L2 holds what neighbours share.
-  // The whole tiles first: the others fill the last round.
-  const int whole = a.plan[a.E + 1], n0 = whole * nct * a.splits, n1 = (a.plan[a.E + 2] - whole) * nct * a.splits;
-  const int per0 = (n0 + 7) >> 3, per1 = (n1 + 7) >> 3;
-  int tile = blockIdx.x >> 3;
-  if (tile < per0) {
-    tile += (blockIdx.x & 7) * per0;
-    if (tile >= n0) return;
-  } else {
-    tile -= per0;
-    if (tile >= per1) return;
-    tile += (blockIdx.x & 7) * per1;
-    if (tile >= n1) return;
-    tile += n0;
-  }
-  const int ct = tile % nct;
-  tile /= nct;
-  const int sp = tile % a.splits;
-  tile /= a.splits;
-  const int e = a.plan[a.E + 3 + 2 * tile], r0 = a.plan[a.E + 4 + 2 * tile];
-  const int left = a.plan[e + 1] - r0, nrows = left < kTileRows ? left : kTileRows;
-  if (tid < kTileRows) {
-    const int p = a.plan[plan_rows_at((int64_t)a.S * a.k, a.E) + r0 + (tid < nrows ? tid : nrows - 1)];
-    srows[tid] = p;
-    srows[kTileRows + tid] = kUp ? p / a.k : p;
-  }
-  __syncthreads();
-  const int c0 = ct * T::kCols * kTileWaves + w * T::kCols;
-  const int ng = a.K >> 7, g0 = ng * sp / a.splits, g1 = ng * (sp + 1) / a.splits;
+  const TileOf t = a.plan ? planned_tile<kUp>(a, nct, srows) : own_tile<kUp>(a, nct, srows, (int*)lds);
+  if (t.n == 0) return;
+  const int c0 = t.ct * T::kCols * kTileWaves + w * T::kCols;
+  const int ng = a.K >> 7, g0 = ng * t.sp / a.splits, g1 = ng * (t.sp + 1) / a.splits;
   uint16_t* tab = (uint16_t*)(lds + 3 * T::kX + 2 * T::kW) + w * kTabGroups * T::kCols;
-  float* y = kUp ? nullptr : a.y + (size_t)sp * a.S * a.k * a.N;
-  switch ((nrows + 31) >> 5) {
-    case 1: return tile_run<kUp, kNT, 1>(a, lds, tab, srows, nrows, e, c0, g0, g1, y);
-    case 2: return tile_run<kUp, kNT, 2>(a, lds, tab, srows, nrows, e, c0, g0, g1, y);
-    case 3: return tile_run<kUp, kNT, 3>(a, lds, tab, srows, nrows, e, c0, g0, g1, y);
-    default: return tile_run<kUp, kNT, 4>(a, lds, tab, srows, nrows, e, c0, g0, g1, y);
+  float* y = kUp ? nullptr : a.y + (size_t)t.sp * a.S * a.k * a.N;
+  switch ((t.n + 31) >> 5) {
+    case 1: return tile_run<kUp, kNT, 1>(a, lds, tab, srows, t.n, t.e, c0, g0, g1, y);
+    case 2: return tile_run<kUp, kNT, 2>(a, lds, tab, srows, t.n, t.e, c0, g0, g1, y);
+    case 3: return tile_run<kUp, kNT, 3>(a, lds, tab, srows, t.n, t.e, c0, g0, g1, y);
+    default: return tile_run<kUp, kNT, 4>(a, lds, tab, srows, t.n, t.e, c0, g0, g1, y);
   }
 }
 
@@ -822,8 +938,9 @@ __global__ __launch_bounds__(64 * kStreamWaves, (2 * Stream<kG, kMT>::kPerUnit))
 // the experts that have a row, so that it can weight the rows and add them to the
 // residual itself, and no launch follows.  The waves split K as above, the weights
 // of the next kRing segments in flight; 8 segments' sums meet at a time.
-// (1 token, 4 of 32 experts of 1792: 5.3 us and 2.4 for the rows' sum so far.)
-constexpr int kFewPairs = 64;
+// (Calls in us, in two launches / so: 1 token, 4 of 32 experts of 1792 11.8 / 8.8;
+// 4 tokens, 16 segments, 16.4 / 19.2.)
+constexpr int kFewPairs = 8;
 
 struct FewArgs {
   MoeArgs m;
@@ -847,13 +964,11 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_few(FewArgs f) {
   // the rows by expert, 16 a segment, as in k_moe_stream
   int id = l < P ? (a.ids ? a.ids[l] : 0) : -1;
   if ((unsigned)id >= (unsigned)a.E) id = -1;
-  // this thread's outputs: column tid & 15 of tokens (tid >> 4) and 32 on
-  float old[2], wt = l < P && f.weights ? f.weights[l] : 1.0f;
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int s = 32 * i + (tid >> 4);
-    old[i] = f.res[(size_t)(s < a.S ? s : 0) * a.N + c0 + (tid & 15)];
-  }
+  // this thread's output: column tid & 15 of token tid >> 4
+  static_assert(kFewPairs <= 32, "a thread an output");
+  const int so = tid >> 4;
+  const float old = f.res[(size_t)(so < a.S ? so : 0) * a.N + c0 + (tid & 15)];
+  const float wt = l < P && f.weights ? f.weights[l] : 1.0f;
   uint64_t same = __ballot(id >= 0);
   const uint64_t live = same;
 #pragma unroll
@@ -865,7 +980,7 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_few(FewArgs f) {
   const int segs = id >= 0 && !(same & below) ? (__popcll(same) + 15) >> 4 : 0;
   int before = 0, nseg = 0;
 #pragma unroll
-  for (int k = 1; k <= kFewPairs / 16; k++) {
+  for (int k = 1; k <= (kFewPairs + 15) / 16; k++) {
     const uint64_t v = __ballot(segs >= k);
     before += __popcll(v & below);
     nseg += __popcll(v);
@@ -961,17 +1076,13 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_few(FewArgs f) {
     }
     __syncthreads();
   }
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int s = 32 * i + (tid >> 4);
-    float v = old[i];
-    for (int j = 0; j < a.k; j++) {
-      const int p = s < a.S ? s * a.k + j : 0;
-      const float wp = __shfl(wt, p);
-      if (live >> p & 1) v = __builtin_fmaf(wp, sums[p][tid & 15], v);
-    }
-    if (s < a.S) f.out[(size_t)s * a.N + c0 + (tid & 15)] = v;
+  float v = old;
+  for (int j = 0; j < a.k; j++) {
+    const int p = so < a.S ? so * a.k + j : 0;
+    const float wp = __shfl(wt, p);
+    if (live >> p & 1) v = __builtin_fmaf(wp, sums[p][tid & 15], v);
   }
+  if (so < a.S) f.out[(size_t)so * a.N + c0 + (tid & 15)] = v;
 }
 
 // ---------------------------------------------------------------- combine
@@ -984,35 +1095,40 @@ struct CombineArgs {
   int S, k, E, H, splits;
 };
 
-// out = res + the k weighted rows of each token, in the order of j
+// out = res + the k weighted rows of each token, in the order of j.  A thread
+// takes 4 columns; bound by memory (4096 tokens of 2048, k = 4: 200 MB, 30 us).
+constexpr unsigned kCombineGrid = 1u << 20;
+
 __global__ __launch_bounds__(256) void k_moe_combine(CombineArgs a) {
-  const int nc = (a.H + 1023) / 1024;
-  const int s = blockIdx.x / nc, c = (blockIdx.x % nc * 256 + threadIdx.x) * 4;
-  if (c >= a.H) return;
-  f32x4 v = *(const f32x4*)(a.res + (size_t)s * a.H + c);
-  for (int j = 0; j < a.k; j++) {
-    const int p = s * a.k + j, e = a.ids ? a.ids[p] : 0;
-    if ((unsigned)e >= (unsigned)a.E) continue;
-    const float w = a.weights ? a.weights[p] : 1.0f;
-    f32x4 y = *(const f32x4*)(a.y + (size_t)p * a.H + c);
-    for (int i = 1; i < a.splits; i++) y += *(const f32x4*)(a.y + ((size_t)i * a.S * a.k + p) * a.H + c);
+  const unsigned nc = (a.H + 1023) / 1024;
+  for (unsigned b = blockIdx.x; b < (unsigned)a.S * nc; b += gridDim.x) {
+    const int s = b / nc, c = (b % nc * 256 + threadIdx.x) * 4;
+    if (c >= a.H) continue;
+    f32x4 v = *(const f32x4*)(a.res + (size_t)s * a.H + c);
+    for (int j = 0; j < a.k; j++) {
+      const int p = s * a.k + j, e = a.ids ? a.ids[p] : 0;
+      if ((unsigned)e >= (unsigned)a.E) continue;
+      const float w = a.weights ? a.weights[p] : 1.0f;
+      f32x4 y = *(const f32x4*)(a.y + (size_t)p * a.H + c);
+      for (int i = 1; i < a.splits; i++) y += *(const f32x4*)(a.y + ((size_t)i * a.S * a.k + p) * a.H + c);
 #pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = __builtin_fmaf(w, y[i], v[i]);
+      for (int i = 0; i < 4; i++) v[i] = __builtin_fmaf(w, y[i], v[i]);
+    }
+    *(f32x4*)(a.out + (size_t)s * a.H + c) = v;
   }
-  *(f32x4*)(a.out + (size_t)s * a.H + c) = v;
 }
 
 // ---------------------------------------------------------------- host
-static int64_t plan_bytes(int64_t P, int E) { return ((plan_rows_at(P, E) + P) * 4 + 255) / 256 * 256; }
+static int64_t plan_bytes(int64_t P, int E) { return ((plan_rows_at(P, E) + P + 3) * 4 + 255) / 256 * 256; }
 
 // Rows of y: P, and room for parts of K where few pairs leave the chip empty
 static int64_t y_rows(int64_t P) { return P >= 4096 ? P : (8 * P < 4096 ? 8 * P : 4096); }
 
-// Parts of K of a down launch: as many as the chip's 512 places hold where the
-// tiles alone leave most of them empty, each of 4 groups or more.
+// Parts of K of a down launch in tiles: as many as the chip's 512 places hold of
+// workgroups of 128 columns, each part of 4 groups or more.
+static int64_t row_tiles(int64_t P, int E);
 static int k_splits(int64_t P, int E, int H, int F) {
-  const int64_t tiles = ((P + kTileRows - 1) / kTileRows + (P < E - 1 ? P : E - 1)) * ((H + 191) / 192);
-  int64_t n = 512 / tiles;
+  int64_t n = 512 / (row_tiles(P, E) * ((H + 127) / 128));
   n = n < y_rows(P) / P ? n : y_rows(P) / P;
   n = n < F / 512 ? n : F / 512;
   return n < 1 ? 1 : (int)n;
@@ -1020,7 +1136,7 @@ static int k_splits(int64_t P, int E, int H, int F) {
 
 static int moe_check(int S, int k, int E, int H, int F, const int32_t* ids) {
   CIA_REQUIRE(S >= 0 && k >= 1 && k <= kMoeMaxK && E >= 1 && E <= kMoeMaxE && H > 0 && F > 0 &&
-                  H % 128 == 0 && F % 128 == 0 && H <= (1 << 20) && F <= (1 << 20) &&
+                  H % 128 == 0 && F % 128 == 0 && H <= kMoeMaxCols && F <= kMoeMaxCols &&
                   (int64_t)S * k <= kMoeMaxPairs,
               CIA_ERR_ARG);
   // without ids there is nothing to choose from
@@ -1043,16 +1159,16 @@ static void set_w(MoeArgs& a, int i, const cia_q4_experts* w) {
   a.sstride[i] = w->scales_stride;
 }
 
-// Whether the weights are streamed rather than multiplied in tiles: up to 8 rows
-// an expert on average, or few pairs at all.  Calls in us, streamed / in tiles:
-// 4 of 32 experts of 1792, H = 2048, 40 tokens up 31 / 34, down 26.5 / 28.1; 64
-// 37 / 41, 31.6 / 32.9; 100 49 / 45, 37.6 / 34.7.  2 of 8 of 2048, H = 1024, 64
-// tokens 15.2 / 18.9, 19.4 / 19.4; 100 17.8 / 21.1, 24.7 / 21.2; 256 25.0 / 26.5,
-// 34 / 26.  The dense form of 7168, H = 2048, 128 rows 23 / 36, 22 / 28; 256 31 /
-// 38, 29 / 30; 400 54 / 41, 48 / 39.  (Down takes a K of two parts as well.)
+// Whether the weights are streamed rather than multiplied in tiles: while experts
+// have 8 (up), 6 (down) rows on average, or pairs are few.  Calls in us, streamed /
+// in tiles: 4 of 32 experts of 1792, H = 2048, up 64 tokens 38 / 43, 100 49 / 46,
+// down 40 27.7 / 30.4, 64 32 / 29; 2 of 8 of 2048, H = 1024, up 100 18 / 18, 170
+// 22 / 21, down 16 14 / 16.5, 40 18 / 17; the dense form of 7168, H = 2048, up 128
+// rows 22 / 24, 170 37 / 25, down 16 12 / 16, 40 16.6 / 16.5.  (Down takes a K of
+// two parts as well.)
 static bool streams(bool up, int64_t P, int E, int K) {
-  const int64_t few = up ? 256 : 128;
-  return P <= kStreamPairs && K <= (up ? 1 : 2) * kStreamMaxK && (P <= 8 * (int64_t)E || P <= few);
+  const int64_t most = up ? 8 * (int64_t)E : 6 * (int64_t)E, few = up ? 128 : 32;
+  return P <= kStreamPairs && K <= (up ? 1 : 2) * kStreamMaxK && P <= (most > few ? most : few);
 }
 
 // 16 rows at a time with two workgroups a compute unit where experts hardly have
@@ -1072,8 +1188,36 @@ static void stream_launch(const MoeArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((k_moe_stream<kUp, kG, kMT>), dim3(kUnits), block, 0, s, a);
 }
 
+// Column tiles a wave, of 1, 2 and 3: time goes with kNT + 1 a round of the 512
+// workgroups that the chip holds, and 0.4 rounds for the last one's end.
+static int64_t row_tiles(int64_t P, int E) {  // about: every expert has a last, partly filled one
+  const int64_t other = P < E ? P : E;
+  return P / kTileRows + (E > 1 ? (other + 1) / 2 : (P % kTileRows != 0));
+}
+static int tile_nt(int64_t P, int E, int nv, int splits) {
+  int best = 1;
+  double least = 0.0;
+  for (int nt = 1; nt <= 3; nt++) {
+    const double rounds = (double)(row_tiles(P, E) * ((nv + 64 * nt - 1) / (64 * nt)) * splits) / 512.0 + 0.4;
+    const double t = (rounds < 1.0 ? 1.0 : rounds) * (nt + 1);
+    if (nt == 1 || t < least) {
+      best = nt;
+      least = t;
+    }
+  }
+  return best;
+}
+
+template <bool kUp, int kNT>
+static void tile_launch(const MoeArgs& a, hipStream_t s) {
+  const int nv = kUp ? 2 * a.N : a.N, cols = 16 * kNT * kTileWaves;
+  const int64_t tiles = max_tiles((int64_t)a.S * a.k, a.E) * ((nv + cols - 1) / cols) * a.splits;
+  hipLaunchKernelGGL((k_moe_tile<kUp, kNT>), dim3((unsigned)((tiles + 7) / 8 * 8 + 8)), dim3(64 * kTileWaves), 0, s, a);
+}
+
+// planned: ws holds the plan of these ids already
 template <bool kUp>
-static int products(MoeArgs& a, void* ws, hipStream_t s) {
+static int products(MoeArgs& a, void* ws, bool planned, hipStream_t s) {
   const int P = a.S * a.k;
   if (streams(kUp, P, a.E, a.K)) {
     const int part = ((a.K >> 7) + a.splits - 1) / a.splits;  // groups
@@ -1085,12 +1229,13 @@ static int products(MoeArgs& a, void* ws, hipStream_t s) {
       stream_launch<kUp, 4>(a, s);
     return launch_status();
   }
-  constexpr int kNT = 3;
-  a.plan = (const int*)ws;
-  hipLaunchKernelGGL(k_moe_plan, dim3(1), dim3(kPlanThreads), 0, s, a.ids, P, a.E, (int*)ws);
-  const int nv = kUp ? 2 * a.N : a.N, cols = 16 * kNT * kTileWaves;
-  const int64_t tiles = max_tiles(P, a.E) * ((nv + cols - 1) / cols) * a.splits;
-  hipLaunchKernelGGL((k_moe_tile<kUp, kNT>), dim3((unsigned)((tiles + 7) / 8 * 8 + 8)), dim3(64 * kTileWaves), 0, s, a);
+  a.plan = P <= kOwnPairs ? nullptr : (const int*)ws;
+  if (a.plan && !planned) hipLaunchKernelGGL(k_moe_plan, dim3(1), dim3(kPlanThreads), 0, s, a.ids, P, a.E, (int*)ws);
+  switch (tile_nt(P, a.E, kUp ? 2 * a.N : a.N, a.splits)) {
+    case 1: tile_launch<kUp, 1>(a, s); break;
+    case 2: tile_launch<kUp, 2>(a, s); break;
+    default: tile_launch<kUp, 3>(a, s);
+  }
   return launch_status();
 }
 
@@ -1104,9 +1249,8 @@ extern "C" int64_t cia_moe_workspace_bytes(int S, int k, int E, int H, int F) {
   return plan_bytes(P, E) + y_rows(P) * H * 4;
 }
 
-extern "C" int cia_moe_up_int4(const uint16_t* x, const int32_t* ids, const cia_q4_experts* w1,
-                               const cia_q4_experts* w3, uint16_t* act, int S, int k, int E, int H,
-                               int F, void* ws, int64_t ws_bytes, void* stream) {
+static int moe_up(const uint16_t* x, const int32_t* ids, const cia_q4_experts* w1, const cia_q4_experts* w3,
+                  uint16_t* act, int S, int k, int E, int H, int F, void* ws, int64_t ws_bytes, void* stream) {
   int st = moe_check(S, k, E, H, F, ids);
   if (st) return st;
   if (S == 0) return CIA_OK;
@@ -1126,12 +1270,19 @@ extern "C" int cia_moe_up_int4(const uint16_t* x, const int32_t* ids, const cia_
   a.E = E;
   a.act = act;
   a.splits = 1;
-  return products<true>(a, ws, (hipStream_t)stream);
+  return products<true>(a, ws, false, (hipStream_t)stream);
 }
 
-extern "C" int cia_moe_down_int4(const uint16_t* act, const int32_t* ids, const float* weights,
-                                 const cia_q4_experts* w2, const float* res, float* out, int S, int k,
-                                 int E, int H, int F, void* ws, int64_t ws_bytes, void* stream) {
+extern "C" int cia_moe_up_int4(const uint16_t* x, const int32_t* ids, const cia_q4_experts* w1,
+                               const cia_q4_experts* w3, uint16_t* act, int S, int k, int E, int H,
+                               int F, void* ws, int64_t ws_bytes, void* stream) {
+  return moe_up(x, ids, w1, w3, act, S, k, E, H, F, ws, ws_bytes, stream);
+}
+
+// planned: ws holds these ids' plan (moe_up's in tiles)
+static int moe_down(const uint16_t* act, const int32_t* ids, const float* weights, const cia_q4_experts* w2,
+                    const float* res, float* out, int S, int k, int E, int H, int F, void* ws, int64_t ws_bytes,
+                    bool planned, void* stream) {
   int st = moe_check(S, k, E, H, F, ids);
   if (st) return st;
   if (S == 0) return CIA_OK;
@@ -1165,10 +1316,17 @@ extern "C" int cia_moe_down_int4(const uint16_t* act, const int32_t* ids, const 
       hipLaunchKernelGGL(k_moe_few<4>, grid, block, 0, s, f);
     return launch_status();
   }
-  if ((st = products<false>(a, ws, s))) return st;
+  if ((st = products<false>(a, ws, planned, s))) return st;
   const CombineArgs c{a.y, ids, weights, res, out, S, k, E, H, a.splits};
-  hipLaunchKernelGGL(k_moe_combine, dim3((unsigned)((H + 1023) / 1024) * (unsigned)S), dim3(256), 0, s, c);
+  const unsigned blocks = (unsigned)((H + 1023) / 1024) * (unsigned)S;
+  hipLaunchKernelGGL(k_moe_combine, dim3(blocks < kCombineGrid ? blocks : kCombineGrid), dim3(256), 0, s, c);
   return launch_status();
+}
+
+extern "C" int cia_moe_down_int4(const uint16_t* act, const int32_t* ids, const float* weights,
+                                 const cia_q4_experts* w2, const float* res, float* out, int S, int k,
+                                 int E, int H, int F, void* ws, int64_t ws_bytes, void* stream) {
+  return moe_down(act, ids, weights, w2, res, out, S, k, E, H, F, ws, ws_bytes, false, stream);
 }
 
 // ---------------------------------------------------------------- the branch
@@ -1226,9 +1384,8 @@ extern "C" int cia_moe_block_forward(const cia_moe* M, float* h, int S, void* st
   if ((st = cia_add_rmsnorm(h, nullptr, M->norm_w, M->norm_eps, nullptr, x, S, M->H, stream))) return st;
   if (M->gate && (st = cia_moe_route(x, M->gate, M->bias, &M->gating, ids, weights, nullptr, S, M->H, stream)))
     return st;
-  if ((st = cia_moe_up_int4(x, ids, &M->w1, &M->w3, act, S, k, E, M->H, M->F, ws + b.moe,
-                            M->ws_bytes - b.moe, stream)))
+  if ((st = moe_up(x, ids, &M->w1, &M->w3, act, S, k, E, M->H, M->F, ws + b.moe, M->ws_bytes - b.moe, stream)))
     return st;
-  return cia_moe_down_int4(act, ids, weights, &M->w2, h, h, S, k, E, M->H, M->F, ws + b.moe,
-                           M->ws_bytes - b.moe, stream);
+  return moe_down(act, ids, weights, &M->w2, h, h, S, k, E, M->H, M->F, ws + b.moe, M->ws_bytes - b.moe,
+                  !streams(true, (int64_t)S * k, E, M->H), stream);
 }

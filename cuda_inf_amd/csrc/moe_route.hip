@@ -384,7 +384,7 @@ static int route_run(const RouteArgs& a, hipStream_t s) {
 static int route_args(RouteArgs& a, const cia_moe_gating* g, int S) {
   CIA_REQUIRE(g, CIA_ERR_NULL);
   CIA_REQUIRE(g->n_experts >= 1 && g->n_experts <= kRouteMaxE && g->top_k >= 1 && g->top_k <= kRouteMaxK &&
-                  g->top_k <= g->n_experts && S >= 0,
+                  g->top_k <= g->n_experts && S >= 0 && S <= CIA_FFN_MAX_TOKENS,
               CIA_ERR_ARG);
   CIA_REQUIRE(g->score == CIA_SCORE_SIGMOID || g->score == CIA_SCORE_SOFTMAX, CIA_ERR_ARG);
   CIA_REQUIRE(g->n_group >= 1 && g->n_experts % g->n_group == 0 && g->topk_group >= 1 &&

@@ -26,6 +26,9 @@ extern "C" {
 
 #define CIA_MOE_MAX_EXPERTS 256
 #define CIA_MOE_MAX_TOP_K 16
+#define CIA_MOE_MAX_WIDTH 32768     /* H and F of the experts */
+#define CIA_MOE_MAX_PAIRS (1 << 20) /* S * k of a call */
+#define CIA_FFN_MAX_TOKENS (1 << 22) /* S of the norm and the router */
 
 /* add_f32_inplace and rmsnorm (engine.cu:533-536, 131-144; launched at 867 and
  * 870): hsum = h + add, out = fp16(hsum * rsqrt(mean(hsum^2) + eps) * w) for
@@ -96,8 +99,9 @@ typedef struct cia_q4_experts {
  * act: fp16 [S][k][F].  A pair whose id is outside [0, E) takes no part (a
  * place of a padded batch, another device's expert): its act row is left as it
  * was.  An id may repeat within a token.  ids NULL: every row is expert 0's
- * (E = k = 1, a dense layer).  H and F multiples of 128, k at most
- * CIA_MOE_MAX_TOP_K, S * k at most 2^24.  x, act and ws 16-byte aligned;
+ * (E = k = 1, a dense layer).  H and F multiples of 128, at most
+ * CIA_MOE_MAX_WIDTH; k at most CIA_MOE_MAX_TOP_K, S * k at most
+ * CIA_MOE_MAX_PAIRS.  x, act and ws 16-byte aligned;
  * ws_bytes at least cia_moe_workspace_bytes(S, k, E, H, F). */
 int cia_moe_up_int4(const uint16_t* x, const int32_t* ids,
                     const cia_q4_experts* w1, const cia_q4_experts* w3,
