@@ -1160,14 +1160,14 @@ static void set_w(MoeArgs& a, int i, const cia_q4_experts* w) {
 }
 
 // Whether the weights are streamed rather than multiplied in tiles: while experts
-// have 8 (up), 6 (down) rows on average, or pairs are few.  Calls in us, streamed /
-// in tiles: 4 of 32 experts of 1792, H = 2048, up 64 tokens 38 / 43, 100 49 / 46,
-// down 40 27.7 / 30.4, 64 32 / 29; 2 of 8 of 2048, H = 1024, up 100 18 / 18, 170
-// 22 / 21, down 16 14 / 16.5, 40 18 / 17; the dense form of 7168, H = 2048, up 128
-// rows 22 / 24, 170 37 / 25, down 16 12 / 16, 40 16.6 / 16.5.  (Down takes a K of
-// two parts as well.)
+// have 8 (up), 4 (down) rows on average, or pairs are few.  Calls in us, streamed /
+// in tiles: 4 of 32 experts of 1792, H = 2048, up 16 tokens 22.7 / 25.7, 40 31 /
+// 36, 64 37 / 41.5, 100 49 / 44, down 16 20.1 / 24.8, 40 27.0 / 27.9, 64 32 / 24.6;
+// 2 of 8 of 2048, H = 1024, up 32 10.8 / 12.1, 40 14.6 / 12.5, down 8 13.9 / 14.2,
+// 16 14.5 / 13.8; the dense form of 7168, H = 2048, up 32 rows 12.4 / 13.2, 64 17.1
+// / 16.1, down 8 12.9 / 15.7, 24 15.0 / 13.8.  (Down takes a K of two parts as well.)
 static bool streams(bool up, int64_t P, int E, int K) {
-  const int64_t most = up ? 8 * (int64_t)E : 6 * (int64_t)E, few = up ? 128 : 32;
+  const int64_t most = (up ? 8 : 4) * (int64_t)E, few = up ? 64 : 16;
   return P <= kStreamPairs && K <= (up ? 1 : 2) * kStreamMaxK && P <= (most > few ? most : few);
 }
 
