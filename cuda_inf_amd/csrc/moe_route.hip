@@ -81,9 +81,11 @@ __device__ __forceinline__ double wave_max_f64(double v) {
 }
 
 // A token's choice by one wave: lg, its logits in LDS; ch, E doubles of LDS for
-// the wave.  Lane l has experts l, l + 64, ..
+// the wave.  Lane l has experts l, l + 64, .., kPer of them.  (A template of kPer:
+// the code of experts that are not there is fetched all the same, and at a few
+// tokens fetching code is much of the time.)
+template <int kPer>
 __device__ __forceinline__ void choose(const RouteArgs& a, int s, const double* lg, double* ch) {
-  constexpr int kPer = kRouteMaxE / 64;
   const int l = threadIdx.x & 63;
   const double ninf = -__builtin_inf();
   double sc[kPer], c[kPer];
@@ -222,7 +224,7 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int s, const double* 
 // lane's 8 elements in four 16-byte pieces kSpan / 8 lanes apart.
 constexpr int kTokWaves = 8;
 
-template <int kT>
+template <int kT, int kPer>
 __global__ __launch_bounds__(64 * kTokWaves) void k_route_tok(RouteArgs a) {
   constexpr int kSpan = 4096 / kT;  // elements of a row in LDS at a time
   __shared__ f64x2 xs[kT][4][kSpan / 8];
@@ -298,7 +300,7 @@ __global__ __launch_bounds__(64 * kTokWaves) void k_route_tok(RouteArgs a) {
     }
     __syncthreads();
   }
-  if (w < kT && s0 + w < a.S) choose(a, s0 + w, lg[w], ch[w]);
+  if (w < kT && s0 + w < a.S) choose<kPer>(a, s0 + w, lg[w], ch[w]);
 }
 
 // Many tokens: 16 a workgroup on the matrix cores in 64 bits
@@ -307,6 +309,7 @@ __global__ __launch_bounds__(64 * kTokWaves) void k_route_tok(RouteArgs a) {
 // 8q + i of row r, in both operands.
 constexpr int kTileToks = 16, kMfmaWaves = 16;
 
+template <int kPer>
 __global__ __launch_bounds__(64 * kMfmaWaves) void k_route_mfma(RouteArgs a) {
   constexpr int kTiles = 2;  // of experts at a time
   __shared__ double part[kMfmaWaves][kTiles][256];  // in the end the waves' choices
@@ -365,18 +368,27 @@ __global__ __launch_bounds__(64 * kMfmaWaves) void k_route_mfma(RouteArgs a) {
     }
     __syncthreads();
   }
-  for (int t = w; t < kTileToks && s0 + t < a.S; t += kMfmaWaves) choose(a, s0 + t, lg[t], part[w][0]);
+  for (int t = w; t < kTileToks && s0 + t < a.S; t += kMfmaWaves) choose<kPer>(a, s0 + t, lg[t], part[w][0]);
+}
+
+template <int kPer>
+static void route_launch(const RouteArgs& a, hipStream_t s) {
+  const dim3 block(64 * kTokWaves);
+  if (a.x && a.S >= 1024)
+    hipLaunchKernelGGL(k_route_mfma<kPer>, dim3((unsigned)((a.S + kTileToks - 1) / kTileToks)), dim3(64 * kMfmaWaves), 0, s, a);
+  else if (!a.x && a.S >= 64)  // (nothing but the choice: a wave a token)
+    hipLaunchKernelGGL((k_route_tok<8, kPer>), dim3((unsigned)((a.S + 7) / 8)), block, 0, s, a);
+  else if (a.S <= 256)
+    hipLaunchKernelGGL((k_route_tok<1, kPer>), dim3((unsigned)a.S), block, 0, s, a);
+  else
+    hipLaunchKernelGGL((k_route_tok<2, kPer>), dim3((unsigned)((a.S + 1) / 2)), block, 0, s, a);
 }
 
 static int route_run(const RouteArgs& a, hipStream_t s) {
-  if (a.x && a.S >= 1024)
-    hipLaunchKernelGGL(k_route_mfma, dim3((unsigned)((a.S + kTileToks - 1) / kTileToks)), dim3(64 * kMfmaWaves), 0, s, a);
-  else if (!a.x && a.S >= 64)  // (nothing but the choice: a wave a token)
-    hipLaunchKernelGGL(k_route_tok<8>, dim3((unsigned)((a.S + 7) / 8)), dim3(64 * kTokWaves), 0, s, a);
-  else if (a.S <= 256)
-    hipLaunchKernelGGL(k_route_tok<1>, dim3((unsigned)a.S), dim3(64 * kTokWaves), 0, s, a);
+  if (a.E <= 64)
+    route_launch<1>(a, s);
   else
-    hipLaunchKernelGGL(k_route_tok<2>, dim3((unsigned)((a.S + 1) / 2)), dim3(64 * kTokWaves), 0, s, a);
+    route_launch<kRouteMaxE / 64>(a, s);
   return launch_status();
 }
 
