@@ -83,9 +83,13 @@ __device__ __forceinline__ double wave_max_f64(double v) {
 // A token's choice by one wave: lg, its logits in LDS; ch, E doubles of LDS for
 // the wave.  Lane l has experts l, l + 64, .., kPer of them.  (A template of kPer:
 // the code of experts that are not there is fetched all the same, and at a few
-// tokens fetching code is much of the time.)
+// tokens fetching code is much of the time.)  far: how far a logit may be off;
+// where logits that near could choose otherwise, the choice is not written, and
+// false returned; doubt[i] then has a bit for each expert 64 i + .. whose exact
+// logit the choice needs.
 template <int kPer>
-__device__ __forceinline__ void choose(const RouteArgs& a, int s, const double* lg, double* ch) {
+__device__ __forceinline__ bool choose(const RouteArgs& a, int s, const double* lg, double* ch, double far,
+                                       uint64_t* doubt) {
   const int l = threadIdx.x & 63;
   const double ninf = -__builtin_inf();
   double sc[kPer], c[kPer];
@@ -99,6 +103,13 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int s, const double* 
     bad = bad || sc[i] != sc[i];
     m = sc[i] > m ? sc[i] : m;
   }
+  // How far a choice may be off: a sigmoid's slope is at most 1/4; a softmax moves by
+  // s (dl - sum s dl), at most 2 s |dl| and its square; and what 64 bits round.
+  auto off = [&](double score, double choice) __attribute__((always_inline)) {
+    return (a.softmax ? 2.05 * score : 0.25) * far + 1e-14 + (choice > ninf ? 1e-15 * __builtin_fabs(choice) : 0.0);
+  };
+  double largest = 1.0;  // no score is above it
+  bool safe = far == 0.0 || !(__any(bad) || !(far < (a.softmax ? 0.01 : 1e30)));
   if (a.softmax) {
     m = wave_max_f64(m);
     // no number among infinities (inf - inf) or beside a NaN; all -inf: scores of 0
@@ -111,6 +122,7 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int s, const double* 
       sum += sc[i];
     }
     sum = wave_sum_f64(sum);
+    largest = 1.0 / sum;  // (the largest logit's)
 #pragma unroll
     for (int i = 0; i < kPer; i++) sc[i] = bad ? __builtin_nan("") : (sum == 0.0 ? 0.0 : sc[i] / sum);
   } else {
@@ -163,9 +175,17 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int s, const double* 
       const int g = l + 64 * i;
       if (64 * i >= a.n_group) break;
       int rank = 0;
+      bool near = false;  // another group's sum of two
+      const double o = 4.0 * off(largest, best[i]);
 #pragma unroll 8
-      for (int j = 0; j < a.n_group; j++) rank += ch[j] > best[i] || (ch[j] == best[i] && j < g);
+      for (int j = 0; j < a.n_group; j++) {
+        rank += ch[j] > best[i] || (ch[j] == best[i] && j < g);
+        near = near || (j != g && __builtin_fabs(ch[j] - best[i]) <= o);
+      }
       keep |= (g < a.n_group && rank < a.topk_group ? 1u : 0u) << i;
+      // (only the last one in and the first one out matter)
+      if (far != 0.0)
+        safe = safe && !__any(g < a.n_group && near && rank >= a.topk_group - 1 && rank <= a.topk_group);
     }
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -176,11 +196,13 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int s, const double* 
     for (int i = 0; i < kPer; i++)
       if (l + 64 * i < a.E && ch[(l + 64 * i) / per] != 0.0) in |= 1u << i;
   }
-  // k rounds: the best choice left, the lowest index among equals; lane j keeps
-  // round j's
+  // k rounds (and one more for how near the next one is): the best choice left, the
+  // lowest index among equals; lane j keeps round j's
+  const bool all = a.n_group > 1 || (a.softmax && a.bias) || !safe;  // of the experts are in doubt, if any
+  const uint32_t in0 = in;
   int id = 0;
-  double w = 0.0;
-  for (int j = 0; j < a.k; j++) {
+  double w = 0.0, above = __builtin_inf(), above_off = 0.0;
+  for (int j = 0; j < a.k + (far != 0.0 ? 1 : 0); j++) {
     double v = ninf;
 #pragma unroll
     for (int i = 0; i < kPer; i++)
@@ -198,15 +220,32 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int s, const double* 
         vs = sc[i];
       }
     }
+    if (!at) break;  // (the choice was all of them)
     const int lane = __builtin_ctzll(at);
     const uint64_t u = __builtin_bit_cast(uint64_t, vs);
     const double ws = f64_of((uint32_t)__builtin_amdgcn_readlane((int)u, lane),
                              (uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), lane));
+    if (far != 0.0) {
+      const double o = off(ws, top);
+      safe = safe && !(above - top <= above_off + o);
+      above = top;
+      above_off = o;
+      if (j == a.k) break;
+    }
     if (l == lane) in &= ~(1u << wi);
     if (l == j) {
       id = lane + 64 * wi;
       w = ws;
     }
+  }
+  if (!safe) {
+    // what is sure to stay below the last one looked at is not in doubt
+#pragma unroll
+    for (int i = 0; i < kPer; i++) {
+      const uint64_t b = __ballot(in0 >> i & 1 && (all || !(c[i] + off(sc[i], c[i]) < above - above_off)));
+      if (l == 0) doubt[i] = b;
+    }
+    return false;
   }
   double f = (double)a.scale;
   if (a.renorm) {
@@ -217,6 +256,7 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int s, const double* 
     a.ids[(size_t)s * a.k + l] = id;
     a.weights[(size_t)s * a.k + l] = (float)(w * f);
   }
+  return true;
 }
 
 // Few tokens: kT a workgroup of 8 waves, a wave every 8th expert, so that a
@@ -300,64 +340,86 @@ __global__ __launch_bounds__(64 * kTokWaves) void k_route_tok(RouteArgs a) {
     }
     __syncthreads();
   }
-  if (w < kT && s0 + w < a.S) choose<kPer>(a, s0 + w, lg[w], ch[w]);
+  if (w < kT && s0 + w < a.S) choose<kPer>(a, s0 + w, lg[w], ch[w], 0.0, nullptr);
 }
 
-// Many tokens: 16 a workgroup on the matrix cores in 64 bits
-// (v_mfma_f64_16x16x4_f64), 16 experts a tile, the 16 waves a part of H each.  A
-// lane's 8 elements of 16 bytes are eight k steps: at step i lane (r, q) holds k =
-// 8q + i of row r, in both operands.
+// More tokens: 16 a workgroup on the fp16 matrix cores, 16 experts a tile, the 16
+// waves a part of H each.  32 products are summed in fp32, the rest in 64 bits; a
+// second product, of the magnitudes, bounds what the fp32 sums have lost.  Tokens
+// whose choice hangs on that (1 of 200 of 32 experts, H = 2048) have the logits that
+// it hangs on taken again, in 64 bits, by all the waves.
+// (4096 tokens of 32 experts, H = 2048: 16.4 us on the 64-bit matrix cores.)
 constexpr int kTileToks = 16, kMfmaWaves = 16;
 
 template <int kPer>
 __global__ __launch_bounds__(64 * kMfmaWaves) void k_route_mfma(RouteArgs a) {
-  constexpr int kTiles = 2;  // of experts at a time
+  constexpr int kTiles = 2, kAhead = 4;  // tiles of experts at a time, steps whose operands are fetched together
   __shared__ double part[kMfmaWaves][kTiles][256];  // in the end the waves' choices
   __shared__ double lg[kTileToks][kRouteMaxE];
-  static_assert(kTiles * 256 >= kRouteMaxE, "a wave's choices");
+  __shared__ u32x4 stage[kMfmaWaves][1 + kTiles][64];
+  __shared__ float mag[kMfmaWaves][kTileToks];
+  __shared__ int again;  // bit t: token t
+  __shared__ uint64_t doubt[kTileToks][kPer];
+  static_assert(kTiles * 256 >= kRouteMaxE && kTileToks == kMfmaWaves, "a wave's choices; a wave a token");
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, r16 = l & 15, q = l >> 4;
   const int s0 = blockIdx.x * kTileToks;
-  const int s = s0 + r16 < a.S ? s0 + r16 : a.S - 1;
   const int n32 = (a.H + 31) / 32;  // steps of 32 elements
+  // Operands are fetched 4 lanes to a row's 64 bytes (16 bytes a lane in rows of
+  // their own take four times as long) and change lanes in the wave's LDS.
+  const int row = l >> 2, to = (l & ~3) | ((l & 3) ^ ((l >> 4) & 3)), from = 4 * r16 + (q ^ ((r16 >> 2) & 3));
+  const uint16_t* const xr = a.x + (size_t)(s0 + row < a.S ? s0 + row : a.S - 1) * a.H;
+  if (tid == 0) again = 0;
+  f32x4 most = {};  // of this wave's sums of magnitudes, tokens 4q .. 4q + 3
   for (int e0 = 0; e0 < a.E; e0 += 16 * kTiles) {
-    f64x4 acc[kTiles] = {};
+    double acc[kTiles][4] = {};
+    f32x4 mags[kTiles] = {};
     const uint16_t* gr[kTiles];
 #pragma unroll
     for (int t = 0; t < kTiles; t++) {
-      const int e = e0 + 16 * t + r16;
+      const int e = e0 + 16 * t + row;
       gr[t] = a.gate + (size_t)(e < a.E ? e : a.E - 1) * a.H;
     }
-    // (elements past H: the last ones of the row times zeros)
-    auto fetch = [&](int i, f16x8& x, f16x8 (&g)[kTiles]) __attribute__((always_inline)) {
-      const int k0 = 32 * i + 8 * q, k = k0 < a.H ? k0 : a.H - 8;
-      x = *(const f16x8*)(a.x + (size_t)s * a.H + k);
+    auto abs8 = [](f16x8 v) __attribute__((always_inline)) {
+      u32x4 u = __builtin_bit_cast(u32x4, v);
 #pragma unroll
-      for (int t = 0; t < kTiles; t++) {
-        g[t] = *(const f16x8*)(gr[t] + k);
-        if (k0 >= a.H) g[t] = f16x8{};
-      }
-      if (k0 >= a.H) x = f16x8{};
+      for (int i = 0; i < 4; i++) u[i] &= 0x7FFF7FFFu;
+      return __builtin_bit_cast(f16x8, u);
     };
-    f16x8 x, g[kTiles], xn, gn[kTiles];
-    fetch(w, xn, gn);
-    for (int i = w; i < n32; i += kMfmaWaves) {
-      x = xn;
+    for (int i0 = w; i0 < n32; i0 += kMfmaWaves * kAhead) {
+      u32x4 x[kAhead], g[kAhead][kTiles];
 #pragma unroll
-      for (int t = 0; t < kTiles; t++) g[t] = gn[t];
-      fetch(i + kMfmaWaves, xn, gn);
+      for (int i = 0; i < kAhead; i++) {
+        // (elements past H: the last ones of the row, and zeros for them)
+        const int k0 = 32 * (i0 + kMfmaWaves * i) + 8 * (l & 3), k = k0 < a.H ? k0 : a.H - 8;
+        x[i] = *(const u32x4*)(xr + k);
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const double xv = (double)(float)x[j];
+        for (int t = 0; t < kTiles; t++) g[i][t] = *(const u32x4*)(gr[t] + k);
+      }
 #pragma unroll
-        for (int t = 0; t < kTiles; t++)
-          acc[t] = __builtin_amdgcn_mfma_f64_16x16x4f64(xv, (double)(float)g[t][j], acc[t], 0, 0, 0);
+      for (int i = 0; i < kAhead; i++) {
+        const bool in = 32 * (i0 + kMfmaWaves * i) + 8 * (l & 3) < a.H;
+        stage[w][0][to] = in ? x[i] : u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < kTiles; t++) stage[w][1 + t][to] = in ? g[i][t] : u32x4{0, 0, 0, 0};
+        const f16x8 xi = __builtin_bit_cast(f16x8, stage[w][0][from]);
+#pragma unroll
+        for (int t = 0; t < kTiles; t++) {
+          const f16x8 gi = __builtin_bit_cast(f16x8, stage[w][1 + t][from]);
+          const f32x4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(xi, gi, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+          mags[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(abs8(xi), abs8(gi), mags[t], 0, 0, 0);
+#pragma unroll
+          for (int j = 0; j < 4; j++) acc[t][j] += (double)p[j];
+        }
       }
     }
-    // lane holds tokens 4 i + q, i = 0 .. 3, of expert r16
+    // lane holds tokens 4q + j, j = 0 .. 3, of expert r16
 #pragma unroll
     for (int t = 0; t < kTiles; t++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) part[w][t][64 * i + l] = acc[t][i];
+      for (int j = 0; j < 4; j++) {
+        part[w][t][16 * (4 * q + j) + r16] = acc[t][j];
+        most[j] = mags[t][j] > most[j] ? mags[t][j] : most[j];
+      }
     __syncthreads();
     for (int i = tid; i < 256 * kTiles; i += 64 * kMfmaWaves) {
       const int t = i >> 8, j = i & 255, e = e0 + 16 * t + (j & 15);
@@ -368,7 +430,67 @@ __global__ __launch_bounds__(64 * kMfmaWaves) void k_route_mfma(RouteArgs a) {
     }
     __syncthreads();
   }
-  for (int t = w; t < kTileToks && s0 + t < a.S; t += kMfmaWaves) choose<kPer>(a, s0 + t, lg[t], part[w][0]);
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    float v = most[j];
+    v = __builtin_fmaxf(v, row_ror<8>(v));
+    v = __builtin_fmaxf(v, row_ror<4>(v));
+    v = __builtin_fmaxf(v, row_ror<2>(v));
+    v = __builtin_fmaxf(v, row_ror<1>(v));
+    if (r16 == 0) mag[w][4 * q + j] = v;
+  }
+  __syncthreads();
+  // A step's 32 additions lose at most half an fp32 step each of the magnitudes'
+  // sum; twice that, as the magnitudes' sums lose as much.  (What is no number shows
+  // in the logits.)
+  double far = 0.0;
+#pragma unroll
+  for (int k = 0; k < kMfmaWaves; k++) far += (double)mag[k][w];
+  far *= 0x1p-18;
+  bool todo = s0 + w < a.S;
+  for (int pass = 0;; pass++) {  // (all waves take the same turns)
+    if (todo && !choose<kPer>(a, s0 + w, lg[w], part[w][0], far, doubt[w]) && l == 0) atomicOr(&again, 1 << w);
+    __syncthreads();
+    const int bits = again;
+    if (pass == 1 || !bits) break;
+    for (int left = bits; left; left &= left - 1) {
+      const int t = __builtin_ctz(left);
+      const uint16_t* xt = a.x + (size_t)(s0 + t) * a.H;
+      uint64_t of[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; i++) of[i] = doubt[t][i];
+      // the n-th of them is wave n's
+      auto take = [&](int n) __attribute__((always_inline)) {
+        int e = -1;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+          const int c = __popcll(of[i]);
+          if (e < 0 && n >= 0 && n < c) {
+            uint64_t b = of[i];
+            for (int k = 0; k < n; k++) b &= b - 1;
+            e = 64 * i + __builtin_ctzll(b);
+          }
+          n -= c;
+        }
+        return e;
+      };
+      for (int n = w, e; (e = take(n)) >= 0; n += kMfmaWaves) {
+        const uint16_t* gr = a.gate + (size_t)e * a.H;
+        double v = 0.0;
+#pragma unroll 4
+        for (int c = 8 * l; c < a.H; c += 512) {
+          const f16x8 xv = *(const f16x8*)(xt + c), gv = *(const f16x8*)(gr + c);
+#pragma unroll
+          for (int j = 0; j < 8; j++) v = __builtin_fma((double)(float)xv[j], (double)(float)gv[j], v);
+        }
+        v = wave_sum_f64(v);
+        if (l == 0) lg[t][e] = v;
+      }
+    }
+    __syncthreads();
+    todo = todo && bits >> w & 1;
+    far = 0.0;
+  }
 }
 
 template <int kPer>

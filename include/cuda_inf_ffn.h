@@ -35,7 +35,8 @@ extern "C" {
  * each of the S rows of H.
  * h, add, hsum: fp32 [S][H]; add may be NULL (nothing is added); hsum may be
  * NULL (the sum is not kept), h or add (in place).  w: fp16 [H].  out: fp16
- * [S][H].  H a multiple of 8; all pointers 16-byte aligned.  Sums are fp32. */
+ * [S][H].  H a multiple of 8, S at most CIA_FFN_MAX_TOKENS; all pointers
+ * 16-byte aligned.  Sums are fp32. */
 int cia_add_rmsnorm(const float* h, const float* add, const uint16_t* w,
                     float eps, float* hsum, uint16_t* out, int S, int H,
                     void* stream);
@@ -65,15 +66,18 @@ typedef struct cia_moe_gating {
  * NULL, used for the choice alone.  ids: int32 [S][top_k]; weights: fp32
  * [S][top_k]; logits: fp32 [S][n_experts], may be NULL.  H a multiple of 8;
  * x and gate 16-byte aligned.
- * Logits, scores and the choice are computed in 64 bits and the outputs rounded
- * once, so a token's experts do not depend on the other tokens of the call.
+ * The choice is the one of logits summed in 64 bits, so a token's experts do
+ * not depend on the other tokens of the call.  Logits are at most 2^-19 of
+ * sum |gate x| and half an fp32 step off, weights as far as that moves them.
  * A c that is not a number ranks with -inf; a softmax over logits that are all
- * -inf gives scores of 0; a sum + eps of 0 gives weights of 0. */
+ * -inf gives scores of 0, one with a NaN or +inf among them NaN; a sum + eps
+ * of 0 gives weights of 0.  S at most CIA_FFN_MAX_TOKENS. */
 int cia_moe_route(const uint16_t* x, const uint16_t* gate, const float* bias,
                   const cia_moe_gating* g, int32_t* ids, float* weights,
                   float* logits, int S, int H, void* stream);
 
-/* The same from logits fp32 [S][n_experts] that the caller has. */
+/* The same from logits fp32 [S][n_experts] that the caller has, in 64 bits up
+ * to one rounding of the weights. */
 int cia_moe_select(const float* logits, const float* bias,
                    const cia_moe_gating* g, int32_t* ids, float* weights, int S,
                    void* stream);

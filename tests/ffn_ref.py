@@ -61,6 +61,23 @@ def choose(logits, bias, k, score="sigmoid", n_group=1, topk_group=1, renorm=Tru
     return ids, wt
 
 
+def weights_bound(logits, far, ids, weights, score="sigmoid", renorm=True, scale=1.0, eps=1e-6, **kw):
+    """Of the weights of experts ids, their logits at most far off."""
+    most = far.max(1, keepdims=True)
+    if score == "sigmoid":  # slope s (1 - s) <= 1/4, and its square
+        s = 1.0 / (1.0 + np.exp(-logits))
+        ds = np.take_along_axis(s * (1 - s) * far + far * far, ids, 1)
+    else:                   # s (dl - sum s dl), and its square
+        p = np.exp(logits - logits.max(1, keepdims=True))
+        s = p / p.sum(1, keepdims=True)
+        ds = np.take_along_axis(s * 2 * most * (1 + 2 * most), ids, 1)
+    s = np.take_along_axis(s, ids, 1)
+    if renorm:
+        total = s.sum(1, keepdims=True) + eps
+        ds = (ds + s / total * ds.sum(1, keepdims=True)) / (total - ds.sum(1, keepdims=True))
+    return abs(scale) * ds * 1.01 + 1.001 * U24 * np.abs(weights) + 1e-12
+
+
 def pairs(ids, S, k, E):
     """(row s * k + j, token s, expert) of the pairs that take part."""
     if ids is None:
