@@ -33,6 +33,8 @@ struct MoeArgs {
   float* y;               // down: [S k][N]
   const int* plan;        // k_moe_plan's; null: every workgroup finds its tile
   int splits;             // down: parts of K, each into its own y
+  const float* res;       // down in tiles of a dense layer, one part: straight into out
+  float* out;             // null: into y
 };
 
 // Rows of a row tile.  The plan lists the tiles: the whole ones of all experts,
@@ -361,6 +363,9 @@ struct TileLoop {
         load_a(at, 0, A[0]);
       }
       __builtin_amdgcn_sched_barrier(0);
+      // (the wave with products before the one that dequantises: 2 %)
+      if (u == 0) __builtin_amdgcn_s_setprio(0);
+      if (u == 1) __builtin_amdgcn_s_setprio(1);
       if (u + 1 < kUnits && u != 3) load_a(at, u + 1, A[(u + 1) & 1]);
 #pragma unroll
       for (int s = 0; s < 4; s++)
@@ -375,23 +380,6 @@ struct TileLoop {
         scale(kUnits - 1, 1, scl_old);
       else
         scale(u - 1, (u - 1) & 1, scl);
-#pragma unroll
-      for (int k = 0; k < 4; k++)
-        if (u == 0) {
-#pragma unroll
-          for (int j = 0; j < kNT; j++) {
-            __builtin_amdgcn_sched_group_barrier(0x002, 13, 0);  // vector instructions
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // one MFMA
-          }
-          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // one LDS read
-        } else {
-#pragma unroll
-          for (int j = 0; j < kNT; j++) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x002, 1, 0);
-          }
-          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        }
     }
     return after(at);
   }
@@ -499,9 +487,12 @@ __device__ __forceinline__ void tile_run(const MoeArgs& a, uint8_t* lds, uint16_
 #pragma unroll
       for (int k = 0; k < 4 * kNT; k++) {
         const int i = 64 * k + l, r = i / (4 * kNT), ch = i % (4 * kNT), n = c0 + 4 * ch;
-        if (64 * half + r < nrows && n < a.N)
-          *(f32x4*)(y + (uint64_t)(uint32_t)rows[64 * half + r] * (uint32_t)a.N + n) =
-              *(const f32x4*)((const float*)out + r * kRow + 4 * ch);
+        if (64 * half + r < nrows && n < a.N) {
+          const uint64_t o = (uint64_t)(uint32_t)rows[64 * half + r] * (uint32_t)a.N + n;
+          f32x4 v = *(const f32x4*)((const float*)out + r * kRow + 4 * ch);
+          if (a.out) v += *(const f32x4*)(a.res + o);
+          *(f32x4*)((a.out ? a.out : y) + o) = v;
+        }
       }
     }
   }
@@ -1105,14 +1096,28 @@ __global__ __launch_bounds__(256) void k_moe_combine(CombineArgs a) {
     const int s = b / nc, c = (b % nc * 256 + threadIdx.x) * 4;
     if (c >= a.H) continue;
     f32x4 v = *(const f32x4*)(a.res + (size_t)s * a.H + c);
-    for (int j = 0; j < a.k; j++) {
-      const int p = s * a.k + j, e = a.ids ? a.ids[p] : 0;
-      if ((unsigned)e >= (unsigned)a.E) continue;
-      const float w = a.weights ? a.weights[p] : 1.0f;
-      f32x4 y = *(const f32x4*)(a.y + (size_t)p * a.H + c);
-      for (int i = 1; i < a.splits; i++) y += *(const f32x4*)(a.y + ((size_t)i * a.S * a.k + p) * a.H + c);
+    for (int j0 = 0; j0 < a.k; j0 += 4) {  // 4 rows' loads together
+      f32x4 y[4];
+      float w[4];
+      bool live[4];
 #pragma unroll
-      for (int i = 0; i < 4; i++) v[i] = __builtin_fmaf(w, y[i], v[i]);
+      for (int j = 0; j < 4; j++) {
+        const int p = s * a.k + (j0 + j < a.k ? j0 + j : a.k - 1), e = a.ids ? a.ids[p] : 0;
+        live[j] = j0 + j < a.k && (unsigned)e < (unsigned)a.E;
+        w[j] = a.weights ? a.weights[p] : 1.0f;
+        y[j] = *(const f32x4*)(a.y + (size_t)p * a.H + c);  // (in ws whether written or not)
+      }
+      for (int i = 1; i < a.splits; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int p = s * a.k + (j0 + j < a.k ? j0 + j : a.k - 1);
+          y[j] += *(const f32x4*)(a.y + ((size_t)i * a.S * a.k + p) * a.H + c);
+        }
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (live[j]) v[i] = __builtin_fmaf(w[j], y[j][i], v[i]);
     }
     *(f32x4*)(a.out + (size_t)s * a.H + c) = v;
   }
@@ -1315,6 +1320,11 @@ static int moe_down(const uint16_t* act, const int32_t* ids, const float* weight
     else
       hipLaunchKernelGGL(k_moe_few<4>, grid, block, 0, s, f);
     return launch_status();
+  }
+  if (!ids && !weights && a.splits == 1 && !streams(false, (int64_t)S * k, E, F)) {
+    a.res = res;
+    a.out = out;
+    return products<false>(a, ws, planned, s);
   }
   if ((st = products<false>(a, ws, planned, s))) return st;
   const CombineArgs c{a.y, ids, weights, res, out, S, k, E, H, a.splits};

@@ -225,6 +225,7 @@ SIZES = [
     (300, 3, 6, 384, 256, "holes"),
     (700, 4, 8, 256, 256, "skew"),
     (1111, 1, 1, 256, 384, "dense"),
+    (4200, 1, 1, 128, 256, "dense"),
     (1500, 2, 16, 2048, 128, "even"),
     (1300, 2, 4, 128, 2304, "holes"),
 ]
