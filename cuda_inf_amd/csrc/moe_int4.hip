@@ -324,11 +324,13 @@ struct TileLoop {
       for (int r = 0; r < 4; r++) C[row_tile][j][r] = __builtin_fmaf(P[p][j][r], sc[j], C[row_tile][j][r]);
   }
   __device__ __forceinline__ static int after(int at) { return at == 2 * T::kX ? 0 : at + T::kX; }
-  // all but the last kLeft fetches have landed
+  // All but the last kLeft fetches have landed, and every LDS read has its data:
+  // products are not held by the barrier, and the wait of the last ones for their
+  // operands could follow it, with the operands' slot already being fetched into.
   template <int kLeft>
   __device__ __forceinline__ static void meet() {
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0F70 | kLeft);  // vmcnt
+    __builtin_amdgcn_s_waitcnt(0x0070 | kLeft);  // vmcnt(kLeft) lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   }

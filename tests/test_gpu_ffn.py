@@ -323,6 +323,35 @@ def test_a_bad_row_stays_alone(K, dev, S):
     assert not np.isfinite(o[bad]).any() and np.isfinite(o[keep]).all()
 
 
+@pytest.mark.parametrize("S,k,E,H,F", [(2300, 4, 16, 512, 1792), (900, 1, 1, 384, 2048), (700, 2, 8, 1024, 384),
+                                       (40, 4, 32, 1024, 512)])
+def test_passes_without_a_wait(K, dev, S, k, E, H, F):
+    """Passes in a row, two sets of inputs in turn, nothing waiting between them: every
+    one gives the first one's bits."""
+    rng = np.random.default_rng(S)
+    sets = []
+    for _ in range(2):
+        x = t(rng.standard_normal((S, H)).astype(np.float16), dev)
+        w = [tuple(t(a, dev) for a in ref.quant(rng, E, r, c)[:2]) for r, c in ((F, H), (F, H), (H, F))]
+        ids = t(make(rng, S, k, E, H, F, "even" if E > 1 else "dense"), dev)
+        wt = t(rng.random((S, k)).astype(np.float32), dev) if E > 1 else None
+        res = t(rng.standard_normal((S, H)).astype(np.float32), dev)
+        ws = torch.empty(K.moe_workspace_bytes(S, k, E, H, F), dtype=torch.uint8, device=dev)
+        sets.append((x, w, ids, wt, res, ws))
+    got = [[], []]
+    for i in range(24):
+        x, w, ids, wt, res, ws = sets[i & 1]
+        act = torch.empty((S, k, F), dtype=torch.float16, device=dev)
+        out = torch.empty((S, H), device=dev)
+        K.moe_up_int4(x, ids, w[0], w[1], act, S, k, ws)
+        K.moe_down_int4(act, ids, wt, w[2], res, out, S, k, ws)
+        got[i & 1].append((act, out))
+    torch.cuda.synchronize()
+    for passes in got:
+        for act, out in passes[1:]:
+            assert torch.equal(act, passes[0][0]) and torch.equal(out, passes[0][1])
+
+
 # ------------------------------------------------------------------ together
 def block(dev, rng, E, k, H, F, max_batch, **kw):
     from cuda_inf_amd.layer import MoeBlock
