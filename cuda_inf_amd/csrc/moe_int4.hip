@@ -1372,13 +1372,15 @@ extern "C" int64_t cia_moe_block_workspace_bytes(const cia_moe* M, int cap) {
 }
 
 extern "C" int cia_moe_block_forward(const cia_moe* M, float* h, int S, void* stream) {
-  CIA_REQUIRE(M && h, CIA_ERR_NULL);
+  CIA_REQUIRE(M, CIA_ERR_NULL);
   CIA_REQUIRE(S >= 0 && S <= M->cap, CIA_ERR_ARG);
   if (S == 0) return CIA_OK;
+  CIA_REQUIRE(h, CIA_ERR_NULL);
   const int k = M->gate ? M->gating.top_k : 1, E = M->gate ? M->gating.n_experts : 1;
   CIA_REQUIRE(M->ws, CIA_ERR_NULL);
   CIA_REQUIRE(aligned(M->ws, 16), CIA_ERR_ALIGN);
-  // all of the branch's arguments before its first launch
+  // the branch's arguments before its first launch (the norm checks its own, and is
+  // the first; h is written by the last)
   int st = moe_check(S, k, E, M->H, M->F, M->gate ? (const int32_t*)M->ws : nullptr);
   if (st) return st;
   CIA_REQUIRE(M->ws_bytes >= cia_moe_block_workspace_bytes(M, S), CIA_ERR_ARG);

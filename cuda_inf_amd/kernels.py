@@ -257,12 +257,22 @@ def qkv_proj_int4(x, wq, wk, wv, q, k, v, M: int, K: int = 2048) -> None:
 
 
 # ------------------------------------------------------------ feed-forward branch
+def _stream_here(*tensors) -> int:
+    """stream_handle(), once every tensor is found on the current device."""
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{dev}")
+    return stream_handle()
+
+
 def add_rmsnorm(h, w, out, S: int, H: int, eps: float = 1e-5, add=None, hsum=None) -> None:
     """engine.cu:867, 870: hsum = h + add (fp32 [S, H]; add and hsum optional,
     hsum may be h or add), out = fp16(hsum * rsqrt(mean(hsum^2) + eps) * w)."""
     f32 = (torch.float32,)
     call("cia_add_rmsnorm", _dev(h, "h", f32, S * H), _opt(add, "add", f32, S * H), _dev(w, "w", _F16, H),
-         float(eps), _opt(hsum, "hsum", f32, S * H), _dev(out, "out", _F16, S * H), S, H, stream_handle())
+         float(eps), _opt(hsum, "hsum", f32, S * H), _dev(out, "out", _F16, S * H), S, H,
+         _stream_here(h, add, w, hsum, out))
 
 
 def moe_gating(E: int, k: int, score: str = "sigmoid", n_group: int = 1, topk_group: int = 1,
@@ -284,7 +294,7 @@ def moe_route(x, gate, ids, weights, S: int, H: int, E: int, k: int, bias=None, 
     call("cia_moe_route", _dev(x, "x", _F16, S * H), _dev(gate, "gate", _F16, E * H),
          _opt(bias, "bias", f32, E), ctypes.byref(moe_gating(E, k, **gating)),
          _dev(ids, "ids", (torch.int32,), S * k), _dev(weights, "weights", f32, S * k),
-         _opt(logits, "logits", f32, S * E), S, H, stream_handle())
+         _opt(logits, "logits", f32, S * E), S, H, _stream_here(x, gate, bias, ids, weights, logits))
 
 
 def moe_select(logits, ids, weights, S: int, E: int, k: int, bias=None, **gating) -> None:
@@ -292,7 +302,7 @@ def moe_select(logits, ids, weights, S: int, E: int, k: int, bias=None, **gating
     f32 = (torch.float32,)
     call("cia_moe_select", _dev(logits, "logits", f32, S * E), _opt(bias, "bias", f32, E),
          ctypes.byref(moe_gating(E, k, **gating)), _dev(ids, "ids", (torch.int32,), S * k),
-         _dev(weights, "weights", f32, S * k), S, stream_handle())
+         _dev(weights, "weights", f32, S * k), S, _stream_here(logits, bias, ids, weights))
 
 
 def q4_experts(w, name: str):
@@ -338,7 +348,7 @@ def moe_up_int4(x, ids, w1, w3, act, S: int, k: int, ws) -> None:
         raise ValueError(f"w3: experts {(E3, F3, H3)}, but w1 has {(E, F, H)}")
     call("cia_moe_up_int4", _dev(x, "x", _F16, S * H), _opt(ids, "ids", (torch.int32,), S * k),
          ctypes.byref(q1), ctypes.byref(q3), _dev(act, "act", _F16, S * k * F), S, k, E, H, F,
-         _dev(ws, "ws", (torch.uint8,)), ws.numel(), stream_handle())
+         _dev(ws, "ws", (torch.uint8,)), ws.numel(), _stream_here(x, ids, w1[0], w3[0], act, ws))
 
 
 def moe_down_int4(act, ids, weights, w2, res, out, S: int, k: int, ws) -> None:
@@ -350,4 +360,4 @@ def moe_down_int4(act, ids, weights, w2, res, out, S: int, k: int, ws) -> None:
     call("cia_moe_down_int4", _dev(act, "act", _F16, S * k * F), _opt(ids, "ids", (torch.int32,), S * k),
          _opt(weights, "weights", f32, S * k), ctypes.byref(q2), _dev(res, "res", f32, S * H),
          _dev(out, "out", f32, S * H), S, k, E, H, F, _dev(ws, "ws", (torch.uint8,)), ws.numel(),
-         stream_handle())
+         _stream_here(act, ids, weights, w2[0], res, out, ws))

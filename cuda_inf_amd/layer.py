@@ -15,8 +15,8 @@ import torch
 from . import _lib
 from ._lib import (D, KVGROUP, NH, NKV, NSPLIT_DEFAULT, call, cia_append_op, cia_attn_proj,
                    cia_layer, cia_moe)
-from .kernels import (decode_workspace_bytes, h2o_workspace_bytes, moe_gating, q4_experts,
-                      stream_handle)
+from .kernels import (_stream_here, decode_workspace_bytes, h2o_workspace_bytes, moe_gating,
+                      q4_experts, stream_handle)
 
 HIDDEN = _lib.HIDDEN
 
@@ -224,13 +224,13 @@ class MoeBlock:
     ``norm_w``: fp16 [H].  ``w1``, ``w3`` ([E, F, H]) and ``w2`` ([E, H, F]):
     INT4 group-128 experts as (packed u8 [E, rows, cols / 2], scales fp16
     [E, rows, cols / 128]) pairs of device tensors.  ``gate`` (fp16 [E, H]) with
-    ``top_k`` and the other arguments of ``kernels.moe_gating`` routes; without
-    it the layer is dense (E = 1).  ``bias``: fp32 [E], for the choice alone.
-    ``max_batch``: tokens a call may bring.
+    ``top_k``, ``renorm_eps`` and the other arguments of ``kernels.moe_gating``
+    routes; without it the layer is dense (E = 1).  ``bias``: fp32 [E], for the
+    choice alone.  ``eps``: the norm's.  ``max_batch``: tokens a call may bring.
     """
 
     def __init__(self, norm_w, w1, w3, w2, *, gate=None, bias=None, top_k: int = 1, eps: float = 1e-5,
-                 max_batch: int = 4096, device="cuda", **gating):
+                 renorm_eps: float = 1e-6, max_batch: int = 4096, device="cuda", **gating):
         dev = torch.device(device)
         M = cia_moe()
         M.w1, E, F, H = q4_experts(w1, "w1")
@@ -246,8 +246,10 @@ class MoeBlock:
             if t is not None and (t.dtype != dtype or not t.is_cuda or not t.is_contiguous()
                                   or tuple(t.shape) != shape):
                 raise ValueError(f"{name}: need a contiguous device {dtype} tensor {shape}")
+        if dev.index is None:
+            dev = norm_w.device
         for t in (norm_w, *w1, *w3, *w2, gate, bias):
-            if t is not None and dev.index is not None and t.device != dev:
+            if t is not None and t.device != dev:
                 raise ValueError(f"a weight is on {t.device}, the layer on {dev}")
         self.H, self.max_batch = H, max_batch
         self._keep = (norm_w, w1, w3, w2, gate, bias)
@@ -255,7 +257,7 @@ class MoeBlock:
         if gate is not None:
             M.gate = gate.data_ptr()
             M.bias = None if bias is None else bias.data_ptr()
-            M.gating = moe_gating(E, top_k, **gating)
+            M.gating = moe_gating(E, top_k, eps=renorm_eps, **gating)
         M.cap = max_batch
         M.ws_bytes = _lib.lib().cia_moe_block_workspace_bytes(ctypes.byref(M), max_batch)
         self.ws = torch.empty(max(M.ws_bytes, 16), dtype=torch.uint8, device=dev)
@@ -270,4 +272,4 @@ class MoeBlock:
             raise ValueError(f"h: need a contiguous device fp32 tensor [S, {self.H}]")
         if S > self.max_batch:
             raise ValueError(f"S={S} exceeds max_batch={self.max_batch}")
-        call("cia_moe_block_forward", ctypes.byref(self._m), h.data_ptr(), S, stream_handle())
+        call("cia_moe_block_forward", ctypes.byref(self._m), h.data_ptr(), S, _stream_here(h, self.ws))

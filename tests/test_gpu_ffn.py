@@ -226,6 +226,9 @@ SIZES = [
     (700, 4, 8, 256, 256, "skew"),
     (1111, 1, 1, 256, 384, "dense"),
     (4200, 1, 1, 128, 256, "dense"),
+    (20, 1, 1, 256, 256, "holes"),
+    (1400, 1, 1, 128, 128, "holes"),
+    (8500, 2, 6, 128, 128, "holes"),
     (1500, 2, 16, 2048, 128, "even"),
     (1300, 2, 4, 128, 2304, "holes"),
 ]
@@ -470,6 +473,30 @@ def test_block_captured(K, dev):
             B.forward(e)
             torch.cuda.synchronize()
             assert torch.equal(e, o)
+
+
+def test_blocks_refusals(K, dev):
+    rng = np.random.default_rng(3)
+    B, _ = block(dev, rng, 4, 2, 256, 128, max_batch=4, score="softmax", renorm=False, renorm_eps=0.0, scale=1.5)
+    B.forward(torch.zeros((0, 256), device=dev))
+    for bad, what in ((torch.zeros((5, 256), device=dev), "max_batch"), (torch.zeros((1, 255), device=dev), "fp32"),
+                      (torch.zeros((1, 256), dtype=torch.float16, device=dev), "fp32"),
+                      (torch.zeros((1, 256)), "device"), (torch.zeros((256, 2), device=dev).t(), "contiguous")):
+        with pytest.raises(ValueError, match=what):
+            B.forward(bad)
+    norm_w, w1, w3, w2, gate, bias = B._keep
+    from cuda_inf_amd.layer import MoeBlock
+    for args, kw in (((norm_w, w1, w3, w3), dict(gate=gate)), ((norm_w, w1, w3, w2), dict()),
+                     ((norm_w[:-1], w1, w3, w2), dict(gate=gate)), ((norm_w, w1, w3, w2), dict(gate=gate.float())),
+                     ((norm_w, w1, w3, w2), dict(gate=gate, bias=bias[:2]))):
+        with pytest.raises(ValueError):
+            MoeBlock(*args, device=dev, **kw)
+    with pytest.raises(ValueError, match="contiguous"):
+        K.moe_up_int4(norm_w, None, (w1[0][:, :, ::2], w1[1]), w3, norm_w, 1, 1, B.ws)
+    with pytest.raises(ValueError, match="do not fit"):
+        K.moe_up_int4(norm_w, None, (w1[0], w1[1][:, 1:]), w3, norm_w, 1, 1, B.ws)
+    with pytest.raises(ValueError, match="w3: experts"):
+        K.moe_up_int4(norm_w, None, w1, w2, norm_w, 1, 1, B.ws)
 
 
 def test_another_stream(K, dev):
