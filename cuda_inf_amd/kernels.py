@@ -263,7 +263,7 @@ def _stream_here(*tensors) -> int:
     for t in tensors:
         if t is not None and t.get_device() != dev:
             raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{dev}")
-    return stream_handle()
+    return stream_handle() if _raw_stream is None else _raw_stream(dev)
 
 
 def add_rmsnorm(h, w, out, S: int, H: int, eps: float = 1e-5, add=None, hsum=None) -> None:

@@ -272,4 +272,6 @@ class MoeBlock:
             raise ValueError(f"h: need a contiguous device fp32 tensor [S, {self.H}]")
         if S > self.max_batch:
             raise ValueError(f"S={S} exceeds max_batch={self.max_batch}")
-        call("cia_moe_block_forward", ctypes.byref(self._m), h.data_ptr(), S, _stream_here(h, self.ws))
+        if h.device != self.ws.device:
+            raise ValueError(f"h is on {h.device}, the layer on {self.ws.device}")
+        call("cia_moe_block_forward", ctypes.byref(self._m), h.data_ptr(), S, _stream_here(h))
