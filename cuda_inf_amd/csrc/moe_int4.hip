@@ -1,6 +1,6 @@
-// moe_int4.hip -- the experts' INT4 group-128 products (the expert loop of
-// engine.cu:894-905: w1, w3, swiglu, w2, acc_scaled) on gfx950, for all the
-// tokens of a call and the experts each has chosen.
+// moe_int4.hip -- the experts' INT4 group-128 products (w1, w3, swiglu, w2 and
+// acc_scaled of engine.cu:869-905) on gfx950, for all the tokens of a call and the
+// experts each has chosen.
 //
 //   up    act[s][j] = fp16(silu(g) * u),  g = W1[e] x[s], u = W3[e] x[s],
 //         e = ids[s][j], silu(g) = g / (1 + exp(-g))
@@ -930,10 +930,11 @@ __global__ __launch_bounds__(64 * kStreamWaves, (2 * Stream<kG, kMT>::kPerUnit))
 // Down for up to kFewPairs pairs: a workgroup takes 16 columns of out through all
 // the experts that have a row, so that it can weight the rows and add them to the
 // residual itself, and no launch follows.  The waves split K as above, the weights
-// of the next kRing segments in flight; 8 segments' sums meet at a time.
+// of the next kRing experts in flight; all the experts' sums meet in LDS at once.
 // (Calls in us, in two launches / so: 1 token, 4 of 32 experts of 1792 11.8 / 8.8;
 // 4 tokens, 16 segments, 16.4 / 19.2.)
 constexpr int kFewPairs = 8;
+static_assert(kFewPairs <= kStreamWaves && kFewPairs <= 16, "a wave an expert's sums; a row tile an expert");
 
 struct FewArgs {
   MoeArgs m;
@@ -945,16 +946,16 @@ struct FewArgs {
 // grid = N / 16, block = 512; K <= 1024 kG
 template <int kG>
 __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_few(FewArgs f) {
-  constexpr int kRing = kG <= 2 ? 4 : 2, kBatch = 8;
+  constexpr int kRing = kG <= 2 ? 4 : 2;
   const MoeArgs& a = f.m;
-  __shared__ f32x4 part[kBatch][kStreamWaves][64];
+  __shared__ f32x4 part[kFewPairs][kStreamWaves][64];
   __shared__ u32x4 stage[kStreamWaves][2][64];
   __shared__ float sums[kFewPairs][16];
-  __shared__ int rows[kStreamWaves][2 * kBatch][16];
+  __shared__ int rows[kStreamWaves][kFewPairs][kFewPairs];
   const int tid = threadIdx.x, l = tid & 63, n16 = l & 15, q = l >> 4, P = a.S * a.k;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c0 = 16 * blockIdx.x;
-  // the rows by expert, 16 a segment, as in k_moe_stream
+  // the rows by expert, lane i with pair i; an expert's first pair stands for it
   int id = l < P ? (a.ids ? a.ids[l] : 0) : -1;
   if ((unsigned)id >= (unsigned)a.E) id = -1;
   // this thread's output: column tid & 15 of token tid >> 4
@@ -970,35 +971,28 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_few(FewArgs f) {
     same &= id >> b & 1 ? v : ~v;
   }
   const uint64_t below = (1ull << l) - 1;
-  const int segs = id >= 0 && !(same & below) ? (__popcll(same) + 15) >> 4 : 0;
-  int before = 0, nseg = 0;
-#pragma unroll
-  for (int k = 1; k <= (kFewPairs + 15) / 16; k++) {
-    const uint64_t v = __ballot(segs >= k);
-    before += __popcll(v & below);
-    nseg += __popcll(v);
-  }
+  const uint64_t firsts = __ballot(id >= 0 && !(same & below));
+  const int nexp = __popcll(firsts);
   const int ng = a.K >> 7, g0 = w * ng / kStreamWaves, mine = (w + 1) * ng / kStreamWaves - g0;
   typedef const __attribute__((address_space(1))) uint16_t* gs_t;
   typedef const __attribute__((address_space(1))) u32x4* gw_t;
   u32x4 wr[kRing][kG];
   uint32_t sr[kRing][kG];
-  // segment sg's expert and its first row's place among the expert's
-  auto expert = [&](int sg, int& r0) __attribute__((always_inline)) {
-    const int at = __builtin_ctzll(__ballot(segs > 0 && sg >= before && sg < before + segs));
-    r0 = (sg - __builtin_amdgcn_readlane(before, at)) * 16;
-    return __builtin_amdgcn_readlane(id, at);
+  // the n-th expert with a row
+  auto expert = [&](int n) __attribute__((always_inline)) {
+    uint64_t m = firsts;
+    for (int i = 0; i < n; i++) m &= m - 1;
+    return __builtin_amdgcn_readlane(id, __builtin_ctzll(m));
   };
   // its weights, scales and x rows of this wave's groups
   f16x8 A[kRing][kG][4];
-  auto fetch = [&](int sg, int d) __attribute__((always_inline)) {
-    if (sg >= nseg) return;
-    int r0;
-    const int e = expert(sg, r0);
+  auto fetch = [&](int n, int d) __attribute__((always_inline)) {
+    if (n >= nexp) return;
+    const int e = expert(n);
     const uint64_t m = __ballot(id == e);
-    const int r = __popcll(m & below) - r0;
-    int* const list = rows[w][sg % (2 * kBatch)];
-    if (id == e && r >= 0 && r < 16) list[r] = l;
+    const int left = __popcll(m);
+    int* const list = rows[w][n];
+    if (id == e) list[__popcll(m & below)] = l;
     if (mine == 0) return;
     const Cols<false> col(a, e, false);
     const gw_t wp = (gw_t)(col.packed(c0 + (l >> 2)) + 64 * (size_t)g0 + 16 * (l & 3));
@@ -1010,9 +1004,9 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_few(FewArgs f) {
       sr[d][g] = sp[gg];
     }
     // (rows past the last one: the first, its products are not read)
-    const int p = list[n16 < __popcll(m) - r0 ? n16 : 0];
+    const int p = list[n16 < left ? n16 : 0];
     const gw_t xr = (gw_t)(a.x + (uint64_t)(uint32_t)p * (uint32_t)a.K + 128 * g0 + 32 * q);
-    if (n16 < __popcll(m) - r0)
+    if (n16 < left)
 #pragma unroll
       for (int g = 0; g < kG; g++)
 #pragma unroll
@@ -1026,49 +1020,46 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_few(FewArgs f) {
       for (int s = 0; s < 4; s++) A[d][g][s] = f16x8{};
     fetch(d, d);
   }
-  for (int sb = 0; sb < nseg; sb += kBatch) {
 #pragma unroll
-    for (int b = 0; b < kBatch; b++) {
-      const int sg = sb + b, d = b % kRing;
-      if (sg >= nseg) break;
-      f32x4 acc = {};
-      if (mine > 0) {
-        u32x4 wq[kG];
-        float scl[kG];
+  for (int n = 0; n < kFewPairs; n++) {
+    const int d = n % kRing;
+    if (n >= nexp) break;
+    f32x4 acc = {};
+    if (mine > 0) {
+      u32x4 wq[kG];
+      float scl[kG];
 #pragma unroll
-        for (int g = 0; g < kG; g++) {
-          u32x4* st = stage[w][g & 1];
-          st[(l & ~3) | ((l & 3) ^ ((l >> 4) & 3))] = wr[d][g];
-          wq[g] = st[4 * n16 + (q ^ ((n16 >> 2) & 3))];
-          scl[g] = g < mine ? h2f((uint16_t)sr[d][g]) : 0.f;
-        }
-#pragma unroll
-        for (int g = 0; g < kG; g++) {
-          f32x4 Pg = {};
-#pragma unroll
-          for (int s = 0; s < 4; s++) Pg = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[d][g][s], nib8(wq[g][s]), Pg, 0, 0, 0);
-          if (g < mine)
-#pragma unroll
-            for (int i = 0; i < 4; i++) acc[i] = __builtin_fmaf(Pg[i], scl[g], acc[i]);
-        }
+      for (int g = 0; g < kG; g++) {
+        u32x4* st = stage[w][g & 1];
+        st[(l & ~3) | ((l & 3) ^ ((l >> 4) & 3))] = wr[d][g];
+        wq[g] = st[4 * n16 + (q ^ ((n16 >> 2) & 3))];
+        scl[g] = g < mine ? h2f((uint16_t)sr[d][g]) : 0.f;
       }
-      fetch(sg + kRing, d);
-      part[b][w][l] = acc;
-    }
-    __syncthreads();
-    // wave b adds up segment sb + b (its own list of its rows)
-    if (sb + w < nseg) {
-      f32x4 v = {};
 #pragma unroll
-      for (int k = 0; k < kStreamWaves; k++) v += part[w][k][l];
-      int r0;
-      const int e = expert(sb + w, r0), left = __popcll(__ballot(id == e)) - r0;
+      for (int g = 0; g < kG; g++) {
+        f32x4 Pg = {};
 #pragma unroll
-      for (int i = 0; i < 4; i++)
-        if (4 * q + i < left) sums[rows[w][(sb + w) % (2 * kBatch)][4 * q + i]][n16] = v[i];
+        for (int s = 0; s < 4; s++) Pg = __builtin_amdgcn_mfma_f32_16x16x32_f16(A[d][g][s], nib8(wq[g][s]), Pg, 0, 0, 0);
+        if (g < mine)
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc[i] = __builtin_fmaf(Pg[i], scl[g], acc[i]);
+      }
     }
-    __syncthreads();
+    fetch(n + kRing, d);
+    part[n][w][l] = acc;
   }
+  __syncthreads();
+  // wave n adds up the n-th expert's (its own list of its rows)
+  if (w < nexp) {
+    f32x4 v = {};
+#pragma unroll
+    for (int k = 0; k < kStreamWaves; k++) v += part[w][k][l];
+    const int left = __popcll(__ballot(id == expert(w)));
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (4 * q + i < left) sums[rows[w][w][4 * q + i]][n16] = v[i];
+  }
+  __syncthreads();
   float v = old;
   for (int j = 0; j < a.k; j++) {
     const int p = so < a.S ? so * a.k + j : 0;
@@ -1154,7 +1145,7 @@ static int moe_check(int S, int k, int E, int H, int F, const int32_t* ids) {
 // an expert's strides hold its rows
 static int q4_check(const cia_q4_experts* w, int E, int64_t rows, int64_t cols) {
   CIA_REQUIRE(w && w->packed && w->scales, CIA_ERR_NULL);
-  CIA_REQUIRE(aligned(w->packed, 16) && aligned(w->scales, 2) && w->packed_stride % 16 == 0, CIA_ERR_ALIGN);
+  CIA_REQUIRE(aligned(w->packed, 16) && aligned(w->scales, 2) && (E == 1 || w->packed_stride % 16 == 0), CIA_ERR_ALIGN);
   CIA_REQUIRE(E == 1 || (w->packed_stride >= rows * cols / 2 && w->scales_stride >= rows * cols / 128), CIA_ERR_ARG);
   return CIA_OK;
 }
@@ -1251,7 +1242,8 @@ static int products(MoeArgs& a, void* ws, bool planned, hipStream_t s) {
 using namespace cia;
 
 extern "C" int64_t cia_moe_workspace_bytes(int S, int k, int E, int H, int F) {
-  if (S < 0 || k < 1 || E < 1 || H < 1 || F < 1) return 0;
+  if (S < 0 || k < 1 || k > kMoeMaxK || E < 1 || E > kMoeMaxE || H < 1 || H > kMoeMaxCols || F < 1 || F > kMoeMaxCols)
+    return 0;
   const int64_t P = (int64_t)S * k;
   return plan_bytes(P, E) + y_rows(P) * H * 4;
 }
@@ -1366,7 +1358,7 @@ BlockWs block_ws(const cia_moe* M, int S) {
 }  // namespace
 
 extern "C" int64_t cia_moe_block_workspace_bytes(const cia_moe* M, int cap) {
-  if (!M || cap < 0 || M->H < 1 || M->F < 1 || (M->gate && (M->gating.top_k < 1 || M->gating.n_experts < 1)))
+  if (!M || cap < 0 || !cia_moe_workspace_bytes(0, M->gate ? M->gating.top_k : 1, M->gate ? M->gating.n_experts : 1, M->H, M->F))
     return 0;
   return block_ws(M, cap).end;
 }

@@ -1,6 +1,6 @@
 // moe_route.hip -- the router of a layer of experts: logits, scores, choice of
-// k experts and their weights (the host routing of engine.cu:878-893 with its
-// copy of the logits, on the device).
+// k experts and their weights (of engine.cu:869-905, which copies the logits to
+// the host at 880 and chooses there), on the device.
 //
 //   l = gate x,  s = 1 / (1 + exp(-l)) or softmax(l),  c = s + bias
 //   groups: those topk_group of n_group whose two best c have the largest sum
@@ -8,10 +8,12 @@
 //   the lowest index first among equals;  w = s[ids]
 //   renorm: w / (sum w + eps);  then times scale
 //
-// Which experts are chosen is decided in 64 bits from the products on: fp16
-// products are exact there and the order of their sum does not matter (an
-// fp32 sum of 2048 products is 1e-7 off, which moves a choice in one token of
-// some 1e5), so a token's experts do not depend on the batch around it.
+// The experts chosen are those of logits summed in 64 bits: fp16 products are
+// exact there and the order of their sum does not matter (an fp32 sum of 2048
+// products is 1e-7 off, which moves a choice in one token of some 1e5), so a
+// token's experts do not depend on the batch around it.  Few tokens have their sums
+// in 64 bits; of many the matrix cores' fp32 sums decide where their error cannot
+// matter, and 64 bits the rest.
 #include "common.h"
 #include "cuda_inf_ffn.h"
 
@@ -259,13 +261,18 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, int s, const double* 
   return true;
 }
 
-// Few tokens: kT a workgroup of 8 waves, a wave every 8th expert, so that a
-// token's gate is read by all of a compute unit.  x lies in LDS in 64 bits, a
-// lane's 8 elements in four 16-byte pieces kSpan / 8 lanes apart.
-constexpr int kTokWaves = 8;
+// Few tokens: kT a workgroup, its waves every 8th (of many experts every 16th)
+// expert each, so that a token's gate is read by all of a compute unit.  x lies in
+// LDS in 64 bits, a lane's 8 elements in four 16-byte pieces kSpan / 8 lanes apart.
+//   Bound by what the conversions to 64 bits and their products take of a compute
+// unit, and by latency: a token of 32 experts, H = 2048, 6.5 us, 300 of 128, H =
+// 1280, in 8 groups, 18.8 us a call (20.8 with 8 waves; of 32 experts 16 waves take
+// 10.1 instead of 8.3).
+constexpr int tok_waves(int kT, int kPer) { return kT <= 2 && kPer > 1 ? 16 : 8; }
 
 template <int kT, int kPer>
-__global__ __launch_bounds__(64 * kTokWaves) void k_route_tok(RouteArgs a) {
+__global__ __launch_bounds__(64 * tok_waves(kT, kPer)) void k_route_tok(RouteArgs a) {
+  constexpr int kTokWaves = tok_waves(kT, kPer);
   constexpr int kSpan = 4096 / kT;  // elements of a row in LDS at a time
   __shared__ f64x2 xs[kT][4][kSpan / 8];
   __shared__ double lg[kT][kRouteMaxE];
@@ -495,15 +502,18 @@ __global__ __launch_bounds__(64 * kMfmaWaves) void k_route_mfma(RouteArgs a) {
 
 template <int kPer>
 static void route_launch(const RouteArgs& a, hipStream_t s) {
-  const dim3 block(64 * kTokWaves);
-  if (a.x && a.S >= 1024)
+  // Calls in us, 1 token a workgroup / 2 / 16 in tiles: 32 experts, H = 2048, 256
+  // tokens 8.1 / 9.2 / 13.9, 512 10.1 / 9.1 / 14.0, 1024 15.7 / 12.2 / 14.1, 2048
+  // 26.3 / 20.6 / 15.6; 128 experts, H = 1280, 256 15.0 / 18.3 / 28.3, 512 22.8 /
+  // 19.1 / 28.5, 1024 36.3 / 28.9 / 29.0, 2048 65 / 50 / 30.
+  if (a.x && a.S > 1024)
     hipLaunchKernelGGL(k_route_mfma<kPer>, dim3((unsigned)((a.S + kTileToks - 1) / kTileToks)), dim3(64 * kMfmaWaves), 0, s, a);
   else if (!a.x && a.S >= 64)  // (nothing but the choice: a wave a token)
-    hipLaunchKernelGGL((k_route_tok<8, kPer>), dim3((unsigned)((a.S + 7) / 8)), block, 0, s, a);
+    hipLaunchKernelGGL((k_route_tok<8, kPer>), dim3((unsigned)((a.S + 7) / 8)), dim3(64 * tok_waves(8, kPer)), 0, s, a);
   else if (a.S <= 256)
-    hipLaunchKernelGGL((k_route_tok<1, kPer>), dim3((unsigned)a.S), block, 0, s, a);
+    hipLaunchKernelGGL((k_route_tok<1, kPer>), dim3((unsigned)a.S), dim3(64 * tok_waves(1, kPer)), 0, s, a);
   else
-    hipLaunchKernelGGL((k_route_tok<2, kPer>), dim3((unsigned)((a.S + 1) / 2)), block, 0, s, a);
+    hipLaunchKernelGGL((k_route_tok<2, kPer>), dim3((unsigned)((a.S + 1) / 2)), dim3(64 * tok_waves(2, kPer)), 0, s, a);
 }
 
 static int route_run(const RouteArgs& a, hipStream_t s) {
@@ -547,7 +557,7 @@ extern "C" int cia_moe_route(const uint16_t* x, const uint16_t* gate, const floa
   RouteArgs a{};
   const int st = route_args(a, g, S);
   if (st) return st;
-  CIA_REQUIRE(H > 0 && H % 8 == 0, CIA_ERR_ARG);
+  CIA_REQUIRE(H > 0 && H <= CIA_FFN_MAX_WIDTH && H % 8 == 0, CIA_ERR_ARG);
   if (S == 0) return CIA_OK;
   CIA_REQUIRE(x && gate && ids && weights, CIA_ERR_NULL);
   CIA_REQUIRE(aligned(x, 16) && aligned(gate, 16) && aligned(bias, 4) && aligned(ids, 4) &&

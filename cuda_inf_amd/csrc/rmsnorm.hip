@@ -1,5 +1,5 @@
 // rmsnorm.hip -- residual addition and hidden-state RMSNorm (add_f32_inplace,
-// engine.cu:533-536, and rmsnorm, engine.cu:131-144) in one pass on gfx950.
+// engine.cu:527-559, and rmsnorm, engine.cu:131-144) in one pass on gfx950.
 //
 //   hsum = h + add,   out = fp16(hsum * rsqrt(mean(hsum^2) + eps) * w)
 //
@@ -121,7 +121,7 @@ using namespace cia;
 
 extern "C" int cia_add_rmsnorm(const float* h, const float* add, const uint16_t* w, float eps,
                                float* hsum, uint16_t* out, int S, int H, void* stream) {
-  CIA_REQUIRE(S >= 0 && S <= CIA_FFN_MAX_TOKENS && H > 0 && H % kNormVec == 0 && eps >= 0.0f, CIA_ERR_ARG);
+  CIA_REQUIRE(S >= 0 && S <= CIA_FFN_MAX_TOKENS && H > 0 && H <= CIA_FFN_MAX_WIDTH && H % kNormVec == 0 && eps >= 0.0f, CIA_ERR_ARG);
   if (S == 0) return CIA_OK;
   CIA_REQUIRE(h && w && out, CIA_ERR_NULL);
   CIA_REQUIRE(aligned(h, 16) && aligned(add, 16) && aligned(w, 16) && aligned(hsum, 16) && aligned(out, 16),

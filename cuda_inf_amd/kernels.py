@@ -267,7 +267,7 @@ def _stream_here(*tensors) -> int:
 
 
 def add_rmsnorm(h, w, out, S: int, H: int, eps: float = 1e-5, add=None, hsum=None) -> None:
-    """engine.cu:867, 870: hsum = h + add (fp32 [S, H]; add and hsum optional,
+    """add_f32_inplace (engine.cu:867) and rmsnorm (870): hsum = h + add (fp32 [S, H]; add and hsum optional,
     hsum may be h or add), out = fp16(hsum * rsqrt(mean(hsum^2) + eps) * w)."""
     f32 = (torch.float32,)
     call("cia_add_rmsnorm", _dev(h, "h", f32, S * H), _opt(add, "add", f32, S * H), _dev(w, "w", _F16, H),
@@ -286,7 +286,7 @@ def moe_gating(E: int, k: int, score: str = "sigmoid", n_group: int = 1, topk_gr
 
 def moe_route(x, gate, ids, weights, S: int, H: int, E: int, k: int, bias=None, logits=None,
               **gating) -> None:
-    """engine.cu:878-893 on the device: the k experts of each of the S rows of x
+    """The router of engine.cu:869-905 on the device: the k experts of each of the S rows of x
     (fp16 [S, H]; gate fp16 [E, H]; bias fp32 [E], for the choice alone) into
     ids int32 [S, k] and weights fp32 [S, k]; logits fp32 [S, E], optional.
     gating: score, n_group, topk_group, renorm, eps, scale, as moe_gating."""
@@ -338,7 +338,8 @@ def moe_workspace_bytes(S: int, k: int, E: int, H: int, F: int) -> int:
 
 
 def moe_up_int4(x, ids, w1, w3, act, S: int, k: int, ws) -> None:
-    """engine.cu:896-899 for every token and chosen expert: act [S, k, F] fp16 =
+    """w1, w3 and swiglu of engine.cu:869-905 for every token and chosen expert:
+    act [S, k, F] fp16 =
     silu(W1[e] x) * (W3[e] x), e = ids[s, j]; x fp16 [S, H], ids int32 [S, k]
     (outside [0, E): the pair's act row is left as it was; None: one expert,
     every row), w1 and w3 as q4_experts takes them, [E, F, H]."""
@@ -352,8 +353,8 @@ def moe_up_int4(x, ids, w1, w3, act, S: int, k: int, ws) -> None:
 
 
 def moe_down_int4(act, ids, weights, w2, res, out, S: int, k: int, ws) -> None:
-    """engine.cu:900-904 for every token and chosen expert: out [S, H] fp32 = res
-    + sum over j of weights[s, j] * (W2[e] act[s, j]); out may be res; weights
+    """w2 and acc_scaled of engine.cu:869-905 for every token and chosen expert:
+    out [S, H] fp32 = res + sum over j of weights[s, j] * (W2[e] act[s, j]); out may be res; weights
     fp32 [S, k] or None (1); ids as moe_up_int4's; w2 [E, H, F]."""
     q2, E, H, F = q4_experts(w2, "w2")
     f32 = (torch.float32,)

@@ -29,14 +29,15 @@ extern "C" {
 #define CIA_MOE_MAX_WIDTH 32768     /* H and F of the experts */
 #define CIA_MOE_MAX_PAIRS (1 << 20) /* S * k of a call */
 #define CIA_FFN_MAX_TOKENS (1 << 22) /* S of the norm and the router */
+#define CIA_FFN_MAX_WIDTH (1 << 24)  /* their H */
 
-/* add_f32_inplace and rmsnorm (engine.cu:533-536, 131-144; launched at 867 and
+/* add_f32_inplace and rmsnorm (engine.cu:527-559, 131-144; launched at 867 and
  * 870): hsum = h + add, out = fp16(hsum * rsqrt(mean(hsum^2) + eps) * w) for
  * each of the S rows of H.
  * h, add, hsum: fp32 [S][H]; add may be NULL (nothing is added); hsum may be
  * NULL (the sum is not kept), h or add (in place).  w: fp16 [H].  out: fp16
- * [S][H].  H a multiple of 8, S at most CIA_FFN_MAX_TOKENS; all pointers
- * 16-byte aligned.  Sums are fp32. */
+ * [S][H].  H a multiple of 8 and at most CIA_FFN_MAX_WIDTH, S at most
+ * CIA_FFN_MAX_TOKENS; all pointers 16-byte aligned.  Sums are fp32. */
 int cia_add_rmsnorm(const float* h, const float* add, const uint16_t* w,
                     float eps, float* hsum, uint16_t* out, int S, int H,
                     void* stream);
@@ -56,7 +57,8 @@ typedef struct cia_moe_gating {
   float scale;     /* every weight is multiplied by it; finite */
 } cia_moe_gating;
 
-/* The router (engine.cu:878-893, which copies the logits to the host):
+/* The router (of engine.cu:869-905, which copies the logits to the host at 880
+ * and chooses there):
  *   l = gate x;  s = score(l);  c = s + bias;
  *   of the groups, the topk_group whose two best c have the largest sum;
  *   ids = the top_k largest c among the experts of those groups, largest
@@ -64,8 +66,8 @@ typedef struct cia_moe_gating {
  *   (their sum + eps) if renorm, times scale.
  * x: fp16 [S][H]; gate: fp16 [n_experts][H]; bias: fp32 [n_experts], may be
  * NULL, used for the choice alone.  ids: int32 [S][top_k]; weights: fp32
- * [S][top_k]; logits: fp32 [S][n_experts], may be NULL.  H a multiple of 8;
- * x and gate 16-byte aligned.
+ * [S][top_k]; logits: fp32 [S][n_experts], may be NULL.  H a multiple of 8
+ * and at most CIA_FFN_MAX_WIDTH; x and gate 16-byte aligned.
  * The choice is the one of logits summed in 64 bits, so a token's experts do
  * not depend on the other tokens of the call.  Logits are at most 2^-19 of
  * sum |gate x| and half an fp32 step off, weights as far as that moves them.
@@ -85,9 +87,9 @@ int cia_moe_select(const float* logits, const float* bias,
 /* INT4 group-128 weights of E experts, each [rows][cols] in the format of
  * cia_gemv_int4: expert e's packed bytes [rows][cols/2] at
  * packed + e * packed_stride and its fp16 scales [rows][cols/128] at
- * scales + e * scales_stride (elements).  packed 16-byte aligned and
- * packed_stride a multiple of 16; scales 2-byte aligned.  Strides are read only
- * where E > 1 and must then hold an expert: rows * cols / 2 bytes and
+ * scales + e * scales_stride (elements).  packed 16-byte aligned;
+ * scales 2-byte aligned.  Strides are read only where E > 1: packed_stride is
+ * then a multiple of 16, and they hold an expert, rows * cols / 2 bytes and
  * rows * cols / 128 elements at least. */
 typedef struct cia_q4_experts {
   const uint8_t* packed;
@@ -96,7 +98,7 @@ typedef struct cia_q4_experts {
   int64_t scales_stride;
 } cia_q4_experts;
 
-/* The experts' gate and up products with SwiGLU (engine.cu:896-899 for every
+/* The experts' gate and up products with SwiGLU (of engine.cu:869-905, for every
  * token and chosen expert): act[s][j] = fp16(g / (1 + exp(-g)) * u) with
  * g = W1[e] x[s], u = W3[e] x[s], e = ids[s][j].
  * x: fp16 [S][H]; ids: int32 [S][k]; w1, w3: E experts of [F][H];
@@ -113,7 +115,7 @@ int cia_moe_up_int4(const uint16_t* x, const int32_t* ids,
                     int64_t ws_bytes, void* stream);
 
 /* The experts' down products, weighted and added to the residual
- * (engine.cu:900-904): out[s] = res[s] + sum over j, in order, of
+ * (of engine.cu:869-905): out[s] = res[s] + sum over j, in order, of
  * weights[s][j] * (W2[e] act[s][j]).
  * act: fp16 [S][k][F]; weights: fp32 [S][k], NULL: 1; w2: E experts of [H][F];
  * res, out: fp32 [S][H], out may be res.  Pairs outside [0, E) add nothing,
@@ -125,7 +127,7 @@ int cia_moe_down_int4(const uint16_t* act, const int32_t* ids,
                       int F, void* ws, int64_t ws_bytes, void* stream);
 
 /* Workspace bytes of cia_moe_up_int4 and cia_moe_down_int4 for up to S tokens;
- * 0 where the arguments are not positive. */
+ * 0 where S is negative or another argument outside its limits. */
 int64_t cia_moe_workspace_bytes(int S, int k, int E, int H, int F);
 
 /* The feed-forward branch of one layer. */

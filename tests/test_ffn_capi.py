@@ -35,6 +35,8 @@ def test_every_declared_symbol(L):
     ((A, None, A, 1e-5, None, A, -1, 64), ARG),
     ((A, None, A, 1e-5, None, A, 1, 0), ARG),
     ((A, None, A, 1e-5, None, A, 1, 60), ARG),
+    ((A, None, A, 1e-5, None, A, 1, (1 << 24) + 8), ARG),
+    ((A, None, A, 1e-5, None, A, (1 << 22) + 1, 64), ARG),
     ((A, None, A, -1e-5, None, A, 1, 64), ARG),
     ((A, None, A, float("nan"), None, A, 1, 64), ARG),
     ((A + 8, None, A, 1e-5, None, A, 1, 64), ALIGN),
@@ -70,7 +72,7 @@ def test_gating_refusals(L, kw, code):
     ((None, A, None, A, A, None, 1, 64), NULL), ((A, None, None, A, A, None, 1, 64), NULL),
     ((A, A, None, None, A, None, 1, 64), NULL), ((A, A, None, A, None, None, 1, 64), NULL),
     ((A, A, None, A, A, None, -1, 64), ARG), ((A, A, None, A, A, None, 1, 0), ARG),
-    ((A, A, None, A, A, None, 1, 68), ARG), ((A + 8, A, None, A, A, None, 1, 64), ALIGN),
+    ((A, A, None, A, A, None, 1, 68), ARG), ((A, A, None, A, A, None, 1, (1 << 24) + 8), ARG), ((A + 8, A, None, A, A, None, 1, 64), ALIGN),
     ((A, A + 2, None, A, A, None, 1, 64), ALIGN), ((A, A, A + 2, A, A, None, 1, 64), ALIGN),
     ((A, A, None, A + 2, A, None, 1, 64), ALIGN), ((A, A, None, A, A + 1, None, 1, 64), ALIGN),
     ((A, A, None, A, A, A + 2, 1, 64), ALIGN), ((None, None, None, None, None, None, 0, 64), OK),
@@ -151,6 +153,7 @@ def test_down_refusals(L, kw, code):
 def test_workspace_bytes(L):
     f = L.cia_moe_workspace_bytes
     assert f(-1, 4, 32, 2048, 1792) == 0 and f(1, 0, 32, 2048, 1792) == 0 and f(1, 4, 0, 2048, 1792) == 0
+    assert f(1, 17, 32, 2048, 1792) == f(1, 4, 257, 2048, 1792) == f(1, 4, 32, 40000, 1792) == 0
     # more tokens never need less, and sizes past 32 bits are whole
     last = 0
     for S in (0, 1, 2, 7, 100, 5000, 1 << 20):
@@ -158,6 +161,15 @@ def test_workspace_bytes(L):
         assert n >= last
         last = n
     assert last > 1 << 32
+
+
+def test_strides_of_one_expert_are_not_read(L):
+    w = q4(1, 128, 256, packed_stride=-7, scales_stride=-1)
+    n = L.cia_moe_workspace_bytes(1, 1, 1, 256, 128)
+    w2 = q4(1, 256, 128, packed_stride=1, scales_stride=0)
+    # (refused for what is looked at after the strides)
+    assert L.cia_moe_up_int4(A, None, ctypes.byref(w), ctypes.byref(w), A, 1, 1, 1, 256, 128, A, n - 1, None) == ARG
+    assert L.cia_moe_down_int4(A, None, None, ctypes.byref(w2), A, A, 1, 1, 1, 256, 128, A, n - 1, None) == ARG
 
 
 def test_block_refusals(L):

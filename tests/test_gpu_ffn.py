@@ -281,6 +281,52 @@ def test_down(K, dev, S, k, E, H, F, how, weighted):
     assert torch.equal(rd, out)
 
 
+@pytest.mark.parametrize("S,k,E", [(2, 2, 4), (30, 2, 4), (400, 2, 4), (700, 2, 4)])
+def test_small_numbers(K, dev, S, k, E):
+    """fp16 numbers below the normal ones keep their value, in x, scales and act."""
+    H, F = 512, 256
+    rng = np.random.default_rng(S)
+    small = lambda *n: (rng.integers(-1000, 1001, n) * 2.0 ** -24).astype(np.float16)
+    ids = make(rng, S, k, E, H, F)
+    p1, s1, _ = ref.quant(rng, E, F, H)
+    p3, s3, _ = ref.quant(rng, E, F, H)
+    p2, s2, _ = ref.quant(rng, E, H, F)
+    wide = lambda p, s: (np.stack((p & 15, p >> 4), -1).reshape(E, p.shape[1], -1).astype(np.float64) - 8.0
+                         ) * np.repeat(s.astype(np.float64), 128, axis=2)
+    res = np.zeros((S, H), np.float32)
+    ws = torch.empty(K.moe_workspace_bytes(S, k, E, H, F), dtype=torch.uint8, device=dev)
+    act, out = torch.empty((S, k, F), dtype=torch.float16, device=dev), torch.empty((S, H), device=dev)
+    for tiny_x in (True, False):
+        big = lambda s: (s.astype(np.float64) * 3000).astype(np.float16)
+        if tiny_x:
+            x, a, c1, c3, c2 = small(S, H), small(S * k, F), big(s1), big(s3), big(s2)
+        else:
+            x, a = (100 * rng.standard_normal((S, H))).astype(np.float16), rng.standard_normal((S * k, F)).astype(np.float16)
+            c1, c3, c2 = (np.abs(small(*s.shape)) for s in (s1, s3, s2))
+        want, bound = ref.up(x, ids, wide(p1, c1), wide(p3, c3), k)
+        K.moe_up_int4(t(x, dev), t(ids, dev), (t(p1, dev), t(c1, dev)), (t(p3, dev), t(c3, dev)), act, S, k, ws)
+        within(act.view(S * k, F).cpu().numpy(), want, bound, "act")
+        want, bound = ref.down(a, ids, None, wide(p2, c2), res, k)
+        K.moe_down_int4(t(a, dev), t(ids, dev), None, (t(p2, dev), t(c2, dev)), t(res, dev), out, S, k, ws)
+        within(out.cpu().numpy(), want, bound, "out")
+
+
+@pytest.mark.parametrize("S", [3, 300, 1100])
+def test_route_of_small_numbers(K, dev, S):
+    rng = np.random.default_rng(S)
+    H, E, k = 640, 20, 4
+    x = (rng.integers(-1000, 1001, (S, H)) * 2.0 ** -24).astype(np.float16)
+    gate = (1000 * rng.standard_normal((E, H))).astype(np.float16)
+    l = x.astype(np.float64) @ gate.astype(np.float64).T
+    ids, wt = ref.choose(l, None, k)
+    gi, gw = torch.empty((S, k), dtype=torch.int32, device=dev), torch.empty((S, k), device=dev)
+    gl = torch.empty((S, E), device=dev)
+    K.moe_route(t(x, dev), t(gate, dev), gi, gw, S, H, E, k, logits=gl)
+    assert np.array_equal(gi.cpu().numpy(), ids)
+    far = 32 * ref.U24 * (np.abs(x.astype(np.float64)) @ np.abs(gate.astype(np.float64)).T)
+    within(gl.cpu().numpy(), l, ref.U24 * np.abs(l) + far, "logits")
+
+
 def test_experts_apart(K, dev):
     """Experts at a stride larger than an expert, as tensors of a weight blob lie."""
     rng = np.random.default_rng(11)
