@@ -317,7 +317,7 @@ def q4_experts(w, name: str):
     groups = half // 64
     ps, ss = packed.stride(), scales.stride()
     # (one condition: a decode token's call is bound by the host)
-    if not (packed.is_cuda and scales.is_cuda and packed.dtype is torch.uint8 and scales.dtype in _F16
+    if not (packed.is_cuda and scales.get_device() == packed.get_device() and packed.dtype is torch.uint8 and scales.dtype in _F16
             and half == 64 * groups and scales.shape == (E, rows, groups)
             and ps[1] == half and ps[2] == 1 and ss[1] == groups and ss[2] == 1):
         for t, part, dtypes in ((packed, ".packed", (torch.uint8,)), (scales, ".scales", _F16)):
@@ -327,6 +327,8 @@ def q4_experts(w, name: str):
                 raise TypeError(f"{name}{part}: dtype {t.dtype} not in {dtypes}")
             if t.stride()[1:] != (t.shape[2], 1):
                 raise ValueError(f"{name}{part}: an expert must be contiguous")
+        if packed.device != scales.device:
+            raise ValueError(f"{name}: packed is on {packed.device}, scales on {scales.device}")
         raise ValueError(f"{name}: packed {tuple(packed.shape)} and scales {tuple(scales.shape)} do not fit: "
                          "[E, rows, cols / 2] and [E, rows, cols / 128], cols a multiple of 128")
     return _lib.cia_q4_experts(packed.data_ptr(), scales.data_ptr(), ps[0], ss[0]), E, rows, 2 * half
