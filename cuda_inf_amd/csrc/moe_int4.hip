@@ -931,10 +931,12 @@ __global__ __launch_bounds__(64 * kStreamWaves, (2 * Stream<kG, kMT>::kPerUnit))
 // the experts that have a row, so that it can weight the rows and add them to the
 // residual itself, and no launch follows.  The waves split K as above, the weights
 // of the next kRing experts in flight; all the experts' sums meet in LDS at once.
-// (Calls in us, in two launches / so: 1 token, 4 of 32 experts of 1792 11.8 / 8.8;
-// 4 tokens, 16 segments, 16.4 / 19.2.)
+//   Bound by latency: ids, then weights and x, then two meetings of the waves.  16
+// waves where K has more than 8 groups: 1 token of 4 of 32 experts of 1792, H =
+// 2048, 8.1 us with 8 waves, 7.4 with 16; 6 of 64 of 768 6.8 / 7.4.  (Calls in us,
+// in two launches / so: the first 11.8 / 8.8, 4 such tokens, 16 pairs, 16.4 / 19.2.)
 constexpr int kFewPairs = 8;
-static_assert(kFewPairs <= kStreamWaves && kFewPairs <= 16, "a wave an expert's sums; a row tile an expert");
+static_assert(kFewPairs <= 8, "a wave an expert's sums; an expert's rows in a row tile");
 
 struct FewArgs {
   MoeArgs m;
@@ -943,15 +945,15 @@ struct FewArgs {
   float* out;
 };
 
-// grid = N / 16, block = 512; K <= 1024 kG
-template <int kG>
-__global__ __launch_bounds__(64 * kStreamWaves) void k_moe_few(FewArgs f) {
-  constexpr int kRing = kG <= 2 ? 4 : 2;
+// grid = N / 16, block = 64 kWaves; K <= 128 kWaves kG
+template <int kWaves, int kG>
+__global__ __launch_bounds__(64 * kWaves) void k_moe_few(FewArgs f) {
+  constexpr int kRing = kG == 1 ? 4 : 2;
   const MoeArgs& a = f.m;
-  __shared__ f32x4 part[kFewPairs][kStreamWaves][64];
-  __shared__ u32x4 stage[kStreamWaves][2][64];
+  __shared__ f32x4 part[kFewPairs][kWaves][64];
+  __shared__ u32x4 stage[kWaves][64];
   __shared__ float sums[kFewPairs][16];
-  __shared__ int rows[kStreamWaves][kFewPairs][kFewPairs];
+  __shared__ int rows[kWaves][kFewPairs][kFewPairs];
   const int tid = threadIdx.x, l = tid & 63, n16 = l & 15, q = l >> 4, P = a.S * a.k;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c0 = 16 * blockIdx.x;
@@ -973,7 +975,7 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_few(FewArgs f) {
   const uint64_t below = (1ull << l) - 1;
   const uint64_t firsts = __ballot(id >= 0 && !(same & below));
   const int nexp = __popcll(firsts);
-  const int ng = a.K >> 7, g0 = w * ng / kStreamWaves, mine = (w + 1) * ng / kStreamWaves - g0;
+  const int ng = a.K >> 7, g0 = w * ng / kWaves, mine = (w + 1) * ng / kWaves - g0;
   typedef const __attribute__((address_space(1))) uint16_t* gs_t;
   typedef const __attribute__((address_space(1))) u32x4* gw_t;
   u32x4 wr[kRing][kG];
@@ -1030,7 +1032,7 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_few(FewArgs f) {
       float scl[kG];
 #pragma unroll
       for (int g = 0; g < kG; g++) {
-        u32x4* st = stage[w][g & 1];
+        u32x4* st = stage[w];
         st[(l & ~3) | ((l & 3) ^ ((l >> 4) & 3))] = wr[d][g];
         wq[g] = st[4 * n16 + (q ^ ((n16 >> 2) & 3))];
         scl[g] = g < mine ? h2f((uint16_t)sr[d][g]) : 0.f;
@@ -1053,7 +1055,7 @@ __global__ __launch_bounds__(64 * kStreamWaves) void k_moe_few(FewArgs f) {
   if (w < nexp) {
     f32x4 v = {};
 #pragma unroll
-    for (int k = 0; k < kStreamWaves; k++) v += part[w][k][l];
+    for (int k = 0; k < kWaves; k++) v += part[w][k][l];
     const int left = __popcll(__ballot(id == expert(w)));
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -1306,13 +1308,13 @@ static int moe_down(const uint16_t* act, const int32_t* ids, const float* weight
   hipStream_t s = (hipStream_t)stream;
   if (S * (int64_t)k <= kFewPairs && F <= kStreamMaxK) {
     const FewArgs f{a, weights, res, out};
-    const dim3 grid((unsigned)(H / 16)), block(64 * kStreamWaves);
+    const dim3 grid((unsigned)(H / 16));
     if (F <= 1024)
-      hipLaunchKernelGGL(k_moe_few<1>, grid, block, 0, s, f);
+      hipLaunchKernelGGL((k_moe_few<8, 1>), grid, dim3(512), 0, s, f);
     else if (F <= 2048)
-      hipLaunchKernelGGL(k_moe_few<2>, grid, block, 0, s, f);
+      hipLaunchKernelGGL((k_moe_few<16, 1>), grid, dim3(1024), 0, s, f);
     else
-      hipLaunchKernelGGL(k_moe_few<4>, grid, block, 0, s, f);
+      hipLaunchKernelGGL((k_moe_few<16, 2>), grid, dim3(1024), 0, s, f);
     return launch_status();
   }
   if (!ids && !weights && a.splits == 1 && !streams(false, (int64_t)S * k, E, F)) {
