@@ -673,7 +673,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void k_moe_tile(MoeArgs a) {
 //         kRing tiles meet in LDS and are added there in the order of the groups.
 // Rows by expert are found by the workgroup itself, from up to kStreamPairs ids:
 // no launch before this one.
-constexpr int kStreamWaves = 8, kStreamPairs = 1024, kUnits = 256;  // compute units
+constexpr int kStreamWaves = 8, kStreamPairs = 64 * kStreamWaves, kUnits = 256;  // compute units
 constexpr int kStreamMaxK = 4 * 8 * 128;  // 4 groups a wave, of one part of K
 
 // groups a wave -> row tiles that x leaves registers for
@@ -691,7 +691,7 @@ struct Stream {
     f32x4 part[kPart][kStreamWaves][64];
     u32x4 stage[kStreamWaves][kStage][64];
     int cnt[kMoeMaxE], seg[kMoeMaxE];
-    int sum[4], wave[2][kStreamWaves], rows[kRows], expert[2];
+    int sum[4], wave[kStreamWaves], rows[kRows], expert[2];
   };
 };
 
@@ -818,7 +818,8 @@ __device__ __forceinline__ void stream_rows(const MoeArgs& a, typename St::Lds& 
   __syncthreads();  // the sums and rows are read
 }
 
-// grid = any, block = 512; S k <= kStreamPairs, a part of K at most 1024 kG
+// grid = any, block = 512; S k <= kStreamPairs (64 if kMT > 1), a part of K at most
+// 1024 kG
 template <bool kUp, int kG, int kMT>
 __global__ __launch_bounds__(64 * kStreamWaves, (2 * Stream<kG, kMT>::kPerUnit)) void k_moe_stream(MoeArgs a) {
   using St = Stream<kG, kMT>;
@@ -827,7 +828,7 @@ __global__ __launch_bounds__(64 * kStreamWaves, (2 * Stream<kG, kMT>::kPerUnit))
   const int nct = (kUp ? 2 * a.N : a.N) >> 4, parts = kUp ? 1 : a.splits;
   // Segments: an expert's rows kRows at a time, in the order of the pairs, the same
   // in every workgroup.  Each takes an equal run of all the segments' column tiles.
-  if (P <= 64) {
+  if (kMT > 1 || P <= 64) {  // (more pairs are 16 rows at a time)
     // every wave finds its own, lane i with pair i, and waits for no other
     int id = l < P ? (a.ids ? a.ids[l] : 0) : -1;
     if ((unsigned)id >= (unsigned)a.E) id = -1;
@@ -865,18 +866,11 @@ __global__ __launch_bounds__(64 * kStreamWaves, (2 * Stream<kG, kMT>::kPerUnit))
     }
     return;
   }
-  int id[2];
-#pragma unroll
-  for (int j = 0; j < 2; j++) {
-    const int i = 512 * j + tid;
-    id[j] = i < P ? (a.ids ? a.ids[i] : 0) : -1;
-    if ((unsigned)id[j] >= (unsigned)a.E) id[j] = -1;
-  }
+  int id = tid < P ? (a.ids ? a.ids[tid] : 0) : -1;
+  if ((unsigned)id >= (unsigned)a.E) id = -1;
   if (tid < kMoeMaxE) L.cnt[tid] = 0;
   __syncthreads();
-#pragma unroll
-  for (int j = 0; j < 2; j++)
-    if (id[j] >= 0) atomicAdd(&L.cnt[id[j]], 1);
+  if (id >= 0) atomicAdd(&L.cnt[id], 1);
   __syncthreads();
   const int segs = tid < kMoeMaxE ? (L.cnt[tid] + St::kRows - 1) / St::kRows : 0;
   int before = segs;
@@ -908,19 +902,12 @@ __global__ __launch_bounds__(64 * kStreamWaves, (2 * Stream<kG, kMT>::kPerUnit))
     __syncthreads();
     const int e = __builtin_amdgcn_readfirstlane(L.expert[0]);
     const int r0 = __builtin_amdgcn_readfirstlane(L.expert[1]) * St::kRows;
-    uint64_t b[2];
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-      b[j] = __ballot(id[j] == e);
-      if (l == 0) L.wave[j][w] = __popcll(b[j]);
-    }
+    const uint64_t b = __ballot(id == e);
+    if (l == 0) L.wave[w] = __popcll(b);
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-      int r = __popcll(b[j] & ((1ull << l) - 1)) - r0;
-      for (int k = 0; k < 8 * j + w; k++) r += L.wave[k >> 3][k & 7];
-      if (id[j] == e && r >= 0 && r < St::kRows) L.rows[r] = 512 * j + tid;
-    }
+    int r = __popcll(b & ((1ull << l) - 1)) - r0;
+    for (int k = 0; k < w; k++) r += L.wave[k];
+    if (id == e && r >= 0 && r < St::kRows) L.rows[r] = tid;
     __syncthreads();
     const int left = L.cnt[e] - r0, n = __builtin_amdgcn_readfirstlane(left < St::kRows ? left : St::kRows);
     stream_rows<kUp, kG, St>(a, L, e, part_k, n, t0, t1);
@@ -1126,9 +1113,9 @@ static int64_t y_rows(int64_t P) { return P >= 4096 ? P : (8 * P < 4096 ? 8 * P 
 
 // Parts of K of a down launch in tiles: as many as the chip's 512 places hold of
 // workgroups of 128 columns, each part of 4 groups or more.
-static int64_t row_tiles(int64_t P, int E);
+static double row_tiles(int64_t P, int E);
 static int k_splits(int64_t P, int E, int H, int F) {
-  int64_t n = 512 / (row_tiles(P, E) * ((H + 127) / 128));
+  int64_t n = (int64_t)(512.0 / (row_tiles(P, E) * ((H + 127) / 128)));
   n = n < y_rows(P) / P ? n : y_rows(P) / P;
   n = n < F / 512 ? n : F / 512;
   return n < 1 ? 1 : (int)n;
@@ -1160,46 +1147,52 @@ static void set_w(MoeArgs& a, int i, const cia_q4_experts* w) {
 }
 
 // Whether the weights are streamed rather than multiplied in tiles: while experts
-// have 8 (up), 4 (down) rows on average, or pairs are few.  Calls in us, streamed /
-// in tiles: 4 of 32 experts of 1792, H = 2048, up 16 tokens 22.7 / 25.7, 40 31 /
-// 36, 64 37 / 41.5, 100 49 / 44, down 16 20.1 / 24.8, 40 27.0 / 27.9, 64 32 / 24.6;
-// 2 of 8 of 2048, H = 1024, up 32 10.8 / 12.1, 40 14.6 / 12.5, down 8 13.9 / 14.2,
-// 16 14.5 / 13.8; the dense form of 7168, H = 2048, up 32 rows 12.4 / 13.2, 64 17.1
-// / 16.1, down 8 12.9 / 15.7, 24 15.0 / 13.8.  (Down takes a K of two parts as well.)
+// have 2 (up), 1.5 (down) rows on average, or pairs are few.  Calls in us, streamed /
+// in tiles: 4 of 32 experts of 1792, H = 2048, up 16 tokens 21.0 / 24.5, 20 26.9 /
+// 25.0, 40 30.6 / 30.4, down 12 15.6 / 16.7, 20 23.7 / 18.1; 8 of 128 of 1536, H =
+// 4096, up 8 66 / 76, 32 119 / 114, down 24 64 / 67, 64 90 / 87; 2 of 8 of 2048, H =
+// 1024, up 32 9.7 / 10.5, 40 13.3 / 11.1, down 4 8.5 / 8.5, 12 13.7 / 11.0; the dense
+// form of 7168, H = 2048, up 32 rows 11.5 / 12.3, 64 16.1 / 14.6, down 16 12.1 / 13.8,
+// 24 14.4 / 13.9.  (Down takes a K of two parts as well.)
 static bool streams(bool up, int64_t P, int E, int K) {
-  const int64_t most = (up ? 8 : 4) * (int64_t)E, few = up ? 64 : 16;
-  return P <= kStreamPairs && K <= (up ? 1 : 2) * kStreamMaxK && P <= (most > few ? most : few);
+  const int64_t most = up ? 2 * (int64_t)E : 3 * (int64_t)E / 2, few = up ? 64 : 16;
+  return P <= (most > few ? most : few) && K <= (up ? 1 : 2) * kStreamMaxK;
 }
+static_assert(2 * kMoeMaxE <= kStreamPairs && 64 <= kStreamPairs, "a thread a pair");
 
 // 16 rows at a time with two workgroups a compute unit where experts hardly have
-// more
+// more; up to 64 rows of up's few pairs of few experts
 template <bool kUp, int kG>
 static void stream_launch(const MoeArgs& a, hipStream_t s) {
-  constexpr int kMT = stream_mt(kG);
   const dim3 block(64 * kStreamWaves);
   const int64_t P = (int64_t)a.S * a.k;
-  if (P <= 8 * (int64_t)a.E) {
-    // (as many workgroups as tiles to take 4 of)
-    const int64_t tiles = (P < a.E ? P : a.E) * ((kUp ? 2 * a.N : a.N) >> 4) * (kUp ? 1 : a.splits);
-    const int n = tiles <= 4 * kUnits ? kUnits : kUnits * Stream<kG, 1>::kPerUnit;
-    hipLaunchKernelGGL((k_moe_stream<kUp, kG, 1>), dim3(n), block, 0, s, a);
+  if (kUp && P > 8 * (int64_t)a.E) {
+    hipLaunchKernelGGL((k_moe_stream<kUp, kG, kUp ? stream_mt(kG) : 1>), dim3(kUnits), block, 0, s, a);
+    return;
   }
-  else
-    hipLaunchKernelGGL((k_moe_stream<kUp, kG, kMT>), dim3(kUnits), block, 0, s, a);
+  // (as many workgroups as tiles to take 4 of)
+  const int64_t tiles = (P < a.E ? P : a.E) * ((kUp ? 2 * a.N : a.N) >> 4) * (kUp ? 1 : a.splits);
+  const int n = tiles <= 4 * kUnits ? kUnits : kUnits * Stream<kG, 1>::kPerUnit;
+  hipLaunchKernelGGL((k_moe_stream<kUp, kG, 1>), dim3(n), block, 0, s, a);
 }
 
-// Column tiles a wave, of 1, 2 and 3: time goes with kNT + 1 a round of the 512
-// workgroups that the chip holds, and 0.4 rounds for the last one's end.
-static int64_t row_tiles(int64_t P, int E) {  // about: every expert has a last, partly filled one
-  const int64_t other = P < E ? P : E;
-  return P / kTileRows + (E > 1 ? (other + 1) / 2 : (P % kTileRows != 0));
+// Column tiles a wave, of 1, 2 and 3: a workgroup's time goes with kNT + 3, and the
+// call's with its rounds of the 512 workgroups that the chip holds, of which the
+// first is never less than nine tenths.  (Of 125 sizes of 5 layers the choice is 1 %
+// slower on average than the best of the three, always 2 would be 5 %, always 1 19 %;
+// 45 tokens of 4 of 32 experts, H = 2048, down 1792 25.7 / 21.3 / 24.7 us, 4096
+// tokens up 352 / 275 / 263.)
+// Row tiles, about: an expert's last one is partly filled, and with few rows costs
+// less.
+static double row_tiles(int64_t P, int E) {
+  return E > 1 ? (double)P / kTileRows + 0.75 * (double)(P < E ? P : E) : (double)((P + kTileRows - 1) / kTileRows);
 }
 static int tile_nt(int64_t P, int E, int nv, int splits) {
   int best = 1;
   double least = 0.0;
   for (int nt = 1; nt <= 3; nt++) {
-    const double rounds = (double)(row_tiles(P, E) * ((nv + 64 * nt - 1) / (64 * nt)) * splits) / 512.0 + 0.4;
-    const double t = (rounds < 1.0 ? 1.0 : rounds) * (nt + 1);
+    const double rounds = row_tiles(P, E) * ((nv + 64 * nt - 1) / (64 * nt)) * splits / 512.0;
+    const double t = (rounds < 0.9 ? 0.9 : rounds) * (nt + 3);
     if (nt == 1 || t < least) {
       best = nt;
       least = t;
