@@ -4,7 +4,9 @@
 //   hsum = h + add,   out = fp16(hsum * rsqrt(mean(hsum^2) + eps) * w)
 //
 // Bound by memory: 6 bytes an element, 14 with the addition.  A row stays in
-// registers between its sum of squares and its outputs, so h is read once.
+// registers between its sum of squares and its outputs, so h is read once.  4096
+// rows of 2048 with the addition: 27 us, 4.35 TB/s, where a large copy reaches 4.78;
+// one row 2.1 us, little more than an empty launch.
 #include "common.h"
 #include "cuda_inf_ffn.h"
 
@@ -49,7 +51,8 @@ __device__ __forceinline__ void norm_store(const NormArgs& a, size_t at, int c, 
 }
 
 // kWaves waves a row, kSteps steps of 512 kWaves elements held in registers
-// (H up to kSteps * 512 * kWaves).  block = 256: 4 / kWaves rows.
+// (H up to kSteps * 512 * kWaves).  block = 256: 4 / kWaves rows.  A wave a row
+// while a row's 32 values a lane fit, as its sum then needs no meeting of waves.
 template <int kWaves, int kSteps>
 __global__ __launch_bounds__(256) void k_rmsnorm(NormArgs a) {
   __shared__ float part[4];
