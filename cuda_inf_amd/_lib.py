@@ -148,7 +148,9 @@ def check(fn: str, code: int) -> None:
 
 
 def call(fn: str, *args) -> None:
-    check(fn, getattr(lib(), fn)(*args))
+    code = getattr(_lib or lib(), fn)(*args)
+    if code:
+        check(fn, code)
 
 
 class cia_tensor_desc(ctypes.Structure):

@@ -257,22 +257,42 @@ def qkv_proj_int4(x, wq, wk, wv, q, k, v, M: int, K: int = 2048) -> None:
 
 
 # ------------------------------------------------------------ feed-forward branch
-def _stream_here(*tensors) -> int:
-    """stream_handle(), once every tensor is found on the current device."""
-    dev = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"a tensor is on {t.device}, the current device is cuda:{dev}")
+# A decode token's call of these is bound by the host, so a tensor is looked at in one
+# condition, and again in detail where it does not hold (moe_up_int4 of one token: 7.5
+# us of host time, 8.7 with _dev() for each; the foreign call with its launch is 3.9).
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _at(t, name: str, dtypes, numel: int, dev: int):
+    """_dev() of a tensor that has to be on device dev."""
+    try:
+        if t.get_device() == dev and t.is_contiguous() and t.dtype in dtypes and t.numel() >= numel:
+            return t.data_ptr()
+    except AttributeError:
+        pass  # no tensor
+    _dev(t, name, dtypes, numel)
+    raise ValueError(f"{name}: on {t.device}, and other tensors of the call on cuda:{dev}")
+
+
+def _stream_on(dev: int) -> int:
+    """stream_handle() of device dev, which has to be the current one, where the
+    call runs."""
+    if _current_device() != dev:
+        raise ValueError(f"the tensors are on cuda:{dev}, the current device is cuda:{_current_device()}")
     return stream_handle() if _raw_stream is None else _raw_stream(dev)
 
 
+_F32, _I32, _U8 = (torch.float32,), (torch.int32,), (torch.uint8,)
+
+
 def add_rmsnorm(h, w, out, S: int, H: int, eps: float = 1e-5, add=None, hsum=None) -> None:
-    """add_f32_inplace (engine.cu:867) and rmsnorm (870): hsum = h + add (fp32 [S, H]; add and hsum optional,
-    hsum may be h or add), out = fp16(hsum * rsqrt(mean(hsum^2) + eps) * w)."""
-    f32 = (torch.float32,)
-    call("cia_add_rmsnorm", _dev(h, "h", f32, S * H), _opt(add, "add", f32, S * H), _dev(w, "w", _F16, H),
-         float(eps), _opt(hsum, "hsum", f32, S * H), _dev(out, "out", _F16, S * H), S, H,
-         _stream_here(h, add, w, hsum, out))
+    """add_f32_inplace (engine.cu:867) and rmsnorm (870): hsum = h + add (fp32 [S, H];
+    add and hsum optional, hsum may be h or add), out = fp16(hsum *
+    rsqrt(mean(hsum^2) + eps) * w)."""
+    hp, dev, n = _dev(h, "h", _F32, S * H), h.get_device(), S * H
+    call("cia_add_rmsnorm", hp, None if add is None else _at(add, "add", _F32, n, dev), _at(w, "w", _F16, H, dev),
+         eps, None if hsum is None else _at(hsum, "hsum", _F32, n, dev), _at(out, "out", _F16, n, dev), S, H,
+         _stream_on(dev))
 
 
 def moe_gating(E: int, k: int, score: str = "sigmoid", n_group: int = 1, topk_group: int = 1,
@@ -280,58 +300,69 @@ def moe_gating(E: int, k: int, score: str = "sigmoid", n_group: int = 1, topk_gr
     """How a router chooses, as moe_route and moe_select take it."""
     if score not in _lib.SCORES:
         raise ValueError(f"score: {score!r} is not one of {sorted(_lib.SCORES)}")
-    return _lib.cia_moe_gating(E, k, _lib.SCORES[score], n_group, topk_group, int(bool(renorm)),
-                               float(eps), float(scale))
+    return _lib.cia_moe_gating(E, k, _lib.SCORES[score], n_group, topk_group, bool(renorm), eps, scale)
 
 
 def moe_route(x, gate, ids, weights, S: int, H: int, E: int, k: int, bias=None, logits=None,
               **gating) -> None:
-    """The router of engine.cu:869-905 on the device: the k experts of each of the S rows of x
-    (fp16 [S, H]; gate fp16 [E, H]; bias fp32 [E], for the choice alone) into
-    ids int32 [S, k] and weights fp32 [S, k]; logits fp32 [S, E], optional.
+    """The router of engine.cu:869-905 on the device: the k experts of each of the S
+    rows of x (fp16 [S, H]; gate fp16 [E, H]; bias fp32 [E], for the choice alone)
+    into ids int32 [S, k] and weights fp32 [S, k]; logits fp32 [S, E], optional.
     gating: score, n_group, topk_group, renorm, eps, scale, as moe_gating."""
-    f32 = (torch.float32,)
-    call("cia_moe_route", _dev(x, "x", _F16, S * H), _dev(gate, "gate", _F16, E * H),
-         _opt(bias, "bias", f32, E), ctypes.byref(moe_gating(E, k, **gating)),
-         _dev(ids, "ids", (torch.int32,), S * k), _dev(weights, "weights", f32, S * k),
-         _opt(logits, "logits", f32, S * E), S, H, _stream_here(x, gate, bias, ids, weights, logits))
+    xp, dev = _dev(x, "x", _F16, S * H), x.get_device()
+    call("cia_moe_route", xp, _at(gate, "gate", _F16, E * H, dev),
+         None if bias is None else _at(bias, "bias", _F32, E, dev), ctypes.byref(moe_gating(E, k, **gating)),
+         _at(ids, "ids", _I32, S * k, dev), _at(weights, "weights", _F32, S * k, dev),
+         None if logits is None else _at(logits, "logits", _F32, S * E, dev), S, H, _stream_on(dev))
 
 
 def moe_select(logits, ids, weights, S: int, E: int, k: int, bias=None, **gating) -> None:
-    """moe_route's choice from logits fp32 [S, E]."""
-    f32 = (torch.float32,)
-    call("cia_moe_select", _dev(logits, "logits", f32, S * E), _opt(bias, "bias", f32, E),
-         ctypes.byref(moe_gating(E, k, **gating)), _dev(ids, "ids", (torch.int32,), S * k),
-         _dev(weights, "weights", f32, S * k), S, _stream_here(logits, bias, ids, weights))
+    """moe_route from logits fp32 [S, E] that the caller has."""
+    lp, dev = _dev(logits, "logits", _F32, S * E), logits.get_device()
+    call("cia_moe_select", lp, None if bias is None else _at(bias, "bias", _F32, E, dev),
+         ctypes.byref(moe_gating(E, k, **gating)), _at(ids, "ids", _I32, S * k, dev),
+         _at(weights, "weights", _F32, S * k, dev), S, _stream_on(dev))
 
 
 def q4_experts(w, name: str):
     """(cia_q4_experts, E, rows, cols) of INT4 group-128 experts: w = (packed u8
     [E, rows, cols / 2], scales fp16 [E, rows, cols / 128]) on the device.  Each
     expert is contiguous; the experts may lie apart, at one stride."""
+    return _q4(w, name, None)
+
+
+def _q4(w, name: str, dev):
+    """q4_experts of a call whose tensors are on device dev (None: any)."""
     packed, scales = w
+    try:
+        E, rows, half = packed.shape
+        groups = half // 64
+        on = packed.get_device() if dev is None else dev
+        if (on >= 0 and packed.get_device() == on and scales.get_device() == on and packed.dtype is torch.uint8
+                and scales.dtype in _F16 and half == 64 * groups and scales.shape == (E, rows, groups)):
+            if packed.is_contiguous() and scales.is_contiguous():
+                return (_lib.cia_q4_experts(packed.data_ptr(), scales.data_ptr(), rows * half, rows * groups),
+                        E, rows, 2 * half)
+            ps, ss = packed.stride(), scales.stride()
+            if ps[1:] == (half, 1) and ss[1:] == (groups, 1):
+                return _lib.cia_q4_experts(packed.data_ptr(), scales.data_ptr(), ps[0], ss[0]), E, rows, 2 * half
+    except (AttributeError, ValueError):
+        pass  # no tensors, or not of three dimensions
     if not (isinstance(packed, torch.Tensor) and isinstance(scales, torch.Tensor) and packed.dim() == 3
             and scales.dim() == 3):
         raise ValueError(f"{name}: need two tensors [experts, rows, columns], packed and scales")
-    E, rows, half = packed.shape
-    groups = half // 64
-    ps, ss = packed.stride(), scales.stride()
-    # (one condition: a decode token's call is bound by the host)
-    if not (packed.is_cuda and scales.get_device() == packed.get_device() and packed.dtype is torch.uint8 and scales.dtype in _F16
-            and half == 64 * groups and scales.shape == (E, rows, groups)
-            and ps[1] == half and ps[2] == 1 and ss[1] == groups and ss[2] == 1):
-        for t, part, dtypes in ((packed, ".packed", (torch.uint8,)), (scales, ".scales", _F16)):
-            if not t.is_cuda:
-                raise ValueError(f"{name}{part}: must be a device tensor")
-            if t.dtype not in dtypes:
-                raise TypeError(f"{name}{part}: dtype {t.dtype} not in {dtypes}")
-            if t.stride()[1:] != (t.shape[2], 1):
-                raise ValueError(f"{name}{part}: an expert must be contiguous")
-        if packed.device != scales.device:
-            raise ValueError(f"{name}: packed is on {packed.device}, scales on {scales.device}")
-        raise ValueError(f"{name}: packed {tuple(packed.shape)} and scales {tuple(scales.shape)} do not fit: "
-                         "[E, rows, cols / 2] and [E, rows, cols / 128], cols a multiple of 128")
-    return _lib.cia_q4_experts(packed.data_ptr(), scales.data_ptr(), ps[0], ss[0]), E, rows, 2 * half
+    for t, part, dtypes in ((packed, ".packed", _U8), (scales, ".scales", _F16)):
+        if not t.is_cuda:
+            raise ValueError(f"{name}{part}: must be a device tensor")
+        if t.dtype not in dtypes:
+            raise TypeError(f"{name}{part}: dtype {t.dtype} not in {dtypes}")
+        if t.stride()[1:] != (t.shape[2], 1):
+            raise ValueError(f"{name}{part}: an expert must be contiguous")
+    if packed.device != scales.device or dev not in (None, packed.get_device()):
+        raise ValueError(f"{name}: packed is on {packed.device}, scales on {scales.device}"
+                         + ("" if dev is None else f", other tensors of the call on cuda:{dev}"))
+    raise ValueError(f"{name}: packed {tuple(packed.shape)} and scales {tuple(scales.shape)} do not fit: "
+                     "[E, rows, cols / 2] and [E, rows, cols / 128], cols a multiple of 128")
 
 
 def moe_workspace_bytes(S: int, k: int, E: int, H: int, F: int) -> int:
@@ -341,26 +372,26 @@ def moe_workspace_bytes(S: int, k: int, E: int, H: int, F: int) -> int:
 
 def moe_up_int4(x, ids, w1, w3, act, S: int, k: int, ws) -> None:
     """w1, w3 and swiglu of engine.cu:869-905 for every token and chosen expert:
-    act [S, k, F] fp16 =
-    silu(W1[e] x) * (W3[e] x), e = ids[s, j]; x fp16 [S, H], ids int32 [S, k]
-    (outside [0, E): the pair's act row is left as it was; None: one expert,
-    every row), w1 and w3 as q4_experts takes them, [E, F, H]."""
-    q1, E, F, H = q4_experts(w1, "w1")
-    q3, E3, F3, H3 = q4_experts(w3, "w3")
-    if (E3, F3, H3) != (E, F, H):
+    act [S, k, F] fp16 = silu(W1[e] x) * (W3[e] x), e = ids[s, j]; x fp16 [S, H],
+    ids int32 [S, k] (outside [0, E): the pair's act row is left as it was; None:
+    one expert, every row), w1 and w3 as q4_experts takes them, [E, F, H]."""
+    q1, E, F, H = _q4(w1, "w1", None)
+    dev = w1[0].get_device()
+    q3, E3, F3, H3 = _q4(w3, "w3", dev)
+    if F3 != F or H3 != H or E3 != E:
         raise ValueError(f"w3: experts {(E3, F3, H3)}, but w1 has {(E, F, H)}")
-    call("cia_moe_up_int4", _dev(x, "x", _F16, S * H), _opt(ids, "ids", (torch.int32,), S * k),
-         ctypes.byref(q1), ctypes.byref(q3), _dev(act, "act", _F16, S * k * F), S, k, E, H, F,
-         _dev(ws, "ws", (torch.uint8,)), ws.numel(), _stream_here(x, ids, w1[0], w3[0], act, ws))
+    call("cia_moe_up_int4", _at(x, "x", _F16, S * H, dev), None if ids is None else _at(ids, "ids", _I32, S * k, dev),
+         ctypes.byref(q1), ctypes.byref(q3), _at(act, "act", _F16, S * k * F, dev), S, k, E, H, F,
+         _at(ws, "ws", _U8, 0, dev), ws.numel(), _stream_on(dev))
 
 
 def moe_down_int4(act, ids, weights, w2, res, out, S: int, k: int, ws) -> None:
     """w2 and acc_scaled of engine.cu:869-905 for every token and chosen expert:
-    out [S, H] fp32 = res + sum over j of weights[s, j] * (W2[e] act[s, j]); out may be res; weights
-    fp32 [S, k] or None (1); ids as moe_up_int4's; w2 [E, H, F]."""
-    q2, E, H, F = q4_experts(w2, "w2")
-    f32 = (torch.float32,)
-    call("cia_moe_down_int4", _dev(act, "act", _F16, S * k * F), _opt(ids, "ids", (torch.int32,), S * k),
-         _opt(weights, "weights", f32, S * k), ctypes.byref(q2), _dev(res, "res", f32, S * H),
-         _dev(out, "out", f32, S * H), S, k, E, H, F, _dev(ws, "ws", (torch.uint8,)), ws.numel(),
-         _stream_here(act, ids, weights, w2[0], res, out, ws))
+    out [S, H] fp32 = res + sum over j of weights[s, j] * (W2[e] act[s, j]); out may
+    be res; weights fp32 [S, k] or None (1); ids as moe_up_int4's; w2 [E, H, F]."""
+    q2, E, H, F = _q4(w2, "w2", None)
+    dev, n = w2[0].get_device(), S * k
+    call("cia_moe_down_int4", _at(act, "act", _F16, n * F, dev), None if ids is None else _at(ids, "ids", _I32, n, dev),
+         None if weights is None else _at(weights, "weights", _F32, n, dev), ctypes.byref(q2),
+         _at(res, "res", _F32, S * H, dev), _at(out, "out", _F32, S * H, dev), S, k, E, H, F,
+         _at(ws, "ws", _U8, 0, dev), ws.numel(), _stream_on(dev))

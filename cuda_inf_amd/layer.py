@@ -15,7 +15,7 @@ import torch
 from . import _lib
 from ._lib import (D, KVGROUP, NH, NKV, NSPLIT_DEFAULT, call, cia_append_op, cia_attn_proj,
                    cia_layer, cia_moe)
-from .kernels import (_stream_here, decode_workspace_bytes, h2o_workspace_bytes, moe_gating,
+from .kernels import (_stream_on, decode_workspace_bytes, h2o_workspace_bytes, moe_gating,
                       q4_experts, stream_handle)
 
 HIDDEN = _lib.HIDDEN
@@ -274,4 +274,4 @@ class MoeBlock:
             raise ValueError(f"S={S} exceeds max_batch={self.max_batch}")
         if h.device != self.ws.device:
             raise ValueError(f"h is on {h.device}, the layer on {self.ws.device}")
-        call("cia_moe_block_forward", ctypes.byref(self._m), h.data_ptr(), S, _stream_here(h))
+        call("cia_moe_block_forward", ctypes.byref(self._m), h.data_ptr(), S, _stream_on(h.get_device()))
