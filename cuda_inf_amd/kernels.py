@@ -358,7 +358,7 @@ def _q4(w, name: str, dev):
             raise TypeError(f"{name}{part}: dtype {t.dtype} not in {dtypes}")
         if t.stride()[1:] != (t.shape[2], 1):
             raise ValueError(f"{name}{part}: an expert must be contiguous")
-    if packed.device != scales.device or dev not in (None, packed.get_device()):
+    if packed.get_device() != scales.get_device() or dev not in (None, packed.get_device()):
         raise ValueError(f"{name}: packed is on {packed.device}, scales on {scales.device}"
                          + ("" if dev is None else f", other tensors of the call on cuda:{dev}"))
     raise ValueError(f"{name}: packed {tuple(packed.shape)} and scales {tuple(scales.shape)} do not fit: "

@@ -228,3 +228,39 @@ def test_choice_oracle():
     assert ids.tolist() == [[3, 2]]
     ids, _ = ref.choose(np.zeros((1, 4)), None, 3)
     assert ids.tolist() == [[0, 1, 2]]
+
+
+def test_tensors_of_another_device(cia, monkeypatch):
+    import torch
+
+    from cuda_inf_amd import kernels as K
+
+    class On(torch.Tensor):  # a tensor that says it is on a device
+        is_cuda = True
+        index = 0
+
+        def get_device(self):
+            return self.index
+
+    def on(t, index):
+        t = t.as_subclass(On)
+        t.index = index
+        return t
+
+    x = on(torch.zeros((2, 256)), 0)
+    assert K._at(x, "x", (torch.float32,), 512, 0) == x.data_ptr()
+    with pytest.raises(ValueError, match="x: on .*other tensors of the call on cuda:1"):
+        K._at(x, "x", (torch.float32,), 512, 1)
+    with pytest.raises(ValueError, match="x: needs at least 513"):
+        K._at(x, "x", (torch.float32,), 513, 0)
+    with pytest.raises(TypeError, match="x: expected a torch.Tensor"):
+        K._at(None, "x", (torch.float32,), 512, 0)
+    packed, scales = torch.zeros((2, 4, 64), dtype=torch.uint8), torch.zeros((2, 4, 1), dtype=torch.float16)
+    q, E, rows, cols = K.q4_experts((on(packed, 0), on(scales, 0)), "w")
+    assert (E, rows, cols, q.packed_stride, q.scales_stride) == (2, 4, 128, 256, 4)
+    for a, b, dev in ((0, 1, None), (1, 1, 0)):
+        with pytest.raises(ValueError, match="w: packed is on"):
+            K._q4((on(packed, a), on(scales, b)), "w", dev)
+    monkeypatch.setattr(K, "_current_device", lambda: 1)
+    with pytest.raises(ValueError, match="the current device is cuda:1"):
+        K._stream_on(0)

@@ -557,3 +557,50 @@ def test_another_stream(K, dev):
         B.forward(h)
     s.synchronize()
     assert torch.equal(h, want)
+
+
+def test_offsets_past_32_bits(K, dev):
+    """Rows whose elements lie past the 2^32nd, against the same rows on their own and
+    64-bit forms."""
+    rng = np.random.default_rng(12)
+    S, H, E, k = (1 << 21) + 3, 2056, 8, 2
+    assert S * H > 1 << 32
+    h = torch.empty((S, H), device=dev).normal_()
+    x = torch.empty((S, H), dtype=torch.float16, device=dev)
+    w = torch.ones(H, dtype=torch.float16, device=dev)
+    gate = t((rng.standard_normal((E, H)) / 45).astype(np.float16), dev)
+    K.add_rmsnorm(h, w, x, S, H)
+    ids, wt = torch.empty((S, k), dtype=torch.int32, device=dev), torch.empty((S, k), device=dev)
+    K.moe_route(x, gate, ids, wt, S, H, E, k)
+    for i in (0, S // 2, S - 3):
+        o, i1, w1 = torch.empty_like(x[:3]), torch.empty_like(ids[:3]), torch.empty_like(wt[:3])
+        K.add_rmsnorm(h[i:i + 3].clone(), w, o, 3, H)
+        assert torch.equal(o, x[i:i + 3])
+        K.moe_route(o, gate, i1, w1, 3, H, E, k)
+        assert torch.equal(i1, ids[i:i + 3])
+    del h, x, ids, wt
+    S, k, E, n, wide = 1 << 18, 4, 3, 128, 4224
+    assert S * k * wide > 1 << 32
+    ids = np.stack([rng.permutation(E + 1)[:k] for _ in range(1024)]).astype(np.int32)
+    ids = np.tile(ids, (S // 1024, 1))  # (id E: no expert)
+    rows = np.array([0, S // 2 + 1, S - 2, S - 1])
+    x = t(rng.standard_normal((1024, n)).astype(np.float16), dev).repeat(S // 1024, 1)
+    p1, s1, W1 = ref.quant(rng, E, wide, n)
+    p3, s3, W3 = ref.quant(rng, E, wide, n)
+    act = torch.full((S, k, wide), 3.0, dtype=torch.float16, device=dev)
+    ws = torch.empty(K.moe_workspace_bytes(S, k, E, n, wide), dtype=torch.uint8, device=dev)
+    K.moe_up_int4(x, t(ids, dev), (t(p1, dev), t(s1, dev)), (t(p3, dev), t(s3, dev)), act, S, k, ws)
+    want, bound = ref.up(x[rows].cpu().numpy(), ids[rows], W1, W3, k)
+    got = act[rows].view(-1, wide).cpu().numpy()
+    dead = ids[rows].reshape(-1) == E
+    assert (got[dead] == 3.0).all()
+    within(got[~dead], want[~dead], bound[~dead], "act")
+    del act, ws
+    p2, s2, W2 = ref.quant(rng, E, wide, n)
+    a = t(rng.standard_normal((1024 * k, n)).astype(np.float16), dev).repeat(S // 1024, 1)
+    out = torch.ones((S, wide), device=dev)
+    ws = torch.empty(K.moe_workspace_bytes(S, k, E, wide, n), dtype=torch.uint8, device=dev)
+    K.moe_down_int4(a, t(ids, dev), None, (t(p2, dev), t(s2, dev)), out, out, S, k, ws)
+    want, bound = ref.down(a.view(S, k, n)[rows].view(-1, n).cpu().numpy(), ids[rows], None, W2,
+                           np.ones((len(rows), wide), np.float32), k)
+    within(out[rows].cpu().numpy(), want, bound, "out")
