@@ -278,7 +278,7 @@ __global__ __launch_bounds__(64 * tok_waves(kT, kPer)) void k_route_tok(RouteArg
   __shared__ double lg[kT][kRouteMaxE];
   __shared__ double ch[kT][kRouteMaxE];
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, s0 = blockIdx.x * kT;
-  if (a.x) {
+  if (kT <= 2 && a.x) {  // (8 tokens bring their logits)
     for (int h0 = 0; h0 < a.H; h0 += kSpan) {
       const int n8 = (a.H - h0 < kSpan ? a.H - h0 : kSpan) / 8;
       if (h0) __syncthreads();

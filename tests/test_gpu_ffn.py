@@ -327,6 +327,26 @@ def test_route_of_small_numbers(K, dev, S):
     within(gl.cpu().numpy(), l, ref.U24 * np.abs(l) + far, "logits")
 
 
+@pytest.mark.parametrize("S,E", [(2, 20), (2, 100), (300, 20), (300, 100), (1100, 20)])
+def test_route_of_a_bad_gate(K, dev, S, E):
+    """Infinities and NaN in two experts' gates reach those experts' logits alone."""
+    rng = np.random.default_rng(S + E)
+    H, k = 4168, 4
+    x = rng.standard_normal((S, H)).astype(np.float16)
+    gate = (rng.standard_normal((E, H)) / 64).astype(np.float16)
+    gate[3, 5], gate[7, 4100], gate[9, 0], gate[9, 1] = np.nan, np.inf, np.inf, -np.inf
+    with np.errstate(invalid="ignore"):
+        l = x.astype(np.float64) @ gate.astype(np.float64).T
+    assert np.isnan(l[:, 3]).all() and np.isinf(l[:, 7]).all()
+    ids, _ = ref.choose(l, None, k)
+    gi, gw = torch.empty((S, k), dtype=torch.int32, device=dev), torch.empty((S, k), device=dev)
+    gl = torch.empty((S, E), device=dev)
+    K.moe_route(t(x, dev), t(gate, dev), gi, gw, S, H, E, k, logits=gl)
+    got = gl.cpu().numpy()
+    assert np.array_equal(np.isnan(got), np.isnan(l)) and np.array_equal(got[:, 7], l[:, 7].astype(np.float32))
+    assert np.array_equal(gi.cpu().numpy(), ids)
+
+
 def test_experts_apart(K, dev):
     """Experts at a stride larger than an expert, as tensors of a weight blob lie."""
     rng = np.random.default_rng(11)
