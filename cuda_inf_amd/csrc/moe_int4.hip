@@ -37,9 +37,30 @@ struct MoeArgs {
   float* out;             // null: into y
 };
 
-// Rows of a row tile.  The plan lists the tiles: the whole ones of all experts,
-// then the experts' last, partly filled ones.
+// Rows of a row tile.  Tiles are in the order of the whole ones of all experts, then
+// the experts' last, partly filled ones, those of the most rows first, as the last
+// round of workgroups ends with the shortest.
 constexpr int kTileRows = 128;
+
+// An expert's n rows: its whole tiles (if whole), and its partly filled one under how
+// many times 32 rows it has, 4 first, in fields of kBits from the lowest.  256 experts'
+// sums fit 12 bits where all have fewer than 4096 tiles.
+template <int kBits>
+__device__ __forceinline__ uint64_t tile_counts(int n, bool whole) {
+  const int c = (n % kTileRows + 31) >> 5;  // 0: none
+  uint64_t v = c ? 1ull << kBits * (whole ? 5 - c : 4 - c) : 0;
+  return whole ? v + (uint64_t)(n / kTileRows) : v;
+}
+// Of the wave's lanes up to this one
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
+  const int l = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint64_t u = __shfl_up(v, d);
+    if (l >= d) v += u;
+  }
+  return v;
+}
 
 // The most row tiles P pairs of E experts can make
 __host__ __device__ constexpr int64_t max_tiles(int64_t P, int E) { return P / kTileRows + (P < E ? P : E); }
@@ -59,7 +80,7 @@ constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 
 __global__ __launch_bounds__(kPlanThreads) void k_moe_plan(const int32_t* ids, int P, int E, int* plan) {
   __shared__ int cnt[kPlanWaves][kMoeMaxE];  // of a wave, then the first place of its pairs
-  __shared__ int part[3][4];  // of 64 experts
+  __shared__ uint64_t part[2][4];  // of 64 experts: pairs and whole tiles, the others
   __shared__ __attribute__((aligned(16))) int order[16 * kPlanThreads];
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63;
   int* rows = plan + plan_rows_at(P, E);
@@ -87,49 +108,58 @@ __global__ __launch_bounds__(kPlanThreads) void k_moe_plan(const int32_t* ids, i
     }
   }
   __syncthreads();
-  // thread e: its pairs, whole tiles and partly filled tile, and how many of each
-  // the experts before it have
-  int n = 0, before[3] = {};
+  // thread e: its pairs and whole tiles (in the halves of a word), its partly filled
+  // tile, and how many of each the experts before it have
+  int n = 0;
+  uint64_t own[2] = {}, before[2] = {};
   if (tid < kMoeMaxE) {
     for (int i = 0; i < kPlanWaves; i++) n += cnt[i][tid];
-    const int own[3] = {n, n / kTileRows, n % kTileRows != 0};
+    own[0] = (uint64_t)(n / kTileRows) << 32 | (uint32_t)n;
+    own[1] = tile_counts<16>(n, false);
 #pragma unroll
-    for (int k = 0; k < 3; k++) {
-      int v = own[k];
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int u = __shfl_up(v, d);
-        if (l >= d) v += u;
-      }
+    for (int k = 0; k < 2; k++) {
+      const uint64_t v = wave_scan(own[k]);
       before[k] = v - own[k];
       if (l == 63) part[k][w] = v;
     }
   }
   __syncthreads();
-  if (tid < kMoeMaxE) {
-    const int whole = part[1][0] + part[1][1] + part[1][2] + part[1][3];
+  uint64_t total[2] = {};
 #pragma unroll
-    for (int k = 0; k < 3; k++)
-      for (int i = 0; i < w; i++) before[k] += part[k][i];
+  for (int k = 0; k < 2; k++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if (i < w) before[k] += part[k][i];
+      total[k] += part[k][i];
+    }
+  if (tid < kMoeMaxE) {
+    const int whole = (int)(total[0] >> 32), first = (int)(uint32_t)before[0];
     if (tid < E) {
-      plan[tid] = before[0];
+      plan[tid] = first;
       int* tiles = plan + E + 3;
-      const int full = n / kTileRows, other = whole + before[2];
+      const int full = n / kTileRows;
       for (int i = 0; i < full; i++) {
-        tiles[2 * (before[1] + i)] = tid;
-        tiles[2 * (before[1] + i) + 1] = before[0] + i * kTileRows;
+        const int at = (int)(before[0] >> 32) + i;
+        tiles[2 * at] = tid;
+        tiles[2 * at + 1] = first + i * kTileRows;
       }
-      if (n % kTileRows) {
-        tiles[2 * other] = tid;
-        tiles[2 * other + 1] = before[0] + full * kTileRows;
+      int others = 0;
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        if (own[1] >> 16 * c & 1) {
+          const int at = whole + others + (int)(before[1] >> 16 * c & 0xFFFF);
+          tiles[2 * at] = tid;
+          tiles[2 * at + 1] = first + full * kTileRows;
+        }
+        others += (int)(total[1] >> 16 * c & 0xFFFF);
       }
       if (tid == E - 1) {
-        plan[E] = before[0] + n;
+        plan[E] = first + n;
         plan[E + 1] = whole;
-        plan[E + 2] = other + (n % kTileRows != 0);
+        plan[E + 2] = whole + others;
       }
     }
-    int at = before[0];
+    int at = first;
     for (int i = 0; i < kPlanWaves; i++) {
       const int c = cnt[i][tid];
       cnt[i][tid] = at;
@@ -144,8 +174,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_moe_plan(const int32_t* ids, i
     for (int j = 0; j < kPer; j++)
       if ((unsigned)id[j] < (unsigned)E) order[cnt[w][id[j]] + rank[j]] = kPlanThreads * j + tid;
     __syncthreads();
-    const int total = (part[0][0] + part[0][1] + part[0][2] + part[0][3] + 3) / 4;
-    for (int i = tid; i < total; i += kPlanThreads) ((u32x4*)rows)[i] = ((const u32x4*)order)[i];
+    const int quads = ((int)(uint32_t)total[0] + 3) / 4;
+    for (int i = tid; i < quads; i += kPlanThreads) ((u32x4*)rows)[i] = ((const u32x4*)order)[i];
   } else {
     for (int i = tid; i < P; i += kPlanThreads) {
       const int e = ids[i];
@@ -516,20 +546,17 @@ struct TileOf {
   int ct, sp;
 };
 
-// Workgroups go to the 8 XCDs in turn: each takes a run of tiles, row tiles
-// slowest, so that its L2 holds what neighbours share.  The whole tiles first: the
-// others fill the last round.  Returns the row tile, or -1.
+// Workgroups go to the 8 XCDs in turn: each takes a run of the whole tiles, row tiles
+// slowest, so that its L2 holds what neighbours share.  The others, whose neighbours
+// share few rows and no weights, in their order.  Returns the row tile, or -1.
 __device__ __forceinline__ int tile_index(int whole, int others, int nct, int splits, TileOf& t) {
-  const int n0 = whole * nct * splits, n1 = others * nct * splits;
-  const int per0 = (n0 + 7) >> 3, per1 = (n1 + 7) >> 3;
+  const int n0 = whole * nct * splits, n1 = others * nct * splits, per0 = (n0 + 7) >> 3;
   int i = blockIdx.x >> 3;
   if (i < per0) {
     i += (blockIdx.x & 7) * per0;
     if (i >= n0) return -1;
   } else {
-    i -= per0;
-    if (i >= per1) return -1;
-    i += (blockIdx.x & 7) * per1;
+    i = blockIdx.x - 8 * per0;
     if (i >= n1) return -1;
     i += n0;
   }
@@ -564,8 +591,8 @@ __device__ __forceinline__ TileOf own_tile(const MoeArgs& a, int nct, int* rows,
   static_assert(kMoeMaxE <= 64 * kTileWaves, "a thread an expert");
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, P = a.S * a.k;
   int* const cnt = scratch;               // [256]
-  int* const part = scratch + kMoeMaxE;   // [2][4]: whole tiles and others of 64 experts
-  int* const found = part + 2 * kTileWaves;
+  uint64_t* const part = (uint64_t*)(scratch + kMoeMaxE);  // [4]: tiles of 64 experts
+  int* const found = (int*)(part + kTileWaves);
   int* const wave = found + 2;            // [kPer][4]: pairs of the expert
   int id[kPer];
 #pragma unroll
@@ -580,39 +607,37 @@ __device__ __forceinline__ TileOf own_tile(const MoeArgs& a, int nct, int* rows,
   for (int j = 0; j < kPer; j++)
     if (id[j] >= 0) atomicAdd(&cnt[id[j]], 1);
   __syncthreads();
-  const int mine = cnt[tid], own[2] = {mine / kTileRows, mine % kTileRows != 0};
-  int before[2];
-#pragma unroll
-  for (int k = 0; k < 2; k++) {
-    int v = own[k];
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int u = __shfl_up(v, d);
-      if (l >= d) v += u;
-    }
-    before[k] = v - own[k];
-    if (l == 63) part[k * kTileWaves + w] = v;
-  }
+  static_assert(kOwnPairs / kTileRows < 4096 && kMoeMaxE < 4096, "tile_counts in 12 bits");
+  const int mine = cnt[tid];
+  const uint64_t own = tile_counts<12>(mine, true), upto = wave_scan(own);
+  uint64_t before = upto - own, total = 0;
+  if (l == 63) part[w] = upto;
   __syncthreads();
-  int total[2] = {};
 #pragma unroll
-  for (int k = 0; k < 2; k++)
-#pragma unroll
-    for (int i = 0; i < kTileWaves; i++) {
-      const int v = part[k * kTileWaves + i];
-      if (i < w) before[k] += v;
-      total[k] += v;
-    }
-  TileOf t{};
-  const int tile = tile_index(total[0], total[1], nct, a.splits, t);
-  if (tile < 0) return t;
-  if (tile >= before[0] && tile < before[0] + own[0]) {
-    found[0] = tid;
-    found[1] = (tile - before[0]) * kTileRows;
+  for (int i = 0; i < kTileWaves; i++) {
+    if (i < w) before += part[i];
+    total += part[i];
   }
-  if (own[1] && tile == total[0] + before[1]) {
+  const int whole = (int)(total & 0xFFF), full = mine / kTileRows;
+  int others = 0;
+#pragma unroll
+  for (int c = 1; c <= 4; c++) others += (int)(total >> 12 * c & 0xFFF);
+  TileOf t{};
+  const int tile = tile_index(whole, others, nct, a.splits, t);
+  if (tile < 0) return t;
+  const int first = (int)(before & 0xFFF);
+  if (tile >= first && tile < first + full) {
     found[0] = tid;
-    found[1] = own[0] * kTileRows;
+    found[1] = (tile - first) * kTileRows;
+  }
+  int at = whole;
+#pragma unroll
+  for (int c = 1; c <= 4; c++) {
+    if ((own >> 12 * c & 1) && tile == at + (int)(before >> 12 * c & 0xFFF)) {
+      found[0] = tid;
+      found[1] = full * kTileRows;
+    }
+    at += (int)(total >> 12 * c & 0xFFF);
   }
   __syncthreads();
   t.e = __builtin_amdgcn_readfirstlane(found[0]);
