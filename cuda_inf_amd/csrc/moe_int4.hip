@@ -39,7 +39,9 @@ struct MoeArgs {
 
 // Rows of a row tile.  Tiles are in the order of the whole ones of all experts, then
 // the experts' last, partly filled ones, those of the most rows first, as the last
-// round of workgroups ends with the shortest.
+// round of workgroups ends with the shortest.  (4 of 32 experts of 1792, H = 2048, up:
+// 500 tokens 62 us, 77 with these in the order of the experts and a run of them on
+// each XCD.)
 constexpr int kTileRows = 128;
 
 // An expert's n rows: its whole tiles (if whole), and its partly filled one under how
@@ -278,10 +280,10 @@ struct Cols {
 // s, so one 16-byte read brings a column's nibbles for all four steps.
 //   One barrier a half: past the one before half h, h has landed, and all have
 // read h - 1, whose slot h + 2 takes.
-//   4096 tokens of 4 of 32 experts of 1792, H = 2048, up: 252 us, 955 TFLOP/s, where
-// a large fp16 product reaches 1140-1306.  The matrix cores are busy 46 % of it: 3.7
+//   4096 tokens of 4 of 32 experts of 1792, H = 2048, up: 243 us, 990 TFLOP/s, where
+// a large fp16 product reaches 1140-1306.  The matrix cores are busy 49 % of it: 3.7
 // vector instructions (dequantisation, scales) go with a product, and the operands'
-// LDS reads alone take 30 % of the cycles at 128 bytes each.  Few rows an expert are bound by memory: 45 tokens, down,
+// LDS reads alone take 32 % of the cycles at 128 bytes each.  Few rows an expert are bound by memory: 45 tokens, down,
 // 16 us for 59 MB.  (W and X fetched 3 groups ahead instead, where 32 rows leave the
 // slots room: 1 % slower.)
 typedef __attribute__((address_space(3))) void lds_void_t;
@@ -1211,10 +1213,10 @@ static void stream_launch(const MoeArgs& a, hipStream_t s) {
 
 // Column tiles a wave, of 1, 2 and 3: a workgroup's time goes with kNT + 3, and the
 // call's with its rounds of the 512 workgroups that the chip holds, of which the
-// first is never less than nine tenths.  (Of 125 sizes of 5 layers the choice is 1 %
-// slower on average than the best of the three, always 2 would be 5 %, always 1 19 %;
-// 45 tokens of 4 of 32 experts, H = 2048, down 1792 25.7 / 21.3 / 24.7 us, 4096
-// tokens up 352 / 275 / 263.)
+// first is never less than nine tenths.  (Of 125 sizes of 7 layers the choice is 0.6 %
+// slower on average than the best of the three, always 2 would be 5 %, always 1 21 %;
+// 4 of 32 experts of 1792, H = 2048, in us: 45 tokens down 25.7 / 21.3 / 24.7, 220 up
+// 62.4 / 47.0 / 50.8.)
 // Row tiles, about: an expert's last one is partly filled, and with few rows costs
 // less.
 static double row_tiles(int64_t P, int E) {
