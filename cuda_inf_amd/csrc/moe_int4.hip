@@ -427,8 +427,7 @@ struct TileLoop {
   // groups g0 .. g1 - 1; scales(c, g) is column c's
   template <class F>
   __device__ __forceinline__ void run(int g0, const F& scales) {
-    const int l = threadIdx.x & 63;
-    auto refill = [&](int g) __attribute__((always_inline)) {
+    auto refill = [&](int g, int l) __attribute__((always_inline)) {
       constexpr int n = T::kCols * kTabGroups / 64;  // 16 neighbouring lanes a column
       const int gg = g + l % kTabGroups;
       uint16_t v[n];
@@ -443,7 +442,7 @@ struct TileLoop {
       fetch_x<1>(T::kX, g0);
     else
       fetch_x<0>(T::kX, g0 + 1);
-    refill(g0);
+    refill(g0, threadIdx.x & 63);
 #pragma unroll
     for (int j = 0; j < kNT; j++) {
 #pragma unroll
@@ -453,7 +452,13 @@ struct TileLoop {
     }
     int at = 0;
     for (int i = 0; g0 + i < g1; i++) {
-      if (i > 0 && i % kTabGroups == 0) refill(g0 + i);
+      if (i > 0 && i % kTabGroups == 0) {
+        // (worked out anew: kept over the loop its addresses go to scratch, and loads from
+        // there into the count that meet() waits for)
+        int l = threadIdx.x & 63;
+        asm volatile("" : "+v"(l));
+        refill(g0 + i, l);
+      }
       at = group(i, g0 + i, at);
     }
     scale(kUnits - 1, 1, scl);
