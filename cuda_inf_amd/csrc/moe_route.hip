@@ -145,9 +145,10 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, int s, const double* 
       ch[e] = c[i];
     }
   }
-  uint32_t in = 0;  // bit i: expert l + 64 i may be chosen
+  uint32_t real = 0;  // bit i: there is an expert l + 64 i
 #pragma unroll
-  for (int i = 0; i < kPer; i++) in |= (l + 64 * i < a.E ? 1u : 0u) << i;
+  for (int i = 0; i < kPer; i++) real |= (l + 64 * i < a.E ? 1u : 0u) << i;
+  uint32_t in = real;  // that may be chosen
   if (a.n_group > 1) {
     // lane l has groups l, l + 64, ..: the sum of a group's two best choices
     const int per = a.E / a.n_group;
@@ -200,8 +201,8 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, int s, const double* 
   }
   // k rounds (and one more for how near the next one is): the best choice left, the
   // lowest index among equals; lane j keeps round j's
-  const bool all = a.n_group > 1 || (a.softmax && a.bias) || !safe;  // of the experts are in doubt, if any
-  const uint32_t in0 = in;
+  const bool all = a.n_group > 1 || (a.softmax && a.bias) || !safe;  // of those below are in doubt, if any
+  const uint32_t in0 = safe ? in : real;  // (where the groups are in doubt, the ones left out as well)
   int id = 0;
   double w = 0.0, above = __builtin_inf(), above_off = 0.0;
   for (int j = 0; j < a.k + (far != 0.0 ? 1 : 0); j++) {

@@ -144,6 +144,44 @@ def test_route_of_near_choices(K, dev, S, E, kw):
         assert len(set(r.tolist())) == k and (r >= 0).all() and (r < E).all()
 
 
+@pytest.mark.parametrize("S", [40, 1100, 2050])
+@pytest.mark.parametrize("E,kw", [(32, dict(k=4, n_group=2, topk_group=1)), (64, dict(k=6, n_group=8, topk_group=3)),
+                                  (64, dict(k=3, n_group=8, topk_group=1, score="softmax")),
+                                  (132, dict(k=5, n_group=12, topk_group=5, score="softmax"))])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("apart", [False, True])
+def test_route_of_near_groups(K, dev, S, E, kw, bias, apart):
+    """Groups in pairs of equal gate rows, or of rows whose logits are 2^-26 apart, with
+    an odd number of groups kept: the last one kept and the first one left out are
+    such a pair.  Numbers are whole multiples of small powers of two, so that 64 bits
+    hold every sum exactly, in any order, and fp32 does not."""
+    kw = dict(kw)
+    k, H, per = kw.pop("k"), 512, E // kw["n_group"]
+    rng = np.random.default_rng(E + S)
+    x = rng.integers(-2047, 2048, (S, H)) / 1024.0
+    gate = rng.integers(-2047, 2048, (E // 2, H)) / 65536.0
+    gate = np.repeat(gate.reshape(-1, 1, per, H), 2, axis=1).reshape(E, H)
+    if apart:
+        x[:, 7] = rng.integers(-1, 2, S) / 1024.0
+        gate[:, 7] = rng.integers(-2047, 2047, E) / 65536.0
+        second = np.arange(E) // per % 2 == 1
+        gate[second, 7] = gate[np.flatnonzero(second) - per, 7] + 1.0 / 65536.0
+    x, gate = x.astype(np.float16), gate.astype(np.float16)
+    b = np.repeat(0.1 * rng.standard_normal((E // 2 // per, 1, per)), 2, axis=1).reshape(E).astype(np.float32) if bias else None
+    l = (x.astype(np.float64) * 2.0 ** 10) @ (gate.astype(np.float64) * 2.0 ** 16).T * 2.0 ** -26
+    ids, wt = ref.choose(l, b, k, **kw)
+    gi, gw = torch.full((S, k), -7, dtype=torch.int32, device=dev), torch.zeros((S, k), device=dev)
+    K.moe_route(t(x, dev), t(gate, dev), gi, gw, S, H, E, k, bias=t(b, dev), **kw)
+    wrong = (gi.cpu().numpy() != ids).any(1)
+    assert not wrong.any(), f"{wrong.sum()} of {S} tokens, first {np.flatnonzero(wrong)[0]}"
+    far = 32 * ref.U24 * (np.abs(x.astype(np.float64)) @ np.abs(gate.astype(np.float64)).T)
+    within(gw.cpu().numpy(), wt, ref.weights_bound(l, far, ids, wt, **kw), "weights")
+    i1, w1 = torch.empty((1, k), dtype=torch.int32, device=dev), torch.empty((1, k), device=dev)
+    for i in range(0, S, S // 13):
+        K.moe_route(t(x[i:i + 1], dev), t(gate, dev), i1, w1, 1, H, E, k, bias=t(b, dev), **kw)
+        assert torch.equal(i1[0], gi[i])
+
+
 @pytest.mark.parametrize("E,kw", [(32, dict(k=4)), (9, dict(k=3, score="softmax")),
                                   (64, dict(k=5, n_group=8, topk_group=2, score="softmax", renorm=False)),
                                   (256, dict(k=8, n_group=4, topk_group=2)), (100, dict(k=10))])
