@@ -37,7 +37,8 @@ extern "C" {
  * h, add, hsum: fp32 [S][H]; add may be NULL (nothing is added); hsum may be
  * NULL (the sum is not kept), h or add (in place).  w: fp16 [H].  out: fp16
  * [S][H].  H a multiple of 8 and at most CIA_FFN_MAX_WIDTH, S at most
- * CIA_FFN_MAX_TOKENS; all pointers 16-byte aligned.  Sums are fp32. */
+ * CIA_FFN_MAX_TOKENS; all pointers 16-byte aligned.  Sums are fp32, a lane's
+ * part of a row above 8192 in 64 bits. */
 int cia_add_rmsnorm(const float* h, const float* add, const uint16_t* w,
                     float eps, float* hsum, uint16_t* out, int S, int H,
                     void* stream);

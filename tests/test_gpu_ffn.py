@@ -48,6 +48,27 @@ def test_norm(K, dev, S, H, add):
     assert torch.equal(out, out2) and torch.equal(hd, hs)
 
 
+@pytest.mark.parametrize("H", [(1 << 24) - 8, 1 << 24, (1 << 22) + 8])
+def test_norm_of_the_longest_rows(K, dev, H):
+    """Rows whose elements are all alike, whose squares lose the same at every addition
+    where they are added up in one fp32 chain: the bound does not grow with H."""
+    rng = np.random.default_rng(H)
+    w = (1 + rng.random(H)).astype(np.float16)
+    value = np.array([1.3361171, 1.0165276, 0.03], np.float32)
+    h = np.repeat(value[:, None], H, 1)
+    h[2] = rng.standard_normal(H)
+    out = torch.empty((3, H), dtype=torch.float16, device=dev)
+    K.add_rmsnorm(t(h, dev), t(w, dev), out, 3, H, 1e-5)
+    got = out.cpu().numpy()
+    for r in range(3):
+        s = h[r].astype(np.float64)
+        y = s / np.sqrt((s * s).mean() + 1e-5) * w.astype(np.float64)
+        # 8 squares a step, the steps in 64 bits, at most 16 additions where the row's
+        # parts meet: 24 half steps, halved by the root; mean, eps, root, quotient, two
+        # products; then fp16
+        within(got[r], y, np.abs(y) * (ref.U11 * 1.001 + (12 + 8) * ref.U24) + 2.0 ** -25, f"row {r}")
+
+
 def test_norm_rows_of_zeros_and_beyond_numbers(K, dev):
     h = torch.zeros((4, 256), device=dev)
     h[1, 3], h[2, 5] = float("nan"), float("inf")
