@@ -1284,7 +1284,8 @@ static int products(MoeArgs& a, void* ws, bool planned, hipStream_t s) {
 using namespace cia;
 
 extern "C" int64_t cia_moe_workspace_bytes(int S, int k, int E, int H, int F) {
-  if (S < 0 || k < 1 || k > kMoeMaxK || E < 1 || E > kMoeMaxE || H < 1 || H > kMoeMaxCols || F < 1 || F > kMoeMaxCols)
+  if (S < 0 || k < 1 || k > kMoeMaxK || E < 1 || E > kMoeMaxE || H < 1 || H > kMoeMaxCols || H % 128 || F < 1 ||
+      F > kMoeMaxCols || F % 128)
     return 0;
   const int64_t P = (int64_t)S * k;
   return plan_bytes(P, E) + y_rows(P) * H * 4;
@@ -1404,8 +1405,9 @@ BlockWs block_ws(const cia_moe* M, int S) {
 }  // namespace
 
 extern "C" int64_t cia_moe_block_workspace_bytes(const cia_moe* M, int cap) {
-  if (!M || cap < 0 || !cia_moe_workspace_bytes(0, M->gate ? M->gating.top_k : 1, M->gate ? M->gating.n_experts : 1, M->H, M->F))
-    return 0;
+  if (!M || cap < 0) return 0;
+  const int k = M->gate ? M->gating.top_k : 1, E = M->gate ? M->gating.n_experts : 1;
+  if (!cia_moe_workspace_bytes(0, k, E, M->H, M->F) || (int64_t)cap * k > kMoeMaxPairs) return 0;
   return block_ws(M, cap).end;
 }
 

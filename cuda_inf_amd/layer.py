@@ -260,7 +260,9 @@ class MoeBlock:
             M.gating = moe_gating(E, top_k, eps=renorm_eps, **gating)
         M.cap = max_batch
         M.ws_bytes = _lib.lib().cia_moe_block_workspace_bytes(ctypes.byref(M), max_batch)
-        self.ws = torch.empty(max(M.ws_bytes, 16), dtype=torch.uint8, device=dev)
+        if not M.ws_bytes:
+            raise ValueError(f"max_batch={max_batch}, top_k={top_k}, {E} experts of {F}, H={H}: beyond what a call takes")
+        self.ws = torch.empty(M.ws_bytes, dtype=torch.uint8, device=dev)
         M.ws = self.ws.data_ptr()
         self._m = M
 

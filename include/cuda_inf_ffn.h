@@ -128,7 +128,8 @@ int cia_moe_down_int4(const uint16_t* act, const int32_t* ids,
                       int F, void* ws, int64_t ws_bytes, void* stream);
 
 /* Workspace bytes of cia_moe_up_int4 and cia_moe_down_int4 for up to S tokens;
- * 0 where S is negative or another argument outside its limits. */
+ * 0 where S is negative, or k, E, H or F is one that they refuse.  (More than
+ * CIA_MOE_MAX_PAIRS pairs have a size as well, though no call takes them.) */
 int64_t cia_moe_workspace_bytes(int S, int k, int E, int H, int F);
 
 /* The feed-forward branch of one layer. */
@@ -147,7 +148,9 @@ typedef struct cia_moe {
   int cap;                 /* tokens a call may bring */
 } cia_moe;
 
-/* Scratch bytes of a branch for calls of up to cap tokens. */
+/* Scratch bytes of a branch for calls of up to cap tokens; 0 where cap is
+ * negative, cap tokens make more than CIA_MOE_MAX_PAIRS pairs, or top_k,
+ * n_experts, H or F is one that cia_moe_workspace_bytes gives 0 for. */
 int64_t cia_moe_block_workspace_bytes(const cia_moe* M, int cap);
 
 /* The feed-forward branch (engine.cu:869-905) for S <= M->cap tokens, from the

@@ -163,6 +163,26 @@ def test_workspace_bytes(L):
     assert last > 1 << 32
 
 
+@pytest.mark.parametrize("H,F", [(192, 1792), (2048, 64), (2049, 128), (2048, 32768 + 128), (32768 + 128, 128)])
+def test_workspace_bytes_of_widths_that_no_call_takes(L, H, F):
+    from cuda_inf_amd import _lib
+    assert L.cia_moe_workspace_bytes(1, 4, 32, H, F) == 0
+    M = _lib.cia_moe(H=H, F=F, gate=A, gating=_lib.cia_moe_gating(*GOOD.values()))
+    assert L.cia_moe_block_workspace_bytes(ctypes.byref(M), 8) == 0
+    M.H, M.F = 32768, 32768  # the widest
+    assert L.cia_moe_workspace_bytes(1, 4, 32, 32768, 32768) > 0
+    assert L.cia_moe_block_workspace_bytes(ctypes.byref(M), 8) > 0
+
+
+def test_block_workspace_bytes_of_batches_that_no_call_takes(L):
+    from cuda_inf_amd import _lib
+    M = _lib.cia_moe(H=2048, F=1792, gate=A, gating=_lib.cia_moe_gating(*GOOD.values()))
+    f = L.cia_moe_block_workspace_bytes
+    assert f(ctypes.byref(M), 1 << 18) > 1 << 32 and f(ctypes.byref(M), (1 << 18) + 1) == 0
+    M.gate = None  # a dense layer: a row a token
+    assert f(ctypes.byref(M), 1 << 20) > 1 << 32 and f(ctypes.byref(M), (1 << 20) + 1) == 0
+
+
 def test_strides_of_one_expert_are_not_read(L):
     w = q4(1, 128, 256, packed_stride=-7, scales_stride=-1)
     n = L.cia_moe_workspace_bytes(1, 1, 1, 256, 128)

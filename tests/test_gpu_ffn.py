@@ -624,6 +624,14 @@ def test_blocks_refusals(K, dev):
         K.moe_up_int4(norm_w, None, w1, w2, norm_w, 1, 1, B.ws)
 
 
+def test_a_block_for_a_batch_that_no_call_takes(K, dev):
+    rng = np.random.default_rng(4)
+    for E, k, most in ((4, 2, 1 << 19), (1, 1, 1 << 20)):
+        for n in (-1, most + 1):
+            with pytest.raises(ValueError, match="max_batch"):
+                block(dev, rng, E, k, 128, 128, max_batch=n)
+
+
 def test_another_stream(K, dev):
     rng = np.random.default_rng(10)
     B, _ = block(dev, rng, 8, 2, 256, 384, max_batch=64)
