@@ -250,7 +250,7 @@ struct Cols {
     last = a.N - 1;
     ng = a.K >> 7;
   }
-  // (an expert's bytes and scales: at most 2^39 and 2^33)
+  // (an expert's bytes and scales: at most 2^29 and 2^23)
   __device__ __forceinline__ size_t row(int c) const {
     const int n = kUp ? c >> 1 : c;
     return (size_t)((uint64_t)(uint32_t)(n < last ? n : last) * (uint32_t)ng);

@@ -150,6 +150,21 @@ def test_down_refusals(L, kw, code):
     assert L.cia_moe_down_int4(A, A, A, None, A, A, 3, 2, 4, 256, 128, A, 1 << 30, None) == NULL
 
 
+@pytest.mark.parametrize("kw,code", [
+    (dict(H=32768, F=32768), OK), (dict(H=32768 + 128), ARG), (dict(F=32768 + 128), ARG), (dict(E=256, k=16), OK),
+    (dict(S=1 << 19, k=2, ws_less=1), ARG), (dict(S=(1 << 19) + 1, k=2), ARG)])
+def test_limits_of_the_products(L, kw, code):
+    """The largest of each argument (of no tokens, or refused for what is looked at
+    later), and one more."""
+    d = put({"S": 0, **kw})
+    n = L.cia_moe_workspace_bytes(*(d[i] for i in "SkEHF")) - d["ws_less"]
+    assert (n > 0) == (d["H"] <= 32768 and d["F"] <= 32768)
+    w, w2 = q4(d["E"], d["F"], d["H"]), q4(d["E"], d["H"], d["F"])
+    sizes = [d[i] for i in "SkEHF"]
+    assert L.cia_moe_up_int4(A, A, ctypes.byref(w), ctypes.byref(w), A, *sizes, A, n, None) == code
+    assert L.cia_moe_down_int4(A, A, A, ctypes.byref(w2), A, A, *sizes, A, n, None) == code
+
+
 def test_workspace_bytes(L):
     f = L.cia_moe_workspace_bytes
     assert f(-1, 4, 32, 2048, 1792) == 0 and f(1, 0, 32, 2048, 1792) == 0 and f(1, 4, 0, 2048, 1792) == 0
