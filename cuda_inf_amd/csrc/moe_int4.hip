@@ -14,6 +14,7 @@
 // part: its act row is left as it is, and it adds nothing to out.
 #include "common.h"
 #include "cuda_inf_ffn.h"
+#include "moe_shape.h"
 
 namespace cia {
 
@@ -37,12 +38,11 @@ struct MoeArgs {
   float* out;             // null: into y
 };
 
-// Rows of a row tile.  Tiles are in the order of the whole ones of all experts, then
+// Row tiles of kTileRows are in the order of the whole ones of all experts, then
 // the experts' last, partly filled ones, those of the most rows first, as the last
 // round of workgroups ends with the shortest.  (4 of 32 experts of 1792, H = 2048, up:
 // 500 tokens 62 us, 77 with these in the order of the experts and a run of them on
 // each XCD.)
-constexpr int kTileRows = 128;
 
 // An expert's n rows: its whole tiles (if whole), and its partly filled one under how
 // many times 32 rows it has, 4 first, in fields of kBits from the lowest.  256 experts'
@@ -64,8 +64,6 @@ __device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
   return v;
 }
 
-// The most row tiles P pairs of E experts can make
-__host__ __device__ constexpr int64_t max_tiles(int64_t P, int E) { return P / kTileRows + (P < E ? P : E); }
 // plan: offs[E + 1], whole tiles, tiles, (expert, first) of each, rows[P]
 // (rows 16-byte aligned, and written 4 at a time)
 __host__ __device__ constexpr int64_t plan_rows_at(int64_t P, int E) { return (E + 3 + 2 * max_tiles(P, E) + 3) / 4 * 4; }
@@ -544,10 +542,7 @@ __device__ __forceinline__ void tile_run(const MoeArgs& a, uint8_t* lds, uint16_
 }
 
 // A workgroup's tile: its expert, rows and their rows of x, in rows[128] and
-// rows[128 + ..].  From the plan, or from up to kOwnPairs ids by itself (which
-// saves the plan's launch, 4 us).
-constexpr int kOwnPairs = 1024;
-
+// rows[128 + ..].  From the plan, or from up to kOwnPairs ids by itself.
 struct TileOf {
   int e, n;  // n = 0: none
   int ct, sp;
@@ -713,12 +708,6 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void k_moe_tile(MoeArgs a) {
 // and 3.2 the weights at a copy's rate; 12 such tokens 17.4 us.
 // Rows by expert are found by the workgroup itself, from up to kStreamPairs ids:
 // no launch before this one.
-constexpr int kStreamWaves = 8, kStreamPairs = 64 * kStreamWaves, kUnits = 256;  // compute units
-constexpr int kStreamMaxK = 4 * 8 * 128;  // 4 groups a wave, of one part of K
-
-// groups a wave -> row tiles that x leaves registers for
-__host__ __device__ constexpr int stream_mt(int kg) { return kg <= 2 ? 4 : 2; }
-
 template <int kG, int kMT>
 struct Stream {
   static constexpr int kRing = kG <= 2 ? 4 : 2;
@@ -962,7 +951,6 @@ __global__ __launch_bounds__(64 * kStreamWaves, (2 * Stream<kG, kMT>::kPerUnit))
 // waves where K has more than 8 groups: 1 token of 4 of 32 experts of 1792, H =
 // 2048, 8.1 us with 8 waves, 7.4 with 16; 6 of 64 of 768 6.8 / 7.4.  (Calls in us,
 // in two launches / so: the first 11.8 / 8.8, 4 such tokens, 16 pairs, 16.4 / 19.2.)
-constexpr int kFewPairs = 8;
 static_assert(kFewPairs <= 8, "a wave an expert's sums; an expert's rows in a row tile");
 
 struct FewArgs {
@@ -1155,19 +1143,6 @@ __global__ __launch_bounds__(256) void k_moe_combine(CombineArgs a) {
 // ---------------------------------------------------------------- host
 static int64_t plan_bytes(int64_t P, int E) { return ((plan_rows_at(P, E) + P + 3) * 4 + 255) / 256 * 256; }
 
-// Rows of y: P, and room for parts of K where few pairs leave the chip empty
-static int64_t y_rows(int64_t P) { return P >= 4096 ? P : (8 * P < 4096 ? 8 * P : 4096); }
-
-// Parts of K of a down launch in tiles: as many as the chip's 512 places hold of
-// workgroups of 128 columns, each part of 4 groups or more.
-static double row_tiles(int64_t P, int E);
-static int k_splits(int64_t P, int E, int H, int F) {
-  int64_t n = (int64_t)(512.0 / (row_tiles(P, E) * ((H + 127) / 128)));
-  n = n < y_rows(P) / P ? n : y_rows(P) / P;
-  n = n < F / 512 ? n : F / 512;
-  return n < 1 ? 1 : (int)n;
-}
-
 static int moe_check(int S, int k, int E, int H, int F, const int32_t* ids) {
   CIA_REQUIRE(S >= 0 && k >= 1 && k <= kMoeMaxK && E >= 1 && E <= kMoeMaxE && H > 0 && F > 0 &&
                   H % 128 == 0 && F % 128 == 0 && H <= kMoeMaxCols && F <= kMoeMaxCols &&
@@ -1193,27 +1168,14 @@ static void set_w(MoeArgs& a, int i, const cia_q4_experts* w) {
   a.sstride[i] = w->scales_stride;
 }
 
-// Whether the weights are streamed rather than multiplied in tiles: while experts
-// have 2 (up), 1.5 (down) rows on average, or pairs are few.  Calls in us, streamed /
-// in tiles: 4 of 32 experts of 1792, H = 2048, up 16 tokens 21.0 / 24.5, 20 26.9 /
-// 25.0, 40 30.6 / 30.4, down 12 15.6 / 16.7, 20 23.7 / 18.1; 8 of 128 of 1536, H =
-// 4096, up 8 66 / 76, 32 119 / 114, down 24 64 / 67, 64 90 / 87; 2 of 8 of 2048, H =
-// 1024, up 32 9.7 / 10.5, 40 13.3 / 11.1, down 4 8.5 / 8.5, 12 13.7 / 11.0; the dense
-// form of 7168, H = 2048, up 32 rows 11.5 / 12.3, 64 16.1 / 14.6, down 16 12.1 / 13.8,
-// 24 14.4 / 13.9.  (Down takes a K of two parts as well.)
-static bool streams(bool up, int64_t P, int E, int K) {
-  const int64_t most = up ? 2 * (int64_t)E : 3 * (int64_t)E / 2, few = up ? 64 : 16;
-  return P <= (most > few ? most : few) && K <= (up ? 1 : 2) * kStreamMaxK;
-}
 static_assert(2 * kMoeMaxE <= kStreamPairs && 64 <= kStreamPairs, "a thread a pair");
 
-// 16 rows at a time with two workgroups a compute unit where experts hardly have
-// more; up to 64 rows of up's few pairs of few experts
+// (16 rows at a time: two workgroups a compute unit)
 template <bool kUp, int kG>
-static void stream_launch(const MoeArgs& a, hipStream_t s) {
+static void stream_launch(const MoeArgs& a, int mt, hipStream_t s) {
   const dim3 block(64 * kStreamWaves);
   const int64_t P = (int64_t)a.S * a.k;
-  if (kUp && P > 8 * (int64_t)a.E) {
+  if (kUp && mt > 1) {
     hipLaunchKernelGGL((k_moe_stream<kUp, kG, kUp ? stream_mt(kG) : 1>), dim3(kUnits), block, 0, s, a);
     return;
   }
@@ -1221,31 +1183,6 @@ static void stream_launch(const MoeArgs& a, hipStream_t s) {
   const int64_t tiles = (P < a.E ? P : a.E) * ((kUp ? 2 * a.N : a.N) >> 4) * (kUp ? 1 : a.splits);
   const int n = tiles <= 4 * kUnits ? kUnits : kUnits * Stream<kG, 1>::kPerUnit;
   hipLaunchKernelGGL((k_moe_stream<kUp, kG, 1>), dim3(n), block, 0, s, a);
-}
-
-// Column tiles a wave, of 1, 2 and 3: a workgroup's time goes with kNT + 3, and the
-// call's with its rounds of the 512 workgroups that the chip holds, of which the
-// first is never less than nine tenths.  (Of 125 sizes of 7 layers the choice is 0.6 %
-// slower on average than the best of the three, always 2 would be 5 %, always 1 21 %;
-// 4 of 32 experts of 1792, H = 2048, in us: 45 tokens down 25.7 / 21.3 / 24.7, 220 up
-// 62.4 / 47.0 / 50.8.)
-// Row tiles, about: an expert's last one is partly filled, and with few rows costs
-// less.
-static double row_tiles(int64_t P, int E) {
-  return E > 1 ? (double)P / kTileRows + 0.75 * (double)(P < E ? P : E) : (double)((P + kTileRows - 1) / kTileRows);
-}
-static int tile_nt(int64_t P, int E, int nv, int splits) {
-  int best = 1;
-  double least = 0.0;
-  for (int nt = 1; nt <= 3; nt++) {
-    const double rounds = row_tiles(P, E) * ((nv + 64 * nt - 1) / (64 * nt)) * splits / 512.0;
-    const double t = (rounds < 0.9 ? 0.9 : rounds) * (nt + 3);
-    if (nt == 1 || t < least) {
-      best = nt;
-      least = t;
-    }
-  }
-  return best;
 }
 
 template <bool kUp, int kNT>
@@ -1257,21 +1194,19 @@ static void tile_launch(const MoeArgs& a, hipStream_t s) {
 
 // planned: ws holds the plan of these ids already
 template <bool kUp>
-static int products(MoeArgs& a, void* ws, bool planned, hipStream_t s) {
-  const int P = a.S * a.k;
-  if (streams(kUp, P, a.E, a.K)) {
-    const int part = ((a.K >> 7) + a.splits - 1) / a.splits;  // groups
-    if (part <= 8)
-      stream_launch<kUp, 1>(a, s);
-    else if (part <= 16)
-      stream_launch<kUp, 2>(a, s);
-    else
-      stream_launch<kUp, 4>(a, s);
+static int products(MoeArgs& a, const MoeShape& shape, void* ws, bool planned, hipStream_t s) {
+  if (shape.kernel == kMoeStream) {
+    switch (shape.a) {
+      case 1: stream_launch<kUp, 1>(a, shape.b, s); break;
+      case 2: stream_launch<kUp, 2>(a, shape.b, s); break;
+      default: stream_launch<kUp, 4>(a, shape.b, s);
+    }
     return launch_status();
   }
-  a.plan = P <= kOwnPairs ? nullptr : (const int*)ws;
-  if (a.plan && !planned) hipLaunchKernelGGL(k_moe_plan, dim3(1), dim3(kPlanThreads), 0, s, a.ids, P, a.E, (int*)ws);
-  switch (tile_nt(P, a.E, kUp ? 2 * a.N : a.N, a.splits)) {
+  a.plan = shape.b ? (const int*)ws : nullptr;
+  if (a.plan && !planned)
+    hipLaunchKernelGGL(k_moe_plan, dim3(1), dim3(kPlanThreads), 0, s, a.ids, a.S * a.k, a.E, (int*)ws);
+  switch (shape.a) {
     case 1: tile_launch<kUp, 1>(a, s); break;
     case 2: tile_launch<kUp, 2>(a, s); break;
     default: tile_launch<kUp, 3>(a, s);
@@ -1311,8 +1246,9 @@ static int moe_up(const uint16_t* x, const int32_t* ids, const cia_q4_experts* w
   a.k = k;
   a.E = E;
   a.act = act;
-  a.splits = 1;
-  return products<true>(a, ws, false, (hipStream_t)stream);
+  const MoeShape shape = moe_shape(true, (int64_t)S * k, E, H, F);
+  a.splits = shape.splits;
+  return products<true>(a, shape, ws, false, (hipStream_t)stream);
 }
 
 extern "C" int cia_moe_up_int4(const uint16_t* x, const int32_t* ids, const cia_q4_experts* w1,
@@ -1345,25 +1281,26 @@ static int moe_down(const uint16_t* act, const int32_t* ids, const float* weight
   a.k = k;
   a.E = E;
   a.y = (float*)((char*)ws + plan_bytes((int64_t)S * k, E));
-  a.splits = streams(false, (int64_t)S * k, E, F) ? (F + kStreamMaxK - 1) / kStreamMaxK : k_splits((int64_t)S * k, E, H, F);
+  const MoeShape shape = moe_shape(false, (int64_t)S * k, E, F, H);
+  a.splits = shape.splits;
   hipStream_t s = (hipStream_t)stream;
-  if (S * (int64_t)k <= kFewPairs && F <= kStreamMaxK) {
+  if (shape.kernel == kMoeFew) {
     const FewArgs f{a, weights, res, out};
     const dim3 grid((unsigned)(H / 16));
-    if (F <= 1024)
+    if (shape.a == 8)
       hipLaunchKernelGGL((k_moe_few<8, 1>), grid, dim3(512), 0, s, f);
-    else if (F <= 2048)
+    else if (shape.b == 1)
       hipLaunchKernelGGL((k_moe_few<16, 1>), grid, dim3(1024), 0, s, f);
     else
       hipLaunchKernelGGL((k_moe_few<16, 2>), grid, dim3(1024), 0, s, f);
     return launch_status();
   }
-  if (!ids && !weights && a.splits == 1 && !streams(false, (int64_t)S * k, E, F)) {
+  if (!ids && !weights && a.splits == 1 && shape.kernel == kMoeTile) {
     a.res = res;
     a.out = out;
-    return products<false>(a, ws, planned, s);
+    return products<false>(a, shape, ws, planned, s);
   }
-  if ((st = products<false>(a, ws, planned, s))) return st;
+  if ((st = products<false>(a, shape, ws, planned, s))) return st;
   const CombineArgs c{a.y, ids, weights, res, out, S, k, E, H, a.splits};
   const unsigned blocks = (unsigned)((H + 1023) / 1024) * (unsigned)S;
   const dim3 grid(blocks < kCombineGrid ? blocks : kCombineGrid);
