@@ -202,7 +202,9 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, int s, const double* 
   // k rounds (and one more for how near the next one is): the best choice left, the
   // lowest index among equals; lane j keeps round j's
   const bool all = a.n_group > 1 || (a.softmax && a.bias) || !safe;  // of those below are in doubt, if any
-  const uint32_t in0 = safe ? in : real;  // (where the groups are in doubt, the ones left out as well)
+  // (where the groups are in doubt, the ones left out as well; beside a bias the
+  // distance of two scores hangs on the sum over all experts)
+  const uint32_t in0 = safe && !(a.softmax && a.bias) ? in : real;
   int id = 0;
   double w = 0.0, above = __builtin_inf(), above_off = 0.0;
   for (int j = 0; j < a.k + (far != 0.0 ? 1 : 0); j++) {

@@ -203,6 +203,62 @@ def test_route_of_near_groups(K, dev, S, E, kw, bias, apart):
         assert torch.equal(i1[0], gi[i])
 
 
+def near_tokens(rng, S, near, H, E, n_group, topk_group, k, unit):
+    """Whole numbers x [S, H], gate [E, H] (a logit is unit times their product's sum)
+    and bias [E]: of the first tokens, two of the choices by softmax and bias that
+    follow one another lie some 1e-11 apart."""
+    per = E // n_group
+    x = rng.integers(-2047, 2048, (S, H)).astype(np.float64)
+    gate = rng.integers(-2047, 2048, (E, H)).astype(np.float64)
+    gate[:, :16] = rng.integers(-7, 8, (E, 16))  # (x moves the logits little here)
+    bias = (0.2 * rng.standard_normal(E)).astype(np.float32)
+
+    def soft(l):
+        p = np.exp(l - l.max(-1, keepdims=True))
+        return p / p.sum(-1, keepdims=True)
+
+    for t in range(near):
+        l = x[t] @ gate.T * unit
+        c = soft(l) + bias
+        kept = np.argsort(-np.sort(c.reshape(n_group, per), 1)[:, -2:].sum(1), kind="stable")[:topk_group]
+        of = (kept[:, None] * per + np.arange(per)).reshape(-1)
+        of = of[np.argsort(-c[of], kind="stable")][:k + 1]
+        j = int(np.argmin(c[of[:-1]] - c[of[1:]]))
+        a, b = of[j], of[j + 1]
+        for few, most in ((False, 2047), (False, 512), (True, 2047), (True, 2047), (True, 40), (True, 3)):
+            cols = np.arange(16) if few else rng.permutation(np.arange(16, H))[:16]
+            move = rng.integers(-most, most + 1, (3000, 16)) * (rng.random((3000, 16)) < (1.0 if few else 0.3))
+            move[0] = 0
+            move = np.clip(x[t, cols] + move, -2047, 2047) - x[t, cols]
+            s = soft(l + move @ gate[:, cols].T * unit)
+            x[t, cols] += move[np.argmin(np.abs(s[:, a] - s[:, b] + np.float64(bias[a]) - np.float64(bias[b])))]
+            l = x[t] @ gate.T * unit
+    return x, gate, bias
+
+
+@pytest.mark.parametrize("E,H,unit,kw", [(48, 256, 2.0 ** -24, dict(k=4, n_group=6, topk_group=3)),
+                                         (48, 512, 2.0 ** -24, dict(k=4, n_group=12, topk_group=2)),
+                                         (128, 256, 2.0 ** -23, dict(k=6, n_group=8, topk_group=2)),
+                                         (48, 256, 2.0 ** -23, dict(k=4, n_group=1, topk_group=1))])
+def test_route_of_near_choices_by_softmax_and_bias(K, dev, E, H, unit, kw):
+    """Beside a bias a score's distance to another hangs on the sum over all experts,
+    those of the groups that are left out among them."""
+    kw = dict(kw, score="softmax")
+    k, S = kw.pop("k"), 1100
+    X, G, b = near_tokens(np.random.default_rng(E + H), S, 64, H, E, kw["n_group"], kw["topk_group"], k, unit)
+    x, gate = (X * (unit * 65536.0)).astype(np.float16), (G / 65536.0).astype(np.float16)
+    l = X @ G.T * unit  # (exact: whole numbers below 2^31)
+    ids, wt = ref.choose(l, b, k, **kw)
+    # (scores in 64 bits are 1e-16 off: tokens that hang on it say nothing)
+    p = np.exp(l - l.max(1, keepdims=True))
+    clear = (np.diff(np.sort(p / p.sum(1, keepdims=True) + b, 1), axis=1) > 1e-14).all(1)
+    assert clear.sum() > S - 20
+    gi, gw = torch.full((S, k), -7, dtype=torch.int32, device=dev), torch.zeros((S, k), device=dev)
+    K.moe_route(t(x, dev), t(gate, dev), gi, gw, S, H, E, k, bias=t(b, dev), **kw)
+    wrong = (gi.cpu().numpy() != ids).any(1) & clear
+    assert not wrong.any(), f"{wrong.sum()} of {S} tokens, first {np.flatnonzero(wrong)[0]}"
+
+
 @pytest.mark.parametrize("E,kw", [(32, dict(k=4)), (9, dict(k=3, score="softmax")),
                                   (64, dict(k=5, n_group=8, topk_group=2, score="softmax", renorm=False)),
                                   (256, dict(k=8, n_group=4, topk_group=2)), (100, dict(k=10))])
