@@ -148,7 +148,9 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, int s, const double* 
   uint32_t real = 0;  // bit i: there is an expert l + 64 i
 #pragma unroll
   for (int i = 0; i < kPer; i++) real |= (l + 64 * i < a.E ? 1u : 0u) << i;
-  uint32_t in = real;  // that may be chosen
+  uint32_t in = real;     // that may be chosen
+  uint32_t again = real;  // that may turn out to be, where the choice is in doubt
+  bool groups_safe = true;
   if (a.n_group > 1) {
     // lane l has groups l, l + 64, ..: the sum of a group's two best choices
     const int per = a.E / a.n_group;
@@ -172,39 +174,48 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, int s, const double* 
 #pragma unroll
     for (int i = 0; i < kPer; i++)
       if (l + 64 * i < a.n_group) ch[l + 64 * i] = best[i];
-    uint32_t keep = 0;
+    uint32_t keep = 0, open = 0;
 #pragma unroll
     for (int i = 0; i < kPer; i++) {
       const int g = l + 64 * i;
       if (64 * i >= a.n_group) break;
-      int rank = 0;
-      bool near = false;  // another group's sum of two
+      int rank = 0, sure = 0;  // groups that are before it, and that are so for sure
+      bool near = false;       // another group's sum of two
       const double o = 4.0 * off(largest, best[i]);
 #pragma unroll 8
       for (int j = 0; j < a.n_group; j++) {
         rank += ch[j] > best[i] || (ch[j] == best[i] && j < g);
+        sure += ch[j] - best[i] > o;
         near = near || (j != g && __builtin_fabs(ch[j] - best[i]) <= o);
       }
       keep |= (g < a.n_group && rank < a.topk_group ? 1u : 0u) << i;
+      open |= (g < a.n_group && sure < a.topk_group ? 1u : 0u) << i;
       // (only the last one in and the first one out matter)
       if (far != 0.0)
-        safe = safe && !__any(g < a.n_group && near && rank >= a.topk_group - 1 && rank <= a.topk_group);
+        groups_safe = groups_safe && !__any(g < a.n_group && near && rank >= a.topk_group - 1 && rank <= a.topk_group);
     }
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int i = 0; i < kPer; i++)
-      if (l + 64 * i < a.n_group) ch[l + 64 * i] = keep >> i & 1 ? 1.0 : 0.0;
-    in = 0;
+      if (l + 64 * i < a.n_group) ch[l + 64 * i] = keep >> i & 1 ? 2.0 : open >> i & 1 ? 1.0 : 0.0;
+    in = again = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; i++)
-      if (l + 64 * i < a.E && ch[(l + 64 * i) / per] != 0.0) in |= 1u << i;
+    for (int i = 0; i < kPer; i++) {
+      const double of = l + 64 * i < a.E ? ch[(l + 64 * i) / per] : 0.0;
+      in |= (of == 2.0 ? 1u : 0u) << i;
+      again |= (of != 0.0 ? 1u : 0u) << i;
+    }
+    if (groups_safe) again = in;
   }
+  // Beside a bias the distance of two scores hangs on the sum over all experts.  Where
+  // the groups are in doubt, all of those that are not out for sure are looked at
+  // again: the last one kept is then compared with exact sums, or with sums that stay
+  // below it by more than they may be off.
+  if (!safe || (a.softmax && a.bias)) again = real;
+  safe = safe && groups_safe;
+  const bool all = !safe || (a.softmax && a.bias);  // of again are in doubt, if any
   // k rounds (and one more for how near the next one is): the best choice left, the
   // lowest index among equals; lane j keeps round j's
-  const bool all = a.n_group > 1 || (a.softmax && a.bias) || !safe;  // of those below are in doubt, if any
-  // (where the groups are in doubt, the ones left out as well; beside a bias the
-  // distance of two scores hangs on the sum over all experts)
-  const uint32_t in0 = safe && !(a.softmax && a.bias) ? in : real;
   int id = 0;
   double w = 0.0, above = __builtin_inf(), above_off = 0.0;
   for (int j = 0; j < a.k + (far != 0.0 ? 1 : 0); j++) {
@@ -247,7 +258,7 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, int s, const double* 
     // what is sure to stay below the last one looked at is not in doubt
 #pragma unroll
     for (int i = 0; i < kPer; i++) {
-      const uint64_t b = __ballot(in0 >> i & 1 && (all || !(c[i] + off(sc[i], c[i]) < above - above_off)));
+      const uint64_t b = __ballot(again >> i & 1 && (all || !(c[i] + off(sc[i], c[i]) < above - above_off)));
       if (l == 0) doubt[i] = b;
     }
     return false;
