@@ -278,8 +278,8 @@ struct Cols {
 // s, so one 16-byte read brings a column's nibbles for all four steps.
 //   One barrier a half: past the one before half h, h has landed, and all have
 // read h - 1, whose slot h + 2 takes.
-//   4096 tokens of 4 of 32 experts of 1792, H = 2048, up: 243 us, 990 TFLOP/s, where
-// a large fp16 product reaches 1140-1306.  The matrix cores are busy 49 % of it: 3.7
+//   4096 tokens of 4 of 32 experts of 1792, H = 2048, up: 246-252 us, 955-978 TFLOP/s,
+// where a large fp16 product reaches 1140-1306.  The matrix cores are busy 49 % of it: 3.7
 // vector instructions (dequantisation, scales) go with a product, and the operands'
 // LDS reads alone take 32 % of the cycles at 128 bytes each.  Few rows an expert are bound by memory: 45 tokens, down,
 // 16 us for 59 MB.  (W and X fetched 3 groups ahead instead, where 32 rows leave the

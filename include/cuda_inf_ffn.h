@@ -71,7 +71,8 @@ typedef struct cia_moe_gating {
  * and at most CIA_FFN_MAX_WIDTH; x and gate 16-byte aligned.
  * The choice is the one of logits summed in 64 bits, so a token's experts do
  * not depend on the other tokens of the call.  Logits are at most 2^-19 of
- * sum |gate x| and half an fp32 step off, weights as far as that moves them.
+ * sum |gate x| and half an fp32 step off, in calls of up to 1024 tokens the half
+ * step alone; weights as far as that moves them.
  * A c that is not a number ranks with -inf; a softmax over logits that are all
  * -inf gives scores of 0, one with a NaN or +inf among them NaN; a sum + eps
  * of 0 gives weights of 0.  S at most CIA_FFN_MAX_TOKENS. */
