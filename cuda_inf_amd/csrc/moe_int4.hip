@@ -1355,7 +1355,7 @@ extern "C" int cia_moe_block_forward(const cia_moe* M, float* h, int S, void* st
   CIA_REQUIRE(h, CIA_ERR_NULL);
   const int k = M->gate ? M->gating.top_k : 1, E = M->gate ? M->gating.n_experts : 1;
   CIA_REQUIRE(M->ws, CIA_ERR_NULL);
-  CIA_REQUIRE(aligned(M->ws, 16), CIA_ERR_ALIGN);
+  CIA_REQUIRE(aligned(M->ws, 16) && aligned(M->gate, 16) && (!M->gate || aligned(M->bias, 4)), CIA_ERR_ALIGN);
   // the branch's arguments before its first launch (the norm checks its own, and is
   // the first; h is written by the last)
   int st = moe_check(S, k, E, M->H, M->F, M->gate ? (const int32_t*)M->ws : nullptr);

@@ -235,6 +235,15 @@ def test_block_refusals(L):
     assert L.cia_moe_block_workspace_bytes(block(), -1) == 0
 
 
+def test_block_refuses_a_router_out_of_place_before_any_launch(L):
+    from cuda_inf_amd import _lib
+    M = _lib.cia_moe(norm_w=A, norm_eps=1e-5, H=256, F=128, gating=_lib.cia_moe_gating(*{**GOOD, "E": 4, "k": 2}.values()),
+                     w1=q4(4, 128, 256), w3=q4(4, 128, 256), w2=q4(4, 256, 128), ws=A, ws_bytes=1 << 30, cap=8)
+    for gate, bias in ((A + 8, None), (A, A + 2)):
+        M.gate, M.bias = gate, bias
+        assert L.cia_moe_block_forward(ctypes.byref(M), A, 1, None) == ALIGN
+
+
 def test_wrapper_refusals(cia):
     import torch
 
