@@ -78,6 +78,13 @@ SIGNATURES = {
     "cia_moe_workspace_bytes": (ctypes.c_int64, [_I] * 5),
     "cia_moe_block_workspace_bytes": (ctypes.c_int64, [_P, _I]),
     "cia_moe_block_forward": (_I, [_P, _P, _I, _P]),
+    # include/cuda_inf_batch.h
+    "cia_kv_pages_write": (_I, [_P, _P, ctypes.c_int64, _P, ctypes.c_int64, _P, _P, _I, _P]),
+    "cia_kv_pages_read": (_I, [_P, _P, ctypes.c_int64, _P, ctypes.c_int64, _P, _P, _I, _P]),
+    "cia_attn_pages": (_I, [_P, _P, ctypes.c_int64, _P, _P, _I, _I, _F, _I, _P, _P, ctypes.c_int64, _P]),
+    "cia_attn_pages_workspace_bytes": (ctypes.c_int64, [_I] * 3),
+    "cia_sample": (_I, [_P, _I, ctypes.c_int64] + [_P] * 7 + [_I, _I, _P, ctypes.c_int64, _P]),
+    "cia_sample_workspace_bytes": (ctypes.c_int64, [_I, _I]),
     # include/cuda_inf_model.h
     "cia_index_read": (_I, [ctypes.c_char_p, _P, ctypes.c_int64, _P]),
     "cia_file_size": (_I, [ctypes.c_char_p, _P]),
@@ -204,3 +211,10 @@ class cia_moe(ctypes.Structure):
     _fields_ = [("norm_w", _P), ("norm_eps", _F), ("H", _I), ("F", _I), ("gate", _P), ("bias", _P),
                 ("gating", cia_moe_gating), ("w1", cia_q4_experts), ("w3", cia_q4_experts),
                 ("w2", cia_q4_experts), ("ws", _P), ("ws_bytes", ctypes.c_int64), ("cap", _I)]
+
+
+class cia_kv_pages(ctypes.Structure):
+    """Mirror of ``cia_kv_pages`` in include/cuda_inf_batch.h."""
+    _fields_ = [("k", _P), ("v", _P), ("ks", _P), ("vs", _P), ("type", _I), ("n_pages", _I), ("page", _I),
+                ("n_kv", _I), ("head_dim", _I), ("n_seq", _I), ("max_pages", _I), ("table", _P),
+                ("table_stride", ctypes.c_int64)]

@@ -395,3 +395,140 @@ def moe_down_int4(act, ids, weights, w2, res, out, S: int, k: int, ws) -> None:
          None if weights is None else _at(weights, "weights", _F32, n, dev), ctypes.byref(q2),
          _at(res, "res", _F32, S * H, dev), _at(out, "out", _F32, S * H, dev), S, k, E, H, F,
          _at(ws, "ws", _U8, 0, dev), ws.numel(), _stream_on(dev))
+
+
+# ------------------------------------------------------------ a batch's decode step
+class KvPages:
+    """One layer's paged key-value cache for many sequences, as kv_pages_write,
+    kv_pages_read and attn_pages take it (cia_kv_pages).
+
+    ``k``, ``v``: [pages, kv heads, page, dim], contiguous, fp16, or u8 (e4m3) with
+    ``ks``, ``vs`` fp16 [pages, kv heads, page].  ``table``: int32 [sequences, columns],
+    the pages of each sequence in order; rows may lie apart.  Its contents may change
+    between calls, as the pages' may; the tensors are kept."""
+
+    def __init__(self, k, v, table, ks=None, vs=None):
+        if not isinstance(k, torch.Tensor) or k.dim() != 4:
+            raise ValueError("k: need a tensor [pages, kv heads, page, dim]")
+        quant = k.dtype == torch.uint8
+        if not quant and k.dtype not in _F16:
+            raise TypeError(f"k: dtype {k.dtype}: need fp16, or uint8 for e4m3")
+        kp, dev, n = _dev(k, "k"), k.get_device(), k.numel()
+        vp = _at(v, "v", (k.dtype,), n, dev)
+        rows = n // k.shape[3]
+        if quant:
+            sp = [_at(t, name, _F16, rows, dev) for t, name in ((ks, "ks"), (vs, "vs"))]
+        elif ks is not None or vs is not None:
+            raise ValueError("ks, vs: fp16 pages have no scales")
+        else:
+            sp = [None, None]
+        for t, name, like in ((v, "v", k.shape), (ks, "ks", k.shape[:3]), (vs, "vs", k.shape[:3])):
+            if t is not None and t.shape != like:
+                raise ValueError(f"{name}: shape {tuple(t.shape)}, and k's is {tuple(k.shape)}")
+        if (not isinstance(table, torch.Tensor) or table.dim() != 2 or table.dtype != torch.int32
+                or (table.shape[1] > 1 and table.stride(1) != 1)):
+            raise ValueError("table: need an int32 tensor [sequences, columns], rows contiguous")
+        if table.get_device() != dev:
+            raise ValueError(f"table: on {table.device}, and the pages on cuda:{dev}")
+        n_pages, n_kv, page, dim = k.shape
+        stride = table.stride(0) if table.shape[0] > 1 else table.shape[1]
+        self._s = _lib.cia_kv_pages(kp, vp, *sp, 0 if quant else 1, n_pages, page, n_kv, dim, table.shape[0],
+                                    table.shape[1], table.data_ptr(), stride)
+        self._ref, self._device, self._n_seq = ctypes.byref(self._s), dev, table.shape[0]
+        self.k, self.v, self.ks, self.vs, self.table = k, v, ks, vs, table
+        self.n_kv, self.head_dim, self.page = n_kv, dim, page
+
+
+def _rows(t, name: str, heads: int, dim: int, T: int, dev: int):
+    """Address and row stride of fp16 rows [T, heads, dim], each contiguous."""
+    try:
+        if (t.get_device() == dev and t.dtype in _F16 and t.shape == (T, heads, dim)
+                and (t.is_contiguous() or (t.stride(2) == 1 and (heads == 1 or t.stride(1) == dim)))):
+            return t.data_ptr(), t.stride(0) if T > 1 else heads * dim
+    except AttributeError:
+        pass  # no tensor
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
+    if t.dtype not in _F16:
+        raise TypeError(f"{name}: dtype {t.dtype} not in {_F16}")
+    raise ValueError(f"{name}: {tuple(t.shape)} on {t.device}: need rows [{T}, {heads}, {dim}], each contiguous, "
+                     f"on cuda:{dev}")
+
+
+def _move(fn: str, pages: KvPages, k, v, pos, seq) -> None:
+    T, dev = pos.numel(), pages._device
+    kp, ks = _rows(k, "k", pages.n_kv, pages.head_dim, T, dev)
+    vp, vs = _rows(v, "v", pages.n_kv, pages.head_dim, T, dev)
+    call(fn, pages._ref, kp, ks, vp, vs, None if seq is None else _at(seq, "seq", _I32, T, dev),
+         _at(pos, "pos", _I32, T, dev), T, _stream_on(dev))
+
+
+def kv_pages_write(pages: KvPages, k, v, pos, seq=None) -> None:
+    """k and v (fp16 [T, kv heads, dim], rows may lie apart) into the pages at
+    positions ``pos`` (int32 [T]) of sequences ``seq`` (int32 [T]; None: token t is
+    sequence t's), quantised as kv_quant_write does (engine.cu:317-333) in an e4m3
+    cache.  A position of -1, or one without a page, is passed over; two tokens of a
+    call must not have one place."""
+    _move("cia_kv_pages_write", pages, k, v, pos, seq)
+
+
+def kv_pages_read(pages: KvPages, k, v, pos, seq=None) -> None:
+    """The reverse of kv_pages_write: k and v rows from the pages, fp16; rows of
+    tokens without a place are left as they were."""
+    _move("cia_kv_pages_read", pages, k, v, pos, seq)
+
+
+def attn_pages_workspace_bytes(n_q: int, n_kv: int, head_dim: int) -> int:
+    """Workspace bytes of attn_pages, for any number of rows."""
+    return int(_lib.lib().cia_attn_pages_workspace_bytes(n_q, n_kv, head_dim))
+
+
+def new_attn_pages_workspace(pages: KvPages, n_q: int) -> torch.Tensor:
+    """Workspace of attn_pages over these pages with n_q query heads.  Zeroed here;
+    every call leaves its counters at zero."""
+    n = attn_pages_workspace_bytes(n_q, pages.n_kv, pages.head_dim)
+    if not n:
+        raise ValueError(f"{n_q} query heads on {pages.n_kv} kv heads of {pages.head_dim}: beyond what a call takes")
+    return torch.zeros(n, dtype=torch.uint8, device=pages.k.device)
+
+
+def attn_pages(pages: KvPages, q, out, pos, ws, seq=None, scale: float = 0.125, window: int = 0) -> None:
+    """Attention of one query token per row over its sequence's pages: q fp16 [T, query
+    heads, dim] (rows may lie apart) at positions ``pos`` (int32 [T]) of ``seq`` (int32
+    [T]; None: row t is sequence t's), into out fp16 [T, query heads, dim]; all tokens
+    up to pos, the last ``window`` of them if window > 0.  Rows with none (pos -1) are
+    0.  Calls sharing ws must be ordered on one stream."""
+    T, dev = pos.numel(), pages._device
+    n_q = q.shape[1]
+    qp, qs = _rows(q, "q", n_q, pages.head_dim, T, dev)
+    call("cia_attn_pages", pages._ref, qp, qs, None if seq is None else _at(seq, "seq", _I32, T, dev),
+         _at(pos, "pos", _I32, T, dev), T, n_q, scale, window,
+         _at(out, "out", _F16, T * n_q * pages.head_dim, dev), _at(ws, "ws", _U8, 0, dev), ws.numel(), _stream_on(dev))
+
+
+_LOGITS = {torch.float32: 0, torch.float16: 1}  # CIA_LOGITS_*
+
+
+def sample_workspace_bytes(B: int, V: int) -> int:
+    """Workspace bytes of sample for up to B rows of V logits."""
+    return int(_lib.lib().cia_sample_workspace_bytes(B, V))
+
+
+def sample(logits, u, ids, ws, temperature=None, top_k=None, top_p=None, min_p=None, p=None) -> None:
+    """A token for each row of logits (fp32 or fp16 [B, V], rows may lie apart) from the
+    given random numbers u (fp32 [B], in [0, 1)) into ids (int32 [B]), after
+    temperature (0: the largest logit), top_k, top_p and min_p in this order (fp32 [B],
+    top_k int32 [B]; None: 1, and no filter); p (fp32 [B], optional): the probability it
+    was drawn with.  In place of argmax_kernel (engine.cu:562-572)."""
+    try:
+        B, V = logits.shape
+        kind, dev = _LOGITS[logits.dtype], logits.get_device()
+    except (AttributeError, KeyError, ValueError):
+        raise ValueError("logits: need a device tensor [B, V] of fp32 or fp16") from None
+    if dev < 0 or (V > 1 and logits.stride(1) != 1):
+        raise ValueError("logits: need a device tensor [B, V], rows contiguous")
+    f = [None if t is None else _at(t, name, d, B, dev) for t, name, d in (
+        (temperature, "temperature", _F32), (top_k, "top_k", _I32), (top_p, "top_p", _F32), (min_p, "min_p", _F32))]
+    call("cia_sample", logits.data_ptr(), kind, logits.stride(0) if B > 1 else V, *f, _at(u, "u", _F32, B, dev),
+         _at(ids, "ids", _I32, B, dev), None if p is None else _at(p, "p", _F32, B, dev), B, V,
+         _at(ws, "ws", _U8, 0, dev), ws.numel(), _stream_on(dev))
