@@ -13,23 +13,27 @@
 //                  order.
 // Bins lie at whole x, so that those of chunks with other maxima only need a shift.
 // Masses are added as integers, 2^34 for a bin's upper edge, so that sums do not depend
-// on the order of atomics.
+// on the order of atomics; over the largest logit's own, so that rows of equals have
+// whole sums.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "cuda_inf_batch.h"
 
 namespace cia {
 
-constexpr int kSampleThreads = 1024;  // of k_sample_pick
+constexpr int kSampleThreads = 512;  // of k_sample_pick
 constexpr int kSampleWaves = kSampleThreads / 64;
 constexpr int kBins = 336;   // 42 octaves, 8 bins each
-constexpr int kCap = 4096;   // tokens of a bin taken into LDS
+constexpr int kSlots = 32;    // tokens that a thread takes from a row into LDS
+constexpr int kCap = 6144;   // tokens that are tried to be taken: 12 a thread
 constexpr int kSmall = 256;  // tokens put in order by counting the larger ones
-constexpr int kAll = 1024;   // tokens put in order to find all prefixes among them
-constexpr int kSub = 1024;   // parts of a bin that holds more than kSmall
-constexpr int kTile = 4096;  // logits of a step: 4 a thread of k_sample_pick, 16 of k_sample_bins
-constexpr int kMaxChunk = 4 * kTile;
+constexpr int kAll = 1024;   // tokens put in order at all
+constexpr int kSub = kSampleThreads;  // parts of a bin that holds more than kSmall
+constexpr int kStep = 4 * kSampleThreads;  // logits of a step of k_sample_pick
+constexpr int kMinChunk = 4096;
+constexpr int kMaxChunk = 4 * kMinChunk;
 constexpr int kMaxChunks = CIA_SAMPLE_MAX_VOCAB / kMaxChunk;  // 256
 constexpr int kCountShift = 49;  // of a chunk's bin: count << 49 | mass; 2^14 tokens of 2^34
 
@@ -65,84 +69,103 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __builtin_bit_cast(float, k ^ ((uint32_t)((int32_t)~k >> 31) | 0x80000000u));
 }
 
-// four neighbouring logits from i on, -inf where NaN and past the row's end
+// Four neighbouring logits from i on, in two steps, so that many loads can be out before
+// any is looked at.  whole: all four are in the row; else those past its end are -inf.
 template <bool kHalf>
-__device__ __forceinline__ f32x4 load_logits(const void* row, int i, int V) {
-  const float none = -__builtin_inff();
-  f32x4 x{none, none, none, none};
-  if constexpr (kHalf) {
-    const _Float16* r = (const _Float16*)row;
-    if (i + 4 <= V) {
-      f16x4 h;
-      __builtin_memcpy(&h, r + i, 8);
-      for (int e = 0; e < 4; e++) x[e] = (float)h[e];
+struct Logits {
+  using T = typename std::conditional<kHalf, _Float16, float>::type;
+  typename std::conditional<kHalf, f16x4, f32x4>::type x;
+  __device__ __forceinline__ void load(const void* row, int i, int V, bool whole) {
+    const T* const r = (const T*)row;
+    if (whole) {
+      __builtin_memcpy(&x, r + i, sizeof(x));
     } else {
-      for (int e = 0; e < 4; e++)
-        if (i + e < V) x[e] = (float)r[i + e];
-    }
-  } else {
-    const float* r = (const float*)row;
-    if (i + 4 <= V) {
-      __builtin_memcpy(&x, r + i, 16);
-    } else {
-      for (int e = 0; e < 4; e++)
-        if (i + e < V) x[e] = r[i + e];
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[e] = r[min(i + e, V - 1)];
     }
   }
-  for (int e = 0; e < 4; e++) x[e] = x[e] == x[e] ? x[e] : none;
-  return x;
-}
+  __device__ __forceinline__ f32x4 get(int i, int V, bool whole) const {
+    f32x4 y;
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] = whole || i + e < V ? (float)x[e] : -__builtin_inff();
+    return y;
+  }
+};
 
-// 2^(f / 8) in units of 2^-34 for f in (-1, 0]: the exponential's series to its 6th
-// power (the next is 7e-12), rounded by an addition of 2^18
-__device__ __forceinline__ uint64_t bin_mass(double f) {
-  const double y = f * (0.69314718055994530942 / 8);
-  double r = 1.0 / 720;
-  r = __builtin_fma(r, y, 1.0 / 120);
-  r = __builtin_fma(r, y, 1.0 / 24);
-  r = __builtin_fma(r, y, 1.0 / 6);
-  r = __builtin_fma(r, y, 0.5);
-  r = __builtin_fma(r, y, 1.0);
-  r = __builtin_fma(r, y, 1.0);
-  return __builtin_bit_cast(uint64_t, r + 262144.0) - __builtin_bit_cast(uint64_t, 262144.0);
+// 2^(f / 8) for f in (-1, 0]: the polynomial of degree 5 through the Chebyshev points of
+// the interval, 3e-13 off
+__device__ __forceinline__ double bin_power(double f) {
+  double r = 3.896822893996917e-08;
+  r = __builtin_fma(r, f, 2.346252607310361e-06);
+  r = __builtin_fma(r, f, 1.0840546828792358e-04);
+  r = __builtin_fma(r, f, 3.753538938644709e-03);
+  r = __builtin_fma(r, f, 8.66433975500605e-02);
+  return __builtin_fma(r, f, 0.9999999999997227);
 }
-__device__ __forceinline__ double bin_unit(int bin) { return exp2((double)bin * -0.125 - 34.0); }
+// the same in units of 2^-34, rounded by an addition of 2^18
+__device__ __forceinline__ uint64_t bin_mass(double f) {
+  return __builtin_bit_cast(uint64_t, bin_power(f) + 262144.0) - __builtin_bit_cast(uint64_t, 262144.0);
+}
+// a bin's upper edge, bin 0's being 1: 2^(-bin / 8)
+__device__ __forceinline__ double bin_edge(int bin) {
+  constexpr double kEighth[8] = {1.0, 0.91700404320467122, 0.84089641525371454, 0.77110541270397037,
+                                 0.70710678118654752, 0.64841977732550483, 0.59460355750136054, 0.54525386633262882};
+  double e = kEighth[0];
+#pragma unroll
+  for (int i = 1; i < 8; i++) e = (bin & 7) == i ? kEighth[i] : e;
+  return e * __builtin_bit_cast(double, (uint64_t)(1023 - (bin >> 3)) << 52);
+}
 
 __device__ __forceinline__ double temperature_scale(float t) { return 8 * 1.44269504088896340736 / (double)t; }
 
 // ---------------------------------------------------------------- the bins
-// grid = rows * chunks, block = 256, kTiles * kTile logits a workgroup in registers
-template <bool kHalf, int kTiles>
-__global__ __launch_bounds__(256) void k_sample_bins(SampleArgs a) {
+// grid = rows * chunks, block = kThreads, 4 kVec logits of the chunk a thread, in registers
+template <bool kHalf, int kThreads, int kVec>
+__global__ __launch_bounds__(kThreads) void k_sample_bins(SampleArgs a) {
+  constexpr int kWaves = kThreads / 64, kEach = 4 * kThreads;
   __shared__ unsigned long long bins[kBins];
-  __shared__ float wtop[4];
-  __shared__ uint32_t widx[4];
+  __shared__ float wtop[kWaves];
+  __shared__ uint32_t widx[kWaves];
   const int b = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, tid = threadIdx.x;
   const void* row = (const char*)a.logits + (int64_t)b * a.stride * (kHalf ? 2 : 4);
-  const int i0 = chunk * (kTiles * kTile) + 4 * tid;
-  f32x4 x[4 * kTiles];
+  const int i0 = chunk * (kVec * kEach) + 4 * tid;
+  const bool whole = (chunk + 1) * (kVec * kEach) <= a.V;
+  Logits<kHalf> in[kVec];
+  if (whole) {
 #pragma unroll
-  for (int i = 0; i < 4 * kTiles; i++) x[i] = load_logits<kHalf>(row, i0 + 1024 * i, a.V);
+    for (int i = 0; i < kVec; i++) in[i].load(row, i0 + kEach * i, a.V, true);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; i++) in[i].load(row, i0 + kEach * i, a.V, false);
+  }
   const float t = a.temperature ? a.temperature[b] : 1.0f;
-  for (int i = tid; i < kBins; i += 256) bins[i] = 0;
+  for (int i = tid; i < kBins; i += kThreads) bins[i] = 0;
+  f32x4 x[kVec];
+#pragma unroll
+  for (int i = 0; i < kVec; i++) {
+    x[i] = in[i].get(i0 + kEach * i, a.V, whole);
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[i][e] = x[i][e] == x[i][e] ? x[i][e] : -__builtin_inff();
+  }
   float top = -__builtin_inff();
 #pragma unroll
-  for (int i = 0; i < 4 * kTiles; i++)
+  for (int i = 0; i < kVec; i++)
 #pragma unroll
     for (int e = 0; e < 4; e++) top = __builtin_fmaxf(top, x[i][e]);
   top = wave_max_fast(top);
   if ((tid & 63) == 0) wtop[tid >> 6] = top;
   __syncthreads();
-  top = __builtin_fmaxf(__builtin_fmaxf(wtop[0], wtop[1]), __builtin_fmaxf(wtop[2], wtop[3]));
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) top = __builtin_fmaxf(top, wtop[w]);
   ChunkHead* const head = a.heads + (int64_t)b * a.chunks + chunk;
   const bool none = top == -__builtin_inff();
   if (none || !(t > 0.0f)) {  // nothing here, or the largest is all that is asked for
     uint32_t idx = ~0u;
 #pragma unroll
-    for (int i = 4 * kTiles - 1; i >= 0; i--)
+    for (int i = kVec - 1; i >= 0; i--)
 #pragma unroll
       for (int e = 3; e >= 0; e--)
-        if (x[i][e] == top) idx = (uint32_t)(i0 + 1024 * i + e);
+        if (x[i][e] == top) idx = (uint32_t)(i0 + kEach * i + e);
     for (int off = 32; off; off >>= 1) {
       const uint32_t o = __shfl_xor(idx, off);
       idx = o < idx ? o : idx;
@@ -150,7 +173,7 @@ __global__ __launch_bounds__(256) void k_sample_bins(SampleArgs a) {
     if ((tid & 63) == 0) widx[tid >> 6] = idx;
     __syncthreads();
     if (tid == 0) {
-      idx = min(min(widx[0], widx[1]), min(widx[2], widx[3]));
+      for (int w = 0; w < kWaves; w++) idx = min(idx, widx[w]);
       *head = ChunkHead{none ? -__builtin_inf() : 0.0, top, idx};
     }
     return;
@@ -158,7 +181,7 @@ __global__ __launch_bounds__(256) void k_sample_bins(SampleArgs a) {
   const bool inf = top == __builtin_inff();
   const double c = temperature_scale(t), R = inf ? 0.0 : __builtin_ceil(c * (double)top);
 #pragma unroll
-  for (int i = 0; i < 4 * kTiles; i++)
+  for (int i = 0; i < kVec; i++)
 #pragma unroll
     for (int e = 0; e < 4; e++) {
 #pragma clang fp contract(off)
@@ -170,7 +193,7 @@ __global__ __launch_bounds__(256) void k_sample_bins(SampleArgs a) {
     }
   __syncthreads();
   uint64_t* const to = a.bins + ((int64_t)b * a.chunks + chunk) * kBins;
-  for (int i = tid; i < kBins; i += 256) to[i] = bins[i];
+  for (int i = tid; i < kBins; i += kThreads) to[i] = bins[i];
   if (tid == 0) *head = ChunkHead{inf ? __builtin_inf() : R, top, 0};
 }
 
@@ -179,15 +202,17 @@ enum Goal { kNth, kReach, kPass, kRatio };
 
 // where a prefix ends
 struct Ends {
-  double mass;  // of the prefix, the largest bin's upper edge being 1
+  double mass;  // of the prefix
   double w;     // of its last token
   int idx;
 };
 
 struct SampleLds {
-  uint64_t list[kCap];  // key << 32 | ~index
-  uint64_t small[kAll];
-  double run[kAll];     // sums of the ordered list
+  float value[kSlots][kSampleThreads];     // tokens taken from the row, of each thread its own
+  uint16_t nth[kSlots][kSampleThreads];    // and which of the logits it has passed each is
+  uint64_t some[kAll];  // those of one bin
+  uint64_t small[kAll];  // in descending order
+  double run[kAll];     // sums of their weights
   unsigned long long mass[kSub];
   uint32_t cnt[kSub];
   double before[kBins + 1];  // mass of the bins before
@@ -197,12 +222,18 @@ struct SampleLds {
   double dsum[kSampleWaves];
   uint64_t key[kSampleWaves];
   uint32_t lo[kSampleWaves], hi[kSampleWaves];
-  int n, m, at, bin;
+  int n, m, at, bin, last;
   Ends ends;
 };
 
-// one row, all threads of the workgroup
-template <bool kHalf>
+// bins from[r]..to[r] of n ranges
+constexpr int kRanges = 2;
+struct BinSet {
+  int n, from[kRanges], to[kRanges];
+};
+
+// one row, all threads of the workgroup; kPer: steps of a chunk
+template <bool kHalf, int kPer>
 struct SampleRow {
   SampleLds& s;
   const SampleArgs& a;
@@ -211,28 +242,35 @@ struct SampleRow {
   const uint64_t* bins;
   double c;     // x = c l
   double R;     // ceil of the largest x
+  double top_power, top_mass;  // bin_power and bin_mass of the largest logit
   float top;    // the largest logit
   bool inf;     // some are +inf: they count as 0, the others as -inf
   int tid, lane, wave;
+  int taken;    // tokens that the thread has in the list
 
-  __device__ __forceinline__ f32x4 load(int i) const {
-    f32x4 x = load_logits<kHalf>(row, i, a.V);
-    if (inf)
-      for (int e = 0; e < 4; e++) x[e] = x[e] == __builtin_inff() ? 0.0f : -__builtin_inff();
-    return x;
-  }
   // x of a logit, rounded.  (Fused with a difference, a product of 1e39 would be its
   // rounding away from its own ceil.)
   __device__ __forceinline__ double x_of(float l) const {
 #pragma clang fp contract(off)
     return c * (double)l;
   }
+  // w of a token of one of the bins, exactly 1 for the largest logit's
   __device__ __forceinline__ double weight(float l) const {
 #pragma clang fp contract(off)
-    return exp2((x_of(l) - R) * 0.125);
+    const double x = x_of(l), n = __builtin_ceil(x);
+    return bin_power(x - n) / top_power * bin_edge((int)(R - n));
   }
-  // w over the largest
+  // the same for a sum of bin_mass over tokens of one bin: whole for equals of the largest
+  __device__ __forceinline__ double mass_in(int bin, unsigned long long m) const {
+    return (double)m / top_mass * bin_edge(bin);
+  }
+  // the same without the bins' 3e-13
   __device__ __forceinline__ double ratio(float l) const { return exp2(((double)l - (double)top) * c * 0.125); }
+  __device__ __forceinline__ double power_of(float l) const {
+#pragma clang fp contract(off)
+    const double x = x_of(l);
+    return bin_power(x - __builtin_ceil(x));
+  }
   __device__ __forceinline__ uint64_t mass_of(float l) const {
 #pragma clang fp contract(off)
     const double x = x_of(l);
@@ -240,7 +278,7 @@ struct SampleRow {
   }
 
   // the row's largest logit: key << 32 | ~index
-  __device__ uint64_t largest() {
+  __device__ __forceinline__ uint64_t largest() {
     uint64_t best = 0;
     for (int i = tid; i < a.chunks; i += kSampleThreads) {
       const ChunkHead h = heads[i];
@@ -261,117 +299,159 @@ struct SampleRow {
   }
 
   // the row's bins: tokens and mass before each
-  __device__ void add_up() {
-    constexpr int kWays = kSampleThreads / kBins;  // threads of a bin
+  __device__ __forceinline__ void add_up() {
     for (int i = tid; i < a.chunks; i += kSampleThreads) {
       const double n = s.shift[i];
       s.shift[i] = inf ? (n == __builtin_inf() ? 0.0 : (double)kBins) : R - n;
     }
+    if (tid == 0) s.last = 0;
     __syncthreads();
-    const int b = tid % kBins, way = tid / kBins;
     unsigned long long m = 0;
     uint32_t k = 0;
-    if (way < kWays)
+    if (tid < kBins)
 #pragma unroll 8
-      for (int i = way; i < a.chunks; i += kWays) {
-        const double d = (double)b - s.shift[i];
-        const uint64_t v = d >= 0.0 ? bins[(int64_t)i * kBins + (int)d] : 0;
+      for (int i = 0; i < a.chunks; i++) {
+        const double d = (double)tid - s.shift[i];
+        uint64_t v = bins[(int64_t)i * kBins + (int)fmax(d, 0.0)];
+        v = d >= 0.0 ? v : 0;  // (the bins of a chunk without tokens are not written)
         m += v & ((1ull << kCountShift) - 1);
         k += (uint32_t)(v >> kCountShift);
       }
-    if (way < kWays) s.list[tid] = m, s.cnt[tid] = k;  // (tid = way * kBins + b)
-    __syncthreads();
-    if (wave == 0) {  // 6 bins a lane
-      double dm[6], im = 0.0;
-      int dk[6], ik = 0;
-      for (int j = 0; j < 6; j++) {
-        const int i = lane * 6 + j;
-        dm[j] = im, dk[j] = ik;
-        if (i < kBins) {
-          unsigned long long q = 0;
-          for (int w = 0; w < kWays; w++) q += s.list[w * kBins + i], ik += (int)s.cnt[w * kBins + i];
-          im += (double)q * bin_unit(i);
-        }
-      }
-      const double own = im;
-      const int owk = ik;
-      for (int off = 1; off < 64; off <<= 1) {
-        const double um = __shfl_up(im, off);
-        const int uk = __shfl_up(ik, off);
-        if (lane >= off) im += um, ik += uk;
-      }
-      for (int j = 0; j < 6; j++) {
-        const int i = lane * 6 + j;
-        if (i <= kBins) s.before[i] = (im - own) + dm[j], s.count[i] = (ik - owk) + dk[j];
-      }
+    double run = tid < kBins ? mass_in(tid, m) : 0.0;
+    int upto = (int)k;
+    for (int off = 1; off < 64; off <<= 1) {
+      const double um = __shfl_up(run, off);
+      const int uk = __shfl_up(upto, off);
+      if (lane >= off) run += um, upto += uk;
     }
+    if (lane == 63) s.dsum[wave] = run, s.lo[wave] = (uint32_t)upto;
+    if (k) atomicMax(&s.last, tid);
+    __syncthreads();
+    double base = 0.0;
+    int kbase = 0;
+    for (int v = 0; v < wave; v++) base += s.dsum[v], kbase += (int)s.lo[v];
+    if (tid < kBins) s.before[tid + 1] = base + run, s.count[tid + 1] = kbase + upto;
+    if (tid == 0) s.before[0] = 0.0, s.count[0] = 0;
     __syncthreads();
   }
 
   // the bin in which a prefix ends: the first whose sum satisfies the goal, the last
-  // that holds any where none does
-  __device__ int bin_with(Goal how, int nth, double goal) {
-    __syncthreads();
-    if (tid == 0) s.bin = kBins, s.at = 0;
-    __syncthreads();
-    if (tid < kBins && s.count[tid + 1] > s.count[tid]) {
-      const bool here = how == kNth ? s.count[tid + 1] >= nth
-                        : how == kReach ? s.before[tid + 1] >= goal : s.before[tid + 1] > goal;
-      if (here) atomicMin(&s.bin, tid);
-      atomicMax(&s.at, tid);
+  // that holds any where none does; each wave looks by itself, in 56 groups of 6 bins,
+  // then in one of them
+  __device__ __forceinline__ int bin_with(Goal how, int nth, double goal) const {
+    constexpr int kPart = kBins / 56;
+    int at = 0;
+#pragma unroll 1
+    for (int step = kPart; step; step /= kPart) {
+      const int b = min(at + (lane + 1) * step, kBins);
+      const bool here = how == kNth ? s.count[b] >= nth : how == kReach ? s.before[b] >= goal : s.before[b] > goal;
+      const uint64_t set = __ballot(here);
+      if (!set) return __builtin_amdgcn_readfirstlane(s.last);
+      at += __builtin_ctzll(set) * step;
     }
-    __syncthreads();
-    return s.bin < kBins ? s.bin : s.at;
+    return min(at, kBins - 1);
   }
 
-  // the chunks that have tokens in the bins from `b0` to `b1`: how many
-  __device__ int chunks_with(int b0, int b1) {
+  // the chunks that have a token in one of the bins.  (A chunk's first bin has one, its
+  // largest.)
+  __device__ __forceinline__ void chunks_with(const BinSet& w) {
     __syncthreads();
     if (tid == 0) s.m = 0;
     __syncthreads();
     for (int i = tid; i < a.chunks; i += kSampleThreads) {
       const double sh = s.shift[i];
-      // (its first bin has a token, its largest)
-      if (sh > (double)b1) continue;
-      if (b0 == b1) {
-        const uint64_t v = bins[(int64_t)i * kBins + (b1 - (int)sh)];
-        if (!(v >> kCountShift)) continue;
+      bool has = false;
+      for (int r = 0; r < w.n; r++) {
+        if (sh > (double)w.to[r]) continue;
+        has |= w.from[r] < w.to[r] || bins[(int64_t)i * kBins + (w.to[r] - (int)sh)] >> kCountShift;
       }
-      s.use[atomicAdd(&s.m, 1)] = i;
+      if (has) s.use[atomicAdd(&s.m, 1)] = i;
     }
     __syncthreads();
-    return s.m;
   }
 
-  // fn(key, logit, index) for the tokens of the bins from b0 to b1, of the s.m chunks in use
+  // The least key of the tokens of the bins up to `to`: x above R - to - 1.  It is within a
+  // few of the quotient's, of which the lanes try 64.
+  __device__ __forceinline__ uint32_t first_key(int to) const {
+    if (!(c > 0.0)) return order_key(-3.402823466e38f);  // all tokens are in bin 0
+    const uint32_t k = order_key((float)((R - (double)to - 1.0) / c)) - 32 + lane;
+    const float v = key_value(k);
+    const bool in = k > order_key(__builtin_inff()) || R - __builtin_ceil(x_of(v)) <= (double)to;
+    const uint64_t set = __ballot(in);
+    return __builtin_amdgcn_readfirstlane(k) + (set ? __builtin_ctzll(set) : 64);
+  }
+  // the keys of the bins from..to
+  __device__ __forceinline__ void keys_of(int from, int to, uint32_t& lo, uint32_t& hi) const {
+    lo = first_key(to);
+    hi = from ? first_key(from - 1) - 1 : order_key(top);
+    if (hi == 0x7fffffff) hi--;  // (-0, whose key is 0's)
+  }
+
+  // where the nth of the logits that a thread passes lies: four of a step, the steps of the
+  // chunks in use in turn
+  __device__ __forceinline__ int index_of(int nth) const {
+    const int step = nth >> 2;
+    return s.use[step / kPer] * (kPer * kStep) + step % kPer * kStep + 4 * tid + (nth & 3);
+  }
+
+  // fn(nth, x): four neighbouring logits from the thread's nth on, of the s.m chunks in use
   template <typename F>
-  __device__ __forceinline__ void each(int b0, int b1, F fn) {
-    const int steps = s.m * (a.chunk / kTile);
-    for (int k = 0; k < steps; k++) {
-      const int i = s.use[k / (a.chunk / kTile)] * a.chunk + k % (a.chunk / kTile) * kTile + 4 * tid;
-      const f32x4 x = load(i);
+  __device__ __forceinline__ void each(F fn) {
+    constexpr int kAhead = 8, kAt = kAhead / kPer;  // steps whose loads are out together, of kAt chunks
+    const int m = __builtin_amdgcn_readfirstlane(s.m);
+#pragma unroll 1
+    for (int c0 = 0; c0 < m; c0 += kAt) {
+      Logits<kHalf> in[kAhead];
+      int i[kAt];
+      bool whole = true;
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const double d = R - __builtin_ceil(x_of(x[e]));
-        if (d >= (double)b0 && d <= (double)b1) fn(order_key(x[e]), x[e], i + e);
+      for (int q = 0; q < kAt; q++) {  // (past the last: it again, left out below)
+        i[q] = __builtin_amdgcn_readfirstlane(s.use[min(c0 + q, m - 1)]) * (kPer * kStep);
+        whole &= i[q] + kPer * kStep <= a.V;
+      }
+      if (whole) {
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) in[k].load(row, i[k / kPer] + k % kPer * kStep + 4 * tid, a.V, true);
+      } else {
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) in[k].load(row, i[k / kPer] + k % kPer * kStep + 4 * tid, a.V, false);
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; k++) {
+        if (c0 + k / kPer >= m) break;
+        f32x4 x = in[k].get(i[k / kPer] + k % kPer * kStep + 4 * tid, a.V, whole);
+        if (inf)
+#pragma unroll
+          for (int e = 0; e < 4; e++) x[e] = x[e] == __builtin_inff() ? 0.0f : -__builtin_inff();
+        fn((c0 * kPer + k) * 4, x);
       }
     }
   }
 
-  // The tokens of the bins b0..b1 with keys lo..hi into the list: how many there are
-  // (the list holds kCap at most), and their least and largest key.
-  __device__ int gather(int b0, int b1, uint32_t lo, uint32_t hi, uint32_t& least, uint32_t& most) {
-    __syncthreads();
-    if (tid == 0) s.n = 0;
-    __syncthreads();
-    least = ~0u, most = 0;
-    each(b0, b1, [&](uint32_t k, float, int i) {
-      if (k < lo || k > hi) return;
-      least = k < least ? k : least;
-      most = k > most ? k : most;
-      const int n = atomicAdd(&s.n, 1);
-      if (n < kCap) s.list[n] = (uint64_t)k << 32 | (uint32_t)~i;
+  // The tokens with keys in one of two ranges into the list: whether they fit.
+  __device__ __forceinline__ bool take(const uint32_t (&from)[kRanges], const uint32_t (&upto)[kRanges]) {
+    const float lo = key_value(__builtin_amdgcn_readfirstlane(from[0])), hi = key_value(__builtin_amdgcn_readfirstlane(upto[0]));
+    const float lo1 = key_value(__builtin_amdgcn_readfirstlane(from[1])), hi1 = key_value(__builtin_amdgcn_readfirstlane(upto[1]));
+    int have = 0;
+    each([&](int nth, const f32x4& x) __attribute__((always_inline)) {
+      bool in[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) in[e] = ((x[e] >= lo) & (x[e] <= hi)) | ((x[e] >= lo1) & (x[e] <= hi1));
+      if (!__any(in[0] | in[1] | in[2] | in[3])) return;
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (in[e]) {
+          const int at = min(have, kSlots - 1);
+          s.value[at][tid] = x[e];
+          s.nth[at][tid] = (uint16_t)(nth + e);
+          have++;
+        }
     });
+    taken = min(have, kSlots);
+    return !__syncthreads_or(have > kSlots);
+  }
+
+  __device__ __forceinline__ void least_most(uint32_t& least, uint32_t& most) {
     for (int off = 32; off; off >>= 1) {
       const uint32_t u = __shfl_xor(least, off), v = __shfl_xor(most, off);
       least = u < least ? u : least;
@@ -383,20 +463,40 @@ struct SampleRow {
       least = s.lo[w] < least ? s.lo[w] : least;
       most = s.hi[w] > most ? s.hi[w] : most;
     }
-    return s.n;
+  }
+
+  // The tokens in the list with keys lo..hi into s.some (kAll at most): how many there are,
+  // and their least and largest key.
+  __device__ __forceinline__ int select(uint32_t lo, uint32_t hi, uint32_t& least, uint32_t& most) {
+    __syncthreads();
+    if (tid == 0) s.m = 0;
+    __syncthreads();
+    least = ~0u, most = 0;
+    for (int i = 0; i < taken; i++) {
+      const uint32_t k = order_key(s.value[i][tid]);
+      if (k < lo || k > hi) continue;
+      least = k < least ? k : least;
+      most = k > most ? k : most;
+      const int n = atomicAdd(&s.m, 1);
+      if (n < kAll) s.some[n] = (uint64_t)k << 32 | (uint32_t)~index_of(s.nth[i][tid]);
+    }
+    least_most(least, most);
+    return s.m;
   }
 
   // n tokens of `from` into s.small in descending order; n <= kAll
-  __device__ void order(const uint64_t* from, int n) {
+  __device__ __forceinline__ void order(const uint64_t* from, int n) {
     __syncthreads();
     if (n <= kSmall) {
-      // a token's place is how many are larger: 4 threads a token, each a quarter of them
-      const int i = tid & (kSmall - 1), quarter = tid / kSmall, per = (n + 3) / 4;
+      // a token's place is how many are larger: some threads a token, each a part of them
+      constexpr int kWays = kSampleThreads / kSmall;
+      const int i = tid & (kSmall - 1), way = tid / kSmall, per = (n + kWays - 1) / kWays;
       if (tid < kSmall) s.cnt[tid] = 0;
       __syncthreads();
       const uint64_t mine = i < n ? from[i] : ~0ull;
       int larger = 0;
-      for (int k = quarter * per; k < min(n, quarter * per + per); k++) larger += from[k] > mine;
+#pragma unroll 8
+      for (int k = way * per; k < min(n, way * per + per); k++) larger += from[k] > mine;
       if (i < n && larger) atomicAdd(&s.cnt[i], (uint32_t)larger);
       __syncthreads();
       if (tid < n) s.small[s.cnt[tid]] = mine;
@@ -405,12 +505,12 @@ struct SampleRow {
     }
     int size = 2 * kSmall;
     while (size < n) size *= 2;
-    if (tid < size) s.small[tid] = tid < n ? from[tid] : 0;
+    for (int i = tid; i < size; i += kSampleThreads) s.small[i] = i < n ? from[i] : 0;
     __syncthreads();
     for (int k = 2; k <= size; k *= 2)
       for (int j = k / 2; j; j /= 2) {
         if (tid < size / 2) {
-          const int u = (tid / j) * 2 * j + tid % j, v = u + j;
+          const int u = ((tid & ~(j - 1)) << 1) + (tid & (j - 1)), v = u + j;
           const uint64_t x = s.small[u], y = s.small[v];
           if ((x < y) == ((u & k) == 0)) s.small[u] = y, s.small[v] = x;
         }
@@ -418,43 +518,55 @@ struct SampleRow {
       }
   }
 
-  // sums of the weights of the n tokens in s.small, `mass` before them; a thread's own weight
-  __device__ double sums(int n, double mass) {
-    double w = tid < n ? weight(key_value((uint32_t)(s.small[tid] >> 32))) : 0.0, run = w;
-    for (int off = 1; off < 64; off <<= 1) {
-      const double o = __shfl_up(run, off);
-      if (lane >= off) run += o;
+  // sums of the weights of the n tokens in s.small, `mass` before them
+  __device__ __forceinline__ void sums(int n, double mass) {
+    for (int i0 = 0; i0 < n; i0 += kSampleThreads) {
+      const int i = i0 + tid;
+      double run = i < n ? weight(key_value((uint32_t)(s.small[i] >> 32))) : 0.0;
+      for (int off = 1; off < 64; off <<= 1) {
+        const double o = __shfl_up(run, off);
+        if (lane >= off) run += o;
+      }
+      if (lane == 63) s.dsum[wave] = run;
+      __syncthreads();
+      for (int v = 0; v < wave; v++) mass += s.dsum[v];
+      if (i < n) s.run[i] = mass + run;
+      for (int v = wave; v < kSampleWaves; v++) mass += s.dsum[v];
+      __syncthreads();
     }
-    if (lane == 63) s.dsum[wave] = run;
-    __syncthreads();
-    double base = mass;
-    for (int v = 0; v < wave; v++) base += s.dsum[v];
-    if (tid < n) s.run[tid] = base + run;
-    __syncthreads();
-    return w;
   }
 
   // the place in the ordered list of n at which a prefix ends, cnt tokens before the list;
-  // its last where the sum stays below the goal by a rounding; kRatio: -1 if none is large enough
-  __device__ int place(Goal how, int n, int cnt, int nth, double goal) {
-    __syncthreads();
-    if (tid == 0) s.at = n - 1;
-    __syncthreads();
-    if (tid < n) {
-      const bool stop = how == kNth ? cnt + tid + 1 >= nth
-                        : how == kReach ? s.run[tid] >= goal
-                        : how == kPass ? s.run[tid] > goal
-                                       : !(ratio(key_value((uint32_t)(s.small[tid] >> 32))) >= goal);
-      if (stop) atomicMin(&s.at, how == kRatio ? tid - 1 : tid);
+  // its last where the sum stays below the goal by a rounding; kRatio: -1 if none is large
+  // enough.  Each wave looks by itself: a 64th of the list, then the place in it.
+  __device__ __forceinline__ int place(Goal how, int n, int cnt, int nth, double goal) const {
+    if (how == kNth) return min(n, nth - cnt) - 1;
+    constexpr int kLane = kAll / 64;
+    auto past = [&](int i) {  // the prefix has ended at i (kRatio: before it)
+      return how == kReach ? s.run[i] >= goal
+             : how == kPass ? s.run[i] > goal : !(ratio(key_value((uint32_t)(s.small[i] >> 32))) >= goal);
+    };
+    uint64_t set = __ballot(lane * kLane < n && past(min(n - 1, lane * kLane + kLane - 1)));
+    int at = n;
+    if (set) {
+      const int i = __builtin_ctzll(set) * kLane + lane;
+      set = __ballot(lane < kLane && i < n && past(min(i, n - 1)));
+      at = __builtin_amdgcn_readfirstlane(i) + __builtin_ctzll(set);
     }
-    __syncthreads();
-    return s.at;
+    return how == kRatio ? at - 1 : min(at, n - 1);
+  }
+
+  // the token at a place of the ordered list, `mass` before the list
+  __device__ __forceinline__ Ends ends_at(int at, double mass) const {
+    if (at < 0) return Ends{mass, 0.0, -1};
+    const uint64_t v = s.small[at];
+    return Ends{s.run[at], weight(key_value((uint32_t)(v >> 32))), (int)~(uint32_t)v};
   }
 
   // One of kSub parts of the keys least..most, as `each` gives the tokens, in which the prefix ends:
-  // keys lo..hi of it; cnt and mass move to what is before it.
+  // keys lo..hi of it; cnt and mass move to what is before it.  Returns its tokens.
   template <typename E>
-  __device__ void divide(Goal how, int bin, int& cnt, double& mass, int nth, double goal, uint32_t least, uint32_t most,
+  __device__ __forceinline__ int divide(Goal how, int bin, int& cnt, double& mass, int nth, double goal, uint32_t least, uint32_t most,
                          uint32_t& lo, uint32_t& hi, E tokens) {
     int shift = 0;
     while ((most - least) >> shift >= kSub) shift++;
@@ -480,7 +592,7 @@ struct SampleRow {
     if (lane == 63) s.key[wave] = im, s.lo[wave] = (uint32_t)ik;
     __syncthreads();
     for (int w = 0; w < wave; w++) im += s.key[w], ik += (int)s.lo[w];
-    const double unit = bin_unit(bin), after = mass + (double)im * unit;
+    const double after = mass + mass_in(bin, im);
     const uint32_t low = most - ((((uint32_t)tid + 1) << shift) - 1);  // the part's least key
     if (kc) {
       const bool here = how == kNth ? cnt + ik >= nth
@@ -493,8 +605,9 @@ struct SampleRow {
     __syncthreads();
     const int at = s.at < kSub ? s.at : s.bin;
     if (tid == at) {
-      s.ends.mass = mass + (double)(im - km) * unit;
+      s.ends.mass = mass + mass_in(bin, im - km);
       s.ends.idx = cnt + ik - kc;
+      s.n = kc;
     }
     __syncthreads();
     mass = s.ends.mass;
@@ -502,78 +615,55 @@ struct SampleRow {
     hi = most - ((uint32_t)at << shift);
     const uint32_t part = hi - ((1u << shift) - 1);
     lo = part < least || part > hi ? least : part;
+    return s.n;
   }
 
-  // Where in `bin` a prefix ends, cnt tokens and mass before it: at its `nth` token,
-  // where its sum reaches (kReach) or passes (kPass) `goal`, or at its last token of
-  // at least `goal` times the largest weight (kRatio; none of the bin: idx -1).
-  __device__ Ends end_of(Goal how, int bin, int cnt, double mass, int nth, double goal) {
-    uint32_t lo = 0, hi = ~0u, least, most;
-    chunks_with(bin, bin);
-    int n = gather(bin, bin, lo, hi, least, most);
-    while (n > kCap && least < most) {
-      divide(how, bin, cnt, mass, nth, goal, least, most, lo, hi, [&](auto add) {
-        each(bin, bin, [&](uint32_t k, float l, int) {
-          if (k >= least && k <= most) add(k, l);
+  // Where in `bin` a prefix ends, the bins before it summed up: at its `nth` token,
+  // where its sum reaches (kReach) or passes (kPass) `goal`, or at its last token of at
+  // least `goal` times the largest weight (kRatio; none of the bin: idx -1).  listed:
+  // whether the bin's tokens are in the list already.
+  __device__ __forceinline__ Ends end_of(Goal how, int bin, int nth, double goal, bool listed) {
+    int cnt = s.count[bin];
+    double mass = s.before[bin];
+    uint32_t lo, hi, least, most;
+    keys_of(bin, bin, lo, hi);
+    if (!listed) {
+      // divided where it lies until what is left can be taken
+      int n = s.count[bin + 1] - cnt;
+      chunks_with(BinSet{1, {bin, bin}, {bin, bin}});
+      while (n > kCap || !take({lo, lo}, {hi, hi})) {
+        if (lo == hi) return equals(how, cnt, mass, nth, goal, n, key_value(lo));
+        least = lo, most = hi;
+        n = divide(how, bin, cnt, mass, nth, goal, least, most, lo, hi, [&](auto add) {
+          each([&](int, const f32x4& x) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const uint32_t k = order_key(x[e]);
+              if (k >= least && k <= most) add(k, x[e]);
+            }
+          });
         });
-      });
-      n = gather(bin, bin, lo, hi, least, most);
+      }
     }
-    if (n > kCap) return equals(how, cnt, mass, nth, goal, n, key_value(most));
-    const uint64_t* from = s.list;
+    int n = select(lo, hi, least, most);
     while (n > kSmall && least < most) {
       divide(how, bin, cnt, mass, nth, goal, least, most, lo, hi, [&](auto add) {
-        for (int i = tid; i < n; i += kSampleThreads) {
-          const uint32_t k = (uint32_t)(s.list[i] >> 32);
-          if (k >= least && k <= most) add(k, key_value(k));
+        for (int i = 0; i < taken; i++) {
+          const float l = s.value[i][tid];
+          const uint32_t k = order_key(l);
+          if (k >= least && k <= most) add(k, l);
         }
       });
-      // its tokens to the front (a step's are read before any is written)
-      if (tid == 0) s.m = 0;
-      uint32_t l2 = ~0u, m2 = 0;
-      for (int i0 = 0; i0 < n; i0 += kSampleThreads) {
-        const uint64_t v = i0 + tid < n ? s.list[i0 + tid] : 0;
-        const uint32_t k = (uint32_t)(v >> 32);
-        __syncthreads();
-        if (i0 + tid < n && k >= lo && k <= hi) {
-          s.list[atomicAdd(&s.m, 1)] = v;
-          l2 = k < l2 ? k : l2;
-          m2 = k > m2 ? k : m2;
-        }
-      }
-      for (int off = 32; off; off >>= 1) {
-        const uint32_t u = __shfl_xor(l2, off), v = __shfl_xor(m2, off);
-        l2 = u < l2 ? u : l2;
-        m2 = v > m2 ? v : m2;
-      }
-      __syncthreads();
-      if (lane == 0) s.lo[wave] = l2, s.hi[wave] = m2;
-      __syncthreads();
-      n = s.m;
-      least = ~0u, most = 0;
-      for (int w = 0; w < kSampleWaves; w++) {
-        least = s.lo[w] < least ? s.lo[w] : least;
-        most = s.hi[w] > most ? s.hi[w] : most;
-      }
-      __syncthreads();
+      n = select(lo, hi, least, most);
     }
     if (n > kAll) return equals(how, cnt, mass, nth, goal, n, key_value(most));
-    order(from, n);
-    const double w = sums(n, mass);
-    const int at = place(how, n, cnt, nth, goal);
-    if (tid == 0) s.ends = Ends{mass, 0.0, -1};
-    __syncthreads();
-    if (tid == at) s.ends = Ends{s.run[tid], w, (int)~(uint32_t)s.small[tid]};
-    __syncthreads();
-    return s.ends;
-  }
-  __device__ Ends end(Goal how, int nth, double goal) {
-    const int b = bin_with(how, nth, goal);
-    return end_of(how, b, s.count[b], s.before[b], nth, goal);
+    order(s.some, n);
+    sums(n, mass);
+    return ends_at(place(how, n, cnt, nth, goal), mass);
   }
 
   // the same among n tokens of one logit l
-  __device__ Ends equals(Goal how, int cnt, double mass, int nth, double goal, int n, float l) {
+  __device__ __forceinline__ Ends equals(Goal how, int cnt, double mass, int nth, double goal, int n, float l) {
     const double w = weight(l);
     int r;  // tokens of them in the prefix
     if (how == kNth) {
@@ -627,14 +717,14 @@ struct SampleRow {
   }
 };
 
-// grid = rows, block = 1024
-template <bool kHalf>
+// grid = rows, block = kSampleThreads
+template <bool kHalf, int kPer>
 __global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
   __shared__ SampleLds s;
   const int b = blockIdx.x, tid = threadIdx.x;
   const void* row = (const char*)a.logits + (int64_t)b * a.stride * (kHalf ? 2 : 4);
-  SampleRow<kHalf> r{s,   a,   row, a.heads + (int64_t)b * a.chunks, a.bins + (int64_t)b * a.chunks * kBins,
-                     0.0, 0.0, 0.0f, false, tid, tid & 63, tid >> 6};
+  SampleRow<kHalf, kPer> r{s,   a,   row, a.heads + (int64_t)b * a.chunks, a.bins + (int64_t)b * a.chunks * kBins,
+                     0.0, 0.0, 1.0, 1.0, 0.0f, false, tid, tid & 63, tid >> 6, 0};
   const float t = a.temperature ? a.temperature[b] : 1.0f;
   const int k = a.top_k ? a.top_k[b] : 0;
   const float tp = a.top_p ? a.top_p[b] : 1.0f, mp = a.min_p ? a.min_p[b] : 0.0f;
@@ -648,10 +738,12 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
     return;
   }
   r.top = key_value((uint32_t)(best >> 32));
-  r.inf = r.top == __builtin_inff();
+  r.inf = __builtin_amdgcn_readfirstlane((int)(r.top == __builtin_inff()));
   if (r.inf) r.top = 0.0f;
   r.c = temperature_scale(t);
   r.R = __builtin_ceil(r.x_of(r.top));
+  r.top_mass = (double)r.mass_of(r.top);
+  r.top_power = r.power_of(r.top);
   r.add_up();
   const int total = s.count[kBins];
   const double all = s.before[kBins], need = tp > 0.0f ? (double)tp : 0.0, least = mp < 1.0f ? (double)mp : 1.0;
@@ -665,46 +757,83 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
     bm = by_m && bin > 0.0 ? (int)bin : 0;
   }
   const int bk = by_k ? r.bin_with(kNth, k, 0.0) : kBins - 1;
-  const int bp = by_p ? r.bin_with(kReach, 0, need * s.before[bk + 1]) : kBins - 1;
+  // masses that the filters can keep, by whole bins: from .. to
+  double from = by_k ? s.before[bk] : all, to = by_k ? s.before[bk + 1] : all;
+  const int p0 = by_p ? r.bin_with(kReach, 0, need * from) : 1, p1 = by_p ? r.bin_with(kReach, 0, need * to) : 0;
   u = u >= 0.0f ? (u < 1.0f ? u : 0x1.fffffep-1f) : 0.0f;
   double kept = all;  // mass of what the filters keep
   Ends e;
   // top-p's goal is a part of top-k's mass
-  const int last = by_k && by_p ? bk : min(min(bk, bp), by_m ? bm : kBins - 1);
-  if ((by_k || by_p || by_m) && s.count[last + 1] <= kAll) {
-    // few enough: all of them in order, and every prefix among them
-    r.chunks_with(0, last);
+  const int last = by_k && by_p ? bk : min(by_p ? p1 : bk, by_m ? bm : kBins - 1);
+  const bool few = (by_k || by_p || by_m) && s.count[last + 1] <= kAll;
+  BinSet w{1, {0, 0}, {last, last}};  // few enough: all of them
+  int d0 = 0, d1 = 0;
+  bool listed = true;
+  if (!few) {
+    // the bins in which a filter or the draw can end, taken from the row at once if they fit
+    if (by_p) {
+      from = fmin(from, s.before[p0]);
+      to = fmin(to, s.before[p1 + 1]);
+    }
+    if (by_m) {
+      from = fmin(from, s.before[bm]);
+      to = fmin(to, s.before[bm + 1]);
+    }
+    d0 = r.bin_with(kPass, 0, (double)u * from), d1 = r.bin_with(kPass, 0, (double)u * to);
+    // the draw's, and those from the first to the last of the filters'
+    int f0 = kBins, f1 = 0;
+    if (by_p) f0 = p0, f1 = p1;
+    if (by_k) f0 = min(f0, bk), f1 = max(f1, bk);
+    if (by_m) f0 = min(f0, bm), f1 = max(f1, bm);
+    w = BinSet{f0 <= f1 ? 2 : 1, {d0, f0}, {d1, f1}};
+    int tokens = s.count[d1 + 1] - s.count[d0];
+    if (w.n > 1) tokens += s.count[f1 + 1] - s.count[f0];
+    listed = tokens <= kCap;
+  }
+  if (listed) {
+    uint32_t lo[kRanges], hi[kRanges];
+    r.keys_of(w.from[0], w.to[0], lo[0], hi[0]);
+    lo[1] = lo[0], hi[1] = hi[0];
+    if (w.n > 1) r.keys_of(w.from[1], w.to[1], lo[1], hi[1]);
+    r.chunks_with(w);
+    listed = r.take(lo, hi);
+  }
+  if (few) {
+    // every prefix among them, in order
     uint32_t lo, hi;
-    const int n = r.gather(0, last, 0, ~0u, lo, hi);
-    r.order(s.list, n);
-    const double w = r.sums(n, 0.0);
+    const int n = r.select(0, ~0u, lo, hi);
+    r.order(s.some, n);
+    r.sums(n, 0.0);
     if (by_k && k <= n) kept = s.run[k - 1];
-    if (by_p) {
-      const double m = s.run[r.place(kReach, n, 0, 0, need * kept)];
-      kept = m < kept ? m : kept;
-    }
-    if (by_m) {
-      // (all of them, where another filter ends before: its mass is less)
-      const double m = s.run[max(0, r.place(kRatio, n, 0, 0, least))];
-      kept = m < kept ? m : kept;
-    }
-    const int at = r.place(kPass, n, 0, 0, (double)u * kept);
-    if (tid == at) s.ends = Ends{s.run[tid], w, (int)~(uint32_t)s.small[tid]};
-    __syncthreads();
-    e = s.ends;
+    if (by_p) kept = fmin(kept, s.run[r.place(kReach, n, 0, 0, need * kept)]);
+    // (all of them, where another filter ends before: its mass is less)
+    if (by_m) kept = fmin(kept, s.run[max(0, r.place(kRatio, n, 0, 0, least))]);
+    e = r.ends_at(r.place(kPass, n, 0, 0, (double)u * kept), 0.0);
   } else {
-    if (by_k) kept = r.end(kNth, k, 0.0).mass;
-    if (by_p) {
-      const double m = r.end(kReach, 0, need * kept).mass;
-      kept = m < kept ? m : kept;
+    for (int step = by_k ? 0 : 1; step < 4; step++) {  // top-k, top-p, min-p, the draw
+      // (bins by masses that a rounding has moved past their range stay in it)
+      Goal how = kPass;
+      double goal = (double)u * kept;
+      int bin;
+      if (step == 0) {
+        how = kNth, bin = bk;
+      } else if (step == 1) {
+        if (!by_p) continue;
+        how = kReach, goal = need * kept;
+        bin = min(max(r.bin_with(kReach, 0, goal), p0), p1);
+      } else if (step == 2) {
+        if (!by_m) continue;
+        how = kRatio, goal = least, bin = bm;
+        if (s.count[bm + 1] == s.count[bm]) {  // bins before it are kept whole
+          kept = fmin(kept, s.before[bm]);
+          continue;
+        }
+      } else {
+        bin = min(max(r.bin_with(kPass, 0, goal), d0), d1);
+      }
+      e = r.end_of(how, bin, k, goal, listed);
+      if (step < 3) kept = fmin(kept, e.mass);
     }
-    if (by_m) {
-      // bins before the one of `least` times the largest weight are kept whole
-      const double m = s.count[bm + 1] > s.count[bm] ? r.end_of(kRatio, bm, s.count[bm], s.before[bm], 0, least).mass
-                                                     : s.before[bm];
-      kept = m < kept ? m : kept;
-    }
-    e = r.end(kPass, 0, (double)u * kept);
   }
   if (tid == 0) {
     a.ids[b] = e.idx;
@@ -715,7 +844,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
 // Chunks of 16384 logits where that makes two workgroups a compute unit, or a row more than 64
 // of the smaller ones; else of 4096.
 static int sample_chunk(int B, int V) {
-  return (int64_t)B * ((V + kMaxChunk - 1) / kMaxChunk) >= 512 || V > 64 * kTile ? kMaxChunk : kTile;
+  return (int64_t)B * ((V + kMaxChunk - 1) / kMaxChunk) >= 512 || V > 64 * kMinChunk ? kMaxChunk : kMinChunk;
 }
 
 }  // namespace cia
@@ -725,22 +854,25 @@ using namespace cia;
 extern "C" int64_t cia_sample_workspace_bytes(int B, int V) {
   if (B < 0 || B > CIA_SAMPLE_MAX_ROWS || V < 1 || V > CIA_SAMPLE_MAX_VOCAB) return 0;
   // (the most that B rows or fewer need: a smaller batch may have smaller chunks)
-  const int64_t big = (V + kMaxChunk - 1) / kMaxChunk, small = (V + kTile - 1) / kTile;
-  int64_t n = (int64_t)B * (sample_chunk(B, V) == kTile ? small : big);
-  if (sample_chunk(1, V) == kTile) n = std::max(n, std::min<int64_t>(B, 511 / big) * small);
+  const int64_t big = (V + kMaxChunk - 1) / kMaxChunk, small = (V + kMinChunk - 1) / kMinChunk;
+  int64_t n = (int64_t)B * (sample_chunk(B, V) == kMinChunk ? small : big);
+  if (sample_chunk(1, V) == kMinChunk) n = std::max(n, std::min<int64_t>(B, 511 / big) * small);
   return 16 + n * (int64_t)(sizeof(ChunkHead) + kBins * sizeof(uint64_t));
 }
 
 template <bool kHalf>
 static int sample_launch(const SampleArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)(a.B * a.chunks));
-  if (a.chunk == kTile)
-    hipLaunchKernelGGL((k_sample_bins<kHalf, 1>), grid, dim3(256), 0, s, a);
+  if (a.chunk == kMinChunk)
+    hipLaunchKernelGGL((k_sample_bins<kHalf, 256, kMinChunk / 1024>), grid, dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((k_sample_bins<kHalf, kMaxChunk / kTile>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_sample_bins<kHalf, 512, kMaxChunk / 2048>), grid, dim3(512), 0, s, a);
   const int st = launch_status();
   if (st) return st;
-  hipLaunchKernelGGL((k_sample_pick<kHalf>), dim3((unsigned)a.B), dim3(kSampleThreads), 0, s, a);
+  if (a.chunk == kMinChunk)
+    hipLaunchKernelGGL((k_sample_pick<kHalf, kMinChunk / kStep>), dim3((unsigned)a.B), dim3(kSampleThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL((k_sample_pick<kHalf, kMaxChunk / kStep>), dim3((unsigned)a.B), dim3(kSampleThreads), 0, s, a);
   return launch_status();
 }
 
