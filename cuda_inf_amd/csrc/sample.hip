@@ -3,8 +3,8 @@
 //
 // In descending order of the logits (the lowest index first among equals) each filter
 // keeps a prefix, and so does the draw: a prefix sum of w = exp((l - max) / T) that
-// reaches a goal.  No row is sorted.  With x = 8 log2(e) l / T, a token's bin is
-// ceil(x), an eighth of an octave of w, and the counts and masses of the 336 bins
+// reaches a goal.  No row is sorted.  With x = 16 log2(e) l / T, a token's bin is
+// ceil(x), a sixteenth of an octave of w, and the counts and masses of the 672 bins
 // below the largest (42 octaves; what lies lower has no weight) say in which bin a
 // prefix ends:
 //   k_sample_bins  reads the logits once: the bins of each chunk of a row;
@@ -25,7 +25,7 @@ namespace cia {
 
 constexpr int kSampleThreads = 512;  // of k_sample_pick
 constexpr int kSampleWaves = kSampleThreads / 64;
-constexpr int kBins = 336;   // 42 octaves, 8 bins each
+constexpr int kBins = 672;   // 42 octaves, 16 bins each
 constexpr int kSlots = 32;    // tokens that a thread takes from a row into LDS
 constexpr int kCap = 6144;   // tokens that are tried to be taken: 12 a thread
 constexpr int kSmall = 256;  // tokens put in order by counting the larger ones
@@ -92,31 +92,28 @@ struct Logits {
   }
 };
 
-// 2^(f / 8) for f in (-1, 0]: the polynomial of degree 5 through the Chebyshev points of
-// the interval, 3e-13 off
+// 2^(f / 16) for f in (-1, 0]: the polynomial of degree 4 through the Chebyshev points of
+// the interval, 2.5e-12 off
 __device__ __forceinline__ double bin_power(double f) {
-  double r = 3.896822893996917e-08;
-  r = __builtin_fma(r, f, 2.346252607310361e-06);
-  r = __builtin_fma(r, f, 1.0840546828792358e-04);
-  r = __builtin_fma(r, f, 3.753538938644709e-03);
-  r = __builtin_fma(r, f, 8.66433975500605e-02);
-  return __builtin_fma(r, f, 0.9999999999997227);
+  double r = 1.4361898916011284e-07;
+  r = __builtin_fma(r, f, 1.3548068750879863e-05);
+  r = __builtin_fma(r, f, 9.383838162057435e-04);
+  r = __builtin_fma(r, f, 4.3321698663009583e-02);
+  return __builtin_fma(r, f, 0.9999999999975604);
 }
 // the same in units of 2^-34, rounded by an addition of 2^18
 __device__ __forceinline__ uint64_t bin_mass(double f) {
   return __builtin_bit_cast(uint64_t, bin_power(f) + 262144.0) - __builtin_bit_cast(uint64_t, 262144.0);
 }
-// a bin's upper edge, bin 0's being 1: 2^(-bin / 8)
+// a bin's upper edge, bin 0's being 1: 2^(-bin / 16)
 __device__ __forceinline__ double bin_edge(int bin) {
-  constexpr double kEighth[8] = {1.0, 0.91700404320467122, 0.84089641525371454, 0.77110541270397037,
-                                 0.70710678118654752, 0.64841977732550483, 0.59460355750136054, 0.54525386633262882};
-  double e = kEighth[0];
-#pragma unroll
-  for (int i = 1; i < 8; i++) e = (bin & 7) == i ? kEighth[i] : e;
-  return e * __builtin_bit_cast(double, (uint64_t)(1023 - (bin >> 3)) << 52);
+  const int i = bin & 3, j = bin >> 2 & 3;
+  const double e = i == 0 ? 1.0 : i == 1 ? 0.9576032806985737 : i == 2 ? 0.9170040432046712 : 0.8781260801866497;
+  const double q = j == 0 ? 1.0 : j == 1 ? 0.8408964152537145 : j == 2 ? 0.7071067811865476 : 0.5946035575013605;
+  return e * q * __builtin_bit_cast(double, (uint64_t)(1023 - (bin >> 4)) << 52);
 }
 
-__device__ __forceinline__ double temperature_scale(float t) { return 8 * 1.44269504088896340736 / (double)t; }
+__device__ __forceinline__ double temperature_scale(float t) { return 16 * 1.44269504088896340736 / (double)t; }
 
 // ---------------------------------------------------------------- the bins
 // grid = rows * chunks, block = kThreads, 4 kVec logits of the chunk a thread, in registers
@@ -213,8 +210,8 @@ struct SampleLds {
   uint64_t some[kAll];  // those of one bin
   uint64_t small[kAll];  // in descending order
   double run[kAll];     // sums of their weights
-  unsigned long long mass[kSub];
-  uint32_t cnt[kSub];
+  unsigned long long mass[kBins];
+  uint32_t cnt[kBins];
   double before[kBins + 1];  // mass of the bins before
   int count[kBins + 1];      // tokens of the bins before
   double shift[kMaxChunks];  // of a chunk's bins; kBins or more: none of them counts
@@ -264,8 +261,8 @@ struct SampleRow {
   __device__ __forceinline__ double mass_in(int bin, unsigned long long m) const {
     return (double)m / top_mass * bin_edge(bin);
   }
-  // the same without the bins' 3e-13
-  __device__ __forceinline__ double ratio(float l) const { return exp2(((double)l - (double)top) * c * 0.125); }
+  // the same without the bins' 2.5e-12
+  __device__ __forceinline__ double ratio(float l) const { return exp2(((double)l - (double)top) * c * 0.0625); }
   __device__ __forceinline__ double power_of(float l) const {
 #pragma clang fp contract(off)
     const double x = x_of(l);
@@ -277,8 +274,14 @@ struct SampleRow {
     return bin_mass(x - __builtin_ceil(x));
   }
 
-  // the row's largest logit: key << 32 | ~index
-  __device__ __forceinline__ uint64_t largest() {
+  // The row's largest logit, key << 32 | ~index, and the first of its chunks' bins on
+  // their way.
+  static constexpr int kFirst = 12;  // bins of a thread: 9 small chunks at once, or all 8 of 131072 logits
+  __device__ __forceinline__ uint64_t largest(uint64_t (&first)[kFirst]) {
+#pragma unroll
+    for (int i = 0; i < kFirst; i++) first[i] = bins[min(i * kSampleThreads + tid, a.chunks * kBins - 1)];
+    for (int i = tid; i < kBins; i += kSampleThreads) s.mass[i] = 0, s.cnt[i] = 0;
+    if (tid == 0) s.last = 0;
     uint64_t best = 0;
     for (int i = tid; i < a.chunks; i += kSampleThreads) {
       const ChunkHead h = heads[i];
@@ -299,44 +302,54 @@ struct SampleRow {
   }
 
   // the row's bins: tokens and mass before each
-  __device__ __forceinline__ void add_up() {
+  __device__ __forceinline__ void add_up(const uint64_t (&first)[kFirst]) {
     for (int i = tid; i < a.chunks; i += kSampleThreads) {
       const double n = s.shift[i];
-      s.shift[i] = inf ? (n == __builtin_inf() ? 0.0 : (double)kBins) : R - n;
+      s.shift[i] = inf ? (n == __builtin_inf() ? 0.0 : (double)kBins) : fmin(R - n, (double)kBins);
     }
-    if (tid == 0) s.last = 0;
     __syncthreads();
-    unsigned long long m = 0;
-    uint32_t k = 0;
-    if (tid < kBins)
-#pragma unroll 8
-      for (int i = 0; i < a.chunks; i++) {
-        const double d = (double)tid - s.shift[i];
-        uint64_t v = bins[(int64_t)i * kBins + (int)fmax(d, 0.0)];
-        v = d >= 0.0 ? v : 0;  // (the bins of a chunk without tokens are not written)
-        m += v & ((1ull << kCountShift) - 1);
-        k += (uint32_t)(v >> kCountShift);
+    const int all = a.chunks * kBins;
+    auto add = [&](int i, uint64_t v) {
+      const int chunk = i / kBins, b = i - chunk * kBins + (int)s.shift[min(chunk, a.chunks - 1)];
+      // (the bins of a chunk without tokens are not written)
+      if (i < all && b < kBins && v) {
+        atomicAdd(&s.mass[b], (unsigned long long)(v & ((1ull << kCountShift) - 1)));
+        atomicAdd(&s.cnt[b], (uint32_t)(v >> kCountShift));
       }
-    double run = tid < kBins ? mass_in(tid, m) : 0.0;
-    int upto = (int)k;
+    };
+#pragma unroll
+    for (int i = 0; i < kFirst; i++) add(i * kSampleThreads + tid, first[i]);
+#pragma unroll 4
+    for (int i = kFirst * kSampleThreads + tid; i < all; i += kSampleThreads) add(i, bins[i]);
+    __syncthreads();
+    // two bins a thread
+    const int b = min(2 * tid, kBins - 2);
+    const bool mine = 2 * tid < kBins;
+    const int k0 = mine ? (int)s.cnt[b] : 0, k1 = mine ? (int)s.cnt[b + 1] : 0;
+    const double m0 = mine ? mass_in(b, s.mass[b]) : 0.0, m1 = mine ? mass_in(b + 1, s.mass[b + 1]) : 0.0;
+    double run = m0 + m1;
+    int upto = k0 + k1;
     for (int off = 1; off < 64; off <<= 1) {
       const double um = __shfl_up(run, off);
       const int uk = __shfl_up(upto, off);
       if (lane >= off) run += um, upto += uk;
     }
     if (lane == 63) s.dsum[wave] = run, s.lo[wave] = (uint32_t)upto;
-    if (k) atomicMax(&s.last, tid);
+    if (k0 + k1) atomicMax(&s.last, k1 ? b + 1 : b);
     __syncthreads();
     double base = 0.0;
     int kbase = 0;
     for (int v = 0; v < wave; v++) base += s.dsum[v], kbase += (int)s.lo[v];
-    if (tid < kBins) s.before[tid + 1] = base + run, s.count[tid + 1] = kbase + upto;
+    if (mine) {
+      s.before[b + 2] = base + run, s.count[b + 2] = kbase + upto;
+      s.before[b + 1] = base + run - m1, s.count[b + 1] = kbase + upto - k1;
+    }
     if (tid == 0) s.before[0] = 0.0, s.count[0] = 0;
     __syncthreads();
   }
 
   // the bin in which a prefix ends: the first whose sum satisfies the goal, the last
-  // that holds any where none does; each wave looks by itself, in 56 groups of 6 bins,
+  // that holds any where none does; each wave looks by itself, in 56 groups of 12 bins,
   // then in one of them
   __device__ __forceinline__ int bin_with(Goal how, int nth, double goal) const {
     constexpr int kPart = kBins / 56;
@@ -568,8 +581,7 @@ struct SampleRow {
   template <typename E>
   __device__ __forceinline__ int divide(Goal how, int bin, int& cnt, double& mass, int nth, double goal, uint32_t least, uint32_t most,
                          uint32_t& lo, uint32_t& hi, E tokens) {
-    int shift = 0;
-    while ((most - least) >> shift >= kSub) shift++;
+    const int shift = max(0, 32 - __clz((int)(most - least)) - __builtin_ctz(kSub));
     __syncthreads();
     s.mass[tid] = 0, s.cnt[tid] = 0;
     if (tid == 0) s.at = kSub, s.bin = 0;
@@ -627,9 +639,9 @@ struct SampleRow {
     double mass = s.before[bin];
     uint32_t lo, hi, least, most;
     keys_of(bin, bin, lo, hi);
+    int n = s.count[bin + 1] - cnt;
     if (!listed) {
       // divided where it lies until what is left can be taken
-      int n = s.count[bin + 1] - cnt;
       chunks_with(BinSet{1, {bin, bin}, {bin, bin}});
       while (n > kCap || !take({lo, lo}, {hi, hi})) {
         if (lo == hi) return equals(how, cnt, mass, nth, goal, n, key_value(lo));
@@ -645,17 +657,17 @@ struct SampleRow {
         });
       }
     }
-    int n = select(lo, hi, least, most);
-    while (n > kSmall && least < most) {
-      divide(how, bin, cnt, mass, nth, goal, least, most, lo, hi, [&](auto add) {
+    while (n > kSmall && lo < hi) {
+      least = lo, most = hi;
+      n = divide(how, bin, cnt, mass, nth, goal, least, most, lo, hi, [&](auto add) {
         for (int i = 0; i < taken; i++) {
           const float l = s.value[i][tid];
           const uint32_t k = order_key(l);
           if (k >= least && k <= most) add(k, l);
         }
       });
-      n = select(lo, hi, least, most);
     }
+    n = select(lo, hi, least, most);
     if (n > kAll) return equals(how, cnt, mass, nth, goal, n, key_value(most));
     order(s.some, n);
     sums(n, mass);
@@ -729,7 +741,8 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
   const int k = a.top_k ? a.top_k[b] : 0;
   const float tp = a.top_p ? a.top_p[b] : 1.0f, mp = a.min_p ? a.min_p[b] : 0.0f;
   float u = a.u[b];
-  const uint64_t best = r.largest();
+  uint64_t first[SampleRow<kHalf, kPer>::kFirst];
+  const uint64_t best = r.largest(first);
   if (best == 0 || !(t > 0.0f)) {
     if (tid == 0) {
       a.ids[b] = best ? (int)~(uint32_t)best : -1;
@@ -744,7 +757,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
   r.R = __builtin_ceil(r.x_of(r.top));
   r.top_mass = (double)r.mass_of(r.top);
   r.top_power = r.power_of(r.top);
-  r.add_up();
+  r.add_up(first);
   const int total = s.count[kBins];
   const double all = s.before[kBins], need = tp > 0.0f ? (double)tp : 0.0, least = mp < 1.0f ? (double)mp : 1.0;
   const bool by_k = k > 0 && k < total, by_p = tp < 1.0f;
@@ -752,7 +765,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
   // the bin of the last token that each filter can keep
   int bm = 0;
   if (by_m) {
-    const double x = r.x_of(r.top) + 8 * log2(least), bin = r.R - __builtin_ceil(x);
+    const double x = r.x_of(r.top) + 16 * log2(least), bin = r.R - __builtin_ceil(x);
     by_m = bin < (double)kBins;
     bm = by_m && bin > 0.0 ? (int)bin : 0;
   }
