@@ -7,7 +7,8 @@
 //
 // Work.  A row's tokens are units of 128, and the units of all rows one list, of which
 // each of the P workgroups of a kv head takes an equal part, whatever rows it falls
-// into: batches of very different lengths keep every compute unit busy to the end.  The
+// into: batches of very different lengths keep every compute unit busy to the end.  A
+// row's start counts as some units more, or workgroups of many short rows end last.  The
 // list follows from the positions on the device, so a captured call can be replayed with
 // others.  A row in one workgroup's part is finished there; the parts of a longer one are
 // joined by the workgroup that ends last (it counts itself in, nothing waits).
@@ -26,6 +27,7 @@
 namespace cia {
 
 constexpr int kUnit = 128;        // tokens of a unit: 32 a wave
+constexpr int kRowCost = 3;       // units that a row's start and end take the time of
 constexpr int kGroups = 1024;     // workgroups of a call at most
 constexpr int kMaxParts = 256;    // of them for one kv head
 constexpr int kTicketStride = 16;  // uint32 between two counters
@@ -63,8 +65,9 @@ __device__ __forceinline__ Span row_span(const AttnPagesArgs& a, int t) {
   }
   return r;
 }
-__device__ __forceinline__ int span_units(const Span& r) {
-  return r.len ? (r.len + kUnit - 1) / kUnit - r.first / kUnit : 0;
+// a row's cost: its units, and kRowCost for its start
+__device__ __forceinline__ int span_cost(const Span& r) {
+  return r.len ? (r.len + kUnit - 1) / kUnit - r.first / kUnit + kRowCost : 0;
 }
 
 template <int kD, bool kF8, int kNB>
@@ -97,12 +100,17 @@ __device__ __forceinline__ void put(float* p, float x, float y) {
   const uint64_t w = (uint64_t)__builtin_bit_cast(uint32_t, y) << 32 | __builtin_bit_cast(uint32_t, x);
   __hip_atomic_store((uint64_t*)p, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+__device__ __forceinline__ f32x4 take4(const float* p) {
+  const uint64_t u = __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const uint64_t w = __hip_atomic_load((const uint64_t*)p + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return __builtin_bit_cast(f32x4, u32x4{(uint32_t)u, (uint32_t)(u >> 32), (uint32_t)w, (uint32_t)(w >> 32)});
+}
 __device__ __forceinline__ f32x2 take(const float* p) {
   const uint64_t w = __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   return f32x2{__builtin_bit_cast(float, (uint32_t)w), __builtin_bit_cast(float, (uint32_t)(w >> 32))};
 }
 
-// grid = kv heads * cols * parts, block = 256, LDS: a prefix sum of T + 1
+// grid = kv heads * cols * parts, block = 256, LDS: T rows
 template <int kD, bool kF8, int kNB>
 __global__ __launch_bounds__(256, kD == 64 ? 3 : 2) void k_attn_pages(AttnPagesArgs a) {
   using Tile = AttnTile<kD, kF8, kNB>;
@@ -110,7 +118,8 @@ __global__ __launch_bounds__(256, kD == 64 ? 3 : 2) void k_attn_pages(AttnPagesA
   constexpr int kRowB = Tile::kRowB, kR = Tile::kR, kO = kD / 16;
   constexpr int kPart = kRp * (kD + 2);  // floats of a partial: o, then (max, sum) of each head
   constexpr int kVecs = kRp * kD / 4;    // fours of a row's outputs
-  extern __shared__ int pre[];  // units before each row
+  extern __shared__ Span spans[];  // of the rows, and then the cost before each
+  int* const pre = (int*)(spans + a.T);
   __shared__ union {
     struct {
       float o[4][kRp][kD];
@@ -128,37 +137,52 @@ __global__ __launch_bounds__(256, kD == 64 ? 3 : 2) void k_attn_pages(AttnPagesA
   const int head = vh / a.cols, h0 = head * a.group + vh % a.cols * 16;  // kv head, first query head
   const int heads = min(kRp, a.group - vh % a.cols * 16);
 
-  // ---- the list of units; rows without any are zeros
-  int carry = 0;
-  for (int base = 0; base < a.T; base += 256) {
-    const int t = base + tid;
-    int n = 0;
-    if (t < a.T) {
-      n = span_units(row_span(a, t));
-      if (n == 0 && t % a.parts == part)
-        for (int i = 0; i < heads * kD / 8; i++)
-          *(u32x4*)(a.out + ((int64_t)t * a.n_q + h0) * kD + 8 * i) = u32x4{0, 0, 0, 0};
-    }
-    int sum = n;
+  // ---- the list of the rows' costs; rows without any units are zeros
+  auto put_row = [&](int t, const Span& r, int before, int cost) __attribute__((always_inline)) {
+    pre[t] = before;
+    spans[t] = r;
+    if (cost == 0 && t % a.parts == part)
+      for (int i = 0; i < heads * kD / 8; i++)
+        *(u32x4*)(a.out + ((int64_t)t * a.n_q + h0) * kD + 8 * i) = u32x4{0, 0, 0, 0};
+  };
+  auto scan = [&](int n) __attribute__((always_inline)) {
     for (int off = 1; off < 64; off <<= 1) {
-      const int o = __shfl_up(sum, off);
-      if (lane >= off) sum += o;
+      const int o = __shfl_up(n, off);
+      if (lane >= off) n += o;
     }
-    if (lane == 63) wsum[wave] = sum;
-    __syncthreads();
-    int before = carry;
-    for (int w = 0; w < 4; w++) {
-      if (w < wave) before += wsum[w];
-      carry += wsum[w];
+    return n;
+  };
+  int total = 0;
+  if (a.T <= 64) {
+    // every wave for itself: what it reads of the list, it has written
+    const Span r = lane < a.T ? row_span(a, lane) : Span{0, 0, 0};
+    const int cost = span_cost(r), upto = scan(cost);
+    if (lane < a.T) put_row(lane, r, upto - cost, cost);
+    total = __builtin_amdgcn_readlane(upto, 63);
+    if (lane == 0) pre[a.T] = total;
+  } else {
+    for (int base = 0; base < a.T; base += 256) {
+      const int t = base + tid;
+      const Span r = t < a.T ? row_span(a, t) : Span{0, 0, 0};
+      const int cost = span_cost(r), upto = scan(cost);
+      if (lane == 63) wsum[wave] = upto;
+      __syncthreads();
+      int before = total;
+      for (int w = 0; w < 4; w++) {
+        if (w < wave) before += wsum[w];
+        total += wsum[w];
+      }
+      if (t < a.T) put_row(t, r, before + upto - cost, cost);
+      __syncthreads();
     }
-    if (t < a.T) pre[t] = before + sum - n;
+    if (tid == 0) pre[a.T] = total;
     __syncthreads();
   }
-  const int total = carry;
-  if (tid == 0) pre[a.T] = total;
-  __syncthreads();
-  const int from = (int)((int64_t)total * part / a.parts), to = (int)((int64_t)total * (part + 1) / a.parts);
-  if (from >= to) return;
+  if (total == 0) return;
+  // as few parts as make the largest no larger
+  const int most = (total + a.parts - 1) / a.parts, parts = (total + most - 1) / most;
+  if (part >= parts) return;
+  const int from = (int)((int64_t)total * part / parts), to = (int)((int64_t)total * (part + 1) / parts);
 
   // ---- the lane's places
   const int n = lane & 15, g = lane >> 4, j = n / kRp;
@@ -177,12 +201,13 @@ __global__ __launch_bounds__(256, kD == 64 ? 3 : 2) void k_attn_pages(AttnPagesA
       hi = mid - 1;
     }
   }
-  for (int at = from; at < to; row++) {
-    const int r0 = pre[row], r1 = pre[row + 1];
-    if (r1 <= at) continue;
-    const int end = min(r1, to), count = end - at;
-    const Span span = row_span(a, row);
-    const int base = (span.first / kUnit + (at - r0)) * kUnit + 32 * wave;  // the wave's first token
+  for (; row < a.T && pre[row] < to; row++) {
+    // the units [u0, u1) of the row's
+    const int r0 = pre[row] + kRowCost, r1 = pre[row + 1];
+    const int u0 = max(from - r0, 0), u1 = min(to, r1) - r0, count = u1 - u0;
+    if (count <= 0) continue;
+    const Span span = spans[row];
+    const int base = (span.first / kUnit + u0) * kUnit + 32 * wave;  // the wave's first token
 
     f16x8 Q[kD / 32];
 #pragma unroll
@@ -412,8 +437,8 @@ __global__ __launch_bounds__(256, kD == 64 ? 3 : 2) void k_attn_pages(AttnPagesA
       if (g == 0) s.w.m[wave][mine] = M, s.w.l[wave][mine] = l;
     }
     __syncthreads();
-    const bool ends = at == r0 && end == r1;  // the whole row
-    float* const to_ws = a.partial + ((int64_t)(vh * a.parts + part) * 2 + (at == r0 ? 1 : 0)) * kPart;
+    const bool ends = u0 == 0 && r0 + u1 == r1;  // the whole row
+    float* const to_ws = a.partial + ((int64_t)(vh * a.parts + part) * 2 + (u0 == 0 ? 1 : 0)) * kPart;
     for (int i = tid; i < kVecs; i += 256) {
       const int h = i / (kD / 4), d = i % (kD / 4) * 4;
       float top = s.w.m[0][h];
@@ -443,9 +468,9 @@ __global__ __launch_bounds__(256, kD == 64 ? 3 : 2) void k_attn_pages(AttnPagesA
     }
     if (!ends) {
       // the row's parts: the workgroups that have a unit of it, from that of its first
-      const int64_t N = total, W = a.parts;
+      const int64_t N = total, W = parts;
       const int first = (int)(((int64_t)(r0 + 1) * W - 1) / N), fin = (int)(((int64_t)r1 * W - 1) / N);
-      const int pieces = total <= a.parts ? r1 - r0 : fin - first + 1;
+      const int pieces = fin - first + 1;
       stores_acked();
       __syncthreads();
       if (tid == 0) {
@@ -457,9 +482,16 @@ __global__ __launch_bounds__(256, kD == 64 ? 3 : 2) void k_attn_pages(AttnPagesA
       __syncthreads();
       if (last) {
         auto piece = [&](int i) {
-          const int p = total <= a.parts ? (int)(((int64_t)(r0 + i + 1) * W - 1) / N) : first + i;
-          return a.partial + ((int64_t)(vh * a.parts + p) * 2 + (i == 0 ? 1 : 0)) * kPart;
+          return a.partial + ((int64_t)(vh * a.parts + first + i) * 2 + (i == 0 ? 1 : 0)) * kPart;
         };
+        constexpr int kSplit = kVecs < 256 ? 256 / kVecs : 1;  // threads of a four
+        // a thread's first pieces are on their way while the weights are made
+        constexpr int kEarly = 8;
+        const int i4 = tid % kVecs, h_of = i4 / (kD / 4), at4 = h_of * kD + i4 % (kD / 4) * 4, way = tid / kVecs;
+        f32x4 early[kEarly];
+        if constexpr (kVecs <= 256)
+#pragma unroll
+          for (int c = 0; c < kEarly; c++) early[c] = take4(piece(min(way + c * kSplit, pieces - 1)) + at4);
         for (int h = wave; h < kRp; h += 4) {
           float pm[kMaxParts / 64], pl[kMaxParts / 64], top = kLow;
 #pragma unroll
@@ -484,19 +516,28 @@ __global__ __launch_bounds__(256, kD == 64 ? 3 : 2) void k_attn_pages(AttnPagesA
           if (lane == 0) s.j.l[h] = sum;
         }
         __syncthreads();
-        constexpr int kSplit = kVecs < 256 ? 256 / kVecs : 1;  // threads of a four
         for (int v = tid; v < kVecs * kSplit; v += 256) {
           const int i4 = v % kVecs, h = i4 / (kD / 4), d = i4 % (kD / 4) * 4;
           f32x4 o{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-          for (int i = v / kVecs; i < pieces; i += kSplit) {
-            const float* x = piece(i) + h * kD + d;
-            const f32x2 u = take(x), w = take(x + 2);
-            const float e = s.j.weight[h][i];
-            o[0] = __builtin_fmaf(u[0], e, o[0]);
-            o[1] = __builtin_fmaf(u[1], e, o[1]);
-            o[2] = __builtin_fmaf(w[0], e, o[2]);
-            o[3] = __builtin_fmaf(w[1], e, o[3]);
+          int i = v / kVecs;
+          auto add = [&](const f32x4& x, float e) __attribute__((always_inline)) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) o[c] = __builtin_fmaf(x[c], e, o[c]);
+          };
+          if constexpr (kVecs <= 256) {
+#pragma unroll
+            for (int c = 0; c < kEarly; c++)
+              if (i + c * kSplit < pieces) add(early[c], s.j.weight[h][i + c * kSplit]);
+            i += kEarly * kSplit;
+          }
+#pragma unroll 1
+          for (; i < pieces; i += kEarly * kSplit) {
+            f32x4 x[kEarly];
+#pragma unroll
+            for (int c = 0; c < kEarly; c++) x[c] = take4(piece(min(i + c * kSplit, pieces - 1)) + h * kD + d);
+#pragma unroll
+            for (int c = 0; c < kEarly; c++)
+              if (i + c * kSplit < pieces) add(x[c], s.j.weight[h][i + c * kSplit]);
           }
           if constexpr (kSplit > 1) {
             *(f32x4*)&s.j.o[4 * v] = o;
@@ -513,7 +554,6 @@ __global__ __launch_bounds__(256, kD == 64 ? 3 : 2) void k_attn_pages(AttnPagesA
         }
       }
     }
-    at = end;
   }
 }
 
@@ -527,7 +567,7 @@ static int attn_columns(int group) { return group <= 4 ? 4 : group <= 8 ? 8 : 16
 template <int kD, bool kF8>
 static void attn_launch(const AttnPagesArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)(a.P.n_kv * a.cols * a.parts));
-  const size_t lds = (size_t)(a.T + 1) * sizeof(int);
+  const size_t lds = (size_t)a.T * (sizeof(Span) + sizeof(int)) + sizeof(int);
   switch (attn_columns(a.group)) {
     case 4: hipLaunchKernelGGL((k_attn_pages<kD, kF8, 4>), grid, dim3(256), lds, s, a); break;
     case 8: hipLaunchKernelGGL((k_attn_pages<kD, kF8, 2>), grid, dim3(256), lds, s, a); break;
