@@ -28,7 +28,7 @@ namespace cia {
 
 constexpr int kUnit = 128;        // tokens of a unit: 32 a wave
 constexpr int kRowCost = 3;       // units that a row's start and end take the time of
-constexpr int kGroups = 1024;     // workgroups of a call at most
+constexpr int kGroups = 512;      // workgroups of a call, two a compute unit
 constexpr int kMaxParts = 256;    // of them for one kv head
 constexpr int kTicketStride = 16;  // uint32 between two counters
 constexpr int64_t kTicketBytes = (int64_t)kGroups * kTicketStride * 4;
@@ -96,27 +96,22 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[kV]) 
 
 __device__ __forceinline__ uint32_t f16_bits(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
 
-__device__ __forceinline__ void put(float* p, float x, float y) {
-  const uint64_t w = (uint64_t)__builtin_bit_cast(uint32_t, y) << 32 | __builtin_bit_cast(uint32_t, x);
-  __hip_atomic_store((uint64_t*)p, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// Partials cross the XCDs: coherent stores and loads, the workgroup's address plus a
+// uniform offset in floats and a lane's.
+__device__ __forceinline__ void put4(__amdgpu_buffer_rsrc_t ws, int at, int lane_at, const f32x4& x) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), ws, lane_at * 4, at * 4, kCoherent);
 }
-__device__ __forceinline__ f32x4 take4(const float* p) {
-  const uint64_t u = __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  const uint64_t w = __hip_atomic_load((const uint64_t*)p + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return __builtin_bit_cast(f32x4, u32x4{(uint32_t)u, (uint32_t)(u >> 32), (uint32_t)w, (uint32_t)(w >> 32)});
-}
-__device__ __forceinline__ f32x2 take(const float* p) {
-  const uint64_t w = __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return f32x2{__builtin_bit_cast(float, (uint32_t)w), __builtin_bit_cast(float, (uint32_t)(w >> 32))};
+__device__ __forceinline__ f32x4 take4(__amdgpu_buffer_rsrc_t ws, int at, int lane_at) {
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(ws, lane_at * 4, at * 4, kCoherent));
 }
 
 // grid = kv heads * cols * parts, block = 256, LDS: T rows
 template <int kD, bool kF8, int kNB>
-__global__ __launch_bounds__(256, kD == 64 ? 3 : 2) void k_attn_pages(AttnPagesArgs a) {
+__global__ __launch_bounds__(256, 2) void k_attn_pages(AttnPagesArgs a) {
   using Tile = AttnTile<kD, kF8, kNB>;
   constexpr int kRp = 16 / kNB;        // query heads of a workgroup
   constexpr int kRowB = Tile::kRowB, kR = Tile::kR, kO = kD / 16;
-  constexpr int kPart = kRp * (kD + 2);  // floats of a partial: o, then (max, sum) of each head
+  constexpr int kPart = kRp * (kD + 4);  // floats of a partial: o, then (max, sum, -, -) of each head
   constexpr int kVecs = kRp * kD / 4;    // fours of a row's outputs
   extern __shared__ Span spans[];  // of the rows, and then the cost before each
   int* const pre = (int*)(spans + a.T);
@@ -438,7 +433,7 @@ __global__ __launch_bounds__(256, kD == 64 ? 3 : 2) void k_attn_pages(AttnPagesA
     }
     __syncthreads();
     const bool ends = u0 == 0 && r0 + u1 == r1;  // the whole row
-    float* const to_ws = a.partial + ((int64_t)(vh * a.parts + part) * 2 + (u0 == 0 ? 1 : 0)) * kPart;
+    const __amdgpu_buffer_rsrc_t ws = buf_rsrc(a.partial + (int64_t)vh * a.parts * 2 * kPart);
     for (int i = tid; i < kVecs; i += 256) {
       const int h = i / (kD / 4), d = i % (kD / 4) * 4;
       float top = s.w.m[0][h];
@@ -461,9 +456,9 @@ __global__ __launch_bounds__(256, kD == 64 ? 3 : 2) void k_attn_pages(AttnPagesA
               f16x4{(_Float16)(o[0] * inv), (_Float16)(o[1] * inv), (_Float16)(o[2] * inv), (_Float16)(o[3] * inv)};
         }
       } else {
-        put(to_ws + h * kD + d, o[0], o[1]);
-        put(to_ws + h * kD + d + 2, o[2], o[3]);
-        if (d == 0) put(to_ws + kRp * kD + 2 * h, top, sum);
+        const int to = (part * 2 + (u0 == 0 ? 1 : 0)) * kPart;
+        put4(ws, to, h * kD + d, o);
+        if (d == 0) put4(ws, to, kRp * kD + 4 * h, f32x4{top, sum, 0.f, 0.f});
       }
     }
     if (!ends) {
@@ -481,17 +476,18 @@ __global__ __launch_bounds__(256, kD == 64 ? 3 : 2) void k_attn_pages(AttnPagesA
       }
       __syncthreads();
       if (last) {
-        auto piece = [&](int i) {
-          return a.partial + ((int64_t)(vh * a.parts + first + i) * 2 + (i == 0 ? 1 : 0)) * kPart;
-        };
-        constexpr int kSplit = kVecs < 256 ? 256 / kVecs : 1;  // threads of a four
+        auto piece = [&](int i) { return ((first + i) * 2 + (i == 0 ? 1 : 0)) * kPart; };
+        constexpr int kSplit = kVecs < 256 ? 256 / kVecs : 1;  // waves, or more, of a four
         // a thread's first pieces are on their way while the weights are made
-        constexpr int kEarly = 8;
-        const int i4 = tid % kVecs, h_of = i4 / (kD / 4), at4 = h_of * kD + i4 % (kD / 4) * 4, way = tid / kVecs;
+        constexpr int kEarly = 8, kLate = 8;
+        const int way = __builtin_amdgcn_readfirstlane(tid / kVecs);
         f32x4 early[kEarly];
         if constexpr (kVecs <= 256)
 #pragma unroll
-          for (int c = 0; c < kEarly; c++) early[c] = take4(piece(min(way + c * kSplit, pieces - 1)) + at4);
+          for (int c = 0; c < kEarly; c++) {
+            early[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (way + c * kSplit < pieces) early[c] = take4(ws, piece(way + c * kSplit), 4 * (tid % kVecs));
+          }
         for (int h = wave; h < kRp; h += 4) {
           float pm[kMaxParts / 64], pl[kMaxParts / 64], top = kLow;
 #pragma unroll
@@ -499,7 +495,7 @@ __global__ __launch_bounds__(256, kD == 64 ? 3 : 2) void k_attn_pages(AttnPagesA
             const int i = lane + 64 * c;
             pm[c] = kLow, pl[c] = 0.0f;
             if (i < pieces) {
-              const f32x2 x = take(piece(i) + kRp * kD + 2 * h);
+              const f32x4 x = take4(ws, 0, piece(i) + kRp * kD + 4 * h);
               pm[c] = x[0], pl[c] = x[1];
             }
             top = __builtin_fmaxf(top, pm[c]);
@@ -519,24 +515,24 @@ __global__ __launch_bounds__(256, kD == 64 ? 3 : 2) void k_attn_pages(AttnPagesA
         for (int v = tid; v < kVecs * kSplit; v += 256) {
           const int i4 = v % kVecs, h = i4 / (kD / 4), d = i4 % (kD / 4) * 4;
           f32x4 o{0.f, 0.f, 0.f, 0.f};
-          int i = v / kVecs;
+          int i = __builtin_amdgcn_readfirstlane(v / kVecs);
           auto add = [&](const f32x4& x, float e) __attribute__((always_inline)) {
 #pragma unroll
             for (int c = 0; c < 4; c++) o[c] = __builtin_fmaf(x[c], e, o[c]);
           };
           if constexpr (kVecs <= 256) {
 #pragma unroll
-            for (int c = 0; c < kEarly; c++)
-              if (i + c * kSplit < pieces) add(early[c], s.j.weight[h][i + c * kSplit]);
+            for (int c = 0; c < kEarly; c++) add(early[c], s.j.weight[h][i + c * kSplit]);  // (0 past the last)
             i += kEarly * kSplit;
           }
 #pragma unroll 1
-          for (; i < pieces; i += kEarly * kSplit) {
-            f32x4 x[kEarly];
+          for (; i < pieces; i += kLate * kSplit) {
+            f32x4 x[kLate];
 #pragma unroll
-            for (int c = 0; c < kEarly; c++) x[c] = take4(piece(min(i + c * kSplit, pieces - 1)) + h * kD + d);
+            for (int c = 0; c < kLate; c++)
+              if (i + c * kSplit < pieces) x[c] = take4(ws, piece(i + c * kSplit), 4 * i4);
 #pragma unroll
-            for (int c = 0; c < kEarly; c++)
+            for (int c = 0; c < kLate; c++)
               if (i + c * kSplit < pieces) add(x[c], s.j.weight[h][i + c * kSplit]);
           }
           if constexpr (kSplit > 1) {
@@ -557,11 +553,8 @@ __global__ __launch_bounds__(256, kD == 64 ? 3 : 2) void k_attn_pages(AttnPagesA
   }
 }
 
-// workgroups of a kv head (and part of 16 query heads): as many as the registers let
-// 256 compute units hold at once
-static int attn_parts(int vheads, int head_dim) {
-  return std::max(1, std::min(kMaxParts, (head_dim == 64 ? 768 : 512) / vheads));
-}
+// workgroups of a kv head (and part of 16 query heads)
+static int attn_parts(int vheads) { return std::max(1, std::min(kMaxParts, kGroups / vheads)); }
 static int attn_columns(int group) { return group <= 4 ? 4 : group <= 8 ? 8 : 16; }
 
 template <int kD, bool kF8>
@@ -584,7 +577,7 @@ extern "C" int64_t cia_attn_pages_workspace_bytes(int n_q, int n_kv, int head_di
       n_q / n_kv > CIA_PAGES_MAX_GROUP)
     return 0;
   const int group = n_q / n_kv, vheads = n_kv * ((group + 15) / 16);
-  return kTicketBytes + (int64_t)vheads * attn_parts(vheads, head_dim) * 2 * attn_columns(group) * (head_dim + 2) * sizeof(float);
+  return kTicketBytes + (int64_t)vheads * attn_parts(vheads) * 2 * attn_columns(group) * (head_dim + 4) * sizeof(float);
 }
 
 extern "C" int cia_attn_pages(const cia_kv_pages* p, const uint16_t* q, int64_t q_stride, const int32_t* seq,
@@ -604,7 +597,7 @@ extern "C" int cia_attn_pages(const cia_kv_pages* p, const uint16_t* q, int64_t 
   CIA_REQUIRE(ws_bytes >= need, CIA_ERR_ARG);
   const int group = n_q / p->n_kv, cols = (group + 15) / 16;
   const AttnPagesArgs a{pages_of(p), q,    q_stride, seq,           pos,    T,   n_q,
-                        group,       cols, attn_parts(p->n_kv * cols, p->head_dim), scale * kLog2e, window, out,
+                        group,       cols, attn_parts(p->n_kv * cols), scale * kLog2e, window, out,
                         (uint32_t*)ws, (float*)((char*)ws + kTicketBytes)};
   hipStream_t s = (hipStream_t)stream;
   if (p->head_dim == 64) {
