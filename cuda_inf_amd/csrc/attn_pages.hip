@@ -27,7 +27,7 @@
 namespace cia {
 
 constexpr int kUnit = 128;        // tokens of a unit: 32 a wave
-constexpr int kRowCost = 3;       // units that a row's start and end take the time of
+constexpr int kRowCost = 2;       // units that a row's start and end take the time of
 constexpr int kGroups = 512;      // workgroups of a call, two a compute unit
 constexpr int kMaxParts = 256;    // of them for one kv head
 constexpr int kTicketStride = 16;  // uint32 between two counters
@@ -392,14 +392,23 @@ __global__ __launch_bounds__(256, 2) void k_attn_pages(AttnPagesArgs a) {
           }
         }
       };
-      Tile x0, x1;
-      load(x0, 0);
-      for (int i = 0; i < tiles; i += 2) {
-        if (i + 1 < tiles) load(x1, i + 1);
-        compute(x0, i);
-        if (i + 1 < tiles) {
-          if (i + 2 < tiles) load(x0, i + 2);
-          compute(x1, i + 1);
+      if constexpr (kRowB == 256) {
+        // (16 KiB of loads a wave: two tiles of them do not fit the registers beside O)
+        Tile x;
+        for (int i = 0; i < tiles; i++) {
+          load(x, i);
+          compute(x, i);
+        }
+      } else {
+        Tile x0, x1;
+        load(x0, 0);
+        for (int i = 0; i < tiles; i += 2) {
+          if (i + 1 < tiles) load(x1, i + 1);
+          compute(x0, i);
+          if (i + 1 < tiles) {
+            if (i + 2 < tiles) load(x0, i + 2);
+            compute(x1, i + 1);
+          }
         }
       }
     }

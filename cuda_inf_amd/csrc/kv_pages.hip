@@ -70,18 +70,20 @@ template <int kD, bool kF8, bool kWrite>
 __global__ __launch_bounds__(256) void k_pages_move(MoveArgs a) {
   constexpr int kLanes = kD / 8;
   const int t = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes, c = threadIdx.x % kLanes, head = blockIdx.y;
+  const bool here = t < a.T;
+  uint16_t* const k = a.k + (here ? t : 0) * a.k_stride + head * kD + 8 * c;
+  uint16_t* const v = a.v + (here ? t : 0) * a.v_stride + head * kD + 8 * c;
+  u32x4 kw{0, 0, 0, 0}, vw{0, 0, 0, 0};
+  if constexpr (kWrite) kw = *(const u32x4*)k, vw = *(const u32x4*)v;  // (before the place is known)
   int page = -1, pos = -1;
-  if (t < a.T) {
+  if (here) {
     pos = a.pos[t];
     const int s = a.seq ? a.seq[t] : t;
     if (s >= 0 && s < a.P.n_seq && pos >= 0 && pos < a.P.max_tokens) page = page_of(a.P, s, pos);
   }
   const bool live = page >= 0;
   const int64_t row = live ? page_row(a.P, page, head, pos) : 0;
-  uint16_t* const k = a.k + (live ? t : 0) * a.k_stride + head * kD + 8 * c;
-  uint16_t* const v = a.v + (live ? t : 0) * a.v_stride + head * kD + 8 * c;
   if constexpr (kWrite) {
-    const u32x4 kw = *(const u32x4*)k, vw = *(const u32x4*)v;
     if constexpr (kF8) {
       store_e4m3<kD>(kw, (uint8_t*)a.P.k, a.P.ks, row, c, live);
       store_e4m3<kD>(vw, (uint8_t*)a.P.v, a.P.vs, row, c, live);
@@ -92,15 +94,14 @@ __global__ __launch_bounds__(256) void k_pages_move(MoveArgs a) {
   } else if (live) {
     const int64_t at = row * kD + 8 * c;
     if constexpr (kF8) {
-      const u32x4 kw = load_e4m3((const uint8_t*)a.P.k, a.P.ks, at, row);
-      const u32x4 vw = load_e4m3((const uint8_t*)a.P.v, a.P.vs, at, row);
-      *(u32x4*)k = kw;
-      *(u32x4*)v = vw;
+      kw = load_e4m3((const uint8_t*)a.P.k, a.P.ks, at, row);
+      vw = load_e4m3((const uint8_t*)a.P.v, a.P.vs, at, row);
     } else {
-      const u32x4 kw = *(const u32x4*)((const uint16_t*)a.P.k + at);
-      *(u32x4*)v = *(const u32x4*)((const uint16_t*)a.P.v + at);
-      *(u32x4*)k = kw;
+      kw = *(const u32x4*)((const uint16_t*)a.P.k + at);
+      vw = *(const u32x4*)((const uint16_t*)a.P.v + at);
     }
+    *(u32x4*)k = kw;
+    *(u32x4*)v = vw;
   }
 }
 
