@@ -32,16 +32,20 @@ constexpr int kSmall = 256;  // tokens put in order by counting the larger ones
 constexpr int kAll = 1024;   // tokens put in order at all
 constexpr int kSub = kSampleThreads;  // parts of a bin that holds more than kSmall
 constexpr int kStep = 4 * kSampleThreads;  // logits of a step of k_sample_pick
-constexpr int kMinChunk = 4096;
-constexpr int kMaxChunk = 4 * kMinChunk;
+constexpr int kMinChunk = 8192;
+constexpr int kMaxChunk = 2 * kMinChunk;
+constexpr int kTop = 512;  // tokens of a smaller chunk that it puts out by themselves, at most
 constexpr int kMaxChunks = CIA_SAMPLE_MAX_VOCAB / kMaxChunk;  // 256
 constexpr int kCountShift = 49;  // of a chunk's bin: count << 49 | mass; 2^14 tokens of 2^34
 
-// of a chunk of a row; its bins follow the chunks of all rows
+// of a chunk of a row; its bins follow the chunks of all rows, and the tops of smaller
+// chunks those
 struct ChunkHead {
   double n;       // ceil of its largest x; -inf: no token, inf: logits of +inf
   float top;      // its largest logit
   uint32_t idx;   // the first token that has it
+  int depth;      // bins whose tokens are in its top
+  int listed;     // tokens of its top
 };
 
 struct SampleArgs {
@@ -58,6 +62,7 @@ struct SampleArgs {
   int chunk, chunks;  // logits of a chunk, chunks of a row
   ChunkHead* heads;   // [B][chunks]
   uint64_t* bins;     // [B][chunks][kBins]
+  uint64_t* tops;     // [B][chunks][kTop], of smaller chunks
 };
 
 // order-preserving bits of a number; -0 as 0
@@ -120,6 +125,8 @@ __device__ __forceinline__ double temperature_scale(float t) { return 16 * 1.442
 template <bool kHalf, int kThreads, int kVec>
 __global__ __launch_bounds__(kThreads) void k_sample_bins(SampleArgs a) {
   constexpr int kWaves = kThreads / 64, kEach = 4 * kThreads;
+  constexpr bool kTops = kVec * kEach == kMinChunk;
+  __shared__ int wcount[kWaves], depth, listed;
   __shared__ unsigned long long bins[kBins];
   __shared__ float wtop[kWaves];
   __shared__ uint32_t widx[kWaves];
@@ -171,12 +178,13 @@ __global__ __launch_bounds__(kThreads) void k_sample_bins(SampleArgs a) {
     __syncthreads();
     if (tid == 0) {
       for (int w = 0; w < kWaves; w++) idx = min(idx, widx[w]);
-      *head = ChunkHead{none ? -__builtin_inf() : 0.0, top, idx};
+      *head = ChunkHead{none ? -__builtin_inf() : 0.0, top, idx, kBins, 0};
     }
     return;
   }
   const bool inf = top == __builtin_inff();
   const double c = temperature_scale(t), R = inf ? 0.0 : __builtin_ceil(c * (double)top);
+  int bin[kTops ? kVec : 1][4];  // of each logit
 #pragma unroll
   for (int i = 0; i < kVec; i++)
 #pragma unroll
@@ -185,13 +193,56 @@ __global__ __launch_bounds__(kThreads) void k_sample_bins(SampleArgs a) {
       float l = x[i][e];
       if (inf) l = l == top ? 0.0f : -__builtin_inff();
       const double y = c * (double)l, n = __builtin_ceil(y), d = R - n;
-      if (d < (double)kBins)
-        atomicAdd(&bins[(int)d], (unsigned long long)bin_mass(y - n) + (1ull << kCountShift));
+      const bool has = d < (double)kBins;
+      if (has) atomicAdd(&bins[(int)d], (unsigned long long)bin_mass(y - n) + (1ull << kCountShift));
+      if constexpr (kTops) bin[i][e] = has ? (int)d : kBins;
     }
+  if (tid == 0) depth = 0, listed = 0;
   __syncthreads();
   uint64_t* const to = a.bins + ((int64_t)b * a.chunks + chunk) * kBins;
   for (int i = tid; i < kBins; i += kThreads) to[i] = bins[i];
-  if (tid == 0) *head = ChunkHead{inf ? __builtin_inf() : R, top, 0};
+  if constexpr (kTops) {
+    // as many of the first bins as hold no more than kTop tokens, two bins a thread
+    const int lane = tid & 63, wave = tid >> 6, i = min(2 * tid, kBins - 2);
+    const bool mine = 2 * tid < kBins;
+    const int k0 = mine ? (int)(bins[i] >> kCountShift) : 0, k1 = mine ? (int)(bins[i + 1] >> kCountShift) : 0;
+    int upto = k0 + k1;
+    for (int off = 1; off < 64; off <<= 1) {
+      const int o = __shfl_up(upto, off);
+      if (lane >= off) upto += o;
+    }
+    if (lane == 63) wcount[wave] = upto;
+    __syncthreads();
+    for (int w = 0; w < wave; w++) upto += wcount[w];
+    const uint64_t first = __ballot(mine && upto - k1 <= kTop), second = __ballot(mine && upto <= kTop);
+    if (lane == 0) atomicMax(&depth, first ? 2 * 64 * wave + __popcll(first) + __popcll(second) : 0);
+    __syncthreads();
+    uint64_t* const tops = a.tops + ((int64_t)b * a.chunks + chunk) * kTop;
+    const int d = depth;
+    uint64_t set[kVec][4];
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kVec; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        set[i][e] = __ballot(bin[i][e] < d);
+        n += __popcll(set[i][e]);
+      }
+    int at = 0;  // a place in the top for each of the wave's
+    if (lane == 0) at = atomicAdd(&listed, n);
+    at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+    for (int i = 0; i < kVec; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        if (bin[i][e] < d)
+          tops[at + __builtin_amdgcn_mbcnt_hi((uint32_t)(set[i][e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)set[i][e], 0))] =
+              (uint64_t)order_key(inf ? 0.0f : x[i][e]) << 32 | (uint32_t)~(i0 + kEach * i + e);
+        at += __popcll(set[i][e]);
+      }
+    __syncthreads();
+  }
+  if (tid == 0) *head = ChunkHead{inf ? __builtin_inf() : R, top, 0, depth, listed};
 }
 
 // ---------------------------------------------------------------- the choice
@@ -216,10 +267,11 @@ struct SampleLds {
   int count[kBins + 1];      // tokens of the bins before
   double shift[kMaxChunks];  // of a chunk's bins; kBins or more: none of them counts
   int use[kMaxChunks];       // chunks to take tokens from
+  int listed[kMaxChunks];    // tokens of a chunk's top
   double dsum[kSampleWaves];
   uint64_t key[kSampleWaves];
   uint32_t lo[kSampleWaves], hi[kSampleWaves];
-  int n, m, at, bin, last;
+  int n, m, at, bin, last, covered;
   Ends ends;
 };
 
@@ -276,12 +328,12 @@ struct SampleRow {
 
   // The row's largest logit, key << 32 | ~index, and the first of its chunks' bins on
   // their way.
-  static constexpr int kFirst = 12;  // bins of a thread: 9 small chunks at once, or all 8 of 131072 logits
+  static constexpr int kFirst = 12;  // bins of a thread: those of 9 chunks
   __device__ __forceinline__ uint64_t largest(uint64_t (&first)[kFirst]) {
 #pragma unroll
     for (int i = 0; i < kFirst; i++) first[i] = bins[min(i * kSampleThreads + tid, a.chunks * kBins - 1)];
     for (int i = tid; i < kBins; i += kSampleThreads) s.mass[i] = 0, s.cnt[i] = 0;
-    if (tid == 0) s.last = 0;
+    if (tid == 0) s.last = 0, s.covered = kBins;
     uint64_t best = 0;
     for (int i = tid; i < a.chunks; i += kSampleThreads) {
       const ChunkHead h = heads[i];
@@ -290,6 +342,8 @@ struct SampleRow {
         best = k > best ? k : best;
       }
       s.shift[i] = h.n;
+      s.use[i] = h.depth;
+      s.listed[i] = h.listed;
     }
     for (int off = 32; off; off >>= 1) {
       const uint64_t o = __shfl_xor((unsigned long long)best, off);
@@ -306,6 +360,7 @@ struct SampleRow {
     for (int i = tid; i < a.chunks; i += kSampleThreads) {
       const double n = s.shift[i];
       s.shift[i] = inf ? (n == __builtin_inf() ? 0.0 : (double)kBins) : fmin(R - n, (double)kBins);
+      atomicMin(&s.covered, (int)s.shift[i] + s.use[i]);
     }
     __syncthreads();
     const int all = a.chunks * kBins;
@@ -494,6 +549,21 @@ struct SampleRow {
       if (n < kAll) s.some[n] = (uint64_t)k << 32 | (uint32_t)~index_of(s.nth[i][tid]);
     }
     least_most(least, most);
+    return s.m;
+  }
+
+  // The tokens of the chunks' tops with keys from lo on into s.some: how many.
+  __device__ __forceinline__ int select_tops(const uint64_t* tops, uint32_t lo) {
+    __syncthreads();
+    if (tid == 0) s.m = 0;
+    __syncthreads();
+    const int all = a.chunks * kTop;
+#pragma unroll 8
+    for (int i = tid; i < all; i += kSampleThreads) {
+      const uint64_t v = i % kTop < s.listed[i / kTop] ? tops[i] : 0;
+      if ((uint32_t)(v >> 32) >= lo) s.some[atomicAdd(&s.m, 1)] = v;
+    }
+    __syncthreads();
     return s.m;
   }
 
@@ -803,7 +873,8 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
     if (w.n > 1) tokens += s.count[f1 + 1] - s.count[f0];
     listed = tokens <= kCap;
   }
-  if (listed) {
+  const bool tops = kPer * kStep == kMinChunk && few && last < s.covered;  // they are at hand
+  if (listed && !tops) {
     uint32_t lo[kRanges], hi[kRanges];
     r.keys_of(w.from[0], w.to[0], lo[0], hi[0]);
     lo[1] = lo[0], hi[1] = hi[0];
@@ -814,7 +885,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
   if (few) {
     // every prefix among them, in order
     uint32_t lo, hi;
-    const int n = r.select(0, ~0u, lo, hi);
+    const int n = tops ? r.select_tops(a.tops + (int64_t)b * a.chunks * kTop, r.first_key(last)) : r.select(0, ~0u, lo, hi);
     r.order(s.some, n);
     r.sums(n, 0.0);
     if (by_k && k <= n) kept = s.run[k - 1];
@@ -854,10 +925,11 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
   }
 }
 
-// Chunks of 16384 logits where that makes two workgroups a compute unit, or a row more than 64
-// of the smaller ones; else of 4096.
+// Chunks of 16384 logits where that makes two workgroups a compute unit, or a row more than 32
+// of the smaller ones; else of 8192, with their tops: of the largest tokens the choice
+// mostly falls on, the row need not be read again.
 static int sample_chunk(int B, int V) {
-  return (int64_t)B * ((V + kMaxChunk - 1) / kMaxChunk) >= 512 || V > 64 * kMinChunk ? kMaxChunk : kMinChunk;
+  return (int64_t)B * ((V + kMaxChunk - 1) / kMaxChunk) >= 512 || V > 32 * kMinChunk ? kMaxChunk : kMinChunk;
 }
 
 }  // namespace cia
@@ -870,14 +942,14 @@ extern "C" int64_t cia_sample_workspace_bytes(int B, int V) {
   const int64_t big = (V + kMaxChunk - 1) / kMaxChunk, small = (V + kMinChunk - 1) / kMinChunk;
   int64_t n = (int64_t)B * (sample_chunk(B, V) == kMinChunk ? small : big);
   if (sample_chunk(1, V) == kMinChunk) n = std::max(n, std::min<int64_t>(B, 511 / big) * small);
-  return 16 + n * (int64_t)(sizeof(ChunkHead) + kBins * sizeof(uint64_t));
+  return 16 + n * (int64_t)(sizeof(ChunkHead) + (kBins + kTop) * sizeof(uint64_t));
 }
 
 template <bool kHalf>
 static int sample_launch(const SampleArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)(a.B * a.chunks));
   if (a.chunk == kMinChunk)
-    hipLaunchKernelGGL((k_sample_bins<kHalf, 256, kMinChunk / 1024>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_sample_bins<kHalf, 512, kMinChunk / 2048>), grid, dim3(512), 0, s, a);
   else
     hipLaunchKernelGGL((k_sample_bins<kHalf, 512, kMaxChunk / 2048>), grid, dim3(512), 0, s, a);
   const int st = launch_status();
@@ -903,8 +975,9 @@ extern "C" int cia_sample(const void* logits, int type, int64_t stride, const fl
   CIA_REQUIRE(ws_bytes >= need, CIA_ERR_ARG);
   const int chunk = sample_chunk(B, V), chunks = (V + chunk - 1) / chunk;
   ChunkHead* const heads = (ChunkHead*)ws;
+  uint64_t* const bins = (uint64_t*)(heads + (int64_t)B * chunks);
   const SampleArgs a{logits, stride, temperature, top_k, top_p, min_p, u, ids, p, B, V, chunk, chunks, heads,
-                     (uint64_t*)(heads + (int64_t)B * chunks)};
+                     bins, bins + (int64_t)B * chunks * kBins};
   return type == CIA_LOGITS_F16 ? sample_launch<true>(a, (hipStream_t)stream)
                                 : sample_launch<false>(a, (hipStream_t)stream);
 }
