@@ -937,7 +937,8 @@ static int sample_chunk(int B, int V) {
 using namespace cia;
 
 extern "C" int64_t cia_sample_workspace_bytes(int B, int V) {
-  if (B < 0 || B > CIA_SAMPLE_MAX_ROWS || V < 1 || V > CIA_SAMPLE_MAX_VOCAB) return 0;
+  if (B < 0 || B > CIA_SAMPLE_MAX_ROWS || V < 1 || V > CIA_SAMPLE_MAX_VOCAB || (int64_t)B * V > CIA_SAMPLE_MAX_LOGITS)
+    return 0;
   // (the most that B rows or fewer need: a smaller batch may have smaller chunks)
   const int64_t big = (V + kMaxChunk - 1) / kMaxChunk, small = (V + kMinChunk - 1) / kMinChunk;
   int64_t n = (int64_t)B * (sample_chunk(B, V) == kMinChunk ? small : big);

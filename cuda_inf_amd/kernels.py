@@ -455,8 +455,14 @@ def _rows(t, name: str, heads: int, dim: int, T: int, dev: int):
                      f"on cuda:{dev}")
 
 
+def _tokens(pos) -> int:
+    if not isinstance(pos, torch.Tensor):
+        raise TypeError(f"pos: expected a torch.Tensor, got {type(pos).__name__}")
+    return pos.numel()
+
+
 def _move(fn: str, pages: KvPages, k, v, pos, seq) -> None:
-    T, dev = pos.numel(), pages._device
+    T, dev = _tokens(pos), pages._device
     kp, ks = _rows(k, "k", pages.n_kv, pages.head_dim, T, dev)
     vp, vs = _rows(v, "v", pages.n_kv, pages.head_dim, T, dev)
     call(fn, pages._ref, kp, ks, vp, vs, None if seq is None else _at(seq, "seq", _I32, T, dev),
@@ -498,8 +504,8 @@ def attn_pages(pages: KvPages, q, out, pos, ws, seq=None, scale: float = 0.125, 
     [T]; None: row t is sequence t's), into out fp16 [T, query heads, dim]; all tokens
     up to pos, the last ``window`` of them if window > 0.  Rows with none (pos -1) are
     0.  Calls sharing ws must be ordered on one stream."""
-    T, dev = pos.numel(), pages._device
-    n_q = q.shape[1]
+    T, dev = _tokens(pos), pages._device
+    n_q = q.shape[1] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0
     qp, qs = _rows(q, "q", n_q, pages.head_dim, T, dev)
     call("cia_attn_pages", pages._ref, qp, qs, None if seq is None else _at(seq, "seq", _I32, T, dev),
          _at(pos, "pos", _I32, T, dev), T, n_q, scale, window,

@@ -15,8 +15,9 @@ import torch
 from . import _lib
 from ._lib import (D, KVGROUP, NH, NKV, NSPLIT_DEFAULT, call, cia_append_op, cia_attn_proj,
                    cia_layer, cia_moe)
-from .kernels import (_stream_on, decode_workspace_bytes, h2o_workspace_bytes, moe_gating,
-                      q4_experts, stream_handle)
+from .kernels import (KvPages, _stream_on, attn_pages, decode_workspace_bytes, h2o_workspace_bytes,
+                      kv_pages_read, kv_pages_write, moe_gating, new_attn_pages_workspace, q4_experts,
+                      stream_handle)
 
 HIDDEN = _lib.HIDDEN
 
@@ -277,3 +278,88 @@ class MoeBlock:
         if h.device != self.ws.device:
             raise ValueError(f"h is on {h.device}, the layer on {self.ws.device}")
         call("cia_moe_block_forward", ctypes.byref(self._m), h.data_ptr(), S, _stream_on(h.get_device()))
+
+
+# ------------------------------------------------------------ many sequences
+class PageTable:
+    """Which pages hold the tokens of each of ``max_seqs`` sequences: token ``pos`` of
+    sequence ``s`` lies in page ``table[s, pos // page]``, -1 where it has none.  The
+    layers of a model share one: ``n_pages`` pages of ``page`` tokens in each of them,
+    given out and taken back on the host."""
+
+    def __init__(self, max_seqs: int, max_tokens: int, n_pages: int, *, page: int = 64, device="cuda"):
+        self.page, self.n_pages = page, n_pages
+        width = -(-max_tokens // page)
+        self.table = torch.full((max_seqs, width), -1, dtype=torch.int32, device=device)
+        self._held = [[] for _ in range(max_seqs)]
+        self._free = list(range(n_pages - 1, -1, -1))
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def reserve(self, seq: int, tokens: int) -> None:
+        """Pages for the first ``tokens`` tokens of a sequence, those it has among them.
+        Raises RuntimeError, with nothing changed, where not enough are free."""
+        if not 0 <= seq < len(self._held):
+            raise ValueError(f"seq={seq}: the table has {len(self._held)} sequences")
+        held = self._held[seq]
+        need = -(-tokens // self.page) - len(held)
+        if need <= 0:
+            return
+        if len(held) + need > self.table.shape[1]:
+            raise ValueError(f"tokens={tokens}: a sequence holds {self.table.shape[1] * self.page}")
+        if need > len(self._free):
+            raise RuntimeError(f"{need} pages needed, {len(self._free)} free")
+        new = [self._free.pop() for _ in range(need)]
+        self.table[seq, len(held):len(held) + need] = torch.tensor(new, dtype=torch.int32, device=self.table.device)
+        held += new
+
+    def release(self, seq: int) -> None:
+        """A sequence's pages back; its row of the table is -1.  Work that still reads
+        them has to lie before what writes them next (the same stream, or events)."""
+        if not 0 <= seq < len(self._held):
+            raise ValueError(f"seq={seq}: the table has {len(self._held)} sequences")
+        self._free += reversed(self._held[seq])
+        self._held[seq] = []
+        self.table[seq] = -1
+
+
+class PagedAttn:
+    """Attention of one layer for a batch of sequences, over pages that ``table`` gives
+    out: e4m3 with an fp16 scale per token and kv head (engine.cu:317-333), or fp16
+    with ``quant=False``.  ``scale``: of the scores, 1 / sqrt(head_dim) if None;
+    ``window``: tokens attended to, 0 for all.  Positions are int32 device tensors, -1
+    for an empty place of a batch; ``seq`` is the tokens' sequences, None: token t is
+    sequence t's.  Calls of one layer must be ordered on one stream."""
+
+    def __init__(self, table: PageTable, *, n_q: int = NH, n_kv: int = NKV, head_dim: int = D, quant: bool = True,
+                 scale=None, window: int = 0):
+        dev, shape = table.table.device, (table.n_pages, n_kv, table.page, head_dim)
+        new = lambda shape, dtype: torch.zeros(shape, dtype=dtype, device=dev)  # noqa: E731
+        kv = [new(shape, torch.uint8 if quant else torch.float16) for _ in range(2)]
+        scales = [new(shape[:3], torch.float16) for _ in range(2)] if quant else [None, None]
+        self.table = table
+        self.pages = KvPages(*kv, table.table, *scales)
+        self.ws = new_attn_pages_workspace(self.pages, n_q)
+        self.scale, self.window = head_dim ** -0.5 if scale is None else float(scale), window
+
+    def write(self, k, v, pos, seq=None) -> None:
+        """k, v fp16 [T, kv heads, dim] to their places."""
+        kv_pages_write(self.pages, k, v, pos, seq=seq)
+
+    def read(self, k, v, pos, seq=None) -> None:
+        """Rows of k, v fp16 [T, kv heads, dim] from their places."""
+        kv_pages_read(self.pages, k, v, pos, seq=seq)
+
+    def attend(self, q, pos, seq=None, out=None):
+        """out fp16 [T, query heads, dim] of q over its sequences' tokens up to pos."""
+        if out is None:
+            out = torch.empty(q.shape, dtype=torch.float16, device=q.device)
+        attn_pages(self.pages, q, out, pos, self.ws, seq=seq, scale=self.scale, window=self.window)
+        return out
+
+    def decode(self, q, k, v, pos, seq=None, out=None):
+        """One token of each sequence: its k and v written, then q attended."""
+        self.write(k, v, pos, seq=seq)
+        return self.attend(q, pos, seq=seq, out=out)

@@ -34,6 +34,7 @@ extern "C" {
 #define CIA_PAGES_MAX_ROWS 4096        /* rows of an attention call */
 #define CIA_SAMPLE_MAX_ROWS (1 << 16)
 #define CIA_SAMPLE_MAX_VOCAB (1 << 22)
+#define CIA_SAMPLE_MAX_LOGITS ((int64_t)1 << 34) /* B * V */
 
 /* One layer's cache for many sequences.  Token `pos` of sequence `s` is row
  * pos % page of page table[s * table_stride + pos / page].  A token has no
@@ -128,7 +129,8 @@ int64_t cia_attn_pages_workspace_bytes(int n_q, int n_kv, int head_dim);
  * logits aligned to their type, ws to 16 bytes; ws_bytes at least
  * cia_sample_workspace_bytes(B, V); ws holds nothing between calls; calls that
  * share one must be ordered, captured graphs included.  B at most
- * CIA_SAMPLE_MAX_ROWS, V from 1 to CIA_SAMPLE_MAX_VOCAB. */
+ * CIA_SAMPLE_MAX_ROWS, V from 1 to CIA_SAMPLE_MAX_VOCAB, B * V at most
+ * CIA_SAMPLE_MAX_LOGITS. */
 int cia_sample(const void* logits, int type, int64_t stride,
                const float* temperature, const int32_t* top_k,
                const float* top_p, const float* min_p, const float* u,

@@ -115,7 +115,7 @@ def test_sample_refusals(L):
                 ws=A, ws_bytes=n)
     f = lambda **kw: L.cia_sample(*{**good, **kw}.values(), None)  # noqa: E731
     for kw in (dict(type=2), dict(type=-1), dict(stride=99), dict(stride=-100), dict(B=-1), dict(B=(1 << 16) + 1),
-               dict(V=0), dict(V=-1), dict(V=(1 << 22) + 1, stride=1 << 23), dict(ws_bytes=n - 1)):
+               dict(V=0), dict(V=-1), dict(B=1 << 16, V=(1 << 18) + 1, stride=1 << 20), dict(V=(1 << 22) + 1, stride=1 << 23), dict(ws_bytes=n - 1)):
         assert f(**kw) == ARG, kw
     for kw in (dict(logits=None), dict(u=None), dict(ids=None), dict(ws=None)):
         assert f(**kw) == NULL, kw
@@ -128,7 +128,8 @@ def test_sample_refusals(L):
 def test_sample_workspace(L):
     f = L.cia_sample_workspace_bytes
     assert f(-1, 10) == f(1, 0) == f((1 << 16) + 1, 10) == f(1, (1 << 22) + 1) == 0
-    assert f(1, 1) > 0 and f(1 << 16, 1 << 22) >= f(1 << 10, 1 << 22) >= f(1, 1 << 22) > 0
+    assert f(1, 1) > 0 and f(1 << 12, 1 << 22) >= f(1 << 10, 1 << 22) >= f(1, 1 << 22) > 0 and f(1 << 16, 1 << 18) > 0
+    assert f((1 << 12) + 1, 1 << 22) == f(1 << 16, (1 << 18) + 1) == 0  # (more than 2^34 logits)
     # (a smaller batch of the same rows fits what a larger one was given)
     for V in (1, 17, 4096, 16385, 65536, 131073):
         last = 0
@@ -199,6 +200,80 @@ def test_wrapper_checks(cia, monkeypatch):
         K._rows(None, "k", 2, 64, 3, 0)
     with pytest.raises(ValueError, match="beyond what a call takes"):
         K.new_attn_pages_workspace(P, 3)
+
+
+def test_more_wrapper_checks(cia):
+    import torch
+
+    from cuda_inf_amd import kernels as K
+
+    class On(torch.Tensor):
+        is_cuda = True
+
+        def get_device(self):
+            return 0
+
+    k = torch.zeros((4, 2, 16, 64), dtype=torch.float16).as_subclass(On)
+    P = K.KvPages(k, k, torch.zeros((3, 5), dtype=torch.int32).as_subclass(On))
+    pos, row = torch.zeros(2, dtype=torch.int32).as_subclass(On), torch.zeros((2, 2, 64), dtype=torch.float16).as_subclass(On)
+    for f in (K.kv_pages_write, K.kv_pages_read):
+        with pytest.raises(TypeError, match="pos: expected"):
+            f(P, row, row, None)
+        with pytest.raises(TypeError, match="pos: dtype"):
+            f(P, row, row, pos.long())
+        with pytest.raises(ValueError, match="v: "):
+            f(P, row, row[:1], pos)
+        with pytest.raises(ValueError, match="seq: needs at least 2"):
+            f(P, row, row, pos, seq=pos[:1])
+        with pytest.raises(ValueError, match="pos: must be a device tensor"):
+            f(P, row, row, torch.zeros(2, dtype=torch.int32))
+    q = torch.zeros((2, 4, 64), dtype=torch.float16).as_subclass(On)
+    ws = torch.zeros(8, dtype=torch.uint8).as_subclass(On)
+    for bad in (None, q[0], q[:, :, :32], q[:1]):
+        with pytest.raises((TypeError, ValueError), match="q: "):
+            K.attn_pages(P, bad, q, pos, ws)
+    with pytest.raises(ValueError, match="out: needs at least"):
+        K.attn_pages(P, q, q[:1], pos, ws)
+    with pytest.raises(TypeError, match="ws: dtype"):
+        K.attn_pages(P, q, q, pos, q)
+    l, f = torch.zeros((2, 8)).as_subclass(On), torch.zeros(2).as_subclass(On)
+    with pytest.raises(TypeError, match="u: dtype"):
+        K.sample(l, f.half(), pos, ws)
+    with pytest.raises(TypeError, match="top_k: dtype"):
+        K.sample(l, f, pos, ws, top_k=f)
+    with pytest.raises(ValueError, match="top_p: needs at least 2"):
+        K.sample(l, f, pos, ws, top_p=f[:1])
+    with pytest.raises(ValueError, match="logits: need a device tensor"):
+        K.sample(l.t(), f, pos, ws)
+
+
+def test_page_table(cia):
+    from cuda_inf_amd.layer import PageTable
+    t = PageTable(3, 100, 8, page=16, device="cpu")
+    assert t.table.shape == (3, 7) and (t.table == -1).all() and t.free_pages == 8
+    t.reserve(0, 17)
+    t.reserve(1, 0)
+    t.reserve(2, 64)
+    assert t.free_pages == 2
+    got = t.table.tolist()
+    assert got[1] == [-1] * 7 and got[0][2:] == [-1] * 5 and got[2][4:] == [-1] * 3
+    assert sorted(got[0][:2] + got[2][:4]) == [0, 1, 2, 3, 4, 5]
+    t.reserve(0, 20)  # (what it has already)
+    assert t.table.tolist() == got
+    with pytest.raises(RuntimeError, match="3 pages needed, 2 free"):
+        t.reserve(1, 33)
+    with pytest.raises(ValueError, match="a sequence holds 112"):
+        t.reserve(0, 113)
+    for seq in (-1, 3):
+        with pytest.raises(ValueError, match="the table has 3"):
+            t.reserve(seq, 1)
+        with pytest.raises(ValueError, match="the table has 3"):
+            t.release(seq)
+    assert t.table.tolist() == got and t.free_pages == 2
+    t.release(2)
+    assert t.free_pages == 6 and (t.table[2] == -1).all()
+    t.reserve(1, 96)
+    assert t.free_pages == 0 and len(set(t.table[1, :6].tolist() + got[0][:2])) == 8
 
 
 def test_choice_oracle():

@@ -254,6 +254,32 @@ def test_attention_of_many_rows(K, orc, dev, T):
     check(K, c, dev, q, seq, pos, 0.125, 0, what=f"{T} rows")
 
 
+@pytest.mark.parametrize("n_q,n_kv,D,quant", [(128 * 64, 128, 64, True), (128, 128, 128, False), (64 * 5, 5, 64, True),
+                                              (33 * 7, 7, 128, True)])
+def test_attention_of_many_heads(K, orc, dev, n_q, n_kv, D, quant):
+    """Heads at their limits: one workgroup for a kv head and 16 query heads, parts of 16 that are not full."""
+    rng = np.random.default_rng(n_q)
+    lens = [200, 1, 0, 777]
+    c = Cache(K, orc, dev, rng, lens, n_kv, D, 32, quant)
+    q = rng.standard_normal((4, n_q, D)).astype(np.float16)
+    check(K, c, dev, q, None, np.array(lens, np.int32) - 1, D ** -0.5, 0, what="heads")
+
+
+def test_attention_of_the_most_rows_of_wide_heads(K, orc, dev):
+    """4096 rows whose list and joins take the most of a workgroup's LDS."""
+    rng = np.random.default_rng(77)
+    lens = [700, 90]
+    c = Cache(K, orc, dev, rng, lens, 1, 128, 64, False)
+    seq = rng.integers(0, 2, 4096).astype(np.int32)
+    pos = np.where(seq == 0, rng.integers(-1, 700, 4096), rng.integers(-1, 90, 4096)).astype(np.int32)
+    q = rng.standard_normal((4096, 16, 128)).astype(np.float16)
+    out = attend(K, c, dev, q, seq, pos, 0.09, 130)
+    some = np.r_[0:40, 2000:2040, 4056:4096]
+    want, bound = ref.attend(q[some], c.num["k"], c.num["v"], c.table, 64, seq[some], pos[some], 0.09, 130)
+    within(out.cpu().numpy()[some], want, bound, "rows")
+    assert not out.isnan().any() and (out[torch.from_numpy(pos < 0)] == 0).all()
+
+
 @pytest.mark.parametrize("quant", [True, False])
 def test_attention_values(K, orc, dev, quant):
     """Scores far apart and far from zero, all alike, scales of a few steps of fp16's least, rows of zeros."""
@@ -439,6 +465,98 @@ def test_sample_frequencies(K, dev):
     assert (np.abs(np.bincount(ids, minlength=11) - 5000 * w / w.sum()) <= 1).all()
 
 
+@pytest.mark.parametrize("B,V", [(3, 8191), (3, 8192), (3, 8193), (2, 262144), (2, 262145), (70, 65536), (300, 20001),
+                                 (520, 16384), (600, 3)])
+@pytest.mark.parametrize("half", [False, True])
+def test_sample_about_a_chunks_edge(K, dev, B, V, half):
+    """Rows of one chunk and of many, of both sizes, one more logit and one less, batches on both sides of the
+    choice between them; rows in descending and ascending order, whose largest tokens all lie in one chunk."""
+    rng = np.random.default_rng(B + V)
+    n = min(B, 6)
+    l = np.zeros((B, V), np.float16 if half else np.float32)
+    l[:] = (2 * rng.standard_normal((n, V)))[np.arange(B) % n]
+    l[0] = np.sort(l[0])
+    l[1] = np.sort(l[1])[::-1]
+    l[2 % B, V // 2:] = -np.inf
+    check = np.unique(np.r_[0:n, rng.integers(0, B, 3), B - 1])
+    x = t(l, dev)
+    for f in (dict(top_k=30), dict(top_k=800, top_p=0.95), dict(top_p=0.6), dict(min_p=0.2), dict(), dict(temperature=0.0)):
+        u = rng.random(B).astype(np.float32)
+        f = {k: np.full(B, v, np.int32 if k == "top_k" else np.float32) for k, v in f.items()}
+        ids, p = sample(K, dev, x, u, **f)
+        want, q, near = ref.choose(l[check], u[check], **{k: v[check] for k, v in f.items()})
+        sure = near > 1e-9
+        assert sure.mean() > 0.6 and np.array_equal(ids[check][sure], want[sure]), f
+        within(p[check][sure], q[sure], q[sure] * (ref.U24 + 1e-9), f"{f}")
+
+
+@pytest.mark.parametrize("V", [1, 8, 1000, 70000, 140000])
+def test_sample_at_the_border_between_equals(K, dev, V):
+    """Sums of equals are whole: a number on the border between two of them draws the second."""
+    at = np.unique(np.minimum(V - 1, np.array([0, 1, 2, V // 8, V // 4, V // 2, V - 1])))
+    u = (at / V).astype(np.float32)
+    keep = (u.astype(np.float64) * V == at)  # those that fp32 holds
+    at, u = at[keep], u[keep]
+    assert at.size
+    for level, temp in ((0.3, 1.0), (-7.25, 0.7), (1e4, 1.3)):
+        l = np.full((at.size, V), level, np.float32)
+        ids, p = sample(K, dev, l, u, temperature=np.full(at.size, temp))
+        assert np.array_equal(ids, at)
+        assert (p == np.float32(1 / V)).all()
+
+
+def test_calls_of_other_sizes_on_the_same_workspaces(K, orc, dev):
+    """A workspace that a larger call has filled, and one whose contents are anything."""
+    rng = np.random.default_rng(2)
+    l = (2 * rng.standard_normal((40, 30000))).astype(np.float32)
+    x, u = t(l, dev), rng.random(40).astype(np.float32)
+    ws = torch.full((K.sample_workspace_bytes(40, 30000),), 0xFF, dtype=torch.uint8, device=dev)
+    ids = torch.zeros(40, dtype=torch.int32, device=dev)
+    tp = torch.full((40,), 0.8, device=dev)
+    for B, V in ((40, 30000), (3, 29999), (40, 100), (1, 30000), (40, 30000)):
+        K.sample(x[:B, :V], t(u, dev), ids, ws, top_p=tp)
+        want, _, near = ref.choose(l[:B, :V], u[:B], top_p=np.full(B, 0.8, np.float32))
+        assert near.min() > 1e-9 and np.array_equal(ids[:B].cpu().numpy(), want)
+    lens = [3000, 5, 600]
+    c = Cache(K, orc, dev, rng, lens, 2, 64, 16, True)
+    ws = torch.zeros(max(K.attn_pages_workspace_bytes(n, 2, 64) for n in (2, 8, 32)), dtype=torch.uint8, device=dev)
+    for n_q, rows in ((32, 3), (2, 1), (8, 3), (32, 2), (2, 3)):
+        q = rng.standard_normal((rows, n_q, 64)).astype(np.float16)
+        check(K, c, dev, q, None, np.array(lens[:rows], np.int32) - 1, 0.125, 0, ws, f"{n_q} heads")
+
+
+def test_two_streams_at_once(K, orc, dev):
+    """The same calls on two streams, each with its workspaces, one cache between them."""
+    rng = np.random.default_rng(14)
+    lens = [5000, 900, 20]
+    c = Cache(K, orc, dev, rng, lens, 2, 64, 64, True)
+    pos = t(np.array(lens, np.int32) - 1, dev)
+    q = [t((2 * rng.standard_normal((3, 8, 64))).astype(np.float16), dev) for _ in range(2)]
+    l = [t((2 * rng.standard_normal((3, 50000))).astype(np.float32), dev) for _ in range(2)]
+    u = t(rng.random(3).astype(np.float32), dev)
+    ws = [(K.new_attn_pages_workspace(c.P, 8), torch.empty(K.sample_workspace_bytes(3, 50000), dtype=torch.uint8, device=dev))
+          for _ in range(2)]
+    tp = torch.full((3,), 0.9, device=dev)
+
+    def run(i):
+        out, ids = torch.empty_like(q[i]), torch.empty(3, dtype=torch.int32, device=dev)
+        for _ in range(10):
+            K.attn_pages(c.P, q[i], out, pos, ws[i][0])
+            K.sample(l[i], u, ids, ws[i][1], top_p=tp)
+        return out, ids
+
+    alone = [run(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    both = []
+    for i, s in enumerate(streams):
+        with torch.cuda.stream(s):
+            both.append(run(i))
+    torch.cuda.synchronize()
+    for a, b in zip(alone, both):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
 # ------------------------------------------------------------------ together, streams, graphs
 def test_on_another_stream_and_captured(K, orc, dev):
     """Write, attention and sampling captured on a fresh stream, replayed with other inputs and eager work
@@ -506,3 +624,97 @@ def test_on_another_stream_and_captured(K, orc, dev):
     side.synchronize()
     for a, b in zip(eager[4], (out, ids, p)):
         assert torch.equal(a, b)
+
+
+def int4(rng, rows, cols, dev):
+    packed = rng.integers(0, 256, (rows, cols // 2), dtype=np.uint8)
+    scales = ((0.5 + rng.random((rows, cols // 128))) * 0.35 / np.sqrt(cols)).astype(np.float16)
+    return t(packed, dev), t(scales, dev)
+
+
+@pytest.mark.parametrize("quant", [True, False])
+def test_a_batch_decodes(K, orc, dev, quant):
+    """The decode loop of a batch: embedding rows, and in each of two layers norm, q/k/v, producers, pages, attention,
+    out_proj and the dense branch; then logits and a token each, which is the next step's.  Sequences of
+    several lengths, one that ends and one that begins on the way.  Each step's attention and tokens are those of the
+    plain forms on the step's own cache, queries and logits."""
+    from cuda_inf_amd.layer import MoeBlock, PagedAttn, PageTable
+    rng = np.random.default_rng(21)
+    H, V, B, steps = 2048, 1000, 5, 6
+    table = PageTable(B, 400, 12, page=64, device=dev)
+    layers = []
+    for _ in range(2):
+        w = dict(norm=t((1 + 0.1 * rng.standard_normal(H)).astype(np.float16), dev),
+                 q=int4(rng, 2048, H, dev), k=int4(rng, 512, H, dev), v=int4(rng, 512, H, dev), o=int4(rng, H, 2048, dev),
+                 qw=t((1 + 0.1 * rng.standard_normal(64)).astype(np.float16), dev),
+                 kw=t((1 + 0.1 * rng.standard_normal(64)).astype(np.float16), dev))
+        ffn = [int4(rng, *s, dev) for s in ((512, H), (512, H), (H, 512))]
+        w["ffn"] = MoeBlock(w["norm"], *[(p[None], s[None]) for p, s in ffn], max_batch=B, device=dev)
+        w["attn"] = PagedAttn(table, quant=quant)
+        layers.append(w)
+    head, embed = int4(rng, V, H, dev), t(rng.standard_normal((V, H)).astype(np.float32), dev)
+    lens = [100, 3, 64, 0, 300]
+    for s, n in enumerate(lens):
+        if not n:
+            continue
+        table.reserve(s, n + steps)
+        at = torch.arange(n, dtype=torch.int32, device=dev)
+        for w in layers:
+            w["attn"].write(*(t(rng.standard_normal((n, 8, 64)).astype(np.float16), dev) for _ in range(2)), at,
+                            seq=torch.full_like(at, s))
+    assert table.free_pages == 12 - 2 - 1 - 2 - 5
+    with pytest.raises(RuntimeError, match="pages needed"):
+        table.reserve(3, 400)
+    pos = torch.tensor(lens, dtype=torch.int32, device=dev)
+    pos[3] = -1
+    ids = torch.zeros(B, dtype=torch.int32, device=dev)
+    p, u = torch.zeros(B, device=dev), torch.zeros(B, device=dev)
+    ws = torch.empty(K.sample_workspace_bytes(B, V), dtype=torch.uint8, device=dev)
+    f = dict(temperature=np.array([0.7, 0.0, 1.2, 1.0, 0.9], np.float32), top_k=np.array([40, 0, 0, 5, 0], np.int32),
+             top_p=np.array([0.9, 1, 0.95, 1, 1], np.float32), min_p=np.array([0, 0, 0.02, 0, 0.1], np.float32))
+    fd = {k: t(v, dev) for k, v in f.items()}
+    x = torch.zeros((B, H), dtype=torch.float16, device=dev)
+    q = torch.zeros((B, 32, 64), dtype=torch.float16, device=dev)
+    k, v, out = torch.zeros((B, 8, 64), dtype=torch.float16, device=dev), torch.zeros((B, 8, 64), dtype=torch.float16, device=dev), torch.zeros_like(q)
+    logits = torch.zeros((B, V), device=dev)
+    codes = orc.e4m3_decode_table().astype(np.float64)
+    for step in range(steps):
+        if step == 3:
+            table.release(4)
+            pos[4] = -1
+            table.reserve(3, steps)
+            pos[3] = 0
+        h = embed[ids.long()].clone()
+        for w in layers:
+            K.add_rmsnorm(h, w["norm"], x, B, H)
+            K.qkv_proj_int4(x, w["q"], w["k"], w["v"], q, k, v, B)
+            K.qk_norm_rope(q, k, w["qw"], w["kw"], pos.clamp(min=0), B)
+            w["attn"].decode(q, k, v, pos, out=out)
+            P = w["attn"].pages
+            num = [codes[c.cpu().numpy()] * s.cpu().numpy().astype(np.float64)[..., None] if quant else c.cpu().numpy()
+                   for c, s in ((P.k, P.ks), (P.v, P.vs))]
+            want, bound = ref.attend(q.cpu().numpy(), *num, table.table.cpu().numpy(), 64, np.arange(B), pos.cpu().numpy(), 0.125, 0)
+            within(out.cpu().numpy(), want, bound, f"step {step}")
+            back = [torch.full_like(k, 9.0) for _ in range(2)]
+            w["attn"].read(*back, pos)
+            live = pos >= 0
+            for got, new in zip(back, (k, v)):
+                assert (got[~live] == 9).all()
+                # a step of e4m3 is 2^-3 of a value at most, half of it the bytes', and a 2^-11 each of scale and result;
+                # below 2^-6 of 448 scales steps are 2^-9 of the scale
+                far = (got[live].double() - new[live].double()).abs()
+                amax = new[live].double().abs().amax(2, keepdim=True)
+                assert (far <= (new[live].double().abs() * (2.0 ** -4 + 2.0 ** -10) + amax / 448 * 2.0 ** -10 if quant else 0 * amax)).all()
+            K.gemv_int4(out, *w["o"], h, H, 2048, B, add=True)
+            w["ffn"].forward(h)
+        K.add_rmsnorm(h, layers[0]["norm"], x, B, H)
+        K.gemv_int4(x, *head, logits, V, H, B)
+        un = rng.random(B).astype(np.float32)
+        u.copy_(t(un, dev))
+        K.sample(logits, u, ids, ws, p=p, **fd)
+        assert logits.isfinite().all()
+        want, pw, near = ref.choose(logits.cpu().numpy(), un, **f)
+        assert near.min() > 1e-9 and np.array_equal(ids.cpu().numpy(), want)
+        within(p.cpu().numpy(), pw, pw * (ref.U24 + 1e-9), f"p of step {step}")
+        pos += (pos >= 0).int()
+    assert table.free_pages == 12 - 2 - 1 - 2 - 1
