@@ -275,11 +275,7 @@ struct SampleLds {
   Ends ends;
 };
 
-// bins from[r]..to[r] of n ranges
 constexpr int kRanges = 2;
-struct BinSet {
-  int n, from[kRanges], to[kRanges];
-};
 
 // one row, all threads of the workgroup; kPer: steps of a chunk
 template <bool kHalf, int kPer>
@@ -326,12 +322,19 @@ struct SampleRow {
     return bin_mass(x - __builtin_ceil(x));
   }
 
-  // The row's largest logit, key << 32 | ~index, and the first of its chunks' bins on
-  // their way.
-  static constexpr int kFirst = 12;  // bins of a thread: those of 9 chunks
-  __device__ __forceinline__ uint64_t largest(uint64_t (&first)[kFirst]) {
+  // The row's largest logit, key << 32 | ~index, and each wave's first chunk's bins, two
+  // of a lane's at a time, on their way.
+  static constexpr int kPairs = (kBins / 2 + 63) / 64;
+  struct Pairs {
+    u32x4 v[kPairs];
+  };
+  __device__ __forceinline__ void load_pairs(int chunk, Pairs& p) const {
+    const u32x4* const from = (const u32x4*)(bins + (int64_t)chunk * kBins);
 #pragma unroll
-    for (int i = 0; i < kFirst; i++) first[i] = bins[min(i * kSampleThreads + tid, a.chunks * kBins - 1)];
+    for (int i = 0; i < kPairs; i++) p.v[i] = from[min(64 * i + lane, kBins / 2 - 1)];
+  }
+  __device__ __forceinline__ uint64_t largest(Pairs& first) {
+    load_pairs(min(wave, a.chunks - 1), first);
     for (int i = tid; i < kBins; i += kSampleThreads) s.mass[i] = 0, s.cnt[i] = 0;
     if (tid == 0) s.last = 0, s.covered = kBins;
     uint64_t best = 0;
@@ -356,26 +359,29 @@ struct SampleRow {
   }
 
   // the row's bins: tokens and mass before each
-  __device__ __forceinline__ void add_up(const uint64_t (&first)[kFirst]) {
+  __device__ __forceinline__ void add_up(Pairs& p) {
     for (int i = tid; i < a.chunks; i += kSampleThreads) {
       const double n = s.shift[i];
       s.shift[i] = inf ? (n == __builtin_inf() ? 0.0 : (double)kBins) : fmin(R - n, (double)kBins);
       atomicMin(&s.covered, (int)s.shift[i] + s.use[i]);
     }
     __syncthreads();
-    const int all = a.chunks * kBins;
-    auto add = [&](int i, uint64_t v) {
-      const int chunk = i / kBins, b = i - chunk * kBins + (int)s.shift[min(chunk, a.chunks - 1)];
-      // (the bins of a chunk without tokens are not written)
-      if (i < all && b < kBins && v) {
-        atomicAdd(&s.mass[b], (unsigned long long)(v & ((1ull << kCountShift) - 1)));
-        atomicAdd(&s.cnt[b], (uint32_t)(v >> kCountShift));
-      }
-    };
+    for (int chunk = wave; chunk < a.chunks; chunk += kSampleWaves) {
+      if (chunk != wave) load_pairs(chunk, p);
+      const int shift = (int)s.shift[chunk];
 #pragma unroll
-    for (int i = 0; i < kFirst; i++) add(i * kSampleThreads + tid, first[i]);
-#pragma unroll 4
-    for (int i = kFirst * kSampleThreads + tid; i < all; i += kSampleThreads) add(i, bins[i]);
+      for (int i = 0; i < kPairs; i++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const uint64_t v = (uint64_t)p.v[i][2 * e + 1] << 32 | p.v[i][2 * e];
+          const int from = 2 * (64 * i + lane) + e, b = from + shift;
+          // (the bins of a chunk without tokens are not written; they are past the last)
+          if (from < kBins && b < kBins && v) {
+            atomicAdd(&s.mass[b], (unsigned long long)(v & ((1ull << kCountShift) - 1)));
+            atomicAdd(&s.cnt[b], (uint32_t)(v >> kCountShift));
+          }
+        }
+    }
     __syncthreads();
     // two bins a thread
     const int b = min(2 * tid, kBins - 2);
@@ -420,21 +426,13 @@ struct SampleRow {
     return min(at, kBins - 1);
   }
 
-  // the chunks that have a token in one of the bins.  (A chunk's first bin has one, its
-  // largest.)
-  __device__ __forceinline__ void chunks_with(const BinSet& w) {
+  // the chunks that may have a token in the bins up to `to`: whose largest is in one
+  __device__ __forceinline__ void chunks_with(int to) {
     __syncthreads();
     if (tid == 0) s.m = 0;
     __syncthreads();
-    for (int i = tid; i < a.chunks; i += kSampleThreads) {
-      const double sh = s.shift[i];
-      bool has = false;
-      for (int r = 0; r < w.n; r++) {
-        if (sh > (double)w.to[r]) continue;
-        has |= w.from[r] < w.to[r] || bins[(int64_t)i * kBins + (w.to[r] - (int)sh)] >> kCountShift;
-      }
-      if (has) s.use[atomicAdd(&s.m, 1)] = i;
-    }
+    for (int i = tid; i < a.chunks; i += kSampleThreads)
+      if (s.shift[i] <= (double)to) s.use[atomicAdd(&s.m, 1)] = i;
     __syncthreads();
   }
 
@@ -712,7 +710,7 @@ struct SampleRow {
     int n = s.count[bin + 1] - cnt;
     if (!listed) {
       // divided where it lies until what is left can be taken
-      chunks_with(BinSet{1, {bin, bin}, {bin, bin}});
+      chunks_with(bin);
       while (n > kCap || !take({lo, lo}, {hi, hi})) {
         if (lo == hi) return equals(how, cnt, mass, nth, goal, n, key_value(lo));
         least = lo, most = hi;
@@ -811,7 +809,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
   const int k = a.top_k ? a.top_k[b] : 0;
   const float tp = a.top_p ? a.top_p[b] : 1.0f, mp = a.min_p ? a.min_p[b] : 0.0f;
   float u = a.u[b];
-  uint64_t first[SampleRow<kHalf, kPer>::kFirst];
+  typename SampleRow<kHalf, kPer>::Pairs first;
   const uint64_t best = r.largest(first);
   if (best == 0 || !(t > 0.0f)) {
     if (tid == 0) {
@@ -839,50 +837,53 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
     by_m = bin < (double)kBins;
     bm = by_m && bin > 0.0 ? (int)bin : 0;
   }
-  const int bk = by_k ? r.bin_with(kNth, k, 0.0) : kBins - 1;
-  // masses that the filters can keep, by whole bins: from .. to
-  double from = by_k ? s.before[bk] : all, to = by_k ? s.before[bk + 1] : all;
-  const int p0 = by_p ? r.bin_with(kReach, 0, need * from) : 1, p1 = by_p ? r.bin_with(kReach, 0, need * to) : 0;
   u = u >= 0.0f ? (u < 1.0f ? u : 0x1.fffffep-1f) : 0.0f;
+  // Bins in which the prefixes can end, by whole bins of what decides them: top-k's bk,
+  // top-p's p0..p1 for the masses that bk leaves open, the draw's d0..d1 for the masses
+  // that the filters can keep, from..to.  (One loop: its code is fetched once, which is
+  // most of the time of code that runs once.)
+  int bk = kBins - 1, p0 = 1, p1 = 0, d0 = 0, d1 = 0;
+  double from = all, to = all;
+#pragma unroll 1
+  for (int i = by_k ? 0 : by_p ? 1 : 3; i < 5; i++) {
+    if (i == 3 && by_m) from = fmin(from, s.before[bm]), to = fmin(to, s.before[bm + 1]);
+    const double goal = i < 3 ? need * (i == 1 ? from : to) : (double)u * (i == 3 ? from : to);
+    const int bin = r.bin_with(i == 0 ? kNth : i < 3 ? kReach : kPass, k, goal);
+    if (i == 0) {
+      bk = bin, from = s.before[bin], to = s.before[bin + 1];
+      if (!by_p) i = 2;
+    } else if (i == 1) {
+      p0 = bin;
+    } else if (i == 2) {
+      p1 = bin;
+      from = fmin(from, s.before[p0]), to = fmin(to, s.before[p1 + 1]);
+    } else if (i == 3) {
+      d0 = bin;
+    } else {
+      d1 = bin;
+    }
+  }
   double kept = all;  // mass of what the filters keep
   Ends e;
   // top-p's goal is a part of top-k's mass
   const int last = by_k && by_p ? bk : min(by_p ? p1 : bk, by_m ? bm : kBins - 1);
   const bool few = (by_k || by_p || by_m) && s.count[last + 1] <= kAll;
-  BinSet w{1, {0, 0}, {last, last}};  // few enough: all of them
-  int d0 = 0, d1 = 0;
-  bool listed = true;
-  if (!few) {
-    // the bins in which a filter or the draw can end, taken from the row at once if they fit
-    if (by_p) {
-      from = fmin(from, s.before[p0]);
-      to = fmin(to, s.before[p1 + 1]);
-    }
-    if (by_m) {
-      from = fmin(from, s.before[bm]);
-      to = fmin(to, s.before[bm + 1]);
-    }
-    d0 = r.bin_with(kPass, 0, (double)u * from), d1 = r.bin_with(kPass, 0, (double)u * to);
-    // the draw's, and those from the first to the last of the filters'
-    int f0 = kBins, f1 = 0;
-    if (by_p) f0 = p0, f1 = p1;
-    if (by_k) f0 = min(f0, bk), f1 = max(f1, bk);
-    if (by_m) f0 = min(f0, bm), f1 = max(f1, bm);
-    w = BinSet{f0 <= f1 ? 2 : 1, {d0, f0}, {d1, f1}};
-    int tokens = s.count[d1 + 1] - s.count[d0];
-    if (w.n > 1) tokens += s.count[f1 + 1] - s.count[f0];
-    listed = tokens <= kCap;
-  }
+  int f0 = kBins, f1 = 0;  // the bins of the filters, from the first to the last
+  if (by_p) f0 = p0, f1 = p1;
+  if (by_k) f0 = min(f0, bk), f1 = max(f1, bk);
+  if (by_m) f0 = min(f0, bm), f1 = max(f1, bm);
+  // few enough: all of them; else those bins and the draw's, if they fit
+  bool listed = few || s.count[d1 + 1] - s.count[d0] + (f0 <= f1 ? s.count[f1 + 1] - s.count[f0] : 0) <= kCap;
   const bool tops = kPer * kStep == kMinChunk && few && last < s.covered;  // they are at hand
   if (listed && !tops) {
     uint32_t lo[kRanges], hi[kRanges];
-    r.keys_of(w.from[0], w.to[0], lo[0], hi[0]);
+    r.keys_of(few ? 0 : d0, few ? last : d1, lo[0], hi[0]);
     lo[1] = lo[0], hi[1] = hi[0];
-    if (w.n > 1) r.keys_of(w.from[1], w.to[1], lo[1], hi[1]);
-    r.chunks_with(w);
+    if (!few && f0 <= f1) r.keys_of(f0, f1, lo[1], hi[1]);
+    r.chunks_with(few ? last : max(d1, f1));
     listed = r.take(lo, hi);
   }
-  if (few) {
+  if (few && listed) {
     // every prefix among them, in order
     uint32_t lo, hi;
     const int n = tops ? r.select_tops(a.tops + (int64_t)b * a.chunks * kTop, r.first_key(last)) : r.select(0, ~0u, lo, hi);

@@ -490,6 +490,19 @@ def test_sample_about_a_chunks_edge(K, dev, B, V, half):
         within(p[check][sure], q[sure], q[sure] * (ref.U24 + 1e-9), f"{f}")
 
 
+def test_sample_of_tokens_that_one_thread_meets(K, dev):
+    """The likely tokens 2048 apart, and 8192 and 512: more of them a thread than it keeps."""
+    rng = np.random.default_rng(4)
+    V = 1 << 19
+    l = (rng.standard_normal((6, V)) - 30).astype(np.float32)
+    for b, (step, n) in enumerate(((2048, 256), (8192, 64), (512, 1024), (2048, 200), (2048, 256), (4, 1000))):
+        l[b, 5:5 + step * n:step] = 2 * rng.standard_normal(n)
+    l[4, 5::2048] = 1.0  # (equals)
+    for f in (dict(top_k=60), dict(top_p=0.9), dict(top_k=150, top_p=0.7, min_p=0.01), dict(min_p=0.05), dict(),
+              dict(temperature=0.5, top_k=1000)):
+        check_sample(K, dev, l, rng.random(6), f"{f}", **{k: np.full(6, v) for k, v in f.items()})
+
+
 @pytest.mark.parametrize("V", [1, 8, 1000, 70000, 140000])
 def test_sample_at_the_border_between_equals(K, dev, V):
     """Sums of equals are whole: a number on the border between two of them draws the second."""
