@@ -486,72 +486,77 @@ __global__ __launch_bounds__(256, 2) void k_attn_pages(AttnPagesArgs a) {
       __syncthreads();
       if (last) {
         auto piece = [&](int i) { return ((first + i) * 2 + (i == 0 ? 1 : 0)) * kPart; };
-        constexpr int kSplit = kVecs < 256 ? 256 / kVecs : 1;  // waves, or more, of a four
+        constexpr int kSplit = kVecs < 256 ? 256 / kVecs : 1;  // ways that share a four's pieces
+        constexpr int kFours = kVecs > 256 ? kVecs / 256 : 1;  // fours of a thread
         // a thread's first pieces are on their way while the weights are made
-        constexpr int kEarly = 8, kLate = 8;
+        constexpr int kEarly = 8 / kFours, kHeads = kRp / 4;
         const int way = __builtin_amdgcn_readfirstlane(tid / kVecs);
-        f32x4 early[kEarly];
-        if constexpr (kVecs <= 256)
+        f32x4 early[kFours][kEarly];
+#pragma unroll
+        for (int f = 0; f < kFours; f++)
 #pragma unroll
           for (int c = 0; c < kEarly; c++) {
-            early[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (way + c * kSplit < pieces) early[c] = take4(ws, piece(way + c * kSplit), 4 * (tid % kVecs));
+            early[f][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (way + c * kSplit < pieces)
+              early[f][c] = take4(ws, piece(way + c * kSplit), 4 * (tid % kVecs + 256 * f));
           }
-        for (int h = wave; h < kRp; h += 4) {
-          float pm[kMaxParts / 64], pl[kMaxParts / 64], top = kLow;
+        // a wave's heads, a piece a lane
+        float pm[kHeads][kMaxParts / 64], pl[kHeads][kMaxParts / 64];
 #pragma unroll
-          for (int c = 0; c < kMaxParts / 64; c++) {
-            const int i = lane + 64 * c;
-            pm[c] = kLow, pl[c] = 0.0f;
-            if (i < pieces) {
-              const f32x4 x = take4(ws, 0, piece(i) + kRp * kD + 4 * h);
-              pm[c] = x[0], pl[c] = x[1];
+        for (int c = 0; c < kMaxParts / 64; c++)
+#pragma unroll
+          for (int e = 0; e < kHeads; e++) {
+            pm[e][c] = kLow, pl[e][c] = 0.0f;
+            if (64 * c < pieces && lane + 64 * c < pieces) {
+              const f32x4 x = take4(ws, 0, piece(lane + 64 * c) + kRp * kD + 4 * (wave + 4 * e));
+              pm[e][c] = x[0], pl[e][c] = x[1];
             }
-            top = __builtin_fmaxf(top, pm[c]);
           }
+#pragma unroll
+        for (int e = 0; e < kHeads; e++) {
+          float top = pm[e][0], sum = 0.0f;
+#pragma unroll
+          for (int c = 1; c < kMaxParts / 64; c++) top = __builtin_fmaxf(top, pm[e][c]);
           top = wave_max_fast(top);
-          float sum = 0.0f;
 #pragma unroll
           for (int c = 0; c < kMaxParts / 64; c++) {
-            const float e = __builtin_amdgcn_exp2f(pm[c] - top);
-            sum = __builtin_fmaf(pl[c], e, sum);
-            s.j.weight[h][lane + 64 * c] = e;
+            const float w = __builtin_amdgcn_exp2f(pm[e][c] - top);
+            sum = __builtin_fmaf(pl[e][c], w, sum);
+            s.j.weight[wave + 4 * e][lane + 64 * c] = w;
           }
           sum = wave_sum_fast(sum);
-          if (lane == 0) s.j.l[h] = sum;
+          if (lane == 0) s.j.l[wave + 4 * e] = sum;
         }
         __syncthreads();
-        for (int v = tid; v < kVecs * kSplit; v += 256) {
-          const int i4 = v % kVecs, h = i4 / (kD / 4), d = i4 % (kD / 4) * 4;
+#pragma unroll
+        for (int f = 0; f < kFours; f++) {
+          const int i4 = tid % kVecs + 256 * f, h = i4 / (kD / 4), d = i4 % (kD / 4) * 4;
           f32x4 o{0.f, 0.f, 0.f, 0.f};
-          int i = __builtin_amdgcn_readfirstlane(v / kVecs);
-          auto add = [&](const f32x4& x, float e) __attribute__((always_inline)) {
+          auto add = [&](const f32x4& x, int i) __attribute__((always_inline)) {
+            const float e = s.j.weight[h][i];
 #pragma unroll
             for (int c = 0; c < 4; c++) o[c] = __builtin_fmaf(x[c], e, o[c]);
           };
-          if constexpr (kVecs <= 256) {
 #pragma unroll
-            for (int c = 0; c < kEarly; c++) add(early[c], s.j.weight[h][i + c * kSplit]);  // (0 past the last)
-            i += kEarly * kSplit;
-          }
+          for (int c = 0; c < kEarly; c++) add(early[f][c], way + c * kSplit);  // (0 past the last)
 #pragma unroll 1
-          for (; i < pieces; i += kLate * kSplit) {
-            f32x4 x[kLate];
+          for (int i = way + kEarly * kSplit; i < pieces; i += kEarly * kSplit) {
+            f32x4 x[kEarly];
 #pragma unroll
-            for (int c = 0; c < kLate; c++)
+            for (int c = 0; c < kEarly; c++)
               if (i + c * kSplit < pieces) x[c] = take4(ws, piece(i + c * kSplit), 4 * i4);
 #pragma unroll
-            for (int c = 0; c < kLate; c++)
-              if (i + c * kSplit < pieces) add(x[c], s.j.weight[h][i + c * kSplit]);
+            for (int c = 0; c < kEarly; c++)
+              if (i + c * kSplit < pieces) add(x[c], i + c * kSplit);
           }
           if constexpr (kSplit > 1) {
-            *(f32x4*)&s.j.o[4 * v] = o;
+            *(f32x4*)&s.j.o[4 * tid] = o;
             __syncthreads();
-            if (v < kVecs)
+            if (tid < kVecs)
 #pragma unroll
-              for (int c = 1; c < kSplit; c++) o += *(const f32x4*)&s.j.o[4 * (v + c * kVecs)];
+              for (int c = 1; c < kSplit; c++) o += *(const f32x4*)&s.j.o[4 * (tid + c * kVecs)];
           }
-          if (v < kVecs && h < heads) {
+          if (tid < kVecs && h < heads) {
             const float inv = s.j.l[h] == 0.0f ? 0.0f : 1.0f / s.j.l[h];
             *(f16x4*)(a.out + ((int64_t)row * a.n_q + h0 + h) * kD + d) =
                 f16x4{(_Float16)(o[0] * inv), (_Float16)(o[1] * inv), (_Float16)(o[2] * inv), (_Float16)(o[3] * inv)};
