@@ -98,18 +98,23 @@ struct Logits {
 };
 
 // 2^(f / 16) for f in (-1, 0]: the polynomial of degree 4 through the Chebyshev points of
-// the interval, 2.5e-12 off
-__device__ __forceinline__ double bin_power(double f) {
-  double r = 1.4361898916011284e-07;
-  r = __builtin_fma(r, f, 1.3548068750879863e-05);
-  r = __builtin_fma(r, f, 9.383838162057435e-04);
-  r = __builtin_fma(r, f, 4.3321698663009583e-02);
-  return __builtin_fma(r, f, 0.9999999999975604);
-}
-// the same in units of 2^-34, rounded by an addition of 2^18
-__device__ __forceinline__ uint64_t bin_mass(double f) {
-  return __builtin_bit_cast(uint64_t, bin_power(f) + 262144.0) - __builtin_bit_cast(uint64_t, 262144.0);
-}
+// the interval, 2.5e-12 off.  Its coefficients are pinned to scalar registers: as literals
+// each costs two moves a use (8 of the 26 vector instructions of a logit).
+struct PowerOf2 {
+  double c0 = 0.9999999999975604, c1 = 4.3321698663009583e-02, c2 = 9.383838162057435e-04,
+         c3 = 1.3548068750879863e-05, c4 = 1.4361898916011284e-07, unit = 262144.0;
+  __device__ __forceinline__ PowerOf2() {
+    asm("" : "+s"(c0), "+s"(c1), "+s"(c2), "+s"(c3), "+s"(c4), "+s"(unit));
+  }
+  __device__ __forceinline__ double operator()(double f) const {
+    return __builtin_fma(__builtin_fma(__builtin_fma(__builtin_fma(c4, f, c3), f, c2), f, c1), f, c0);
+  }
+  // the same in units of 2^-34, rounded by an addition of 2^18, whose low half is 0
+  __device__ __forceinline__ uint64_t mass(double f) const {
+    return __builtin_bit_cast(uint64_t, (*this)(f) + unit) - __builtin_bit_cast(uint64_t, 262144.0);
+  }
+};
+
 // a bin's upper edge, bin 0's being 1: 2^(-bin / 16)
 __device__ __forceinline__ double bin_edge(int bin) {
   const int i = bin & 3, j = bin >> 2 & 3;
@@ -146,11 +151,8 @@ __global__ __launch_bounds__(kThreads) void k_sample_bins(SampleArgs a) {
   for (int i = tid; i < kBins; i += kThreads) bins[i] = 0;
   f32x4 x[kVec];
 #pragma unroll
-  for (int i = 0; i < kVec; i++) {
-    x[i] = in[i].get(i0 + kEach * i, a.V, whole);
-#pragma unroll
-    for (int e = 0; e < 4; e++) x[i][e] = x[i][e] == x[i][e] ? x[i][e] : -__builtin_inff();
-  }
+  for (int i = 0; i < kVec; i++) x[i] = in[i].get(i0 + kEach * i, a.V, whole);
+  // (a NaN is neither the largest nor of any bin: no comparison holds for it)
   float top = -__builtin_inff();
 #pragma unroll
   for (int i = 0; i < kVec; i++)
@@ -182,19 +184,23 @@ __global__ __launch_bounds__(kThreads) void k_sample_bins(SampleArgs a) {
     }
     return;
   }
-  const bool inf = top == __builtin_inff();
+  const bool inf = __builtin_amdgcn_readfirstlane((int)(top == __builtin_inff()));
+  const PowerOf2 power;
   const double c = temperature_scale(t), R = inf ? 0.0 : __builtin_ceil(c * (double)top);
   int bin[kTops ? kVec : 1][4];  // of each logit
+  if (inf)
+#pragma unroll
+    for (int i = 0; i < kVec; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[i][e] = x[i][e] == top ? 0.0f : -__builtin_inff();
 #pragma unroll
   for (int i = 0; i < kVec; i++)
 #pragma unroll
     for (int e = 0; e < 4; e++) {
 #pragma clang fp contract(off)
-      float l = x[i][e];
-      if (inf) l = l == top ? 0.0f : -__builtin_inff();
-      const double y = c * (double)l, n = __builtin_ceil(y), d = R - n;
+      const double y = c * (double)x[i][e], n = __builtin_ceil(y), d = R - n;
       const bool has = d < (double)kBins;
-      if (has) atomicAdd(&bins[(int)d], (unsigned long long)bin_mass(y - n) + (1ull << kCountShift));
+      if (has) atomicAdd(&bins[(int)d], (unsigned long long)power.mass(y - n) + (1ull << kCountShift));
       if constexpr (kTops) bin[i][e] = has ? (int)d : kBins;
     }
   if (tid == 0) depth = 0, listed = 0;
@@ -237,7 +243,7 @@ __global__ __launch_bounds__(kThreads) void k_sample_bins(SampleArgs a) {
       for (int e = 0; e < 4; e++) {
         if (bin[i][e] < d)
           tops[at + __builtin_amdgcn_mbcnt_hi((uint32_t)(set[i][e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)set[i][e], 0))] =
-              (uint64_t)order_key(inf ? 0.0f : x[i][e]) << 32 | (uint32_t)~(i0 + kEach * i + e);
+              (uint64_t)order_key(x[i][e]) << 32 | (uint32_t)~(i0 + kEach * i + e);
         at += __popcll(set[i][e]);
       }
     __syncthreads();
@@ -287,11 +293,12 @@ struct SampleRow {
   const uint64_t* bins;
   double c;     // x = c l
   double R;     // ceil of the largest x
-  double top_power, top_mass;  // bin_power and bin_mass of the largest logit
+  double top_power, top_mass;  // 2^(f / 16) and its mass, of the largest logit
   float top;    // the largest logit
   bool inf;     // some are +inf: they count as 0, the others as -inf
   int tid, lane, wave;
   int taken;    // tokens that the thread has in the list
+  PowerOf2 power;
 
   // x of a logit, rounded.  (Fused with a difference, a product of 1e39 would be its
   // rounding away from its own ceil.)
@@ -303,9 +310,9 @@ struct SampleRow {
   __device__ __forceinline__ double weight(float l) const {
 #pragma clang fp contract(off)
     const double x = x_of(l), n = __builtin_ceil(x);
-    return bin_power(x - n) / top_power * bin_edge((int)(R - n));
+    return power(x - n) / top_power * bin_edge((int)(R - n));
   }
-  // the same for a sum of bin_mass over tokens of one bin: whole for equals of the largest
+  // the same for a sum of masses of tokens of one bin: whole for equals of the largest
   __device__ __forceinline__ double mass_in(int bin, unsigned long long m) const {
     return (double)m / top_mass * bin_edge(bin);
   }
@@ -314,12 +321,12 @@ struct SampleRow {
   __device__ __forceinline__ double power_of(float l) const {
 #pragma clang fp contract(off)
     const double x = x_of(l);
-    return bin_power(x - __builtin_ceil(x));
+    return power(x - __builtin_ceil(x));
   }
   __device__ __forceinline__ uint64_t mass_of(float l) const {
 #pragma clang fp contract(off)
     const double x = x_of(l);
-    return bin_mass(x - __builtin_ceil(x));
+    return power.mass(x - __builtin_ceil(x));
   }
 
   // The row's largest logit, key << 32 | ~index, and each wave's first chunk's bins, two
