@@ -33,7 +33,10 @@ constexpr int kMaxParts = 256;    // of them for one kv head
 constexpr int kTicketStride = 16;  // uint32 between two counters
 constexpr int64_t kTicketBytes = (int64_t)kGroups * kTicketStride * 4;
 constexpr float kLow = -3.0e38f;  // max of no scores: finite, so that exp2(-inf - kLow) is 0
-constexpr float kSlack = 8.0f;    // numerators may be up to 2^kSlack before the max follows
+// The largest numerator of a column is 2^12, and up to 2^15 until the rest is scaled down to
+// it: fp16's least step is then 2^-36 of it.  (With 1 for the largest, 12 000 tokens of 4e-8
+// of its weight were 1/40 off in their sum.)
+constexpr float kLift = 12.0f, kMost = 15.0f;
 
 struct AttnPagesArgs {
   Pages P;
@@ -304,8 +307,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_pages(AttnPagesArgs a) {
           }
         }
         // The numerators are those of weight times V's scale, so that they fill fp16's
-        // range whatever the scales are: the max is that of s + log2 vs.  It is let lag:
-        // a rescaling only where a score passes it by 2^kSlack.
+        // range whatever the scales are: m is the max of s + log2 vs, less kLift.  It is let
+        // lag: a rescaling only where a numerator would be over 2^kMost.
         float top = -__builtin_inff();
 #pragma unroll
         for (int b = 0; b < 2; b++)
@@ -313,8 +316,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_pages(AttnPagesArgs a) {
           for (int e = 0; e < kR; e++)
             top = __builtin_fmaxf(
                 top, kF8 ? y[b][e] + __builtin_amdgcn_logf(__builtin_fmaxf(vs[b][e], 0x1p-24f)) : y[b][e]);
-        if (__any(top > m + kSlack)) {
-          const float now = __builtin_fmaxf(m, col4_max(top));
+        if (__any(top > m + kMost)) {
+          const float now = __builtin_fmaxf(m, col4_max(top) - kLift);
           const float f = __builtin_amdgcn_exp2f(m - now);
           m = now;
           l *= f;

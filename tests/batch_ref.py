@@ -45,8 +45,9 @@ def attend(q, k, v, table, page, seq, pos, scale, window):
     A score of D products in fp32, scaled: at most (D + 6) half steps of sum |q k| scale
     and 2 of itself, its weight off by as much times itself; the exponential and its
     argument 4 and as many half steps as the score has units; sums over n tokens, in
-    chains and their joins, (n / 16 + 64) half steps of sum w |v|; numerators 22 bits or
-    more: 2^-22 of it.  A scores' error moves numerator and denominator: twice.  Then
+    chains and their joins, (n / 16 + 64) half steps of sum w |v|; numerators are two fp16
+    whose largest is 2^12 or more, each off by 2^-22 of itself or half the least step,
+    2^-25, which is 2^-37 of the largest: n times that of max w times max |v|.  A score's error moves numerator and denominator: twice.  Then
     half an fp16 step."""
     T, n_q, D = q.shape
     n_kv = k.shape[1]
@@ -75,7 +76,7 @@ def attend(q, k, v, table, page, seq, pos, scale, window):
             out[t, h] = o
             mass = w @ np.abs(vv)
             bound[t, h] = (np.expm1(2 * off) * w) @ np.abs(vv) + np.abs(o) * (np.expm1(2 * off) * w).sum(1, keepdims=True) \
-                + mass * ((pid.size / 16 + 64) * 2 * U24 + 2.0 ** -22)
+                + mass * ((pid.size / 16 + 64) * 2 * U24 + 2.0 ** -22) + pid.size * 2.0 ** -37 * w.max() * np.abs(vv).max()
     return out, bound * 1.01 + np.abs(out) * U11 * 1.001 + 2.0 ** -25
 
 

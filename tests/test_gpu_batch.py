@@ -293,6 +293,41 @@ def test_attention_values(K, orc, dev, quant):
         check(K, c, dev, q, None, np.array(lens, np.int32) - 1, 0.0, 0, what="mean")
 
 
+@pytest.mark.parametrize("quant", [True, False])
+@pytest.mark.parametrize("gap", [8.0, 14.0, 17.0, 19.0])
+def test_attention_of_many_small_weights(K, orc, dev, quant, gap):
+    """One token with nearly all the weight and a V of zeros, at the start or the end, 12000 others that the output
+    is made of, each of a weight down to 6e-9 of it; so many rows that a workgroup has all of a row."""
+    rng = np.random.default_rng(1)
+    n, D, T = 12000, 64, 2048
+    c = Cache(K, orc, dev, rng, [n, n], 1, D, 64, quant)
+    q = np.zeros((T, 4, D), np.float16)
+    q[:, :, 0] = 8.0 * gap  # score gap with scale 1/8 for a key of 1 against one of 0
+    for name in "kv":
+        x = np.zeros((c.n_pages, 1, 64, D), np.float16)
+        for s, at in ((0, 0), (1, n - 1)):
+            page = int(c.table[s, at // 64])
+            if name == "v":
+                x[c.table[s, :-(-n // 64)]] = (1 + rng.random((-(-n // 64), 1, 64, D))).astype(np.float16)
+                x[page, 0, at % 64] = 0
+            else:
+                x[page, 0, at % 64, 0] = 1.0
+        if quant:
+            b, sc = ref.quant(orc, x)
+            c.raw[name].copy_(t(b, dev))
+            c.raw[name + "s"].copy_(t(sc, dev))
+            c.num[name] = orc.e4m3_decode_table()[b].astype(np.float64) * sc.astype(np.float64)[..., None]
+        else:
+            c.raw[name].copy_(t(x, dev))
+            c.num[name] = x.astype(np.float64)
+    seq = np.arange(T, dtype=np.int32) % 2
+    pos = np.full(T, n - 1, np.int32)
+    out = attend(K, c, dev, q, seq, pos, 0.125, 0).cpu().numpy()
+    want, bound = ref.attend(q[:2], c.num["k"], c.num["v"], c.table, 64, seq[:2], pos[:2], 0.125, 0)
+    for s in range(2):
+        within(out[s::2], want[s], bound[s], f"gap {gap}, {s}")
+
+
 def test_attention_of_numbers_that_are_none(K, orc, dev):
     """A NaN in a token that is attended to reaches its kv head's rows alone; one outside the window nothing."""
     rng = np.random.default_rng(3)
