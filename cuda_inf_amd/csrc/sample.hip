@@ -26,8 +26,8 @@ namespace cia {
 constexpr int kSampleThreads = 512;  // of k_sample_pick
 constexpr int kSampleWaves = kSampleThreads / 64;
 constexpr int kBins = 672;   // 42 octaves, 16 bins each
-constexpr int kSlots = 32;    // tokens that a thread takes from a row into LDS
-constexpr int kCap = 6144;   // tokens that are tried to be taken: 12 a thread
+constexpr int kSlots = 36;    // tokens that a thread takes from a row into LDS
+constexpr int kCap = 7680;   // tokens that are tried to be taken: 15 a thread
 constexpr int kSmall = 256;  // tokens put in order by counting the larger ones
 constexpr int kAll = 1024;   // tokens put in order at all
 constexpr int kSub = kSampleThreads;  // parts of a bin that holds more than kSmall
