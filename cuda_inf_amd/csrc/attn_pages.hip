@@ -605,7 +605,8 @@ extern "C" int cia_attn_pages(const cia_kv_pages* p, const uint16_t* q, int64_t 
   const int64_t need = cia_attn_pages_workspace_bytes(n_q, p->n_kv, p->head_dim);
   CIA_REQUIRE(need > 0 && T >= 0 && T <= CIA_PAGES_MAX_ROWS && (seq || T <= p->n_seq), CIA_ERR_ARG);
   CIA_REQUIRE(q_stride >= (int64_t)n_q * p->head_dim && q_stride % 8 == 0 && window >= 0, CIA_ERR_ARG);
-  CIA_REQUIRE(scale - scale == 0.0f, CIA_ERR_ARG);  // finite
+  // (scores of finite q and K are below 2^48, so that they stay above kLow times log2 e; no NaN)
+  CIA_REQUIRE(__builtin_fabsf(scale) <= 0x1p64f, CIA_ERR_ARG);
   if (T == 0) return CIA_OK;
   if ((st = pages_check_ptr(p))) return st;
   CIA_REQUIRE(q && pos && out && ws, CIA_ERR_NULL);

@@ -503,7 +503,7 @@ def attn_pages(pages: KvPages, q, out, pos, ws, seq=None, scale: float = 0.125, 
     heads, dim] (rows may lie apart) at positions ``pos`` (int32 [T]) of ``seq`` (int32
     [T]; None: row t is sequence t's), into out fp16 [T, query heads, dim]; all tokens
     up to pos, the last ``window`` of them if window > 0.  Rows with none (pos -1) are
-    0.  Calls sharing ws must be ordered on one stream."""
+    0.  Calls sharing ws must be ordered on one stream, after what zeroed it."""
     T, dev = _tokens(pos), pages._device
     n_q = q.shape[1] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0
     qp, qs = _rows(q, "q", n_q, pages.head_dim, T, dev)

@@ -285,7 +285,7 @@ class PageTable:
     """Which pages hold the tokens of each of ``max_seqs`` sequences: token ``pos`` of
     sequence ``s`` lies in page ``table[s, pos // page]``, -1 where it has none.  The
     layers of a model share one: ``n_pages`` pages of ``page`` tokens in each of them,
-    given out and taken back on the host."""
+    given out and taken back on the host, and written to ``table`` on the current stream."""
 
     def __init__(self, max_seqs: int, max_tokens: int, n_pages: int, *, page: int = 64, device="cuda"):
         self.page, self.n_pages = page, n_pages
@@ -331,7 +331,8 @@ class PagedAttn:
     with ``quant=False``.  ``scale``: of the scores, 1 / sqrt(head_dim) if None;
     ``window``: tokens attended to, 0 for all.  Positions are int32 device tensors, -1
     for an empty place of a batch; ``seq`` is the tokens' sequences, None: token t is
-    sequence t's.  Calls of one layer must be ordered on one stream."""
+    sequence t's.  The layer's making, which clears its buffers, and its calls must be
+    ordered on one stream."""
 
     def __init__(self, table: PageTable, *, n_q: int = NH, n_kv: int = NKV, head_dim: int = D, quant: bool = True,
                  scale=None, window: int = 0):

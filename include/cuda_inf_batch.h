@@ -92,7 +92,10 @@ int cia_kv_pages_read(const cia_kv_pages* P, uint16_t* k, int64_t k_stride,
  * q: fp16, row t's [n_q][head_dim] at q + t * q_stride (a multiple of 8, n_q *
  * head_dim at least); out: fp16 [T][n_q][head_dim]; both 16-byte aligned.  n_q
  * a multiple of n_kv, at most CIA_PAGES_MAX_GROUP times it; T at most
- * CIA_PAGES_MAX_ROWS; scale finite.  Softmax and sums are fp32.
+ * CIA_PAGES_MAX_ROWS; |scale| <= 2^64.  Softmax and sums are fp32.  A NaN or an
+ * infinity in what a row attends to makes its kv head's outputs NaN or
+ * infinite (one in V: those of its dimension), but for a score of -inf, which
+ * has no weight; elsewhere in the cache they do nothing.
  * ws: device scratch of at least cia_attn_pages_workspace_bytes, 16-byte
  * aligned, zeroed before its first use; every call leaves its counters at
  * zero.  Calls that share one must be ordered, captured graphs included. */

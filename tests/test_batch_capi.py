@@ -90,7 +90,8 @@ def test_attn_refusals(L):
     f = lambda **kw: L.cia_attn_pages(pages(), *{**good, **kw}.values(), None)  # noqa: E731
     for kw in (dict(T=-1), dict(T=4097), dict(n_q=0), dict(n_q=33), dict(n_q=4), dict(n_q=-8), dict(n_q=8 * 65, q_stride=1 << 20),
                dict(q_stride=2040), dict(q_stride=2052), dict(window=-1), dict(scale=float("nan")),
-               dict(scale=float("inf")), dict(scale=float("-inf")), dict(ws_bytes=n - 1), dict(ws_bytes=0),
+               dict(scale=float("inf")), dict(scale=float("-inf")), dict(scale=1.0001 * 2.0 ** 64), dict(scale=-1e30),
+               dict(ws_bytes=n - 1), dict(ws_bytes=0),
                dict(seq=None, T=5)):
         assert f(**kw) == ARG, kw
     for kw in (dict(q=None), dict(pos=None), dict(out=None), dict(ws=None)):

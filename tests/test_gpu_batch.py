@@ -342,6 +342,36 @@ def test_attention_of_numbers_that_are_none(K, orc, dev):
     assert not attend(K, c, dev, q, None, pos, 0.125, 162).isnan().any()
 
 
+@pytest.mark.parametrize("group", [1, 4, 8, 16])
+def test_attention_to_an_infinity(K, orc, dev, group):
+    rng = np.random.default_rng(5)
+    c = Cache(K, orc, dev, rng, [50, 50], 1, 64, 16, False)
+    q = rng.standard_normal((2, group, 64)).astype(np.float16)
+    c.raw["v"][int(c.table[0, 1]), 0, 3, 9] = float("inf")  # token 19 of sequence 0, dimension 9
+    pos = np.array([49, 49], np.int32)
+    bad = ~attend(K, c, dev, q, None, pos, 0.125, 0).cpu().isfinite()
+    assert bad[0, :, 9].all() and bad.sum() == group
+    assert attend(K, c, dev, q, None, pos, 0.125, 30).isfinite().all()
+
+
+@pytest.mark.parametrize("quant", [True, False])
+@pytest.mark.parametrize("scale", [2.0 ** 64, -(2.0 ** 64), 2.0 ** 40])
+def test_attention_at_the_largest_scales(K, orc, dev, quant, scale):
+    """Only the largest score's token is left: its V, rounded once (2^-11 of it, or half of the least step)."""
+    rng = np.random.default_rng(6)
+    c = Cache(K, orc, dev, rng, [700, 31], 2, 64, 16, quant)
+    q = rng.standard_normal((2, 8, 64)).astype(np.float16)
+    pos = np.array([699, 30], np.int32)
+    out = attend(K, c, dev, q, None, pos, scale, 0).cpu().numpy()
+    for s in range(2):
+        at = [(int(c.table[s, j // 16]), j % 16) for j in range(pos[s] + 1)]
+        k, v = (np.stack([c.num[name][p, :, r] for p, r in at]) for name in "kv")  # [tokens, kv heads, D]
+        for h in range(8):
+            best = np.argmax(np.sign(scale) * (k[:, h // 4] @ q[s, h].astype(np.float64)))
+            want = v[best, h // 4]
+            within(out[s, h], want, np.abs(want) * 2.0 ** -11 + 2.0 ** -25, f"sequence {s}, head {h}")
+
+
 def test_pages_beyond_32_bits(K, orc, dev):
     """Rows of pages whose bytes lie past 2^32: written, attended and read."""
     n_pages, page, n_kv, D = 2100, 1024, 8, 128
