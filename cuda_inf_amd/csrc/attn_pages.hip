@@ -3,12 +3,16 @@
 //   s_j = scale q . k_j,   out = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s)
 // over the tokens of the row's sequence up to its position, each K and V row read once.
 //
-// Bound by memory: 2 D + 4 bytes a token and kv head in e4m3, 4 D in fp16.
+// Bound by memory: 2 D + 4 bytes a token and kv head in e4m3, 4 D in fp16.  32 query heads
+// on 8 kv heads of 64 in e4m3: 256 rows of 900 to 2048 tokens take 78 us (380 MB, 4.9 TB/s; a
+// large copy reaches 5.1), 58 of 9 to 9000 21.8-22.1 (89 MB, 4.0 TB/s), one of 32 768
+// 13.0 (35 MB in about 6, launch and first loads 4, the join 3), one of 700 6.7.
 //
 // Work.  A row's tokens are units of 128, and the units of all rows one list, of which
 // each of the P workgroups of a kv head takes an equal part, whatever rows it falls
 // into: batches of very different lengths keep every compute unit busy to the end.  A
-// row's start counts as some units more, or workgroups of many short rows end last.  The
+// row's start counts as some units more, or workgroups of many short rows end last (with
+// a better join and fewer parts 27.9 -> 23.5 us for 58 ragged rows).  The
 // list follows from the positions on the device, so a captured call can be replayed with
 // others.  A row in one workgroup's part is finished there; the parts of a longer one are
 // joined by the workgroup that ends last (it counts itself in, nothing waits).
@@ -21,6 +25,7 @@
 // 16 query heads fill the 16 columns several times over (kNB): column block j keeps the
 // scores of r = j alone, so a lane has two exponentials a tile instead of eight, and
 // its products' other places are zeros; the blocks' sums are added at the row's end.
+// Matrix cores are busy 9 % of the time, vector units 33 % (256 rows): neither bounds.
 #include "decode_wave.h"
 #include "pages.h"
 
@@ -28,7 +33,9 @@ namespace cia {
 
 constexpr int kUnit = 128;        // tokens of a unit: 32 a wave
 constexpr int kRowCost = 2;       // units that a row's start and end take the time of
-constexpr int kGroups = 512;      // workgroups of a call, two a compute unit
+// Workgroups of a call, two a compute unit.  (Three: even for 256 rows, 15.5 us for 13.1 for one
+// of 32 768 tokens, whose join has more parts.)
+constexpr int kGroups = 512;
 constexpr int kMaxParts = 256;    // of them for one kv head
 constexpr int kTicketStride = 16;  // uint32 between two counters
 constexpr int64_t kTicketBytes = (int64_t)kGroups * kTicketStride * 4;
@@ -324,7 +331,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_pages(AttnPagesArgs a) {
 #pragma unroll
           for (int i = 0; i < kO; i++) O[i] *= f;
         }
-        // numerators as two fp16: 22 bits
+        // numerators as two fp16: 22 bits (256 rows 80.2 us, with one of 11 bits 79.8)
         uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int b = 0; b < 2; b++) {

@@ -3,6 +3,10 @@
 // s = amax / 448 + 1e-12, bytes e4m3(x / s), fp16(s).
 //
 // Bound by memory: 4 D bytes of K and V in fp16, 2 D + 4 in the cache, a token and head.
+// 8192 tokens of 8 heads of 64 read back take 6.0-6.4 us (4.0-4.2 TB/s; a large copy
+// reaches 5.1), 5001 written 5.8-7.0 (2.2-2.7 TB/s), one token 3.2-3.6, an empty kernel
+// 2.0-2.2: what is left beside the bytes is a chain of three loads, position, page id and
+// row, of which the write has its rows' out before the other two.
 #include "pages.h"
 
 namespace cia {
@@ -64,7 +68,8 @@ __device__ __forceinline__ u32x4 load_e4m3(const uint8_t* rows, const uint16_t* 
 }
 
 // grid = (tokens / (2048 / kD), kv heads), block = 256: kD / 8 lanes a token, 8 values
-// each of K and of V.  Neighbouring tokens of one head are neighbouring rows of a
+// each of K and of V, so that a token's amax stays in a DPP row and every load and store
+// of fp16 is 16 bytes.  Neighbouring tokens of one head are neighbouring rows of a
 // page, so a workgroup's stores fill whole lines though a row is 64 bytes.
 template <int kD, bool kF8, bool kWrite>
 __global__ __launch_bounds__(256) void k_pages_move(MoveArgs a) {
