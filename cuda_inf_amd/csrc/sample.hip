@@ -95,6 +95,20 @@ struct Logits {
       for (int e = 0; e < 4; e++) x[e] = r[min(i + e, V - 1)];
     }
   }
+  // of a row of 4 or more: the last four for those past its end
+  __device__ __forceinline__ void load_in(const void* row, int i, int V) {
+    __builtin_memcpy(&x, (const T*)row + min(i, V - 4), sizeof(x));
+  }
+  __device__ __forceinline__ f32x4 get_in(int i, int V) const {
+    const int past = i - min(i, V - 4);
+    f32x4 y;
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] = (float)x[e];
+    const float none = -__builtin_inff();
+    if (past & 1) y = f32x4{y[1], y[2], y[3], none};
+    if (past & 2) y = f32x4{y[2], y[3], none, none};
+    return past > 3 ? f32x4{none, none, none, none} : y;
+  }
   __device__ __forceinline__ f32x4 get(int i, int V, bool whole) const {
     f32x4 y;
 #pragma unroll
@@ -269,6 +283,7 @@ struct Ends {
   int idx;
 };
 
+template <int kSlots>
 struct SampleLds {
   float value[kSlots][kSampleThreads];     // tokens taken from the row, of each thread its own
   uint16_t nth[kSlots][kSampleThreads];    // and which of the logits it has passed each is
@@ -291,10 +306,13 @@ struct SampleLds {
 
 constexpr int kRanges = 2;
 
-// one row, all threads of the workgroup; kPer: steps of a chunk
-template <bool kHalf, int kPer>
+// one row, all threads of the workgroup; kPer: steps of a chunk, or of the row where the
+// threads keep it (kKept)
+template <bool kHalf, int kPer, bool kKept>
 struct SampleRow {
-  SampleLds& s;
+  static constexpr int kSlots = kKept ? 4 * kPer : cia::kSlots;
+  static constexpr int kCap = kKept ? 1 << 30 : cia::kCap;  // (as many as there are fit)
+  SampleLds<kSlots>& s;
   const SampleArgs& a;
   const void* row;
   const ChunkHead* heads;
@@ -307,6 +325,17 @@ struct SampleRow {
   int tid, lane, wave;
   int taken;    // tokens that the thread has in the list
   PowerOf2 power;
+  f32x4 held[kKept ? kPer : 1];
+
+  // what follows from the largest logit
+  __device__ __forceinline__ void start(float largest, float temperature) {
+    inf = __builtin_amdgcn_readfirstlane((int)(largest == __builtin_inff()));
+    top = inf ? 0.0f : largest;
+    c = temperature_scale(temperature);
+    R = __builtin_ceil(x_of(top));
+    top_mass = (double)mass_of(top);
+    top_power = power_of(top);
+  }
 
   // x of a logit, rounded.  (Fused with a difference, a product of 1e39 would be its
   // rounding away from its own ceil.)
@@ -398,11 +427,58 @@ struct SampleRow {
         }
     }
     __syncthreads();
-    // two bins a thread
+    const int b = min(2 * tid, kBins - 2);
+    scan(s.cnt[b], s.cnt[b + 1], s.mass[b], s.mass[b + 1]);
+  }
+
+  // the largest of the threads' numbers
+  __device__ __forceinline__ float most(float v) const {
+    v = wave_max_fast(v);
+    if (lane == 0) s.lo[wave] = __builtin_bit_cast(uint32_t, v);
+    __syncthreads();
+    for (int w = 0; w < kSampleWaves; w++) v = __builtin_fmaxf(v, __builtin_bit_cast(float, s.lo[w]));
+    return v;
+  }
+  // the first of the row's logits, kept by the threads, that is this one
+  __device__ __forceinline__ int first_of(float l) const {
+    int idx = 0x7fffffff;
+#pragma unroll
+    for (int i = kPer - 1; i >= 0; i--)
+#pragma unroll
+      for (int e = 3; e >= 0; e--)
+        if (held[i][e] == l) idx = kStep * i + 4 * tid + e;
+    for (int off = 32; off; off >>= 1) idx = min(idx, __shfl_xor(idx, off));
+    if (lane == 0) s.hi[wave] = (uint32_t)idx;
+    __syncthreads();
+    for (int w = 0; w < kSampleWaves; w++) idx = min(idx, (int)s.hi[w]);
+    return idx;
+  }
+
+  // The bins of a row that the threads keep, and the sums before each.
+  __device__ __forceinline__ void bin_kept() {
+#pragma unroll
+    for (int i = 0; i < kPer; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+#pragma clang fp contract(off)
+        if (inf) held[i][e] = held[i][e] == __builtin_inff() ? 0.0f : -__builtin_inff();
+        const double y = c * (double)held[i][e], n = __builtin_ceil(y), d = R - n;
+        if (d < (double)kBins)
+          atomicAdd(&s.mass[(int)d], (unsigned long long)power.mass(y - n) + (1ull << kCountShift));
+      }
+    __syncthreads();
+    const int b = min(2 * tid, kBins - 2);
+    constexpr unsigned long long kMass = (1ull << kCountShift) - 1;
+    const unsigned long long v0 = s.mass[b], v1 = s.mass[b + 1];
+    scan((uint32_t)(v0 >> kCountShift), (uint32_t)(v1 >> kCountShift), v0 & kMass, v1 & kMass);
+  }
+
+  // s.count and s.before, from two bins a thread: 2 tid and the next
+  __device__ __forceinline__ void scan(uint32_t c0, uint32_t c1, unsigned long long u0, unsigned long long u1) {
     const int b = min(2 * tid, kBins - 2);
     const bool mine = 2 * tid < kBins;
-    const int k0 = mine ? (int)s.cnt[b] : 0, k1 = mine ? (int)s.cnt[b + 1] : 0;
-    const double m0 = mine ? mass_in(b, s.mass[b]) : 0.0, m1 = mine ? mass_in(b + 1, s.mass[b + 1]) : 0.0;
+    const int k0 = mine ? (int)c0 : 0, k1 = mine ? (int)c1 : 0;
+    const double m0 = mine ? mass_in(b, u0) : 0.0, m1 = mine ? mass_in(b + 1, u1) : 0.0;
     double run = m0 + m1;
     int upto = k0 + k1;
     for (int off = 1; off < 64; off <<= 1) {
@@ -472,13 +548,19 @@ struct SampleRow {
   // chunks in use in turn
   __device__ __forceinline__ int index_of(int nth) const {
     const int step = nth >> 2;
+    if constexpr (kKept) return step * kStep + 4 * tid + (nth & 3);
     return s.use[step / kPer] * (kPer * kStep) + step % kPer * kStep + 4 * tid + (nth & 3);
   }
 
   // fn(nth, x): four neighbouring logits from the thread's nth on, of the s.m chunks in use
   template <typename F>
   __device__ __forceinline__ void each(F fn) {
-    constexpr int kAhead = 8, kAt = kAhead / kPer;  // steps whose loads are out together, of kAt chunks
+    if constexpr (kKept) {
+#pragma unroll
+      for (int k = 0; k < kPer; k++) fn(4 * k, held[k]);
+      return;
+    }
+    constexpr int kAhead = 8, kAt = kAhead / (kKept ? 8 : kPer);  // steps whose loads are out together, of kAt chunks
     const int m = __builtin_amdgcn_readfirstlane(s.m);
 #pragma unroll 1
     for (int c0 = 0; c0 < m; c0 += kAt) {
@@ -723,7 +805,7 @@ struct SampleRow {
     uint32_t lo, hi, least, most;
     keys_of(bin, bin, lo, hi);
     int n = s.count[bin + 1] - cnt;
-    if (!listed) {
+    if (!kKept && !listed) {
       // divided where it lies until what is left can be taken
       chunks_with(bin);
       while (n > kCap || !take({lo, lo}, {hi, hi})) {
@@ -810,6 +892,122 @@ struct SampleRow {
       x = ((const float*)row)[i];
     return inf ? x == __builtin_inff() : x == l;
   }
+
+  // the row's token, after its bins
+  __device__ __forceinline__ void choose(int row_at, int k, float tp, float mp, float u) {
+    const int total = s.count[kBins];
+    const double all = s.before[kBins], need = tp > 0.0f ? (double)tp : 0.0, least = mp < 1.0f ? (double)mp : 1.0;
+    const bool by_k = k > 0 && k < total, by_p = tp < 1.0f;
+    bool by_m = mp > 0.0f;
+    // the bin of the last token that each filter can keep
+    int bm = 0;
+    if (by_m) {
+      const double x = x_of(top) + 16 * log2(least), bin = R - __builtin_ceil(x);
+      by_m = bin < (double)kBins;
+      bm = by_m && bin > 0.0 ? (int)bin : 0;
+    }
+    u = u >= 0.0f ? (u < 1.0f ? u : 0x1.fffffep-1f) : 0.0f;
+    // Bins in which the prefixes can end, by whole bins of what decides them: top-k's bk,
+    // top-p's p0..p1 for the masses that bk leaves open, the draw's d0..d1 for the masses
+    // that the filters can keep, from..to.  (One loop: its code is fetched once, which is
+    // most of the time of code that runs once.)
+    int bk = kBins - 1, p0 = 1, p1 = 0, d0 = 0, d1 = 0;
+    double from = all, to = all;
+#pragma unroll 1
+    for (int i = by_k ? 0 : by_p ? 1 : 3; i < 5; i++) {
+      if (i == 3 && by_m) from = fmin(from, s.before[bm]), to = fmin(to, s.before[bm + 1]);
+      const double goal = i < 3 ? need * (i == 1 ? from : to) : (double)u * (i == 3 ? from : to);
+      const int bin = bin_with(i == 0 ? kNth : i < 3 ? kReach : kPass, k, goal);
+      if (i == 0) {
+        bk = bin, from = s.before[bin], to = s.before[bin + 1];
+        if (!by_p) i = 2;
+      } else if (i == 1) {
+        p0 = bin;
+      } else if (i == 2) {
+        p1 = bin;
+        from = fmin(from, s.before[p0]), to = fmin(to, s.before[p1 + 1]);
+      } else if (i == 3) {
+        d0 = bin;
+      } else {
+        d1 = bin;
+      }
+    }
+    double kept = all;  // mass of what the filters keep
+    Ends e;
+    // top-p's goal is a part of top-k's mass
+    const int last = by_k && by_p ? bk : min(by_p ? p1 : bk, by_m ? bm : kBins - 1);
+    const bool few = (by_k || by_p || by_m) && s.count[last + 1] <= kAll;
+    int f0 = kBins, f1 = 0;  // the bins of the filters, from the first to the last
+    if (by_p) f0 = p0, f1 = p1;
+    if (by_k) f0 = min(f0, bk), f1 = max(f1, bk);
+    if (by_m) f0 = min(f0, bm), f1 = max(f1, bm);
+    // few enough: all of them; else those bins and the draw's, if they fit
+    bool listed = few || s.count[d1 + 1] - s.count[d0] + (f0 <= f1 ? s.count[f1 + 1] - s.count[f0] : 0) <= kCap;
+    const bool tops = !kKept && kPer * kStep == kMinChunk && few && last < s.covered;  // they are at hand
+    if (listed && !tops) {
+      uint32_t lo[kRanges], hi[kRanges];
+      keys_of(few ? 0 : d0, few ? last : d1, lo[0], hi[0]);
+      lo[1] = lo[0], hi[1] = hi[0];
+      if (!few && f0 <= f1) keys_of(f0, f1, lo[1], hi[1]);
+      if constexpr (!kKept) chunks_with(few ? last : max(d1, f1));
+      listed = take(lo, hi);
+    }
+    if (few && listed) {
+      // every prefix among them, in order
+      uint32_t lo, hi;
+      const int n = tops ? select_tops(a.tops + (int64_t)row_at * a.chunks * kTop, first_key(last)) : select(0, ~0u, lo, hi);
+      order(s.some, n);
+      sums(n, 0.0);
+      if (by_k && k <= n) kept = s.run[k - 1];
+      if (by_p) kept = fmin(kept, s.run[place(kReach, n, 0, 0, need * kept)]);
+      // (all of them, where another filter ends before: its mass is less)
+      if (by_m) kept = fmin(kept, s.run[max(0, place(kRatio, n, 0, 0, least))]);
+      e = ends_at(place(kPass, n, 0, 0, (double)u * kept), 0.0);
+    } else {
+      for (int step = by_k ? 0 : 1; step < 4; step++) {  // top-k, top-p, min-p, the draw
+        // (bins by masses that a rounding has moved past their range stay in it)
+        Goal how = kPass;
+        double goal = (double)u * kept;
+        int bin;
+        if (step == 0) {
+          how = kNth, bin = bk;
+        } else if (step == 1) {
+          if (!by_p) continue;
+          how = kReach, goal = need * kept;
+          bin = min(max(bin_with(kReach, 0, goal), p0), p1);
+        } else if (step == 2) {
+          if (!by_m) continue;
+          how = kRatio, goal = least, bin = bm;
+          if (s.count[bm + 1] == s.count[bm]) {  // bins before it are kept whole
+            kept = fmin(kept, s.before[bm]);
+            continue;
+          }
+        } else {
+          bin = min(max(bin_with(kPass, 0, goal), d0), d1);
+        }
+        e = end_of(how, bin, k, goal, listed);
+        if (step < 3) kept = fmin(kept, e.mass);
+      }
+    }
+    put(row_at, e.idx, (float)(e.w / kept));
+  }
+  __device__ __forceinline__ void put(int row_at, int id, float p) const {
+    if (tid) return;
+    a.ids[row_at] = id;
+    if (a.p) a.p[row_at] = p;
+  }
+};
+
+// What a row's choice is given, on its way early.
+struct Given {
+  float t, tp, mp, u;
+  int k;
+  __device__ __forceinline__ Given(const SampleArgs& a, int b)
+      : t(a.temperature ? a.temperature[b] : 1.0f),
+        tp(a.top_p ? a.top_p[b] : 1.0f),
+        mp(a.min_p ? a.min_p[b] : 0.0f),
+        u(a.u[b]),
+        k(a.top_k ? a.top_k[b] : 0) {}
 };
 
 // grid = rows, block = kSampleThreads: one workgroup a row, so that its steps meet at
@@ -817,130 +1015,55 @@ struct SampleRow {
 // tokens and their order 4.6, sums and places 2.2, for one row of 65 536 with all filters).
 template <bool kHalf, int kPer>
 __global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
-  __shared__ SampleLds s;
+  using Row = SampleRow<kHalf, kPer, false>;
+  __shared__ SampleLds<Row::kSlots> s;
   const int b = blockIdx.x, tid = threadIdx.x;
   const void* row = (const char*)a.logits + (int64_t)b * a.stride * (kHalf ? 2 : 4);
-  SampleRow<kHalf, kPer> r{s,   a,   row, a.heads + (int64_t)b * a.chunks, a.bins + (int64_t)b * a.chunks * kBins,
-                     0.0, 0.0, 1.0, 1.0, 0.0f, false, tid, tid & 63, tid >> 6, 0};
-  const float t = a.temperature ? a.temperature[b] : 1.0f;
-  const int k = a.top_k ? a.top_k[b] : 0;
-  const float tp = a.top_p ? a.top_p[b] : 1.0f, mp = a.min_p ? a.min_p[b] : 0.0f;
-  float u = a.u[b];
-  typename SampleRow<kHalf, kPer>::Pairs first;
+  Row r{s,   a,   row, a.heads + (int64_t)b * a.chunks, a.bins + (int64_t)b * a.chunks * kBins,
+        0.0, 0.0, 1.0, 1.0, 0.0f, false, tid, tid & 63, tid >> 6, 0};
+  const Given g(a, b);
+  typename Row::Pairs first;
   const uint64_t best = r.largest(first);
-  if (best == 0 || !(t > 0.0f)) {
-    if (tid == 0) {
-      a.ids[b] = best ? (int)~(uint32_t)best : -1;
-      if (a.p) a.p[b] = best ? 1.0f : 0.0f;
-    }
+  if (best == 0 || !(g.t > 0.0f)) {
+    r.put(b, best ? (int)~(uint32_t)best : -1, best ? 1.0f : 0.0f);
     return;
   }
-  r.top = key_value((uint32_t)(best >> 32));
-  r.inf = __builtin_amdgcn_readfirstlane((int)(r.top == __builtin_inff()));
-  if (r.inf) r.top = 0.0f;
-  r.c = temperature_scale(t);
-  r.R = __builtin_ceil(r.x_of(r.top));
-  r.top_mass = (double)r.mass_of(r.top);
-  r.top_power = r.power_of(r.top);
+  r.start(key_value((uint32_t)(best >> 32)), g.t);
   r.add_up(first);
-  const int total = s.count[kBins];
-  const double all = s.before[kBins], need = tp > 0.0f ? (double)tp : 0.0, least = mp < 1.0f ? (double)mp : 1.0;
-  const bool by_k = k > 0 && k < total, by_p = tp < 1.0f;
-  bool by_m = mp > 0.0f;
-  // the bin of the last token that each filter can keep
-  int bm = 0;
-  if (by_m) {
-    const double x = r.x_of(r.top) + 16 * log2(least), bin = r.R - __builtin_ceil(x);
-    by_m = bin < (double)kBins;
-    bm = by_m && bin > 0.0 ? (int)bin : 0;
+  r.choose(b, g.k, g.tp, g.mp, g.u);
+}
+
+// The same for a row of 4..kPer * kStep logits by itself, which the threads keep in registers.
+template <bool kHalf, int kPer>
+__global__ __launch_bounds__(kSampleThreads) void k_sample_row(SampleArgs a) {
+  using Row = SampleRow<kHalf, kPer, true>;
+  __shared__ SampleLds<Row::kSlots> s;
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const void* row = (const char*)a.logits + (int64_t)b * a.stride * (kHalf ? 2 : 4);
+  Row r{s,   a,   row, nullptr, nullptr, 0.0, 0.0, 1.0, 1.0, 0.0f, false, tid, tid & 63, tid >> 6, 0};
+  Logits<kHalf> in[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; i++) in[i].load_in(row, kStep * i + 4 * tid, a.V);
+  const Given g(a, b);
+  for (int i = tid; i < kBins; i += kSampleThreads) s.mass[i] = 0;
+  if (tid == 0) s.last = 0;
+  float top = -__builtin_inff();
+#pragma unroll
+  for (int i = 0; i < kPer; i++) {
+    r.held[i] = in[i].get_in(kStep * i + 4 * tid, a.V);
+#pragma unroll
+    for (int e = 0; e < 4; e++) top = __builtin_fmaxf(top, r.held[i][e]);
   }
-  u = u >= 0.0f ? (u < 1.0f ? u : 0x1.fffffep-1f) : 0.0f;
-  // Bins in which the prefixes can end, by whole bins of what decides them: top-k's bk,
-  // top-p's p0..p1 for the masses that bk leaves open, the draw's d0..d1 for the masses
-  // that the filters can keep, from..to.  (One loop: its code is fetched once, which is
-  // most of the time of code that runs once.)
-  int bk = kBins - 1, p0 = 1, p1 = 0, d0 = 0, d1 = 0;
-  double from = all, to = all;
-#pragma unroll 1
-  for (int i = by_k ? 0 : by_p ? 1 : 3; i < 5; i++) {
-    if (i == 3 && by_m) from = fmin(from, s.before[bm]), to = fmin(to, s.before[bm + 1]);
-    const double goal = i < 3 ? need * (i == 1 ? from : to) : (double)u * (i == 3 ? from : to);
-    const int bin = r.bin_with(i == 0 ? kNth : i < 3 ? kReach : kPass, k, goal);
-    if (i == 0) {
-      bk = bin, from = s.before[bin], to = s.before[bin + 1];
-      if (!by_p) i = 2;
-    } else if (i == 1) {
-      p0 = bin;
-    } else if (i == 2) {
-      p1 = bin;
-      from = fmin(from, s.before[p0]), to = fmin(to, s.before[p1 + 1]);
-    } else if (i == 3) {
-      d0 = bin;
-    } else {
-      d1 = bin;
-    }
+  top = r.most(top);
+  const bool none = top == -__builtin_inff();
+  if (none || !(g.t > 0.0f)) {
+    const int id = none ? -1 : r.first_of(top);
+    r.put(b, id, none ? 0.0f : 1.0f);
+    return;
   }
-  double kept = all;  // mass of what the filters keep
-  Ends e;
-  // top-p's goal is a part of top-k's mass
-  const int last = by_k && by_p ? bk : min(by_p ? p1 : bk, by_m ? bm : kBins - 1);
-  const bool few = (by_k || by_p || by_m) && s.count[last + 1] <= kAll;
-  int f0 = kBins, f1 = 0;  // the bins of the filters, from the first to the last
-  if (by_p) f0 = p0, f1 = p1;
-  if (by_k) f0 = min(f0, bk), f1 = max(f1, bk);
-  if (by_m) f0 = min(f0, bm), f1 = max(f1, bm);
-  // few enough: all of them; else those bins and the draw's, if they fit
-  bool listed = few || s.count[d1 + 1] - s.count[d0] + (f0 <= f1 ? s.count[f1 + 1] - s.count[f0] : 0) <= kCap;
-  const bool tops = kPer * kStep == kMinChunk && few && last < s.covered;  // they are at hand
-  if (listed && !tops) {
-    uint32_t lo[kRanges], hi[kRanges];
-    r.keys_of(few ? 0 : d0, few ? last : d1, lo[0], hi[0]);
-    lo[1] = lo[0], hi[1] = hi[0];
-    if (!few && f0 <= f1) r.keys_of(f0, f1, lo[1], hi[1]);
-    r.chunks_with(few ? last : max(d1, f1));
-    listed = r.take(lo, hi);
-  }
-  if (few && listed) {
-    // every prefix among them, in order
-    uint32_t lo, hi;
-    const int n = tops ? r.select_tops(a.tops + (int64_t)b * a.chunks * kTop, r.first_key(last)) : r.select(0, ~0u, lo, hi);
-    r.order(s.some, n);
-    r.sums(n, 0.0);
-    if (by_k && k <= n) kept = s.run[k - 1];
-    if (by_p) kept = fmin(kept, s.run[r.place(kReach, n, 0, 0, need * kept)]);
-    // (all of them, where another filter ends before: its mass is less)
-    if (by_m) kept = fmin(kept, s.run[max(0, r.place(kRatio, n, 0, 0, least))]);
-    e = r.ends_at(r.place(kPass, n, 0, 0, (double)u * kept), 0.0);
-  } else {
-    for (int step = by_k ? 0 : 1; step < 4; step++) {  // top-k, top-p, min-p, the draw
-      // (bins by masses that a rounding has moved past their range stay in it)
-      Goal how = kPass;
-      double goal = (double)u * kept;
-      int bin;
-      if (step == 0) {
-        how = kNth, bin = bk;
-      } else if (step == 1) {
-        if (!by_p) continue;
-        how = kReach, goal = need * kept;
-        bin = min(max(r.bin_with(kReach, 0, goal), p0), p1);
-      } else if (step == 2) {
-        if (!by_m) continue;
-        how = kRatio, goal = least, bin = bm;
-        if (s.count[bm + 1] == s.count[bm]) {  // bins before it are kept whole
-          kept = fmin(kept, s.before[bm]);
-          continue;
-        }
-      } else {
-        bin = min(max(r.bin_with(kPass, 0, goal), d0), d1);
-      }
-      e = r.end_of(how, bin, k, goal, listed);
-      if (step < 3) kept = fmin(kept, e.mass);
-    }
-  }
-  if (tid == 0) {
-    a.ids[b] = e.idx;
-    if (a.p) a.p[b] = (float)(e.w / kept);
-  }
+  r.start(top, g.t);
+  r.bin_kept();
+  r.choose(b, g.k, g.tp, g.mp, g.u);
 }
 
 // Chunks of 16384 logits where that makes two workgroups a compute unit, or a row more than 32
@@ -969,6 +1092,18 @@ extern "C" int64_t cia_sample_workspace_bytes(int B, int V) {
 
 template <bool kHalf>
 static int sample_launch(const SampleArgs& a, hipStream_t s) {
+  const dim3 rows((unsigned)a.B), block(kSampleThreads);
+  if (a.V >= 4 && a.V <= 8 * kStep) {
+    if (a.V <= kStep)
+      hipLaunchKernelGGL((k_sample_row<kHalf, 1>), rows, block, 0, s, a);
+    else if (a.V <= 2 * kStep)
+      hipLaunchKernelGGL((k_sample_row<kHalf, 2>), rows, block, 0, s, a);
+    else if (a.V <= 4 * kStep)
+      hipLaunchKernelGGL((k_sample_row<kHalf, 4>), rows, block, 0, s, a);
+    else
+      hipLaunchKernelGGL((k_sample_row<kHalf, 8>), rows, block, 0, s, a);
+    return launch_status();
+  }
   const dim3 grid((unsigned)(a.B * a.chunks));
   if (a.chunk == kMinChunk)
     hipLaunchKernelGGL((k_sample_bins<kHalf, 512, kMinChunk / 2048>), grid, dim3(512), 0, s, a);
