@@ -290,6 +290,7 @@ struct SampleLds {
   uint64_t some[kAll];  // those of one bin
   uint64_t small[kAll];  // in descending order
   double run[kAll];     // sums of their weights
+  int place[kAll];      // places of those of s.some
   unsigned long long mass[kBins];
   uint32_t cnt[kBins];
   double before[kBins + 1];  // mass of the bins before
@@ -662,38 +663,49 @@ struct SampleRow {
     return s.m;
   }
 
-  // n tokens of `from` into s.small in descending order; n <= kAll
-  __device__ __forceinline__ void order(const uint64_t* from, int n) {
+  // n tokens of s.some into s.small in descending order; n <= kAll.  A token's place is how
+  // many are larger: some threads a token, each a part of them.
+  __device__ __forceinline__ void order(int n) {
     __syncthreads();
-    if (n <= kSmall) {
-      // a token's place is how many are larger: some threads a token, each a part of them
-      constexpr int kWays = kSampleThreads / kSmall;
-      const int i = tid & (kSmall - 1), way = tid / kSmall, per = (n + kWays - 1) / kWays;
-      if (tid < kSmall) s.cnt[tid] = 0;
-      __syncthreads();
-      const uint64_t mine = i < n ? from[i] : ~0ull;
+    constexpr int kWays = kSampleThreads / kSmall;
+    const int i = tid & (kSmall - 1), way = tid / kSmall, per = (n + kWays - 1) / kWays;
+    for (int k = tid; k < n; k += kSampleThreads) s.place[k] = 0;
+    __syncthreads();
+    for (int at = i; at < n; at += kSmall) {
+      const uint64_t mine = s.some[at];
       int larger = 0;
 #pragma unroll 8
-      for (int k = way * per; k < min(n, way * per + per); k++) larger += from[k] > mine;
-      if (i < n && larger) atomicAdd(&s.cnt[i], (uint32_t)larger);
-      __syncthreads();
-      if (tid < n) s.small[s.cnt[tid]] = mine;
-      __syncthreads();
-      return;
+      for (int k = way * per; k < min(n, way * per + per); k++) larger += s.some[k] > mine;
+      if (larger) atomicAdd(&s.place[at], larger);
     }
-    int size = 2 * kSmall;
-    while (size < n) size *= 2;
-    for (int i = tid; i < size; i += kSampleThreads) s.small[i] = i < n ? from[i] : 0;
     __syncthreads();
-    for (int k = 2; k <= size; k *= 2)
-      for (int j = k / 2; j; j /= 2) {
-        if (tid < size / 2) {
-          const int u = ((tid & ~(j - 1)) << 1) + (tid & (j - 1)), v = u + j;
-          const uint64_t x = s.small[u], y = s.small[v];
-          if ((x < y) == ((u & k) == 0)) s.small[u] = y, s.small[v] = x;
-        }
-        __syncthreads();
-      }
+    for (int k = tid; k < n; k += kSampleThreads) s.small[s.place[k]] = s.some[k];
+    __syncthreads();
+  }
+
+  // The same for all n tokens of the first bins: a token's place is what its bin starts at
+  // and how many of the bin are larger.
+  __device__ __forceinline__ void order_bins(int n) {
+    __syncthreads();
+    for (int i = tid; i < kBins; i += kSampleThreads) s.cnt[i] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kSampleThreads) {
+      const uint64_t v = s.some[i];
+      const int bin = (int)(R - __builtin_ceil(x_of(key_value((uint32_t)(v >> 32)))));
+      const int at = s.count[bin] + (int)atomicAdd(&s.cnt[bin], 1u);
+      s.run[at] = __builtin_bit_cast(double, v);
+      s.place[at] = bin;
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += kSampleThreads) {
+      const uint64_t mine = __builtin_bit_cast(uint64_t, s.run[i]);
+      const int from = s.count[s.place[i]], to = s.count[s.place[i] + 1];
+      int at = from;
+#pragma unroll 4
+      for (int k = from; k < to; k++) at += __builtin_bit_cast(uint64_t, s.run[k]) > mine;
+      s.small[at] = mine;
+    }
+    __syncthreads();
   }
 
   // sums of the weights of the n tokens in s.small, `mass` before them
@@ -834,7 +846,7 @@ struct SampleRow {
     }
     n = select(lo, hi, least, most);
     if (n > kAll) return equals(how, cnt, mass, nth, goal, n, key_value(most));
-    order(s.some, n);
+    order(n);
     sums(n, mass);
     return ends_at(place(how, n, cnt, nth, goal), mass);
   }
@@ -956,7 +968,7 @@ struct SampleRow {
       // every prefix among them, in order
       uint32_t lo, hi;
       const int n = tops ? select_tops(a.tops + (int64_t)row_at * a.chunks * kTop, first_key(last)) : select(0, ~0u, lo, hi);
-      order(s.some, n);
+      order_bins(n);
       sums(n, 0.0);
       if (by_k && k <= n) kept = s.run[k - 1];
       if (by_p) kept = fmin(kept, s.run[place(kReach, n, 0, 0, need * kept)]);
