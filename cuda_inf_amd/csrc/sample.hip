@@ -919,6 +919,8 @@ struct SampleRow {
       bm = by_m && bin > 0.0 ? (int)bin : 0;
     }
     u = u >= 0.0f ? (u < 1.0f ? u : 0x1.fffffep-1f) : 0.0f;
+    // (a list that the threads' own tokens always fit)
+    const bool every = kKept && total <= kAll;
     // Bins in which the prefixes can end, by whole bins of what decides them: top-k's bk,
     // top-p's p0..p1 for the masses that bk leaves open, the draw's d0..d1 for the masses
     // that the filters can keep, from..to.  (One loop: its code is fetched once, which is
@@ -926,7 +928,7 @@ struct SampleRow {
     int bk = kBins - 1, p0 = 1, p1 = 0, d0 = 0, d1 = 0;
     double from = all, to = all;
 #pragma unroll 1
-    for (int i = by_k ? 0 : by_p ? 1 : 3; i < 5; i++) {
+    for (int i = every ? 5 : by_k ? 0 : by_p ? 1 : 3; i < 5; i++) {
       if (i == 3 && by_m) from = fmin(from, s.before[bm]), to = fmin(to, s.before[bm + 1]);
       const double goal = i < 3 ? need * (i == 1 ? from : to) : (double)u * (i == 3 ? from : to);
       const int bin = bin_with(i == 0 ? kNth : i < 3 ? kReach : kPass, k, goal);
@@ -947,8 +949,8 @@ struct SampleRow {
     double kept = all;  // mass of what the filters keep
     Ends e;
     // top-p's goal is a part of top-k's mass
-    const int last = by_k && by_p ? bk : min(by_p ? p1 : bk, by_m ? bm : kBins - 1);
-    const bool few = (by_k || by_p || by_m) && s.count[last + 1] <= kAll;
+    const int last = every ? __builtin_amdgcn_readfirstlane(s.last) : by_k && by_p ? bk : min(by_p ? p1 : bk, by_m ? bm : kBins - 1);
+    const bool few = every || ((by_k || by_p || by_m) && s.count[last + 1] <= kAll);
     int f0 = kBins, f1 = 0;  // the bins of the filters, from the first to the last
     if (by_p) f0 = p0, f1 = p1;
     if (by_k) f0 = min(f0, bk), f1 = max(f1, bk);
