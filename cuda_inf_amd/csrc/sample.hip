@@ -135,6 +135,29 @@ struct PowerOf2 {
   }
 };
 
+// Sums over the lanes up to each: within 16 of them, then with those before (a step by
+// DPP takes 8 bytes in two moves; by a shuffle through LDS six steps took 850 cycles).
+template <int kCtrl, int kRows, typename T>
+__device__ __forceinline__ T dpp_or_0(T v) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl, kRows, 0xF, false));
+  } else {
+    u32x2 w = __builtin_bit_cast(u32x2, v);
+    w[0] = dpp_or_0<kCtrl, kRows>(w[0]), w[1] = dpp_or_0<kCtrl, kRows>(w[1]);
+    return __builtin_bit_cast(T, w);
+  }
+}
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+  v += dpp_or_0<0x111, 0xF>(v);  // row_shr
+  v += dpp_or_0<0x112, 0xF>(v);
+  v += dpp_or_0<0x114, 0xF>(v);
+  v += dpp_or_0<0x118, 0xF>(v);
+  v += dpp_or_0<0x142, 0xA>(v);  // row_bcast15, to the odd rows
+  v += dpp_or_0<0x143, 0xC>(v);  // row_bcast31, to the upper half
+  return v;
+}
+
 // a bin's upper edge, bin 0's being 1: 2^(-bin / 16)
 __device__ __forceinline__ double bin_edge(int bin) {
   const int i = bin & 3, j = bin >> 2 & 3;
@@ -234,11 +257,7 @@ __global__ __launch_bounds__(kThreads) void k_sample_bins(SampleArgs a) {
     const int lane = tid & 63, wave = tid >> 6, i = min(2 * tid, kBins - 2);
     const bool mine = 2 * tid < kBins;
     const int k0 = mine ? (int)(bins[i] >> kCountShift) : 0, k1 = mine ? (int)(bins[i + 1] >> kCountShift) : 0;
-    int upto = k0 + k1;
-    for (int off = 1; off < 64; off <<= 1) {
-      const int o = __shfl_up(upto, off);
-      if (lane >= off) upto += o;
-    }
+    int upto = wave_scan(k0 + k1);
     if (lane == 63) wcount[wave] = upto;
     __syncthreads();
     for (int w = 0; w < wave; w++) upto += wcount[w];
@@ -325,6 +344,8 @@ struct SampleRow {
   bool inf;     // some are +inf: they count as 0, the others as -inf
   int tid, lane, wave;
   int taken;    // tokens that the thread has in the list
+  int group_count;  // of bin_with
+  double group_before;
   PowerOf2 power;
   f32x4 held[kKept ? kPer : 1];
 
@@ -474,28 +495,36 @@ struct SampleRow {
     scan((uint32_t)(v0 >> kCountShift), (uint32_t)(v1 >> kCountShift), v0 & kMass, v1 & kMass);
   }
 
+  // first and what the waves before this one have
+  template <typename T>
+  __device__ __forceinline__ T before_wave(T first, const T (&of)[kSampleWaves]) const {
+    T at[kSampleWaves];
+#pragma unroll
+    for (int w = 0; w < kSampleWaves; w++) at[w] = of[w];
+#pragma unroll
+    for (int w = 0; w < kSampleWaves - 1; w++) first += w < wave ? at[w] : T(0);
+    return first;
+  }
+
   // s.count and s.before, from two bins a thread: 2 tid and the next
   __device__ __forceinline__ void scan(uint32_t c0, uint32_t c1, unsigned long long u0, unsigned long long u1) {
     const int b = min(2 * tid, kBins - 2);
     const bool mine = 2 * tid < kBins;
     const int k0 = mine ? (int)c0 : 0, k1 = mine ? (int)c1 : 0;
     const double m0 = mine ? mass_in(b, u0) : 0.0, m1 = mine ? mass_in(b + 1, u1) : 0.0;
-    double run = m0 + m1;
-    int upto = k0 + k1;
-    for (int off = 1; off < 64; off <<= 1) {
-      const double um = __shfl_up(run, off);
-      const int uk = __shfl_up(upto, off);
-      if (lane >= off) run += um, upto += uk;
-    }
+    double run = wave_scan(m0 + m1);
+    int upto = wave_scan(k0 + k1);
     if (lane == 63) s.dsum[wave] = run, s.lo[wave] = (uint32_t)upto;
-    if (k0 + k1) atomicMax(&s.last, k1 ? b + 1 : b);
+    const uint64_t any = __ballot(k0 + k1 > 0), odd = __ballot(k1 > 0);
+    if (lane == 0 && any) {
+      const int at = 63 - __builtin_clzll(any);
+      atomicMax(&s.last, 2 * (64 * wave + at) + (int)(odd >> at & 1));
+    }
     __syncthreads();
-    double base = 0.0;
-    int kbase = 0;
-    for (int v = 0; v < wave; v++) base += s.dsum[v], kbase += (int)s.lo[v];
+    run += before_wave(0.0, s.dsum), upto += (int)before_wave(0u, s.lo);
     if (mine) {
-      s.before[b + 2] = base + run, s.count[b + 2] = kbase + upto;
-      s.before[b + 1] = base + run - m1, s.count[b + 1] = kbase + upto - k1;
+      s.before[b + 2] = run, s.count[b + 2] = upto;
+      s.before[b + 1] = run - m1, s.count[b + 1] = upto - k1;
     }
     if (tid == 0) s.before[0] = 0.0, s.count[0] = 0;
     __syncthreads();
@@ -503,19 +532,21 @@ struct SampleRow {
 
   // the bin in which a prefix ends: the first whose sum satisfies the goal, the last
   // that holds any where none does; each wave looks by itself, in 56 groups of 12 bins,
-  // then in one of them
+  // whose sums it keeps (keep_groups), then in one of them
+  static constexpr int kPart = kBins / 56;
+  __device__ __forceinline__ void keep_groups() {
+    const int b = min((lane + 1) * kPart, kBins);
+    group_count = s.count[b], group_before = s.before[b];
+  }
   __device__ __forceinline__ int bin_with(Goal how, int nth, double goal) const {
-    constexpr int kPart = kBins / 56;
-    int at = 0;
-#pragma unroll 1
-    for (int step = kPart; step; step /= kPart) {
-      const int b = min(at + (lane + 1) * step, kBins);
-      const bool here = how == kNth ? s.count[b] >= nth : how == kReach ? s.before[b] >= goal : s.before[b] > goal;
-      const uint64_t set = __ballot(here);
-      if (!set) return __builtin_amdgcn_readfirstlane(s.last);
-      at += __builtin_ctzll(set) * step;
-    }
-    return min(at, kBins - 1);
+    const auto ends = [&](int count, double before) {
+      return __ballot(how == kNth ? count >= nth : how == kReach ? before >= goal : before > goal);
+    };
+    uint64_t set = ends(group_count, group_before);
+    if (!set) return __builtin_amdgcn_readfirstlane(s.last);
+    const int at = __builtin_ctzll(set) * kPart, b = min(at + lane + 1, kBins);
+    set = ends(s.count[b], s.before[b]);
+    return min(at + __builtin_ctzll(set), kBins - 1);
   }
 
   // the chunks that may have a token in the bins up to `to`: whose largest is in one
@@ -648,6 +679,30 @@ struct SampleRow {
     return s.m;
   }
 
+  // The tokens that the threads keep with keys lo..hi into s.some (kAll at most): how many.
+  __device__ __forceinline__ int select_held(uint32_t lo_key, uint32_t hi_key) {
+    const float lo = key_value(__builtin_amdgcn_readfirstlane(lo_key)), hi = key_value(__builtin_amdgcn_readfirstlane(hi_key));
+    int mine = 0;
+    each([&](int, const f32x4& x) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) mine += (x[e] >= lo) & (x[e] <= hi);
+    });
+    int at = wave_scan(mine);
+    if (lane == 63) s.lo[wave] = (uint32_t)at;
+    __syncthreads();
+    at += (int)before_wave(0u, s.lo) - mine;
+    int n = 0;
+    for (int w = 0; w < kSampleWaves; w++) n += (int)s.lo[w];
+    each([&](int nth, const f32x4& x) __attribute__((always_inline)) {
+      if (__any((x[0] >= lo) | (x[1] >= lo) | (x[2] >= lo) | (x[3] >= lo)))
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if ((x[e] >= lo) & (x[e] <= hi)) s.some[min(at++, kAll - 1)] = (uint64_t)order_key(x[e]) << 32 | (uint32_t)~index_of(nth + e);
+    });
+    __syncthreads();
+    return n;
+  }
+
   // The tokens of the chunks' tops with keys from lo on into s.some: how many.
   __device__ __forceinline__ int select_tops(const uint64_t* tops, uint32_t lo) {
     __syncthreads();
@@ -712,16 +767,14 @@ struct SampleRow {
   __device__ __forceinline__ void sums(int n, double mass) {
     for (int i0 = 0; i0 < n; i0 += kSampleThreads) {
       const int i = i0 + tid;
-      double run = i < n ? weight(key_value((uint32_t)(s.small[i] >> 32))) : 0.0;
-      for (int off = 1; off < 64; off <<= 1) {
-        const double o = __shfl_up(run, off);
-        if (lane >= off) run += o;
-      }
+      const double run = wave_scan(i < n ? weight(key_value((uint32_t)(s.small[i] >> 32))) : 0.0);
       if (lane == 63) s.dsum[wave] = run;
       __syncthreads();
-      for (int v = 0; v < wave; v++) mass += s.dsum[v];
-      if (i < n) s.run[i] = mass + run;
-      for (int v = wave; v < kSampleWaves; v++) mass += s.dsum[v];
+      const double base = before_wave(mass, s.dsum);
+      if (i < n) s.run[i] = base + run;
+      if (i0 + kSampleThreads < n) {
+        for (int w = 0; w < kSampleWaves; w++) mass += s.dsum[w];
+      }
       __syncthreads();
     }
   }
@@ -771,26 +824,21 @@ struct SampleRow {
     __syncthreads();
     const int kc = (int)s.cnt[tid];
     const unsigned long long km = s.mass[tid];
-    unsigned long long im = km;
-    int ik = kc;
-    for (int off = 1; off < 64; off <<= 1) {
-      const unsigned long long um = __shfl_up(im, off);
-      const int uk = __shfl_up(ik, off);
-      if (lane >= off) im += um, ik += uk;
-    }
+    unsigned long long im = wave_scan(km);
+    int ik = wave_scan(kc);
     if (lane == 63) s.key[wave] = im, s.lo[wave] = (uint32_t)ik;
     __syncthreads();
-    for (int w = 0; w < wave; w++) im += s.key[w], ik += (int)s.lo[w];
+    im += before_wave((uint64_t)0, s.key), ik += (int)before_wave(0u, s.lo);
     const double after = mass + mass_in(bin, im);
     const uint32_t low = most - ((((uint32_t)tid + 1) << shift) - 1);  // the part's least key
-    if (kc) {
-      const bool here = how == kNth ? cnt + ik >= nth
-                        : how == kReach ? after >= goal
-                        : how == kPass ? after > goal
-                                       : !(ratio(key_value(low < least || low > most ? least : low)) >= goal);
-      if (here) atomicMin(&s.at, tid);
-      atomicMax(&s.bin, tid);
-    }
+    bool here = false;
+    if (kc)
+      here = how == kNth ? cnt + ik >= nth
+             : how == kReach ? after >= goal
+             : how == kPass ? after > goal : !(ratio(key_value(low < least || low > most ? least : low)) >= goal);
+    const uint64_t ends = __ballot(here), any = __ballot(kc > 0);
+    if (lane == 0 && ends) atomicMin(&s.at, 64 * wave + __builtin_ctzll(ends));
+    if (lane == 0 && any) atomicMax(&s.bin, 64 * wave + 63 - __builtin_clzll(any));
     __syncthreads();
     const int at = s.at < kSub ? s.at : s.bin;
     if (tid == at) {
@@ -907,6 +955,7 @@ struct SampleRow {
 
   // the row's token, after its bins
   __device__ __forceinline__ void choose(int row_at, int k, float tp, float mp, float u) {
+    keep_groups();
     const int total = s.count[kBins];
     const double all = s.before[kBins], need = tp > 0.0f ? (double)tp : 0.0, least = mp < 1.0f ? (double)mp : 1.0;
     const bool by_k = k > 0 && k < total, by_p = tp < 1.0f;
@@ -958,18 +1007,21 @@ struct SampleRow {
     // few enough: all of them; else those bins and the draw's, if they fit
     bool listed = few || s.count[d1 + 1] - s.count[d0] + (f0 <= f1 ? s.count[f1 + 1] - s.count[f0] : 0) <= kCap;
     const bool tops = !kKept && kPer * kStep == kMinChunk && few && last < s.covered;  // they are at hand
+    uint32_t lo[kRanges], hi[kRanges];
     if (listed && !tops) {
-      uint32_t lo[kRanges], hi[kRanges];
       keys_of(few ? 0 : d0, few ? last : d1, lo[0], hi[0]);
       lo[1] = lo[0], hi[1] = hi[0];
       if (!few && f0 <= f1) keys_of(f0, f1, lo[1], hi[1]);
       if constexpr (!kKept) chunks_with(few ? last : max(d1, f1));
-      listed = take(lo, hi);
+      if (!kKept || !few) listed = take(lo, hi);
     }
     if (few && listed) {
       // every prefix among them, in order
-      uint32_t lo, hi;
-      const int n = tops ? select_tops(a.tops + (int64_t)row_at * a.chunks * kTop, first_key(last)) : select(0, ~0u, lo, hi);
+      int n;
+      if constexpr (kKept)
+        n = select_held(lo[0], hi[0]);
+      else
+        n = tops ? select_tops(a.tops + (int64_t)row_at * a.chunks * kTop, first_key(last)) : select(0, ~0u, lo[0], hi[0]);
       order_bins(n);
       sums(n, 0.0);
       if (by_k && k <= n) kept = s.run[k - 1];
