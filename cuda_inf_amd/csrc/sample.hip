@@ -646,37 +646,35 @@ struct SampleRow {
     return !__syncthreads_or(have > kSlots);
   }
 
-  __device__ __forceinline__ void least_most(uint32_t& least, uint32_t& most) {
-    for (int off = 32; off; off >>= 1) {
-      const uint32_t u = __shfl_xor(least, off), v = __shfl_xor(most, off);
-      least = u < least ? u : least;
-      most = v > most ? v : most;
-    }
-    if (lane == 0) s.lo[wave] = least, s.hi[wave] = most;
+  // Places in s.some for a thread's `mine` tokens, in the threads' order: from which on;
+  // n: of all.
+  __device__ __forceinline__ int places(int mine, int& n) {
+    int at = wave_scan(mine);
     __syncthreads();
-    for (int w = 0; w < kSampleWaves; w++) {
-      least = s.lo[w] < least ? s.lo[w] : least;
-      most = s.hi[w] > most ? s.hi[w] : most;
-    }
+    if (lane == 63) s.lo[wave] = (uint32_t)at;
+    __syncthreads();
+    at += (int)before_wave(0u, s.lo) - mine;
+    n = 0;
+#pragma unroll
+    for (int w = 0; w < kSampleWaves; w++) n += (int)s.lo[w];
+    return at;
   }
 
-  // The tokens in the list with keys lo..hi into s.some (kAll at most): how many there are,
-  // and their least and largest key.
-  __device__ __forceinline__ int select(uint32_t lo, uint32_t hi, uint32_t& least, uint32_t& most) {
-    __syncthreads();
-    if (tid == 0) s.m = 0;
-    __syncthreads();
-    least = ~0u, most = 0;
+  // The tokens in the list with keys lo..hi into s.some (kAll at most): how many.
+  __device__ __forceinline__ int select(uint32_t lo, uint32_t hi) {
+    uint64_t set = 0;  // which of the thread's
+#pragma unroll 4
     for (int i = 0; i < taken; i++) {
       const uint32_t k = order_key(s.value[i][tid]);
-      if (k < lo || k > hi) continue;
-      least = k < least ? k : least;
-      most = k > most ? k : most;
-      const int n = atomicAdd(&s.m, 1);
-      if (n < kAll) s.some[n] = (uint64_t)k << 32 | (uint32_t)~index_of(s.nth[i][tid]);
+      set |= (uint64_t)(k >= lo && k <= hi) << i;
     }
-    least_most(least, most);
-    return s.m;
+    int n, at = places(__popcll(set), n);
+    for (; set && at < kAll; set &= set - 1, at++) {
+      const int i = __builtin_ctzll(set);
+      s.some[at] = (uint64_t)order_key(s.value[i][tid]) << 32 | (uint32_t)~index_of(s.nth[i][tid]);
+    }
+    __syncthreads();
+    return n;
   }
 
   // The tokens that the threads keep with keys lo..hi into s.some (kAll at most): how many.
@@ -687,12 +685,7 @@ struct SampleRow {
 #pragma unroll
       for (int e = 0; e < 4; e++) mine += (x[e] >= lo) & (x[e] <= hi);
     });
-    int at = wave_scan(mine);
-    if (lane == 63) s.lo[wave] = (uint32_t)at;
-    __syncthreads();
-    at += (int)before_wave(0u, s.lo) - mine;
-    int n = 0;
-    for (int w = 0; w < kSampleWaves; w++) n += (int)s.lo[w];
+    int n, at = places(mine, n);
     each([&](int nth, const f32x4& x) __attribute__((always_inline)) {
       if (__any((x[0] >= lo) | (x[1] >= lo) | (x[2] >= lo) | (x[3] >= lo)))
 #pragma unroll
@@ -703,19 +696,36 @@ struct SampleRow {
     return n;
   }
 
+  // The tops of 8 chunks, one token of each a thread, on their way: those of the first 8
+  // before it is known whether they are enough.
+  static_assert(kTop == kSampleThreads);
+  struct Tops {
+    uint64_t v[8];
+  };
+  __device__ __forceinline__ void load_tops(const uint64_t* tops, int chunk, Tops& t) const {
+#pragma unroll
+    for (int i = 0; i < 8; i++) t.v[i] = tops[min(chunk + i, a.chunks - 1) * kTop + tid];
+  }
   // The tokens of the chunks' tops with keys from lo on into s.some: how many.
-  __device__ __forceinline__ int select_tops(const uint64_t* tops, uint32_t lo) {
-    __syncthreads();
-    if (tid == 0) s.m = 0;
-    __syncthreads();
-    const int all = a.chunks * kTop;
-#pragma unroll 8
-    for (int i = tid; i < all; i += kSampleThreads) {
-      const uint64_t v = i % kTop < s.listed[i / kTop] ? tops[i] : 0;
-      if ((uint32_t)(v >> 32) >= lo) s.some[atomicAdd(&s.m, 1)] = v;
+  __device__ __forceinline__ int select_tops(const uint64_t* tops, Tops& t, uint32_t lo) {
+    int n = 0;
+    for (int chunk = 0; chunk < a.chunks; chunk += 8) {
+      if (chunk) load_tops(tops, chunk, t);
+      int mine = 0;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const bool in = chunk + i < a.chunks && tid < s.listed[min(chunk + i, a.chunks - 1)] && (uint32_t)(t.v[i] >> 32) >= lo;
+        if (!in) t.v[i] = 0;
+        mine += in;
+      }
+      int more, at = n + places(mine, more);
+      n += more;
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (t.v[i]) s.some[min(at++, kAll - 1)] = t.v[i];
     }
     __syncthreads();
-    return s.m;
+    return n;
   }
 
   // n tokens of s.some into s.small in descending order; n <= kAll.  A token's place is how
@@ -763,11 +773,12 @@ struct SampleRow {
     __syncthreads();
   }
 
-  // sums of the weights of the n tokens in s.small, `mass` before them
+  // sums of the weights of the n tokens in s.small, `mass` before them; s.some: the weights
   __device__ __forceinline__ void sums(int n, double mass) {
     for (int i0 = 0; i0 < n; i0 += kSampleThreads) {
       const int i = i0 + tid;
-      const double run = wave_scan(i < n ? weight(key_value((uint32_t)(s.small[i] >> 32))) : 0.0);
+      const double w = i < n ? weight(key_value((uint32_t)(s.small[i] >> 32))) : 0.0, run = wave_scan(w);
+      if (i < n) s.some[i] = __builtin_bit_cast(uint64_t, w);
       if (lane == 63) s.dsum[wave] = run;
       __syncthreads();
       const double base = before_wave(mass, s.dsum);
@@ -802,8 +813,7 @@ struct SampleRow {
   // the token at a place of the ordered list, `mass` before the list
   __device__ __forceinline__ Ends ends_at(int at, double mass) const {
     if (at < 0) return Ends{mass, 0.0, -1};
-    const uint64_t v = s.small[at];
-    return Ends{s.run[at], weight(key_value((uint32_t)(v >> 32))), (int)~(uint32_t)v};
+    return Ends{s.run[at], __builtin_bit_cast(double, s.some[at]), (int)~(uint32_t)s.small[at]};
   }
 
   // One of kSub parts of the keys least..most, as `each` gives the tokens, in which the prefix ends:
@@ -892,8 +902,8 @@ struct SampleRow {
         }
       });
     }
-    n = select(lo, hi, least, most);
-    if (n > kAll) return equals(how, cnt, mass, nth, goal, n, key_value(most));
+    n = select(lo, hi);
+    if (n > kAll) return equals(how, cnt, mass, nth, goal, n, key_value(hi));
     order(n);
     sums(n, mass);
     return ends_at(place(how, n, cnt, nth, goal), mass);
@@ -954,7 +964,7 @@ struct SampleRow {
   }
 
   // the row's token, after its bins
-  __device__ __forceinline__ void choose(int row_at, int k, float tp, float mp, float u) {
+  __device__ __forceinline__ void choose(int row_at, int k, float tp, float mp, float u, const uint64_t* tops_at, Tops& first) {
     keep_groups();
     const int total = s.count[kBins];
     const double all = s.before[kBins], need = tp > 0.0f ? (double)tp : 0.0, least = mp < 1.0f ? (double)mp : 1.0;
@@ -968,38 +978,45 @@ struct SampleRow {
       bm = by_m && bin > 0.0 ? (int)bin : 0;
     }
     u = u >= 0.0f ? (u < 1.0f ? u : 0x1.fffffep-1f) : 0.0f;
-    // (a list that the threads' own tokens always fit)
-    const bool every = kKept && total <= kAll;
     // Bins in which the prefixes can end, by whole bins of what decides them: top-k's bk,
     // top-p's p0..p1 for the masses that bk leaves open, the draw's d0..d1 for the masses
     // that the filters can keep, from..to.  (One loop: its code is fetched once, which is
-    // most of the time of code that runs once.)
-    int bk = kBins - 1, p0 = 1, p1 = 0, d0 = 0, d1 = 0;
+    // most of the time of code that runs once.)  Where all tokens up to a filter's bin are
+    // few, they are put in order and the other bins not looked for.
+    int bk = 0, p0 = 0, p1 = kBins - 1, d0 = 0, d1 = kBins - 1;
+    // (top-p's goal is a part of top-k's mass: min-p does not end before it)
+    int last = __builtin_amdgcn_readfirstlane(s.last);
+    if (by_m && !(by_k && by_p)) last = min(last, bm);
+    bool few = s.count[last + 1] <= kAll;
     double from = all, to = all;
 #pragma unroll 1
-    for (int i = every ? 5 : by_k ? 0 : by_p ? 1 : 3; i < 5; i++) {
+    for (int i = by_k ? 0 : by_p ? 1 : 3; i < 5 && !few; i++) {
       if (i == 3 && by_m) from = fmin(from, s.before[bm]), to = fmin(to, s.before[bm + 1]);
       const double goal = i < 3 ? need * (i == 1 ? from : to) : (double)u * (i == 3 ? from : to);
       const int bin = bin_with(i == 0 ? kNth : i < 3 ? kReach : kPass, k, goal);
       if (i == 0) {
         bk = bin, from = s.before[bin], to = s.before[bin + 1];
-        if (!by_p) i = 2;
       } else if (i == 1) {
-        p0 = bin;
+        p0 = p1 = bin;
+        if (!by_k) i = 2;  // (one goal)
       } else if (i == 2) {
         p1 = bin;
-        from = fmin(from, s.before[p0]), to = fmin(to, s.before[p1 + 1]);
       } else if (i == 3) {
-        d0 = bin;
+        d0 = d1 = bin;
+        if (from == to) i = 4;
       } else {
         d1 = bin;
+      }
+      if (i == 2) from = fmin(from, s.before[p0]), to = fmin(to, s.before[p1 + 1]);
+      if (i == 0 || i == 2) {
+        const int upto = min(last, by_k ? bk : p1);
+        few = s.count[upto + 1] <= kAll;
+        if (few) last = upto;
+        if (!by_p) i = 2;
       }
     }
     double kept = all;  // mass of what the filters keep
     Ends e;
-    // top-p's goal is a part of top-k's mass
-    const int last = every ? __builtin_amdgcn_readfirstlane(s.last) : by_k && by_p ? bk : min(by_p ? p1 : bk, by_m ? bm : kBins - 1);
-    const bool few = every || ((by_k || by_p || by_m) && s.count[last + 1] <= kAll);
     int f0 = kBins, f1 = 0;  // the bins of the filters, from the first to the last
     if (by_p) f0 = p0, f1 = p1;
     if (by_k) f0 = min(f0, bk), f1 = max(f1, bk);
@@ -1021,7 +1038,7 @@ struct SampleRow {
       if constexpr (kKept)
         n = select_held(lo[0], hi[0]);
       else
-        n = tops ? select_tops(a.tops + (int64_t)row_at * a.chunks * kTop, first_key(last)) : select(0, ~0u, lo[0], hi[0]);
+        n = tops ? select_tops(tops_at, first, first_key(last)) : select(0, ~0u);
       order_bins(n);
       sums(n, 0.0);
       if (by_k && k <= n) kept = s.run[k - 1];
@@ -1036,7 +1053,7 @@ struct SampleRow {
         double goal = (double)u * kept;
         int bin;
         if (step == 0) {
-          how = kNth, bin = bk;
+          how = kNth, bin = few ? bin_with(kNth, k, 0.0) : bk;  // (few, but too many for one thread)
         } else if (step == 1) {
           if (!by_p) continue;
           how = kReach, goal = need * kept;
@@ -1089,6 +1106,9 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
         0.0, 0.0, 1.0, 1.0, 0.0f, false, tid, tid & 63, tid >> 6, 0};
   const Given g(a, b);
   typename Row::Pairs first;
+  typename Row::Tops tops;
+  const uint64_t* const tops_at = a.tops + (int64_t)b * a.chunks * kTop;
+  if constexpr (kPer * kStep == kMinChunk) r.load_tops(tops_at, 0, tops);
   const uint64_t best = r.largest(first);
   if (best == 0 || !(g.t > 0.0f)) {
     r.put(b, best ? (int)~(uint32_t)best : -1, best ? 1.0f : 0.0f);
@@ -1096,7 +1116,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
   }
   r.start(key_value((uint32_t)(best >> 32)), g.t);
   r.add_up(first);
-  r.choose(b, g.k, g.tp, g.mp, g.u);
+  r.choose(b, g.k, g.tp, g.mp, g.u, tops_at, tops);
 }
 
 // The same for a row of 4..kPer * kStep logits by itself, which the threads keep in registers.
@@ -1129,7 +1149,8 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_row(SampleArgs a) {
   }
   r.start(top, g.t);
   r.bin_kept();
-  r.choose(b, g.k, g.tp, g.mp, g.u);
+  typename Row::Tops tops;
+  r.choose(b, g.k, g.tp, g.mp, g.u, nullptr, tops);
 }
 
 // Chunks of 16384 logits where that makes two workgroups a compute unit, or a row more than 32
