@@ -1153,14 +1153,15 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_row(SampleArgs a) {
   r.choose(b, g.k, g.tp, g.mp, g.u, nullptr, tops);
 }
 
-// Chunks of 16384 logits where that makes two workgroups a compute unit, or a row more than 32
-// of the smaller ones; else of 8192, with their tops: of the largest tokens the choice
+// Chunks of 16384 logits where there are more than 1024 of them, or a row has more than 32 of
+// the smaller ones; else of 8192, with their tops: of the largest tokens the choice
 // mostly falls on, the row need not be read again.  us with 8192 / 16384, of rows of 131 072:
 //   rows (chunks of 16384)         1 (8)   32 (256)     64 (512)   128 (1024)    256 (2048)
-//   top-k and top-p          27.0 / 34.3  32.6 / 41.4  37.6 / 44.2  46.6 / 51.0   71.3 / 65.8
-//   top-p, broad: read again 34.8 / 36.7  72.2 / 67.0  76.7 / 69.9  88.8 / 78.8  109.9 / 90.7
+//   top-k and top-p          18.6 / 29.3  23.0 / 35.3  27.9 / 38.3  36.6 / 45.0   61.8 / 61.0
+//   top-p, broad: read again 29.0 / 32.2  59.0 / 54.6  63.1 / 57.7  74.6 / 65.9   98.0 / 79.0
+constexpr int kMostTopped = 1024;
 static int sample_chunk(int B, int V) {
-  return (int64_t)B * ((V + kMaxChunk - 1) / kMaxChunk) >= 512 || V > 32 * kMinChunk ? kMaxChunk : kMinChunk;
+  return (int64_t)B * ((V + kMaxChunk - 1) / kMaxChunk) > kMostTopped || V > 32 * kMinChunk ? kMaxChunk : kMinChunk;
 }
 
 }  // namespace cia
@@ -1173,7 +1174,7 @@ extern "C" int64_t cia_sample_workspace_bytes(int B, int V) {
   // (the most that B rows or fewer need: a smaller batch may have smaller chunks)
   const int64_t big = (V + kMaxChunk - 1) / kMaxChunk, small = (V + kMinChunk - 1) / kMinChunk;
   int64_t n = (int64_t)B * (sample_chunk(B, V) == kMinChunk ? small : big);
-  if (sample_chunk(1, V) == kMinChunk) n = std::max(n, std::min<int64_t>(B, 511 / big) * small);
+  if (sample_chunk(1, V) == kMinChunk) n = std::max(n, std::min<int64_t>(B, kMostTopped / big) * small);
   return 16 + n * (int64_t)(sizeof(ChunkHead) + (kBins + kTop) * sizeof(uint64_t));
 }
 

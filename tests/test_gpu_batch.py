@@ -531,7 +531,7 @@ def test_sample_frequencies(K, dev):
 
 
 @pytest.mark.parametrize("B,V", [(3, 8191), (3, 8192), (3, 8193), (2, 262144), (2, 262145), (70, 65536), (300, 20001),
-                                 (520, 16384), (600, 3)])
+                                 (520, 16384), (600, 3), (256, 65536), (257, 65536)])
 @pytest.mark.parametrize("half", [False, True])
 def test_sample_about_a_chunks_edge(K, dev, B, V, half):
     """Rows of one chunk and of many, of both sizes, one more logit and one less, batches on both sides of the
@@ -565,6 +565,19 @@ def test_sample_of_tokens_that_one_thread_meets(K, dev):
     l[4, 5::2048] = 1.0  # (equals)
     for f in (dict(top_k=60), dict(top_p=0.9), dict(top_k=150, top_p=0.7, min_p=0.01), dict(min_p=0.05), dict(),
               dict(temperature=0.5, top_k=1000)):
+        check_sample(K, dev, l, rng.random(6), f"{f}", **{k: np.full(6, v) for k, v in f.items()})
+
+
+@pytest.mark.parametrize("V", [3, 4, 5, 1023, 1025, 2047, 2048, 2049, 4096, 4097, 8191, 8192, 8193, 16383, 16384, 16385, 270000])
+@pytest.mark.parametrize("half", [False, True])
+def test_sample_of_rows_about_the_limits_of_their_kernels(K, dev, V, half):
+    """Broad and narrow rows, one whose likely tokens are the last, one of equals, one with numbers that are none."""
+    rng = np.random.default_rng(V)
+    l = np.stack([1.5 * rng.standard_normal(V), 9 * rng.standard_normal(V), np.where(np.arange(V) >= V - 5, 7.0, 0.0) + rng.random(V),
+                  np.full(V, -3.0), rng.standard_normal(V), -20 * rng.random(V)]).astype(np.float16 if half else np.float32)
+    l[4, V // 2], l[4, 0], l[4, -1] = np.nan, -np.inf, -np.inf
+    for f in (dict(), dict(top_k=1), dict(top_k=40), dict(top_k=1200), dict(top_p=0.8), dict(top_p=0.99, top_k=700), dict(min_p=0.2),
+              dict(top_k=50, top_p=0.6, min_p=0.1), dict(temperature=0.0), dict(temperature=0.3, min_p=0.01)):
         check_sample(K, dev, l, rng.random(6), f"{f}", **{k: np.full(6, v) for k, v in f.items()})
 
 
