@@ -80,39 +80,32 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __builtin_bit_cast(float, k ^ ((uint32_t)((int32_t)~k >> 31) | 0x80000000u));
 }
 
-// Four neighbouring logits from i on, in two steps, so that many loads can be out before
-// any is looked at.  whole: all four are in the row; else those past its end are -inf.
+// Four neighbouring logits of a row from i on, in two steps, so that many loads can be out
+// before any is looked at.  `_in`: those past the row's end V are -inf; the row's last four
+// are read for them, and moved.
 template <bool kHalf>
 struct Logits {
   using T = typename std::conditional<kHalf, _Float16, float>::type;
   typename std::conditional<kHalf, f16x4, f32x4>::type x;
-  __device__ __forceinline__ void load(const void* row, int i, int V, bool whole) {
-    const T* const r = (const T*)row;
-    if (whole) {
-      __builtin_memcpy(&x, r + i, sizeof(x));
-    } else {
+  __device__ __forceinline__ void load(const void* row, int i) { __builtin_memcpy(&x, (const T*)row + i, sizeof(x)); }
+  __device__ __forceinline__ void load_in(const void* row, int i, int V) { load(row, min(i, V - 4)); }
+  // (of a row of less than 4)
+  __device__ __forceinline__ void load_few(const void* row, int V) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) x[e] = r[min(i + e, V - 1)];
-    }
-  }
-  // of a row of 4 or more: the last four for those past its end
-  __device__ __forceinline__ void load_in(const void* row, int i, int V) {
-    __builtin_memcpy(&x, (const T*)row + min(i, V - 4), sizeof(x));
+    for (int e = 0; e < 4; e++) x[e] = ((const T*)row)[max(e + V - 4, 0)];
   }
   __device__ __forceinline__ f32x4 get_in(int i, int V) const {
     const int past = i - min(i, V - 4);
-    f32x4 y;
-#pragma unroll
-    for (int e = 0; e < 4; e++) y[e] = (float)x[e];
+    f32x4 y = get();
     const float none = -__builtin_inff();
     if (past & 1) y = f32x4{y[1], y[2], y[3], none};
     if (past & 2) y = f32x4{y[2], y[3], none, none};
     return past > 3 ? f32x4{none, none, none, none} : y;
   }
-  __device__ __forceinline__ f32x4 get(int i, int V, bool whole) const {
+  __device__ __forceinline__ f32x4 get() const {
     f32x4 y;
 #pragma unroll
-    for (int e = 0; e < 4; e++) y[e] = whole || i + e < V ? (float)x[e] : -__builtin_inff();
+    for (int e = 0; e < 4; e++) y[e] = (float)x[e];
     return y;
   }
 };
@@ -169,7 +162,7 @@ __device__ __forceinline__ double bin_edge(int bin) {
 __device__ __forceinline__ double temperature_scale(float t) { return 16 * 1.44269504088896340736 / (double)t; }
 
 // ---------------------------------------------------------------- the bins
-// grid = rows * chunks, block = kThreads, 4 kVec logits of the chunk a thread, in registers:
+// Of rows of more than kMaxChunk.  grid = rows * chunks, block = kThreads, 4 kVec logits of the chunk a thread, in registers:
 // all loads of a chunk are out together, and its largest is known before its bins.  22 vector
 // instructions a logit with all that is around them, vector units 52 % busy (256 rows of 131 072).
 template <bool kHalf, int kThreads, int kVec>
@@ -185,18 +178,13 @@ __global__ __launch_bounds__(kThreads) void k_sample_bins(SampleArgs a) {
   const int i0 = chunk * (kVec * kEach) + 4 * tid;
   const bool whole = (chunk + 1) * (kVec * kEach) <= a.V;
   Logits<kHalf> in[kVec];
-  if (whole) {
 #pragma unroll
-    for (int i = 0; i < kVec; i++) in[i].load(row, i0 + kEach * i, a.V, true);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kVec; i++) in[i].load(row, i0 + kEach * i, a.V, false);
-  }
+  for (int i = 0; i < kVec; i++) in[i].load_in(row, i0 + kEach * i, a.V);
   const float t = a.temperature ? a.temperature[b] : 1.0f;
   for (int i = tid; i < kBins; i += kThreads) bins[i] = 0;
   f32x4 x[kVec];
 #pragma unroll
-  for (int i = 0; i < kVec; i++) x[i] = in[i].get(i0 + kEach * i, a.V, whole);
+  for (int i = 0; i < kVec; i++) x[i] = whole ? in[i].get() : in[i].get_in(i0 + kEach * i, a.V);
   // (a NaN is neither the largest nor of any bin: no comparison holds for it)
   float top = -__builtin_inff();
 #pragma unroll
@@ -592,33 +580,40 @@ struct SampleRow {
       for (int k = 0; k < kPer; k++) fn(4 * k, held[k]);
       return;
     }
-    constexpr int kAhead = 8, kAt = kAhead / (kKept ? 8 : kPer);  // steps whose loads are out together, of kAt chunks
+    // kAhead steps' loads, of kAt chunks, are out while those before them are looked at
+    constexpr int kAhead = 8, kAt = kAhead / (kKept ? 8 : kPer);
     const int m = __builtin_amdgcn_readfirstlane(s.m);
+    Logits<kHalf> in[kAhead];
+    int i[kAt];
+    const auto load = [&](int c0) __attribute__((always_inline)) {
+#pragma unroll
+      for (int q = 0; q < kAt; q++)  // (past the last: it again, left out below)
+        i[q] = __builtin_amdgcn_readfirstlane(s.use[min(c0 + q, m - 1)]) * (kPer * kStep);
+#pragma unroll
+      for (int k = 0; k < kAhead; k++) in[k].load_in(row, i[k / kPer] + k % kPer * kStep + 4 * tid, a.V);
+    };
+    load(0);
 #pragma unroll 1
     for (int c0 = 0; c0 < m; c0 += kAt) {
-      Logits<kHalf> in[kAhead];
-      int i[kAt];
+      f32x4 x[kAhead];
       bool whole = true;
 #pragma unroll
-      for (int q = 0; q < kAt; q++) {  // (past the last: it again, left out below)
-        i[q] = __builtin_amdgcn_readfirstlane(s.use[min(c0 + q, m - 1)]) * (kPer * kStep);
-        whole &= i[q] + kPer * kStep <= a.V;
-      }
+      for (int q = 0; q < kAt; q++) whole &= i[q] + kPer * kStep <= a.V;
       if (whole) {
 #pragma unroll
-        for (int k = 0; k < kAhead; k++) in[k].load(row, i[k / kPer] + k % kPer * kStep + 4 * tid, a.V, true);
+        for (int k = 0; k < kAhead; k++) x[k] = in[k].get();
       } else {
 #pragma unroll
-        for (int k = 0; k < kAhead; k++) in[k].load(row, i[k / kPer] + k % kPer * kStep + 4 * tid, a.V, false);
+        for (int k = 0; k < kAhead; k++) x[k] = in[k].get_in(i[k / kPer] + k % kPer * kStep + 4 * tid, a.V);
       }
+      if (c0 + kAt < m) load(c0 + kAt);
 #pragma unroll
       for (int k = 0; k < kAhead; k++) {
         if (c0 + k / kPer >= m) break;
-        f32x4 x = in[k].get(i[k / kPer] + k % kPer * kStep + 4 * tid, a.V, whole);
         if (inf)
 #pragma unroll
-          for (int e = 0; e < 4; e++) x[e] = x[e] == __builtin_inff() ? 0.0f : -__builtin_inff();
-        fn((c0 * kPer + k) * 4, x);
+          for (int e = 0; e < 4; e++) x[k][e] = x[k][e] == __builtin_inff() ? 0.0f : -__builtin_inff();
+        fn((c0 * kPer + k) * 4, x[k]);
       }
     }
   }
@@ -1119,7 +1114,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
   r.choose(b, g.k, g.tp, g.mp, g.u, tops_at, tops);
 }
 
-// The same for a row of 4..kPer * kStep logits by itself, which the threads keep in registers.
+// The same for a row of up to kPer * kStep logits by itself, which the threads keep in registers.
 template <bool kHalf, int kPer>
 __global__ __launch_bounds__(kSampleThreads) void k_sample_row(SampleArgs a) {
   using Row = SampleRow<kHalf, kPer, true>;
@@ -1128,8 +1123,12 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_row(SampleArgs a) {
   const void* row = (const char*)a.logits + (int64_t)b * a.stride * (kHalf ? 2 : 4);
   Row r{s,   a,   row, nullptr, nullptr, 0.0, 0.0, 1.0, 1.0, 0.0f, false, tid, tid & 63, tid >> 6, 0};
   Logits<kHalf> in[kPer];
+  if (kPer == 1 && a.V < 4) {
+    in[0].load_few(row, a.V);
+  } else {
 #pragma unroll
-  for (int i = 0; i < kPer; i++) in[i].load_in(row, kStep * i + 4 * tid, a.V);
+    for (int i = 0; i < kPer; i++) in[i].load_in(row, kStep * i + 4 * tid, a.V);
+  }
   const Given g(a, b);
   for (int i = tid; i < kBins; i += kSampleThreads) s.mass[i] = 0;
   if (tid == 0) s.last = 0;
@@ -1181,7 +1180,7 @@ extern "C" int64_t cia_sample_workspace_bytes(int B, int V) {
 template <bool kHalf>
 static int sample_launch(const SampleArgs& a, hipStream_t s) {
   const dim3 rows((unsigned)a.B), block(kSampleThreads);
-  if (a.V >= 4 && a.V <= 8 * kStep) {
+  if (a.V <= kMaxChunk) {
     if (a.V <= kStep)
       hipLaunchKernelGGL((k_sample_row<kHalf, 1>), rows, block, 0, s, a);
     else if (a.V <= 2 * kStep)
@@ -1189,7 +1188,7 @@ static int sample_launch(const SampleArgs& a, hipStream_t s) {
     else if (a.V <= 4 * kStep)
       hipLaunchKernelGGL((k_sample_row<kHalf, 4>), rows, block, 0, s, a);
     else
-      hipLaunchKernelGGL((k_sample_row<kHalf, 8>), rows, block, 0, s, a);
+      hipLaunchKernelGGL((k_sample_row<kHalf, kMaxChunk / kStep>), rows, block, 0, s, a);
     return launch_status();
   }
   const dim3 grid((unsigned)(a.B * a.chunks));
