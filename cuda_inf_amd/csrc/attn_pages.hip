@@ -150,18 +150,11 @@ __global__ __launch_bounds__(256, 2) void k_attn_pages(AttnPagesArgs a) {
       for (int i = 0; i < heads * kD / 8; i++)
         *(u32x4*)(a.out + ((int64_t)t * a.n_q + h0) * kD + 8 * i) = u32x4{0, 0, 0, 0};
   };
-  auto scan = [&](int n) __attribute__((always_inline)) {
-    for (int off = 1; off < 64; off <<= 1) {
-      const int o = __shfl_up(n, off);
-      if (lane >= off) n += o;
-    }
-    return n;
-  };
   int total = 0;
   if (a.T <= 64) {
     // every wave for itself: what it reads of the list, it has written
     const Span r = lane < a.T ? row_span(a, lane) : Span{0, 0, 0};
-    const int cost = span_cost(r), upto = scan(cost);
+    const int cost = span_cost(r), upto = wave_scan(cost);
     if (lane < a.T) put_row(lane, r, upto - cost, cost);
     total = __builtin_amdgcn_readlane(upto, 63);
     if (lane == 0) pre[a.T] = total;
@@ -169,7 +162,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_pages(AttnPagesArgs a) {
     for (int base = 0; base < a.T; base += 256) {
       const int t = base + tid;
       const Span r = t < a.T ? row_span(a, t) : Span{0, 0, 0};
-      const int cost = span_cost(r), upto = scan(cost);
+      const int cost = span_cost(r), upto = wave_scan(cost);
       if (lane == 63) wsum[wave] = upto;
       __syncthreads();
       int before = total;

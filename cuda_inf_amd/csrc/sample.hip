@@ -128,29 +128,6 @@ struct PowerOf2 {
   }
 };
 
-// Sums over the lanes up to each: within 16 of them, then with those before (a step by
-// DPP takes 8 bytes in two moves; by a shuffle through LDS six steps took 850 cycles).
-template <int kCtrl, int kRows, typename T>
-__device__ __forceinline__ T dpp_or_0(T v) {
-  if constexpr (sizeof(T) == 4) {
-    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl, kRows, 0xF, false));
-  } else {
-    u32x2 w = __builtin_bit_cast(u32x2, v);
-    w[0] = dpp_or_0<kCtrl, kRows>(w[0]), w[1] = dpp_or_0<kCtrl, kRows>(w[1]);
-    return __builtin_bit_cast(T, w);
-  }
-}
-template <typename T>
-__device__ __forceinline__ T wave_scan(T v) {
-  v += dpp_or_0<0x111, 0xF>(v);  // row_shr
-  v += dpp_or_0<0x112, 0xF>(v);
-  v += dpp_or_0<0x114, 0xF>(v);
-  v += dpp_or_0<0x118, 0xF>(v);
-  v += dpp_or_0<0x142, 0xA>(v);  // row_bcast15, to the odd rows
-  v += dpp_or_0<0x143, 0xC>(v);  // row_bcast31, to the upper half
-  return v;
-}
-
 // a bin's upper edge, bin 0's being 1: 2^(-bin / 16)
 __device__ __forceinline__ double bin_edge(int bin) {
   const int i = bin & 3, j = bin >> 2 & 3;
