@@ -150,12 +150,12 @@ __global__ __launch_bounds__(256, 2) void k_attn_pages(AttnPagesArgs a) {
       for (int i = 0; i < heads * kD / 8; i++)
         *(u32x4*)(a.out + ((int64_t)t * a.n_q + h0) * kD + 8 * i) = u32x4{0, 0, 0, 0};
   };
-  int total = 0;
+  int total = 0, start = 0x7fffffff;  // start: of row `lane`, up to 64 rows
   if (a.T <= 64) {
     // every wave for itself: what it reads of the list, it has written
     const Span r = lane < a.T ? row_span(a, lane) : Span{0, 0, 0};
     const int cost = span_cost(r), upto = wave_scan(cost);
-    if (lane < a.T) put_row(lane, r, upto - cost, cost);
+    if (lane < a.T) put_row(lane, r, start = upto - cost, cost);
     total = __builtin_amdgcn_readlane(upto, 63);
     if (lane == 0) pre[a.T] = total;
   } else {
@@ -180,7 +180,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_pages(AttnPagesArgs a) {
   // as few parts as make the largest no larger
   const int most = (total + a.parts - 1) / a.parts, parts = (total + most - 1) / most;
   if (part >= parts) return;
-  const int from = (int)((int64_t)total * part / parts), to = (int)((int64_t)total * (part + 1) / parts);
+  // (exact: the quotients' fractions are at least 2^-8, in numbers below 2^31)
+  const int from = (int)((double)total * part / parts), to = (int)((double)total * (part + 1) / parts);
 
   // ---- the lane's places
   const int n = lane & 15, g = lane >> 4, j = n / kRp;
@@ -189,15 +190,14 @@ __global__ __launch_bounds__(256, 2) void k_attn_pages(AttnPagesArgs a) {
   const uint32_t v_lane = (uint32_t)(g * kRowB + n * (kRowB / 16));
   const int page_mask = (1 << a.P.shift) - 1;
 
-  int row = 0;
-  for (int lo = 0, hi = a.T - 1; lo <= hi;) {  // the last row that starts at or before `from`
-    const int mid = (lo + hi) >> 1;
-    if (pre[mid] <= from) {
-      row = mid;
-      lo = mid + 1;
-    } else {
-      hi = mid - 1;
-    }
+  // the last row that starts at or before `from`, among 64 rows or groups of them at once
+  int row;
+  if (a.T <= 64) {
+    row = __popcll(__ballot(start <= from)) - 1;
+  } else {
+    const int per = (a.T + 63) / 64;
+    row = (__popcll(__ballot(lane * per < a.T && pre[min(lane * per, a.T)] <= from)) - 1) * per;
+    row += __popcll(__ballot(lane < per && row + lane < a.T && pre[min(row + lane, a.T)] <= from)) - 1;
   }
   for (; row < a.T && pre[row] < to; row++) {
     // the units [u0, u1) of the row's
@@ -475,8 +475,9 @@ __global__ __launch_bounds__(256, 2) void k_attn_pages(AttnPagesArgs a) {
     }
     if (!ends) {
       // the row's parts: the workgroups that have a unit of it, from that of its first
-      const int64_t N = total, W = parts;
-      const int first = (int)(((int64_t)(r0 + 1) * W - 1) / N), fin = (int)(((int64_t)r1 * W - 1) / N);
+      // (exact as above: fractions of at least 2^-31, in numbers up to 256)
+      const double N = total, W = parts;
+      const int first = (int)(((r0 + 1) * W - 1) / N), fin = (int)((r1 * W - 1) / N);
       const int pieces = fin - first + 1;
       stores_acked();
       __syncthreads();
