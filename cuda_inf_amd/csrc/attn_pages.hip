@@ -5,8 +5,8 @@
 //
 // Bound by memory: 2 D + 4 bytes a token and kv head in e4m3, 4 D in fp16.  32 query heads
 // on 8 kv heads of 64 in e4m3: 256 rows of 900 to 2048 tokens take 78 us (380 MB, 4.9 TB/s; a
-// large copy reaches 5.1), 58 of 9 to 9000 21.8-22.1 (89 MB, 4.0 TB/s), one of 32 768
-// 13.0 (35 MB in about 6, launch and first loads 4, the join 3), one of 700 6.7.
+// large copy reaches 5.1), 58 of 9 to 9000 21.3 (89 MB, 4.2 TB/s), one of 32 768
+// 12.7 (35 MB in about 6, launch and first loads 4, the join 3), one of 700 6.4.
 //
 // Work.  A row's tokens are units of 128, and the units of all rows one list, of which
 // each of the P workgroups of a kv head takes an equal part, whatever rows it falls
@@ -154,7 +154,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_pages(AttnPagesArgs a) {
   if (a.T <= 64) {
     // every wave for itself: what it reads of the list, it has written
     const Span r = lane < a.T ? row_span(a, lane) : Span{0, 0, 0};
-    const int cost = span_cost(r), upto = wave_scan(cost);
+    const int cost = span_cost(r), upto = scan_lanes(cost);
     if (lane < a.T) put_row(lane, r, start = upto - cost, cost);
     total = __builtin_amdgcn_readlane(upto, 63);
     if (lane == 0) pre[a.T] = total;
@@ -162,7 +162,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_pages(AttnPagesArgs a) {
     for (int base = 0; base < a.T; base += 256) {
       const int t = base + tid;
       const Span r = t < a.T ? row_span(a, t) : Span{0, 0, 0};
-      const int cost = span_cost(r), upto = wave_scan(cost);
+      const int cost = span_cost(r), upto = scan_lanes(cost);
       if (lane == 63) wsum[wave] = upto;
       __syncthreads();
       int before = total;

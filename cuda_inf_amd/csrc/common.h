@@ -218,7 +218,7 @@ __device__ __forceinline__ T dpp_or_0(T v) {
   }
 }
 template <typename T>
-__device__ __forceinline__ T wave_scan(T v) {
+__device__ __forceinline__ T scan_lanes(T v) {
   v += dpp_or_0<0x111, 0xF>(v);  // row_shr
   v += dpp_or_0<0x112, 0xF>(v);
   v += dpp_or_0<0x114, 0xF>(v);

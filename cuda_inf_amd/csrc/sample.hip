@@ -10,17 +10,22 @@
 //   k_sample_bins  reads the logits once: the bins of each chunk of a row;
 //   k_sample_pick  adds up a row's chunks, takes the few tokens that a filter or the
 //                  draw can end at from the chunks that have them, and puts those in
-//                  order.
+//                  order;
+//   k_sample_row   does both for a row of up to 16384 logits, which stays in registers.
 // Bins lie at whole x, so that those of chunks with other maxima only need a shift.
 // Masses are added as integers, 2^34 for a bin's upper edge, so that sums do not depend
 // on the order of atomics; over the largest logit's own, so that rows of equals have
 // whole sums.
 //
 // Bound by memory for large batches, which read a row once or, for a broad nucleus,
-// twice (4 V bytes a pass in fp32): 256 rows of 131 072, top-p, take 96 us, 31 of them the
-// bins (4.4 TB/s) and 65 the choice, of which its pass is 21 (6.4 TB/s, part of it from the
-// last-level cache).  By chains of dependent steps for few: one row of 65 536 with all
-// filters takes 24 us, 6 for the bins and 17 for the choice.
+// twice (4 V bytes a pass in fp32): 256 rows of 131 072, top-p, take 80 us, 28-30 of them the
+// bins (134 MB at 4.5-4.8 TB/s; 26.3 without their atomics) and 49-51 the choice, of which its
+// pass is 19 (7 TB/s, part of it from the last-level cache).  By chains of dependent steps
+// for few: one row of 65 536 with all filters takes 16 us, 6 for the bins and 10 for the
+// choice; one row of 4000 8.0 in its one launch, of 60 7.8 (a call alone takes the host
+// about 6).  What such steps cost is not arithmetic: a step of a scan through LDS 140
+// cycles (by DPP a few), an atomic on one word by all threads 4500 (by one lane a wave
+// 200), a barrier with what waits at it 150.
 #include <algorithm>
 #include <type_traits>
 
@@ -140,8 +145,8 @@ __device__ __forceinline__ double temperature_scale(float t) { return 16 * 1.442
 
 // ---------------------------------------------------------------- the bins
 // Of rows of more than kMaxChunk.  grid = rows * chunks, block = kThreads, 4 kVec logits of the chunk a thread, in registers:
-// all loads of a chunk are out together, and its largest is known before its bins.  22 vector
-// instructions a logit with all that is around them, vector units 52 % busy (256 rows of 131 072).
+// all loads of a chunk are out together, and its largest is known before its bins.  19 vector
+// instructions a logit with all that is around them, vector units 47 % busy (256 rows of 131 072).
 template <bool kHalf, int kThreads, int kVec>
 __global__ __launch_bounds__(kThreads) void k_sample_bins(SampleArgs a) {
   constexpr int kWaves = kThreads / 64, kEach = 4 * kThreads;
@@ -222,7 +227,7 @@ __global__ __launch_bounds__(kThreads) void k_sample_bins(SampleArgs a) {
     const int lane = tid & 63, wave = tid >> 6, i = min(2 * tid, kBins - 2);
     const bool mine = 2 * tid < kBins;
     const int k0 = mine ? (int)(bins[i] >> kCountShift) : 0, k1 = mine ? (int)(bins[i + 1] >> kCountShift) : 0;
-    int upto = wave_scan(k0 + k1);
+    int upto = scan_lanes(k0 + k1);
     if (lane == 63) wcount[wave] = upto;
     __syncthreads();
     for (int w = 0; w < wave; w++) upto += wcount[w];
@@ -477,8 +482,8 @@ struct SampleRow {
     const bool mine = 2 * tid < kBins;
     const int k0 = mine ? (int)c0 : 0, k1 = mine ? (int)c1 : 0;
     const double m0 = mine ? mass_in(b, u0) : 0.0, m1 = mine ? mass_in(b + 1, u1) : 0.0;
-    double run = wave_scan(m0 + m1);
-    int upto = wave_scan(k0 + k1);
+    double run = scan_lanes(m0 + m1);
+    int upto = scan_lanes(k0 + k1);
     if (lane == 63) s.dsum[wave] = run, s.lo[wave] = (uint32_t)upto;
     const uint64_t any = __ballot(k0 + k1 > 0), odd = __ballot(k1 > 0);
     if (lane == 0 && any) {
@@ -621,7 +626,7 @@ struct SampleRow {
   // Places in s.some for a thread's `mine` tokens, in the threads' order: from which on;
   // n: of all.
   __device__ __forceinline__ int places(int mine, int& n) {
-    int at = wave_scan(mine);
+    int at = scan_lanes(mine);
     __syncthreads();
     if (lane == 63) s.lo[wave] = (uint32_t)at;
     __syncthreads();
@@ -749,7 +754,7 @@ struct SampleRow {
   __device__ __forceinline__ void sums(int n, double mass) {
     for (int i0 = 0; i0 < n; i0 += kSampleThreads) {
       const int i = i0 + tid;
-      const double w = i < n ? weight(key_value((uint32_t)(s.small[i] >> 32))) : 0.0, run = wave_scan(w);
+      const double w = i < n ? weight(key_value((uint32_t)(s.small[i] >> 32))) : 0.0, run = scan_lanes(w);
       if (i < n) s.some[i] = __builtin_bit_cast(uint64_t, w);
       if (lane == 63) s.dsum[wave] = run;
       __syncthreads();
@@ -806,8 +811,8 @@ struct SampleRow {
     __syncthreads();
     const int kc = (int)s.cnt[tid];
     const unsigned long long km = s.mass[tid];
-    unsigned long long im = wave_scan(km);
-    int ik = wave_scan(kc);
+    unsigned long long im = scan_lanes(km);
+    int ik = scan_lanes(kc);
     if (lane == 63) s.key[wave] = im, s.lo[wave] = (uint32_t)ik;
     __syncthreads();
     im += before_wave((uint64_t)0, s.key), ik += (int)before_wave(0u, s.lo);
@@ -1066,8 +1071,8 @@ struct Given {
 };
 
 // grid = rows, block = kSampleThreads: one workgroup a row, so that its steps meet at
-// barriers (about 2 us each: the largest 1.6, bins added up 4.6, goals' bins 3.3, the few
-// tokens and their order 4.6, sums and places 2.2, for one row of 65 536 with all filters).
+// barriers.  us of them, of one row of 65 536 with all filters: the largest 2.4, bins added up 2.5,
+// goals' bins 0.9, the few tokens 1.6, their order 0.8, sums 0.7, places 1.0.
 template <bool kHalf, int kPer>
 __global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
   using Row = SampleRow<kHalf, kPer, false>;
@@ -1091,7 +1096,11 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
   r.choose(b, g.k, g.tp, g.mp, g.u, tops_at, tops);
 }
 
-// The same for a row of up to kPer * kStep logits by itself, which the threads keep in registers.
+// The same for a row of up to kPer * kStep logits by itself, which the threads keep in registers:
+// one launch, no bins through memory, no second pass.  us against the two kernels: one row
+// of 1000 with top-k and top-p 12.3 / 18.0, 256 of 4000 15.5 / 21.7, 256 of 16 384 with a broad
+// top-p 31.0 / 39.7.  (Longer rows chunk by chunk in one workgroup: 5.7 us a chunk of 16384,
+// even at 32 768 and 97 / 92 for 256 rows of 131 072.)
 template <bool kHalf, int kPer>
 __global__ __launch_bounds__(kSampleThreads) void k_sample_row(SampleArgs a) {
   using Row = SampleRow<kHalf, kPer, true>;
