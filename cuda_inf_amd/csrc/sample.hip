@@ -399,6 +399,9 @@ struct SampleRow {
     for (int i = tid; i < a.chunks; i += kSampleThreads) {
       const double n = s.shift[i];
       s.shift[i] = inf ? (n == __builtin_inf() ? 0.0 : (double)kBins) : fmin(R - n, (double)kBins);
+      // (none of its tokens counts; of a chunk without +inf in a row that has some they are
+      // the chunk's own logits, which may lie above the 0 that +inf stands for)
+      if (s.shift[i] >= (double)kBins) s.listed[i] = 0;
       atomicMin(&s.covered, (int)s.shift[i] + s.use[i]);
     }
     __syncthreads();

@@ -512,6 +512,31 @@ def test_sample_of_numbers_that_are_none(K, dev):
         assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
 
 
+@pytest.mark.parametrize("V", [1000, 16384, 16385, 20000, 65536, 70000, 262144, 262145, 270000])
+@pytest.mark.parametrize("half", [False, True])
+def test_sample_of_rows_with_infinities(K, dev, V, half):
+    """+inf in rows of one chunk and of many, of both sizes, beside finite logits far above 0: one, a few of one
+    chunk, some of all chunks, more in one chunk than it lists, more than are put in order at once, and a row of
+    them alone; a NaN and -inf between them.  They are the choice, all alike; a row without any is as ever."""
+    rng = np.random.default_rng(V + half)
+    dtype = np.float16 if half else np.float32
+    spots = [[V // 2], [V - 1], [0, 3, 250], rng.permutation(V)[:40], rng.permutation(min(V, 8192))[:700],
+             rng.permutation(V)[:900], np.arange(0, V, max(1, V // 1500)), rng.permutation(V)[:V // 3], np.arange(V), []]
+    l = (2 * rng.standard_normal((len(spots), V)) + np.linspace(-30, 30, len(spots))[:, None]).astype(dtype)
+    for row, at in zip(l, spots):
+        row[at] = np.inf
+    l[1:3, 5], l[1:3, 7] = np.nan, -np.inf
+    B = len(spots)
+    for f in (dict(), dict(top_k=1), dict(top_k=2), dict(top_k=500), dict(top_p=0.6), dict(min_p=0.3),
+              dict(top_k=650, top_p=0.7, min_p=0.5), dict(temperature=0.0), dict(temperature=np.inf, top_k=100),
+              dict(temperature=1e-3)):
+        f = {k: np.full(B, v) for k, v in f.items()}
+        u = (rng.integers(0, 2 ** 20, B) + 0.37) / 2 ** 20
+        ids, _ = sample(K, dev, l, u, **f)
+        assert (ids >= 0).all() and (ids < V).all(), f"{V} {f}"
+        check_sample(K, dev, l, u, f"{V} {f}", **f)
+
+
 def test_sample_of_the_longest_rows(K, dev):
     rng = np.random.default_rng(6)
     V = 1 << 22
