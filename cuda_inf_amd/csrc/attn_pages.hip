@@ -44,6 +44,11 @@ constexpr float kLow = -3.0e38f;  // max of no scores: finite, so that exp2(-inf
 // it: fp16's least step is then 2^-36 of it.  (With 1 for the largest, 12 000 tokens of 4e-8
 // of its weight were 1/40 off in their sum.)
 constexpr float kLift = 12.0f, kMost = 15.0f;
+// Scores from here on have steps of 1/2 and more in fp32, and less kLift they are rounded: by
+// steps of 4 to 16 about 2^26, which made numerators of 2^16 and more, that fp16 has not.  Of
+// these the largest score itself is taken off, which leaves numerators of at most V's scale;
+// the bits of small weights are lost in the scores' steps there.
+constexpr float kFar = 0x1p22f;
 
 struct AttnPagesArgs {
   Pages P;
@@ -308,7 +313,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_pages(AttnPagesArgs a) {
         }
         // The numerators are those of weight times V's scale, so that they fill fp16's
         // range whatever the scales are: m is the max of s + log2 vs, less kLift.  It is let
-        // lag: a rescaling only where a numerator would be over 2^kMost.
+        // lag: a rescaling only where a numerator would be over 2^kMost (told by the
+        // difference, as the sum m + kMost is rounded too).
         float top = -__builtin_inff();
 #pragma unroll
         for (int b = 0; b < 2; b++)
@@ -316,8 +322,14 @@ __global__ __launch_bounds__(256, 2) void k_attn_pages(AttnPagesArgs a) {
           for (int e = 0; e < kR; e++)
             top = __builtin_fmaxf(
                 top, kF8 ? y[b][e] + __builtin_amdgcn_logf(__builtin_fmaxf(vs[b][e], 0x1p-24f)) : y[b][e]);
-        if (__any(top > m + kMost)) {
-          const float now = __builtin_fmaxf(m, col4_max(top) - kLift);
+        if (__any(top - m > kMost)) {
+          float score = -__builtin_inff();
+#pragma unroll
+          for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int e = 0; e < kR; e++) score = __builtin_fmaxf(score, y[b][e]);
+          score = col4_max(score), top = col4_max(top);
+          const float now = __builtin_fmaxf(m, __builtin_fabsf(top) < kFar ? top - kLift : score);
           const float f = __builtin_amdgcn_exp2f(m - now);
           m = now;
           l *= f;

@@ -372,6 +372,49 @@ def test_attention_at_the_largest_scales(K, orc, dev, quant, scale):
             within(out[s, h], want, np.abs(want) * 2.0 ** -11 + 2.0 ** -25, f"sequence {s}, head {h}")
 
 
+@pytest.mark.parametrize("quant", [True, False])
+@pytest.mark.parametrize("units", [2.0 ** 20, *(f * 2.0 ** e for e in (21, 22, 23, 24, 25, 26, 27, 28, 29) for f in (1.02, 1.3, 1.7)), 2.0 ** 40])
+def test_attention_of_equals_among_large_scores(K, orc, dev, quant, units):
+    """Scores of `units` powers of 2, where fp32's steps reach and pass those that numerators are kept within.  All alike:
+    the mean of V, whose tokens' sizes (e4m3: scales) lie 2^16 apart; weights are equal, so that only the sums' terms
+    of ref.attend's bound count.  The later ones higher by 16 or more, and still so where both are rounded to steps of
+    up to 16: their mean, and 128 / 100 * 2^-16 of the first ones' at most.  A call of two rows, and of so many that a
+    workgroup has all units of a row."""
+    rng = np.random.default_rng(8)
+    n, D = 228, 64
+    c = Cache(K, orc, dev, rng, [n, n], 1, D, 16, quant)
+    shape = (c.n_pages, 1, 16)
+    size = (2.0 ** rng.integers(-10, 7, shape)).astype(np.float16)
+    v = rng.integers(-16, 17, (*shape, D)).astype(np.float32)  # (whole numbers to 16: exact in e4m3)
+    k = np.zeros((*shape, D), np.float32)
+    k[..., 0] = 448.0
+    step = 2.0 ** min(7.0, max(0.0, 27 - np.floor(np.log2(units))))
+    for j in range(128, n):  # 448 and 2^-14 `step`: 2^-22.8 of it higher for a step of 1
+        k[int(c.table[1, j // 16]), 0, j % 16, 1] = step
+    if quant:
+        for name, x, s in (("k", k, np.ones(shape, np.float16)), ("v", v, size)):
+            c.raw[name].copy_(t(orc.e4m3_encode(x.reshape(-1)).reshape(x.shape), dev))
+            c.raw[name + "s"].copy_(t(s, dev))
+    else:
+        c.raw["k"].copy_(t(k.astype(np.float16), dev))
+        c.raw["v"].copy_(t((v * size[..., None]).astype(np.float16), dev))
+    num = v.astype(np.float64) * size.astype(np.float64)[..., None]
+    rows = [np.stack([num[int(c.table[s, j // 16]), 0, j % 16] for j in range(n)]) for s in range(2)]
+    apart = units * step * 2.0 ** -14 / 448 >= 16
+    for T in (2, 1024):
+        q = np.zeros((T, 4, D), np.float16)
+        q[..., 0], q[..., 1] = 1.0, 2.0 ** -14
+        out = attend(K, c, dev, q, np.arange(T, dtype=np.int32) % 2, np.full(T, n - 1, np.int32),
+                     units * np.log(2.0) / 448, 0).cpu().numpy()
+        for s in range(2 if apart else 1):
+            x = rows[s][128:] if s else rows[s]
+            want, mass = x.mean(0), np.abs(x).mean(0)
+            bound = mass * ((n / 16 + 64) * 2 * ref.U24 + 2.0 ** -22) + n * 2.0 ** -37 * np.abs(x).max()
+            if s:
+                bound = bound + 1.28 * 2.0 ** -16 * (mass + np.abs(rows[s][:128]).mean(0))
+            within(out[s::2], want, bound + np.abs(want) * ref.U11 * 1.001 + 2.0 ** -25, f"{T} rows, sequence {s}")
+
+
 def test_pages_beyond_32_bits(K, orc, dev):
     """Rows of pages whose bytes lie past 2^32: written, attended and read."""
     n_pages, page, n_kv, D = 2100, 1024, 8, 128
