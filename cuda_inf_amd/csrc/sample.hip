@@ -26,38 +26,24 @@
 // about 6).  What such steps cost is not arithmetic: a step of a scan through LDS 140
 // cycles (by DPP a few), an atomic on one word by all threads 4500 (by one lane a wave
 // 200), a barrier with what waits at it 150.
-#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
 #include "cuda_inf_batch.h"
+#include "sample_shape.h"
 
 namespace cia {
 
 constexpr int kSampleThreads = 512;  // of a row's workgroup
 constexpr int kSampleWaves = kSampleThreads / 64;
-constexpr int kBins = 672;   // 42 octaves, 16 bins each
 constexpr int kSlots = 36;    // tokens that a thread takes from a row into LDS
 constexpr int kCap = 7680;   // tokens that are tried to be taken: 15 a thread
 constexpr int kSmall = 16;  // tokens put in order by one wave (256 broad rows 74.2 us for 76.8; up to 48 slower)
 constexpr int kAll = 1024;   // tokens put in order at all
 constexpr int kSub = kSampleThreads;  // parts of a bin's keys
 constexpr int kStep = 4 * kSampleThreads;  // logits of a step of k_sample_pick
-constexpr int kMinChunk = 8192;
-constexpr int kMaxChunk = 2 * kMinChunk;
-constexpr int kTop = 512;  // tokens of a smaller chunk that it puts out by themselves, at most
 constexpr int kMaxChunks = CIA_SAMPLE_MAX_VOCAB / kMaxChunk;  // 256
 constexpr int kCountShift = 49;  // of a chunk's bin: count << 49 | mass; 2^14 tokens of 2^34
-
-// of a chunk of a row; its bins follow the chunks of all rows, and the tops of smaller
-// chunks those
-struct ChunkHead {
-  double n;       // ceil of its largest x; -inf: no token, inf: logits of +inf
-  float top;      // its largest logit
-  uint32_t idx;   // the first token that has it
-  int depth;      // bins whose tokens are in its top
-  int listed;     // tokens of its top
-};
 
 struct SampleArgs {
   const void* logits;
@@ -1183,17 +1169,6 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_row(SampleArgs a) {
   r.choose(b, g.k, g.tp, g.mp, g.u, nullptr, tops);
 }
 
-// Chunks of 16384 logits where there are more than 1024 of them, or a row has more than 32 of
-// the smaller ones; else of 8192, with their tops: of the largest tokens the choice
-// mostly falls on, the row need not be read again.  us with 8192 / 16384, of rows of 131 072:
-//   rows (chunks of 16384)         1 (8)   32 (256)     64 (512)   128 (1024)    256 (2048)
-//   top-k and top-p          18.6 / 29.3  23.0 / 35.3  27.9 / 38.3  36.6 / 45.0   61.8 / 61.0
-//   top-p, broad: read again 29.0 / 32.2  59.0 / 54.6  63.1 / 57.7  74.6 / 65.9   98.0 / 79.0
-constexpr int kMostTopped = 1024;
-static int sample_chunk(int B, int V) {
-  return (int64_t)B * ((V + kMaxChunk - 1) / kMaxChunk) > kMostTopped || V > 32 * kMinChunk ? kMaxChunk : kMinChunk;
-}
-
 }  // namespace cia
 
 using namespace cia;
@@ -1201,11 +1176,7 @@ using namespace cia;
 extern "C" int64_t cia_sample_workspace_bytes(int B, int V) {
   if (B < 0 || B > CIA_SAMPLE_MAX_ROWS || V < 1 || V > CIA_SAMPLE_MAX_VOCAB || (int64_t)B * V > CIA_SAMPLE_MAX_LOGITS)
     return 0;
-  // (the most that B rows or fewer need: a smaller batch may have smaller chunks)
-  const int64_t big = (V + kMaxChunk - 1) / kMaxChunk, small = (V + kMinChunk - 1) / kMinChunk;
-  int64_t n = (int64_t)B * (sample_chunk(B, V) == kMinChunk ? small : big);
-  if (sample_chunk(1, V) == kMinChunk) n = std::max(n, std::min<int64_t>(B, kMostTopped / big) * small);
-  return 16 + n * (int64_t)(sizeof(ChunkHead) + (kBins + kTop) * sizeof(uint64_t));
+  return sample_space_bytes(B, V);
 }
 
 template <bool kHalf>
@@ -1248,11 +1219,10 @@ extern "C" int cia_sample(const void* logits, int type, int64_t stride, const fl
                   aligned(ws, 16),
               CIA_ERR_ALIGN);
   CIA_REQUIRE(ws_bytes >= need, CIA_ERR_ARG);
-  const int chunk = sample_chunk(B, V), chunks = (V + chunk - 1) / chunk;
-  ChunkHead* const heads = (ChunkHead*)ws;
-  uint64_t* const bins = (uint64_t*)(heads + (int64_t)B * chunks);
-  const SampleArgs a{logits, stride, temperature, top_k, top_p, min_p, u, ids, p, B, V, chunk, chunks, heads,
-                     bins, bins + (int64_t)B * chunks * kBins};
+  const SampleSpace at = sample_space(B, V);
+  char* const space = (char*)ws;
+  const SampleArgs a{logits, stride, temperature, top_k, top_p, min_p, u, ids, p, B, V, at.chunk, at.chunks,
+                     (ChunkHead*)space, (uint64_t*)(space + at.bins), (uint64_t*)(space + at.tops)};
   return type == CIA_LOGITS_F16 ? sample_launch<true>(a, (hipStream_t)stream)
                                 : sample_launch<false>(a, (hipStream_t)stream);
 }
