@@ -33,29 +33,26 @@ constexpr int sample_chunk(int B, int V) {
 }
 
 // Where a workspace of B rows has its parts, in bytes from its start: the heads of all chunks
-// of all rows, [kBins] uint64 of each, [kTop] uint64 of each.
+// of all rows, [kBins] uint64 of each, and of smaller chunks [kTop] uint64 of each.  Rows of up
+// to kMaxChunk are read by their own workgroups, which need none of it.
 struct SampleSpace {
   int chunk, chunks;  // logits of a chunk, chunks of a row
   int64_t bins, tops, end;
 };
 constexpr SampleSpace sample_space(int B, int V) {
   const int chunk = sample_chunk(B, V), chunks = row_chunks(V, chunk);
-  const int64_t n = (int64_t)B * chunks;
+  const int64_t n = V > kMaxChunk ? (int64_t)B * chunks : 0;
   // (bins are read 16 bytes at a time)
   const int64_t bins = (n * (int64_t)sizeof(ChunkHead) + 15) & ~(int64_t)15;
   const int64_t tops = bins + n * kBins * 8;
-  return SampleSpace{chunk, chunks, bins, tops, tops + n * kTop * 8};
+  return SampleSpace{chunk, chunks, bins, tops, tops + (chunk == kMinChunk ? n * kTop * 8 : 0)};
 }
 
 // Bytes for B rows of V or fewer: a smaller batch may have smaller chunks.
 constexpr int64_t sample_space_bytes(int B, int V) {
-  const int big = row_chunks(V, kMaxChunk), small = row_chunks(V, kMinChunk);
-  int64_t n = (int64_t)B * (sample_chunk(B, V) == kMinChunk ? small : big);
-  if (sample_chunk(1, V) == kMinChunk) {
-    const int64_t rows = B < kMostTopped / big ? B : kMostTopped / big;
-    n = n < rows * small ? rows * small : n;
-  }
-  return 16 + n * ((int64_t)sizeof(ChunkHead) + (kBins + kTop) * 8);
+  const int topped = kMostTopped / row_chunks(V, kMaxChunk);  // rows
+  const int64_t all = sample_space(B, V).end, fewer = sample_space(B < topped ? B : topped, V).end;
+  return 16 + (all > fewer ? all : fewer);
 }
 
 }  // namespace cia

@@ -684,6 +684,25 @@ def test_calls_of_other_sizes_on_the_same_workspaces(K, orc, dev):
         check(K, c, dev, q, None, np.array(lens[:rows], np.int32) - 1, 0.125, 0, ws, f"{n_q} heads")
 
 
+@pytest.mark.parametrize("B,V", [(1, 300), (5, 16384), (1, 16385), (3, 20000), (31, 65536), (65, 262144), (3, 262145), (300, 70000)])
+def test_sample_stays_in_its_workspace(K, dev, B, V):
+    """A workspace of the stated size, odd numbers of chunks among them, with nothing written beside it."""
+    n, edge = K.sample_workspace_bytes(B, V), 4096
+    assert V > 16384 or n <= 64  # (rows of one launch need none)
+    whole = torch.full((edge + n + edge,), 0xA5, dtype=torch.uint8, device=dev)
+    rng = np.random.default_rng(V)
+    l = (2 * rng.standard_normal((min(B, 7), V))).astype(np.float32)[np.arange(B) % 7]
+    x, u = t(l, dev), rng.random(B).astype(np.float32)
+    ids = torch.empty(B, dtype=torch.int32, device=dev)
+    for f in (dict(top_k=40), dict(top_p=0.9)):
+        f = {k: np.full(B, v, np.int32 if k == "top_k" else np.float32) for k, v in f.items()}
+        K.sample(x, t(u, dev), ids, whole[edge:edge + n], **{k: t(v, dev) for k, v in f.items()})
+        some = np.unique(np.r_[0:min(B, 3), B - 1])
+        want, _, near = ref.choose(l[some], u[some], **{k: v[some] for k, v in f.items()})
+        assert near.min() > 1e-9 and np.array_equal(ids.cpu().numpy()[some], want)
+        assert (whole[:edge] == 0xA5).all() and (whole[edge + n:] == 0xA5).all()
+
+
 def test_two_streams_at_once(K, orc, dev):
     """The same calls on two streams, each with its workspaces, one cache between them."""
     rng = np.random.default_rng(14)
