@@ -19,6 +19,7 @@ NH, NKV, GQA, D, KVGROUP = 32, 8, 4, 64, 64
 NSPLIT_DEFAULT = 16
 HIDDEN = 2048  # hidden size H (engine.cu:33)
 NSPLIT_MAX = 4096
+PAGE_MIN, PAGE_MAX, PAGES_MAX_TOKENS = 16, 1024, 1 << 25  # of a paged cache (include/cuda_inf_batch.h)
 
 STATUS = {0: "CIA_OK", 1: "CIA_ERR_NULL", 2: "CIA_ERR_ALIGN", 3: "CIA_ERR_ARG",
           4: "CIA_ERR_HIP", 5: "CIA_ERR_STATE", 6: "CIA_ERR_NOSLOT",

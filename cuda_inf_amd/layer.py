@@ -13,8 +13,8 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import (D, KVGROUP, NH, NKV, NSPLIT_DEFAULT, call, cia_append_op, cia_attn_proj,
-                   cia_layer, cia_moe)
+from ._lib import (D, KVGROUP, NH, NKV, NSPLIT_DEFAULT, PAGE_MAX, PAGE_MIN, PAGES_MAX_TOKENS, call,
+                   cia_append_op, cia_attn_proj, cia_layer, cia_moe)
 from .kernels import (KvPages, _stream_on, attn_pages, decode_workspace_bytes, h2o_workspace_bytes,
                       kv_pages_read, kv_pages_write, moe_gating, new_attn_pages_workspace, q4_experts,
                       stream_handle)
@@ -288,6 +288,13 @@ class PageTable:
     given out and taken back on the host, and written to ``table`` on the current stream."""
 
     def __init__(self, max_seqs: int, max_tokens: int, n_pages: int, *, page: int = 64, device="cuda"):
+        if not PAGE_MIN <= page <= PAGE_MAX or page & (page - 1):
+            raise ValueError(f"page={page}: need a power of two, {PAGE_MIN} to {PAGE_MAX}")
+        for n, name in ((max_seqs, "max_seqs"), (max_tokens, "max_tokens"), (n_pages, "n_pages")):
+            if n < 1:
+                raise ValueError(f"{name}={n}: need 1 or more")
+        if max_tokens > PAGES_MAX_TOKENS:
+            raise ValueError(f"max_tokens={max_tokens}: a sequence holds {PAGES_MAX_TOKENS} at most")
         self.page, self.n_pages = page, n_pages
         width = -(-max_tokens // page)
         self.table = torch.full((max_seqs, width), -1, dtype=torch.int32, device=device)

@@ -277,6 +277,23 @@ def test_page_table(cia):
     assert t.free_pages == 0 and len(set(t.table[1, :6].tolist() + got[0][:2])) == 8
 
 
+def test_page_table_refusals(cia):
+    """What the calls over its pages would refuse, it refuses when it is made."""
+    from cuda_inf_amd import _lib
+    from cuda_inf_amd.layer import PageTable
+    text = open(os.path.join(ROOT, "include", "cuda_inf_batch.h")).read()
+    assert [int(re.search(rf"{n} (\d+)", text)[1]) for n in ("CIA_PAGE_MIN", "CIA_PAGE_MAX")] == [_lib.PAGE_MIN, _lib.PAGE_MAX]
+    assert "CIA_PAGES_MAX_TOKENS (1 << 25)" in text and _lib.PAGES_MAX_TOKENS == 1 << 25
+    for page in (0, 1, 8, 24, 48, 2048, -16):
+        with pytest.raises(ValueError, match="page="):
+            PageTable(2, 100, 4, page=page, device="cpu")
+    for kw in (dict(max_seqs=0), dict(max_seqs=-1), dict(n_pages=0), dict(max_tokens=0), dict(max_tokens=(1 << 25) + 1)):
+        with pytest.raises(ValueError, match=f"{list(kw)[0]}="):
+            PageTable(**{**dict(max_seqs=2, max_tokens=100, n_pages=4), **kw}, device="cpu")
+    for page in (16, 1024):
+        assert PageTable(1, 1 << 25, 1, page=page, device="cpu").table.shape == (1, (1 << 25) // page)
+
+
 def test_choice_oracle():
     """The tests' own choice: hand-made rows."""
     import batch_ref as ref
