@@ -285,7 +285,8 @@ class PageTable:
     """Which pages hold the tokens of each of ``max_seqs`` sequences: token ``pos`` of
     sequence ``s`` lies in page ``table[s, pos // page]``, -1 where it has none.  The
     layers of a model share one: ``n_pages`` pages of ``page`` tokens in each of them,
-    given out and taken back on the host, and written to ``table`` on the current stream."""
+    given out and taken back on the host, and written to ``table`` on the current stream,
+    which must not be capturing a graph."""
 
     def __init__(self, max_seqs: int, max_tokens: int, n_pages: int, *, page: int = 64, device="cuda"):
         if not PAGE_MIN <= page <= PAGE_MAX or page & (page - 1):
@@ -305,12 +306,19 @@ class PageTable:
     def free_pages(self) -> int:
         return len(self._free)
 
+    def _row(self, seq: int):
+        if not 0 <= seq < len(self._held):
+            raise ValueError(f"seq={seq}: the table has {len(self._held)} sequences")
+        return self._held[seq]
+
+    def _no_capture(self) -> None:
+        if self.table.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("pages change hands outside a graph's capture: a replay would do it again")
+
     def reserve(self, seq: int, tokens: int) -> None:
         """Pages for the first ``tokens`` tokens of a sequence, those it has among them.
         Raises RuntimeError, with nothing changed, where not enough are free."""
-        if not 0 <= seq < len(self._held):
-            raise ValueError(f"seq={seq}: the table has {len(self._held)} sequences")
-        held = self._held[seq]
+        held = self._row(seq)
         need = -(-tokens // self.page) - len(held)
         if need <= 0:
             return
@@ -318,18 +326,20 @@ class PageTable:
             raise ValueError(f"tokens={tokens}: a sequence holds {self.table.shape[1] * self.page}")
         if need > len(self._free):
             raise RuntimeError(f"{need} pages needed, {len(self._free)} free")
-        new = [self._free.pop() for _ in range(need)]
+        new = self._free[:-need - 1:-1]
+        self._no_capture()
         self.table[seq, len(held):len(held) + need] = torch.tensor(new, dtype=torch.int32, device=self.table.device)
+        del self._free[-need:]  # (once they are in the table)
         held += new
 
     def release(self, seq: int) -> None:
         """A sequence's pages back; its row of the table is -1.  Work that still reads
         them has to lie before what writes them next (the same stream, or events)."""
-        if not 0 <= seq < len(self._held):
-            raise ValueError(f"seq={seq}: the table has {len(self._held)} sequences")
-        self._free += reversed(self._held[seq])
-        self._held[seq] = []
+        held = self._row(seq)
+        self._no_capture()
         self.table[seq] = -1
+        self._free += reversed(held)
+        self._held[seq] = []
 
 
 class PagedAttn:

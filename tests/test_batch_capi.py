@@ -294,6 +294,37 @@ def test_page_table_refusals(cia):
         assert PageTable(1, 1 << 25, 1, page=page, device="cpu").table.shape == (1, (1 << 25) // page)
 
 
+def test_page_table_keeps_its_count(cia):
+    """A table that cannot be written (its device out of memory, a stream that captures) leaves the pages where they were."""
+    import torch
+
+    from cuda_inf_amd.layer import PageTable
+    t = PageTable(2, 100, 8, page=16, device="cpu")
+    t.reserve(0, 40)
+    whole = t.table
+
+    class Closed(torch.Tensor):
+        def __setitem__(self, at, what):
+            raise RuntimeError("closed")
+
+    t.table = whole.as_subclass(Closed)
+    with pytest.raises(RuntimeError, match="closed"):
+        t.reserve(1, 80)
+    with pytest.raises(RuntimeError, match="closed"):
+        t.reserve(0, 90)
+    with pytest.raises(RuntimeError, match="closed"):
+        t.release(0)
+    t.table = whole
+    assert t.free_pages == 5
+    t.reserve(0, 48)  # (what it has)
+    assert t.free_pages == 5 and (t.table[0, :3] >= 0).all() and (t.table[0, 3:] == -1).all() and (t.table[1] == -1).all()
+    t.reserve(1, 80)
+    assert t.free_pages == 0 and sorted(t.table[t.table >= 0].tolist()) == list(range(8))
+    t.release(0)
+    t.release(1)
+    assert t.free_pages == 8 and (t.table == -1).all()
+
+
 def test_choice_oracle():
     """The tests' own choice: hand-made rows."""
     import batch_ref as ref

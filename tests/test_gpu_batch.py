@@ -805,6 +805,23 @@ def test_on_another_stream_and_captured(K, orc, dev, V):
         assert torch.equal(a, b)
 
 
+def test_pages_change_hands_outside_a_capture(cia, dev):
+    from cuda_inf_amd.layer import PageTable
+    table = PageTable(2, 100, 8, page=16, device=dev)
+    table.reserve(0, 40)
+    x = torch.zeros(4, device=dev)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x += 1
+        for change in (lambda: table.reserve(1, 40), lambda: table.release(0)):
+            with pytest.raises(RuntimeError, match="outside a graph's capture"):
+                change()
+    graph.replay()
+    table.reserve(1, 80)
+    assert (x == 1).all() and table.free_pages == 0
+    assert sorted(table.table[table.table >= 0].tolist()) == list(range(8)) and (table.table[0, 3:] == -1).all()
+
+
 def int4(rng, rows, cols, dev):
     packed = rng.integers(0, 256, (rows, cols // 2), dtype=np.uint8)
     scales = ((0.5 + rng.random((rows, cols // 128))) * 0.35 / np.sqrt(cols)).astype(np.float16)
