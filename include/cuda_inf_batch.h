@@ -126,9 +126,11 @@ int64_t cia_attn_pages_workspace_bytes(int n_q, int n_kv, int head_dim);
  * them, NaN as 0.  ids: int32 [B]; p: fp32 [B], may be NULL.
  * A NaN logit counts as -inf; -inf is never chosen; where logits are +inf they
  * alone are, all alike; a row of none gives id -1 and p 0.  Weights below
- * 2^-41 of the largest count as 0.  Sums are 64 bits wide: weights are good to
- * 2^-34 of themselves in them, so that a u within about that of a border can
- * fall on its other side.
+ * 2^-41 of the largest may count as 0: all V of them are up to V 2^-41 of a sum.
+ * Sums are 64 bits wide: weights are good to 2^-34 + |l| / temperature 2^-52 of
+ * themselves in them.  A u within about the sum of these (2^-34 to 2^-33 for an
+ * ordinary row of up to 128 tokens below 2^-41, 2^-24 for 131 072 of them) of a
+ * border can fall on its other side, and p is as far off.
  * logits aligned to their type, ws to 16 bytes; ws_bytes at least
  * cia_sample_workspace_bytes(B, V); ws holds nothing between calls; calls that
  * share one must be ordered, captured graphs included.  B at most

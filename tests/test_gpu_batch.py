@@ -588,6 +588,47 @@ def test_sample_of_the_longest_rows(K, dev):
         check_sample(K, dev, l, [0.83, 0.21], f"{f}", **{k: np.full(2, v) for k, v in f.items()})
 
 
+def sample_within(K, dev, l, u, temperature, bound, what):
+    """Tokens equal where the draw is further than `bound` (of the kept mass) from a border, valid everywhere; p half
+    an fp32 step and twice the bound, once for the weight and once for the sum."""
+    ids, p = sample(K, dev, l, u, temperature=temperature)
+    want, q, near = ref.choose(l, np.asarray(u, np.float32), temperature=temperature.astype(np.float32))
+    sure = near > bound
+    assert np.array_equal(ids[sure], want[sure]), what
+    assert ((ids >= 0) & (ids < l.shape[1])).all()
+    same = ids == want
+    within(p[same], q[same], q[same] * (ref.U24 + 2 * bound), what)
+    return sure
+
+
+@pytest.mark.parametrize("V", [16384, 131072, 262144, 1 << 22])
+def test_sample_of_a_peak_and_a_far_tail(K, dev, V):
+    """One token and V - 1 alike far below it, on both sides of the weight from which on they may count as 0."""
+    gaps = np.array([20.0, 28.0, 28.4, 28.6, 29.0, 29.07, 29.2, 30.0])
+    l = np.repeat(-gaps[:, None].astype(np.float32), V, 1)
+    l[:, V // 3] = 0.0
+    far = 2.0 ** -34 + V * 2.0 ** -41
+    for u in (0.5, 1 - 2.0 ** -24):
+        sure = sample_within(K, dev, l, np.full(8, u), np.ones(8), far, f"{V} {u}")
+        assert u > 0.5 or sure.all()
+        # weights of 2^-41 and more (e^-28.4) count: bounds of their own alone
+        sample_within(K, dev, l[:3], np.full(3, u), np.ones(3), 2.0 ** -33, f"{V} {u}, counted")
+
+
+@pytest.mark.parametrize("V", [50, 20000])
+def test_sample_of_cold_rows(K, dev, V):
+    """Temperatures down to 2^-28 beside logits of 1, whose neighbours' weights are e^-1 to e^-16."""
+    rng = np.random.default_rng(V)
+    for e in (10, 18, 20, 22, 24, 26, 28):
+        T = 2.0 ** -e
+        l = np.zeros((6, V), np.float32)
+        for row in l:
+            row[rng.permutation(V)[:40]] = 1.0 - np.arange(40) * max(T, 2.0 ** -23)
+        if e == 10:
+            l[l == 0] = -1.0
+        assert sample_within(K, dev, l, rng.random(6), np.full(6, T), 2.0 ** -34 + 2.0 ** (e - 52) + V * 2.0 ** -41, f"2^-{e}").all()
+
+
 def test_sample_frequencies(K, dev):
     """Equally spaced numbers draw every token as often as its probability says."""
     rng = np.random.default_rng(0)
