@@ -408,7 +408,7 @@ class KvPages:
     between calls, as the pages' may; the tensors are kept."""
 
     def __init__(self, k, v, table, ks=None, vs=None):
-        if not isinstance(k, torch.Tensor) or k.dim() != 4:
+        if not isinstance(k, torch.Tensor) or k.dim() != 4 or not k.numel():
             raise ValueError("k: need a tensor [pages, kv heads, page, dim]")
         quant = k.dtype == torch.uint8
         if not quant and k.dtype not in _F16:

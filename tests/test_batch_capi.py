@@ -248,6 +248,16 @@ def test_more_wrapper_checks(cia):
         K.sample(l.t(), f, pos, ws)
 
 
+def test_pages_of_no_elements(cia):
+    import torch
+
+    from cuda_inf_amd import kernels as K
+    for shape in ((4, 2, 16, 0), (0, 2, 16, 64), (4, 0, 16, 64)):
+        k = torch.zeros(shape, dtype=torch.float16)
+        with pytest.raises(ValueError, match="k: need a tensor"):
+            K.KvPages(k, k, torch.zeros((1, 1), dtype=torch.int32))
+
+
 def test_page_table(cia):
     from cuda_inf_amd.layer import PageTable
     t = PageTable(3, 100, 8, page=16, device="cpu")
