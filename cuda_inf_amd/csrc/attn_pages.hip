@@ -313,8 +313,9 @@ __global__ __launch_bounds__(256, 2) void k_attn_pages(AttnPagesArgs a) {
         }
         // The numerators are those of weight times V's scale, so that they fill fp16's
         // range whatever the scales are: m is the max of s + log2 vs, less kLift.  It is let
-        // lag: a rescaling only where a numerator would be over 2^kMost (told by the
-        // difference, as the sum m + kMost is rounded too).
+        // lag: a rescaling only where a numerator would be 2^kMost or more.  (With steps of
+        // u there, top is off by u / 2 and so is the sum with kMost; of two numbers in these
+        // steps the smaller is less by u: what is not rescaled is below 2^kMost or at it.)
         float top = -__builtin_inff();
 #pragma unroll
         for (int b = 0; b < 2; b++)
@@ -322,7 +323,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_pages(AttnPagesArgs a) {
           for (int e = 0; e < kR; e++)
             top = __builtin_fmaxf(
                 top, kF8 ? y[b][e] + __builtin_amdgcn_logf(__builtin_fmaxf(vs[b][e], 0x1p-24f)) : y[b][e]);
-        if (__any(top - m > kMost)) {
+        if (__any(top >= m + kMost)) {
           float score = -__builtin_inff();
 #pragma unroll
           for (int b = 0; b < 2; b++)

@@ -372,11 +372,12 @@ def test_attention_at_the_largest_scales(K, orc, dev, quant, scale):
             within(out[s, h], want, np.abs(want) * 2.0 ** -11 + 2.0 ** -25, f"sequence {s}, head {h}")
 
 
+@pytest.mark.parametrize("sizes", [(-10, 7), (-16, -15), (-8, -7), (6, 7)])
 @pytest.mark.parametrize("quant", [True, False])
-@pytest.mark.parametrize("units", [2.0 ** 20, *(f * 2.0 ** e for e in (21, 22, 23, 24, 25, 26, 27, 28, 29) for f in (1.02, 1.3, 1.7)), 2.0 ** 40])
-def test_attention_of_equals_among_large_scores(K, orc, dev, quant, units):
+@pytest.mark.parametrize("units", [2.0 ** 20, *(f * 2.0 ** e for e in (21, 22, 23, 24, 25, 26, 27, 28, 29) for f in (1.02, 1.11, 1.3, 1.47, 1.7, 1.83)), 2.0 ** 40])
+def test_attention_of_equals_among_large_scores(K, orc, dev, quant, units, sizes):
     """Scores of `units` powers of 2, where fp32's steps reach and pass those that numerators are kept within.  All alike:
-    the mean of V, whose tokens' sizes (e4m3: scales) lie 2^16 apart; weights are equal, so that only the sums' terms
+    the mean of V, whose tokens' sizes (e4m3: scales) lie 2^16 apart or are all of one; weights are equal, so that only the sums' terms
     of ref.attend's bound count.  The later ones higher by 16 or more, and still so where both are rounded to steps of
     up to 16: their mean, and 128 / 100 * 2^-16 of the first ones' at most.  A call of two rows, and of so many that a
     workgroup has all units of a row."""
@@ -384,7 +385,7 @@ def test_attention_of_equals_among_large_scores(K, orc, dev, quant, units):
     n, D = 228, 64
     c = Cache(K, orc, dev, rng, [n, n], 1, D, 16, quant)
     shape = (c.n_pages, 1, 16)
-    size = (2.0 ** rng.integers(-10, 7, shape)).astype(np.float16)
+    size = (2.0 ** rng.integers(*sizes, shape)).astype(np.float16)
     v = rng.integers(-16, 17, (*shape, D)).astype(np.float32)  # (whole numbers to 16: exact in e4m3)
     k = np.zeros((*shape, D), np.float32)
     k[..., 0] = 448.0
