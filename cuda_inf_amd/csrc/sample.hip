@@ -18,8 +18,8 @@
 // whole sums.
 //
 // Bound by memory for large batches, which read a row once or, for a broad nucleus,
-// twice (4 V bytes a pass in fp32): 256 rows of 131 072, top-p, take 80 us, 28-30 of them the
-// bins (134 MB at 4.5-4.8 TB/s; 26.3 without their atomics) and 49-51 the choice, of which its
+// twice (4 V bytes a pass in fp32): 256 rows of 131 072, top-p, take 79 us, 29-30 of them the
+// bins (134 MB at 4.5-4.7 TB/s; their atomics are 3 % of it) and 48-50 the choice, of which its
 // pass is 19 (7 TB/s, part of it from the last-level cache).  By chains of dependent steps
 // for few: one row of 65 536 with all filters takes 16 us, 6 for the bins and 10 for the
 // choice; one row of 4000 8.0 in its one launch, of 60 7.8 (a call alone takes the host
@@ -1128,10 +1128,13 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_pick(SampleArgs a) {
 }
 
 // The same for a row of up to kPer * kStep logits by itself, which the threads keep in registers:
-// one launch, no bins through memory, no second pass.  us against the two kernels: one row
-// of 1000 with top-k and top-p 12.3 / 18.0, 256 of 4000 15.5 / 21.7, 256 of 16 384 with a broad
-// top-p 31.0 / 39.7.  (Longer rows chunk by chunk in one workgroup: 5.7 us a chunk of 16384,
-// even at 32 768 and 97 / 92 for 256 rows of 131 072.)
+// one launch, no bins through memory, no second pass.  us of the two kernels / of this one:
+//   logits                        1000         4000         8192        16 384
+//   one row, top-k and top-p   16.8 / 7.8   13.6 / 8.1   14.0 / 8.7   14.6 / 11.6
+//   256 rows, top-k and top-p  18.8 / 8.5   15.4 / 8.5   15.9 / 10.1  19.9 / 13.6
+//   256 rows, broad top-p      18.4 / 8.5   24.4 / 15.1  24.8 / 17.2  31.0 / 21.0
+// (Longer rows chunk by chunk in one workgroup: 5.7 us a chunk of 16384, even at 32 768 and 97
+// for 92 with 256 rows of 131 072.)
 template <bool kHalf, int kPer>
 __global__ __launch_bounds__(kSampleThreads) void k_sample_row(SampleArgs a) {
   using Row = SampleRow<kHalf, kPer, true>;
